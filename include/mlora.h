@@ -337,6 +337,82 @@ typedef struct MloraInstallState {
 
 int mlora_install_slots(const MloraInstallArgs* list, const MloraInstallState* states, int32_t count);
 
+/* ---- the attention block between the q|k|v and the o linear --------------------------------------- */
+
+#define MLORA_MAX_HEAD_DIM 256
+
+/* Norm, rotation and store of one batch's query, key and value heads in one launch.  For every token t and every head of q
+ * and k:  y = x * rsqrt(mean(x^2) + eps) * weight  where a weight is given, else y = x;  then the first `rotary` elements of y
+ * are turned in pairs by the angle of the token's position, (i, i + rotary / 2) or, interleaved, (2 i, 2 i + 1):
+ * (a, b) -> (a cos - b sin, a sin + b cos).  All of it in fp32, rounded once to the element type.  q goes to q_out, k to k_out
+ * and, with v, to the pages of a cache: row slot % page of block slot / page for slot = slots[t].  A token whose slot is negative or
+ * behind the last block is not stored; a position outside the table turns by NaN.  No two tokens of a call share a slot.
+ * An output may be its input's own memory with the same strides.  (reference: nanovllm_voxcpm/layers/rotary_embedding.py,
+ * layers/attention.py:10-50) */
+typedef struct MloraRotateArgs {
+  void* stream;
+  const void* q;            /* [T, heads, dim], unit stride inside a head; strides of rows and heads in elements */
+  const void* k;            /* [T, kv_heads, dim] */
+  const void* v;            /* [T, kv_heads, dim], or NULL when there is no cache */
+  void* q_out;              /* [T, heads, dim] */
+  void* k_out;              /* [T, kv_heads, dim], or NULL */
+  void* k_cache;            /* [num_blocks, page, kv_heads, dim], or NULL */
+  void* v_cache;
+  int64_t q_row, q_head, k_row, k_head, v_row, v_head, q_out_row, q_out_head, k_out_row, k_out_head;
+  int64_t k_block, k_cache_row, k_cache_head, v_block, v_cache_row, v_cache_head;
+  const void* positions;    /* [T] int32, or int64 with positions64 */
+  const void* slots;        /* [T] int32, or int64 with slots64; NULL when there is no cache */
+  const float* cos_sin;     /* [num_positions, rotary]: cosines, then sines; row stride table_row elements */
+  const void* q_weight;     /* [dim] of `dtype`, or fp32 with weights32; NULL: no norm */
+  const void* k_weight;
+  int64_t table_row, num_positions;
+  int32_t num_tokens, heads, kv_heads, dim, rotary;
+  int32_t num_blocks, page;
+  int32_t dtype;            /* of q, k, v, the outputs and the cache */
+  int32_t weights32, positions64, slots64, interleaved;
+  float eps;
+} MloraRotateArgs;
+
+int mlora_rotate_qk(const MloraRotateArgs* args);
+
+/* Attention of packed rows of queries over the keys and values of their sequences:
+ * out = sum_j p_j v_j, p = softmax over the visible keys j of scale * q . k_j, softmax and sums in fp32, one rounding at the
+ * end; in the 16-bit types p is rounded to the element type before it meets v.  Head h reads key-value head h / (heads / kv_heads).
+ * The query row i of a sequence with Lq rows and Lk keys stands at position p = Lk - Lq + i.  In causal order it sees the keys
+ * j <= p with j > p - window (window 0: all of them) or j < sinks; without it, all Lk.  A row that sees nothing is 0.  What lies in hidden
+ * places (infinities and NaN too) does not reach the result.  Keys and values lie packed, [num_keys, kv_heads, dim], or in the pages of a
+ * cache, [num_blocks, page, kv_heads, dim]; a page id outside the cache stands for keys that nobody sees.
+ * (reference: nanovllm_voxcpm/layers/attention.py:70-105) */
+typedef struct MloraAttentionArgs {
+  void* stream;
+  const void* q;                /* [num_rows, heads, dim], strides of rows and heads in elements */
+  void* out;                    /* the same */
+  const void* k;
+  const void* v;
+  int64_t q_row, q_head, out_row, out_head;
+  int64_t k_block, k_row, k_head, v_block, v_row, v_head; /* packed keys: *_block unused */
+  const int32_t* starts;        /* prompts: [sequences + 1] first query row of every sequence (the rows behind the last
+                                   sequence are left as they were); decode: unused, row i is sequence i */
+  const int32_t* key_starts;    /* packed keys: [sequences + 1] first key row of every sequence, NULL: starts */
+  const int32_t* block_tables;  /* pages: [sequences, table_width], row stride table_row; NULL: packed keys */
+  const int32_t* context_lens;  /* pages: [sequences] keys of every sequence, its query rows' among them */
+  int64_t table_row;
+  int32_t table_width, num_blocks, page;
+  int32_t num_rows, num_keys, sequences, heads, kv_heads, dim;
+  int32_t dtype;                /* of q, k, v and out */
+  int32_t causal, window, sinks;
+  float scale;
+  void* workspace;              /* decode only: 16-byte aligned scratch of mlora_decode_attention_workspace_bytes, needed only
+                                   while the call's work is under way; without it a sequence is not split */
+  int64_t workspace_bytes;
+} MloraAttentionArgs;
+
+/* One query row per sequence over a paged cache (num_rows == sequences). */
+int mlora_decode_attention(const MloraAttentionArgs* args);
+size_t mlora_decode_attention_workspace_bytes(int32_t sequences, int32_t heads, int32_t kv_heads, int32_t dim);
+/* Any number of query rows per sequence, packed one sequence behind the other. */
+int mlora_prompt_attention(const MloraAttentionArgs* args);
+
 /* Identifier of the graph capture in progress on `stream`, 0 when the stream is not
  * capturing.  No counterpart in the reference: lets a host-side cache tell work recorded
  * into one capture from work run eagerly or recorded into another capture. */

@@ -68,6 +68,10 @@ EXPORTS = (
     "mlora_meta_build_runs",
     "mlora_install_slot",
     "mlora_install_slots",
+    "mlora_rotate_qk",
+    "mlora_decode_attention",
+    "mlora_decode_attention_workspace_bytes",
+    "mlora_prompt_attention",
     "mlora_stream_capture_id",
     "mlora_abi_version",
     "mlora_last_error",
@@ -194,6 +198,33 @@ class MloraInstallState(C.Structure):
     _fields_ = [("rank", C.c_void_p), ("scaling", C.c_void_p * 2), ("dtype", C.c_int32)]
 
 
+class MloraRotateArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("stream", "q", "k", "v", "q_out", "k_out", "k_cache", "v_cache")),
+        *((n, C.c_int64) for n in ("q_row", "q_head", "k_row", "k_head", "v_row", "v_head", "q_out_row", "q_out_head", "k_out_row", "k_out_head",
+                                   "k_block", "k_cache_row", "k_cache_head", "v_block", "v_cache_row", "v_cache_head")),
+        *((n, C.c_void_p) for n in ("positions", "slots", "cos_sin", "q_weight", "k_weight")),
+        *((n, C.c_int64) for n in ("table_row", "num_positions")),
+        *((n, C.c_int32) for n in ("num_tokens", "heads", "kv_heads", "dim", "rotary", "num_blocks", "page", "dtype", "weights32", "positions64",
+                                   "slots64", "interleaved")),
+        ("eps", C.c_float),
+    ]
+
+
+class MloraAttentionArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("stream", "q", "out", "k", "v")),
+        *((n, C.c_int64) for n in ("q_row", "q_head", "out_row", "out_head", "k_block", "k_row", "k_head", "v_block", "v_row", "v_head")),
+        *((n, C.c_void_p) for n in ("starts", "key_starts", "block_tables", "context_lens")),
+        ("table_row", C.c_int64),
+        *((n, C.c_int32) for n in ("table_width", "num_blocks", "page", "num_rows", "num_keys", "sequences", "heads", "kv_heads", "dim", "dtype",
+                                   "causal", "window", "sinks")),
+        ("scale", C.c_float),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
 _LIB: C.CDLL | None = None
 _LOAD_ERROR: str | None = None
 
@@ -229,6 +260,9 @@ def load() -> C.CDLL:
         ("mlora_expand", MloraExpandArgs),
         ("mlora_meta_build", MloraMetaArgs),
         ("mlora_install_slot", MloraInstallArgs),
+        ("mlora_rotate_qk", MloraRotateArgs),
+        ("mlora_decode_attention", MloraAttentionArgs),
+        ("mlora_prompt_attention", MloraAttentionArgs),
     ):
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(args)]
@@ -249,6 +283,8 @@ def load() -> C.CDLL:
     lib.mlora_add_workspace_bytes.restype = C.c_size_t
     lib.mlora_workspace_init.argtypes = [C.c_void_p, C.c_int64, C.c_void_p]
     lib.mlora_workspace_init.restype = C.c_int
+    lib.mlora_decode_attention_workspace_bytes.argtypes = [C.c_int32] * 4
+    lib.mlora_decode_attention_workspace_bytes.restype = C.c_size_t
     lib.mlora_stream_capture_id.argtypes = [C.c_void_p]
     lib.mlora_stream_capture_id.restype = C.c_uint64
     _declare_diag(lib)
@@ -718,6 +754,91 @@ def install_slot(
     args.num_slots = a_dst.size(0)
     with _on(a_dst.device):
         _check(lib.mlora_install_slot(C.byref(args)), "mlora_install_slot")
+
+
+def _strides(args, names: tuple[str, ...], t: torch.Tensor) -> None:
+    """Strides of t but for its last dimension, in elements, into the named fields."""
+    for name, stride in zip(names, t.stride()):
+        setattr(args, name, stride)
+
+
+def rotate_qk(q, k, v, q_out, k_out, k_cache, v_cache, positions, slots, cos_sin, q_weight, k_weight, eps: float, interleaved: bool) -> None:
+    """Norm, rotation and cache store of a batch's heads; tensors checked by ``attention_ops.rotate_qk``."""
+    lib = load()
+    _require_cuda(q, "q")
+    args = MloraRotateArgs()
+    args.stream = _stream(q.device)
+    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out), ("k_cache", k_cache), ("v_cache", v_cache),
+                    ("positions", positions), ("slots", slots), ("cos_sin", cos_sin), ("q_weight", q_weight), ("k_weight", k_weight)):
+        if t is not None:
+            setattr(args, name, t.data_ptr())
+    for name, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out), ("k_out", k_out)):
+        if t is not None:
+            _strides(args, (f"{name}_row", f"{name}_head"), t)
+    if k_cache is not None:
+        _strides(args, ("k_block", "k_cache_row", "k_cache_head"), k_cache)
+        _strides(args, ("v_block", "v_cache_row", "v_cache_head"), v_cache)
+        args.num_blocks, args.page = k_cache.size(0), k_cache.size(1)
+        args.slots64 = slots.dtype == torch.int64
+    args.table_row, args.num_positions = cos_sin.stride(0), cos_sin.size(0)
+    args.num_tokens, args.heads, args.dim = q.shape
+    args.kv_heads, args.rotary = k.size(1), cos_sin.size(1)
+    args.dtype = dtype_code(q.dtype)
+    weight = q_weight if q_weight is not None else k_weight
+    args.weights32 = weight is not None and weight.dtype == torch.float32
+    args.positions64 = positions.dtype == torch.int64
+    args.interleaved, args.eps = interleaved, eps
+    with _on(q.device):
+        _check(lib.mlora_rotate_qk(C.byref(args)), "mlora_rotate_qk")
+
+
+def _attention_args(q, out, k, v, block_tables, context_lens, causal: bool, scale: float, window: int, sinks: int) -> MloraAttentionArgs:
+    _require_cuda(q, "q")
+    args = MloraAttentionArgs()
+    args.stream = _stream(q.device)
+    args.q, args.out, args.k, args.v = q.data_ptr(), out.data_ptr(), k.data_ptr(), v.data_ptr()
+    _strides(args, ("q_row", "q_head"), q)
+    _strides(args, ("out_row", "out_head"), out)
+    if block_tables is not None:
+        _strides(args, ("k_block", "k_row", "k_head"), k)
+        _strides(args, ("v_block", "v_row", "v_head"), v)
+        args.block_tables, args.context_lens = block_tables.data_ptr(), context_lens.data_ptr()
+        args.table_row, args.table_width = block_tables.stride(0), block_tables.size(1)
+        args.num_blocks, args.page = k.size(0), k.size(1)
+    else:
+        _strides(args, ("k_row", "k_head"), k)
+        _strides(args, ("v_row", "v_head"), v)
+        args.num_keys = k.size(0)
+    args.num_rows, args.heads, args.dim = q.shape
+    args.kv_heads = k.size(-2)
+    args.dtype = dtype_code(q.dtype)
+    args.causal, args.scale, args.window, args.sinks = causal, scale, min(window, 2**31 - 1), min(sinks, 2**31 - 1)
+    return args
+
+
+def decode_attention(q, out, k_cache, v_cache, block_tables, context_lens, scale: float, window: int, sinks: int) -> None:
+    """One query row per sequence over a paged cache; tensors checked by ``attention_ops.decode_attention``."""
+    lib = load()
+    args = _attention_args(q, out, k_cache, v_cache, block_tables, context_lens, True, scale, window, sinks)
+    args.sequences = q.size(0)
+    nbytes = lib.mlora_decode_attention_workspace_bytes(args.sequences, args.heads, args.kv_heads, args.dim)
+    if nbytes:  # scratch of this call alone: the allocator hands it to nobody before the stream (or the graph) is past the call
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+        args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
+    with _on(q.device):
+        _check(lib.mlora_decode_attention(C.byref(args)), "mlora_decode_attention")
+
+
+def prompt_attention(q, out, k, v, starts, key_starts, block_tables, context_lens, causal: bool, scale: float, window: int, sinks: int) -> None:
+    """Packed query rows over packed or paged keys; tensors checked by ``attention_ops.prompt_attention``."""
+    lib = load()
+    args = _attention_args(q, out, k, v, block_tables, context_lens, causal, scale, window, sinks)
+    args.starts = starts.data_ptr()
+    if key_starts is not None:
+        args.key_starts = key_starts.data_ptr()
+    args.sequences = starts.numel() - 1
+    with _on(q.device):
+        _check(lib.mlora_prompt_attention(C.byref(args)), "mlora_prompt_attention")
 
 
 def stream_capture_id(device: torch.device, stream: int | None = None) -> int:

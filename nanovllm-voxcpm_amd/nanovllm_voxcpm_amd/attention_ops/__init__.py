@@ -1,0 +1,298 @@
+"""The attention block between the q|k|v and the o linear, executed by the HIP library.
+
+``rotate_qk`` norms and rotates the query and key heads of a batch and writes keys and values into the pages of a cache
+(reference: nanovllm_voxcpm/layers/rotary_embedding.py, layers/attention.py:10-50); ``decode_attention`` attends with one new
+token per sequence to such a cache, ``prompt_attention`` with any number of rows per sequence to packed keys or to a cache
+(reference: nanovllm_voxcpm/layers/attention.py:70-105).
+
+All three enqueue work on torch's current stream and neither synchronise nor read device data on the host, so they may be
+captured into a graph.  They have no backward: call them under ``torch.no_grad()`` or ``torch.inference_mode()``.
+Element types are fp32, fp16 and bf16, head sizes multiples of 8 up to 256; index vectors are int32 (positions and slots may
+be int64).  Tensors may be strided views as long as a head's elements lie side by side.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from nanovllm_voxcpm_amd import _hip
+
+__all__ = ["decode_attention", "prompt_attention", "rotary_table", "rotate_qk"]
+
+
+def rotary_table(rotary_dim: int, num_positions: int, *, base: float = 10000.0, factors: torch.Tensor | list[float] | None = None,
+                 scale: float = 1.0, device: torch.device | str | None = None) -> torch.Tensor:
+    """The fp32 table ``[num_positions, rotary_dim]`` of ``rotate_qk``: cosines, then sines, of position * base ** (-2 i / rotary_dim) /
+    factors[i] (``factors``: one per pair, for long-context models), times ``scale``.  Angles are computed in 64 bits: in 32
+    those of far positions are off by thousandths."""
+    if rotary_dim < 2 or rotary_dim % 2:
+        raise ValueError(f"rotary_dim must be an even number, got {rotary_dim}")
+    if num_positions < 1:
+        raise ValueError(f"num_positions must be positive, got {num_positions}")
+    half = rotary_dim // 2
+    inverse = float(base) ** (-torch.arange(half, dtype=torch.float64) / half)
+    if factors is not None:
+        factors = torch.as_tensor(factors, dtype=torch.float64).cpu()
+        if factors.shape != (half,):
+            raise ValueError(f"factors must hold one value for each of the {half} pairs, got shape {tuple(factors.shape)}")
+        inverse = inverse / factors
+    angles = torch.arange(num_positions, dtype=torch.float64)[:, None] * inverse[None, :]
+    return (torch.cat([angles.cos(), angles.sin()], dim=1) * scale).float().to(device or "cpu")
+
+
+def _heads(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be [rows, heads, head size], got shape {tuple(t.shape)}")
+    if t.numel() and t.stride(2) != 1 and t.size(2) != 1:
+        raise ValueError(f"the elements of a head of {name} must lie side by side")
+    _same(t, name, like)
+
+
+def _same(t: torch.Tensor, name: str, like: torch.Tensor | None) -> None:
+    if like is None:
+        return
+    if t.device != like.device:
+        raise ValueError(f"{name} lives on {t.device}, q on {like.device}")
+    if t.dtype != like.dtype:
+        raise ValueError(f"{name} has element type {t.dtype}, q has {like.dtype}")
+
+
+def _index(t: torch.Tensor, name: str, device: torch.device, least: int, dtypes=(torch.int32,)) -> None:
+    if t.dtype not in dtypes or t.dim() != 1 or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {' or '.join(str(d).replace('torch.', '') for d in dtypes)} vector")
+    if t.device != device:
+        raise ValueError(f"{name} lives on {t.device}, q on {device}")
+    if t.numel() < least:
+        raise ValueError(f"{name} has {t.numel()} entries, {least} are needed")
+
+
+def _cache(k: torch.Tensor, v: torch.Tensor, kv_heads: int | None, q: torch.Tensor, names=("k_cache", "v_cache")) -> None:
+    for t, name in ((k, names[0]), (v, names[1])):
+        if t.dim() != 4:
+            raise ValueError(f"{name} must be [blocks, rows of a block, heads, head size], got shape {tuple(t.shape)}")
+        if t.numel() and t.stride(3) != 1 and t.size(3) != 1:
+            raise ValueError(f"the elements of a head of {name} must lie side by side")
+        _same(t, name, q)
+    if k.shape != v.shape:
+        raise ValueError(f"{names[0]} {tuple(k.shape)} and {names[1]} {tuple(v.shape)} differ")
+    if k.size(1) < 1:
+        raise ValueError(f"{names[0]} has blocks without rows")
+    if k.size(3) != q.size(2) or (kv_heads is not None and k.size(2) != kv_heads):
+        raise ValueError(f"{names[0]} {tuple(k.shape)} does not hold heads of size {q.size(2)}" + (f", {kv_heads} of them" if kv_heads is not None else ""))
+
+
+def _no_grad(*tensors: torch.Tensor | None) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError("the attention ops have no backward: call them under torch.no_grad() or torch.inference_mode()")
+
+
+def _memory(t: torch.Tensor) -> tuple[int, int]:
+    """First byte of a strided tensor and the one behind its last."""
+    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _rows_apart(t: torch.Tensor, name: str) -> None:
+    """An output's elements must not lie on one another (an expanded view)."""
+    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+        raise ValueError(f"rows or heads of {name} share memory")
+
+
+def _result(out: torch.Tensor | None, source: torch.Tensor, name: str) -> torch.Tensor:
+    """The caller's output, or a new one; it may be the source's own memory with the same strides."""
+    if out is None:
+        return torch.empty(source.shape, dtype=source.dtype, device=source.device)
+    if out.shape != source.shape:
+        raise ValueError(f"{name} has shape {tuple(out.shape)}, {tuple(source.shape)} is needed")
+    _heads(out, name, source)
+    _rows_apart(out, name)
+    if out.numel() and not (out.data_ptr() == source.data_ptr() and out.stride() == source.stride()):
+        (a, b), (c, d) = _memory(out), _memory(source)
+        if a < d and c < b and not (out.untyped_storage().data_ptr() == source.untyped_storage().data_ptr() and out.stride(0) == source.stride(0)):
+            raise ValueError(f"{name} overlaps its input")
+    return out
+
+
+def rotate_qk(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    positions: torch.Tensor,
+    cos_sin: torch.Tensor,
+    *,
+    q_weight: torch.Tensor | None = None,
+    k_weight: torch.Tensor | None = None,
+    eps: float = 1e-6,
+    interleaved: bool = False,
+    v: torch.Tensor | None = None,
+    k_cache: torch.Tensor | None = None,
+    v_cache: torch.Tensor | None = None,
+    slot_mapping: torch.Tensor | None = None,
+    q_out: torch.Tensor | None = None,
+    k_out: torch.Tensor | None = None,
+) -> tuple[torch.Tensor, torch.Tensor | None]:
+    """Norm and rotate the heads of ``q [T, heads, D]`` and ``k [T, kv_heads, D]`` and store k and v in a cache, in one launch.
+
+    ``q_weight``, ``k_weight`` (``[D]``, the element type of q or fp32): RMS norm of every head first, x * rsqrt(mean(x^2) + eps) *
+    weight; None leaves the heads as they are.  The first ``cos_sin.size(1)`` elements of a head are then turned by row
+    ``positions[t]`` of the table (``rotary_table``), in pairs (i, i + half) or, ``interleaved``, (2 i, 2 i + 1).  Everything is
+    computed in fp32 and rounded once.  A position outside the table gives NaN.
+
+    With ``k_cache``, ``v_cache [blocks, rows of a block, kv_heads, D]``, ``v`` and ``slot_mapping [T]`` the new k and v of token t go to row
+    ``slot_mapping[t]`` of the cache, counted over all blocks; a negative slot (padding) or one behind the last block is
+    not stored.  No two tokens may share a slot.
+
+    Returns (q, k): in ``q_out`` and ``k_out`` where given (an input itself is fine), else new tensors; k is None with a cache
+    and without ``k_out``, since the cache has it.
+    """
+    _heads(q, "q")
+    _heads(k, "k", q)
+    _no_grad(q, k, v, q_weight, k_weight)
+    rows, dim = q.size(0), q.size(2)
+    if k.size(0) != rows or k.size(2) != dim:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in rows or head size")
+    _index(positions, "positions", q.device, rows, (torch.int32, torch.int64))
+    if cos_sin.dim() != 2 or cos_sin.dtype != torch.float32 or (cos_sin.numel() and cos_sin.stride(1) != 1):
+        raise ValueError("cos_sin must be an fp32 [positions, rotary size] table with rows side by side")
+    if cos_sin.device != q.device:
+        raise ValueError(f"cos_sin lives on {cos_sin.device}, q on {q.device}")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is None:
+            continue
+        if w.device != q.device:
+            raise ValueError(f"{name} lives on {w.device}, q on {q.device}")
+        if w.dtype not in (q.dtype, torch.float32) or w.shape != (dim,) or not w.is_contiguous():
+            raise ValueError(f"{name} must be a contiguous vector of {dim} elements, fp32 or {q.dtype}")
+    if q_weight is not None and k_weight is not None and q_weight.dtype != k_weight.dtype:
+        raise ValueError("q_weight and k_weight must have the same element type")
+    cached = [t is not None for t in (v, k_cache, v_cache, slot_mapping)]
+    if any(cached) and not all(cached):
+        raise ValueError("v, k_cache, v_cache and slot_mapping are given together or not at all")
+    if all(cached):
+        _heads(v, "v", q)
+        if v.shape != k.shape:
+            raise ValueError(f"v {tuple(v.shape)} and k {tuple(k.shape)} differ")
+        _cache(k_cache, v_cache, k.size(1), q)
+        for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+            _rows_apart(t, name)
+        _index(slot_mapping, "slot_mapping", q.device, rows, (torch.int32, torch.int64))
+    q_out = _result(q_out, q, "q_out")
+    if k_out is not None or not all(cached):
+        k_out = _result(k_out, k, "k_out")
+    _hip.rotate_qk(q, k, v, q_out, k_out, k_cache, v_cache, positions, slot_mapping, cos_sin, q_weight, k_weight, float(eps), bool(interleaved))
+    return q_out, k_out
+
+
+def _masks(window: int, sinks: int) -> None:
+    if window < 0 or sinks < 0:
+        raise ValueError(f"window and sinks must not be negative, got {window} and {sinks}")
+
+
+def _table(block_tables: torch.Tensor, context_lens: torch.Tensor, sequences: int, device: torch.device) -> None:
+    if block_tables.dim() != 2 or block_tables.dtype != torch.int32 or (block_tables.numel() and block_tables.size(1) > 1 and block_tables.stride(1) != 1):
+        raise ValueError("block_tables must be an int32 [sequences, blocks] table with rows side by side")
+    if block_tables.device != device:
+        raise ValueError(f"block_tables lives on {block_tables.device}, q on {device}")
+    if block_tables.size(0) < sequences:
+        raise ValueError(f"block_tables has {block_tables.size(0)} rows for {sequences} sequences")
+    _index(context_lens, "context_lens", device, sequences)
+
+
+def _output(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if out.shape != q.shape:
+        raise ValueError(f"out has shape {tuple(out.shape)}, {tuple(q.shape)} is needed")
+    _heads(out, "out", q)
+    _rows_apart(out, "out")
+    if out.numel():
+        (a, b), (c, d) = _memory(out), _memory(q)
+        if a < d and c < b:
+            raise ValueError("out overlaps q")
+    return out
+
+
+def _shared_heads(heads: int, kv_heads: int) -> None:
+    if heads and (kv_heads < 1 or heads % kv_heads):
+        raise ValueError(f"{heads} query heads do not share {kv_heads} key-value heads evenly")
+
+
+def decode_attention(
+    q: torch.Tensor,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor,
+    block_tables: torch.Tensor,
+    context_lens: torch.Tensor,
+    *,
+    scale: float | None = None,
+    window: int = 0,
+    sinks: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of one new token per sequence, ``q [sequences, heads, D]``, over the first ``context_lens[s]`` rows (the new token's among
+    them) of the pages ``block_tables[s]`` of ``k_cache``, ``v_cache [blocks, rows of a block, kv_heads, D]``.
+
+    ``scale``: of the scores, D ** -0.5 by default.  ``window``: only the last ``window`` rows are seen (0: all), and the
+    first ``sinks`` beside them.  A sequence of no rows (padding) gives 0.  Lengths beyond the table's pages end there; the rows of a page
+    id outside the cache are not seen.  What lies in rows that are not seen does not matter.
+    """
+    _heads(q, "q")
+    _cache(k_cache, v_cache, None, q)
+    _no_grad(q, k_cache, v_cache)
+    _shared_heads(q.size(1), k_cache.size(2))
+    _masks(window, sinks)
+    _table(block_tables, context_lens, q.size(0), q.device)
+    out = _output(out, q)
+    _hip.decode_attention(q, out, k_cache, v_cache, block_tables, context_lens, q.size(2) ** -0.5 if scale is None else float(scale), window, sinks)
+    return out
+
+
+def prompt_attention(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    cu_seqlens: torch.Tensor,
+    *,
+    cu_seqlens_k: torch.Tensor | None = None,
+    block_tables: torch.Tensor | None = None,
+    context_lens: torch.Tensor | None = None,
+    causal: bool = True,
+    scale: float | None = None,
+    window: int = 0,
+    sinks: int = 0,
+    out: torch.Tensor | None = None,
+) -> torch.Tensor:
+    """Attention of packed sequences: rows ``cu_seqlens[s] : cu_seqlens[s + 1]`` of ``q [T, heads, D]`` are the last rows of sequence s.
+
+    Keys and values lie packed, ``k``, ``v [rows, kv_heads, D]`` with sequence s at ``cu_seqlens_k[s] : cu_seqlens_k[s + 1]`` (``cu_seqlens`` by
+    default), or, with ``block_tables`` and ``context_lens``, in the pages of a cache, ``[blocks, rows of a block, kv_heads, D]``, as in
+    ``decode_attention``.  ``causal``: a row sees its own key and those in front of it, with ``window`` only the last ``window`` of
+    them and the first ``sinks`` keys; without ``causal`` every row sees the whole sequence.  Rows that see nothing are 0, rows of
+    ``out`` behind the last sequence are left as they are (a new ``out`` holds anything there).
+    """
+    _heads(q, "q")
+    _masks(window, sinks)
+    if not causal and (window or sinks):
+        raise ValueError("a window or sinks need causal order")
+    _index(cu_seqlens, "cu_seqlens", q.device, 1)
+    sequences = cu_seqlens.numel() - 1
+    if (block_tables is None) != (context_lens is None):
+        raise ValueError("block_tables and context_lens are given together or not at all")
+    if block_tables is not None:
+        if cu_seqlens_k is not None:
+            raise ValueError("cu_seqlens_k is for packed keys: with block_tables context_lens says how many there are")
+        _cache(k, v, None, q, ("k", "v"))
+        _shared_heads(q.size(1), k.size(2))
+        _table(block_tables, context_lens, sequences, q.device)
+    else:
+        _heads(k, "k", q)
+        _heads(v, "v", q)
+        if k.shape != v.shape or k.size(2) != q.size(2):
+            raise ValueError(f"k {tuple(k.shape)} and v {tuple(v.shape)} must be alike, with heads of size {q.size(2)}")
+        _shared_heads(q.size(1), k.size(1))
+        if cu_seqlens_k is not None:
+            _index(cu_seqlens_k, "cu_seqlens_k", q.device, sequences + 1)
+    _no_grad(q, k, v)
+    out = _output(out, q)
+    _hip.prompt_attention(q, out, k, v, cu_seqlens, cu_seqlens_k, block_tables, context_lens, bool(causal),
+                          q.size(2) ** -0.5 if scale is None else float(scale), window, sinks)
+    return out
