@@ -9,6 +9,11 @@ namespace mlora {
 bool attention_vectors_ok(const MloraAttentionArgs* a);  // every row of q, out, k and v starts on a 16-byte boundary
 int launch_attend_rows(const MloraAttentionArgs* a);     // any head size, stride and page
 
+// paged.hip: one row per sequence over pages, head sizes 64 and 128
+bool paged_supported(const MloraAttentionArgs* a);
+size_t paged_workspace_bytes(int sequences, int heads, int kv_heads, int dim);
+int launch_paged(const MloraAttentionArgs* a);
+
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;

@@ -85,6 +85,7 @@ int check_attention(const MloraAttentionArgs* a, const char* what, bool decode) 
     if (!a->context_lens || a->page < 1) { set_error("%s: pages need context_lens and a page of at least one row", what); return MLORA_E_INVALID; }
     if (static_cast<int64_t>(a->table_width) * a->page > INT32_MAX / 2) { set_error("%s: %d pages of %d rows are more positions than 2^30", what, a->table_width, a->page); return MLORA_E_TOO_LARGE; }
   }
+  if (reinterpret_cast<uintptr_t>(a->workspace) & 15) { set_error("%s: workspace is not 16-byte aligned", what); return MLORA_E_INVALID; }
   const bool keys = a->block_tables ? a->num_blocks > 0 && a->table_width > 0 : a->num_keys > 0;
   if (keys && (!a->k || !a->v)) { set_error("%s: NULL pointer", what); return MLORA_E_INVALID; }
   if (static_cast<int64_t>(a->num_rows) * a->heads > (1ll << 30)) { set_error("%s: %d rows of %d heads are more than one launch holds", what, a->num_rows, a->heads); return MLORA_E_TOO_LARGE; }
@@ -98,11 +99,13 @@ extern "C" int mlora_decode_attention(const MloraAttentionArgs* a) {
   if (rc) return rc == kNothing ? 0 : rc;
   MloraAttentionArgs b = *a;
   b.starts = nullptr;
+  if (paged_supported(&b)) return launch_paged(&b);
   return launch_attend_rows(&b);
 }
 
 extern "C" size_t mlora_decode_attention_workspace_bytes(int32_t sequences, int32_t heads, int32_t kv_heads, int32_t dim) {
-  return 0;
+  if (sequences <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || (dim != 64 && dim != 128)) return 0;
+  return paged_workspace_bytes(sequences, heads, kv_heads, dim);
 }
 
 extern "C" int mlora_prompt_attention(const MloraAttentionArgs* a) {
