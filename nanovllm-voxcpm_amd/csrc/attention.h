@@ -14,6 +14,10 @@ bool paged_supported(const MloraAttentionArgs* a);
 size_t paged_workspace_bytes(int sequences, int heads, int kv_heads, int dim);
 int launch_paged(const MloraAttentionArgs* a);
 
+// prompt.hip: packed rows, head sizes 64 and 128
+bool prompt_supported(const MloraAttentionArgs* a);
+int launch_prompt(const MloraAttentionArgs* a);
+
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;

@@ -111,5 +111,6 @@ extern "C" size_t mlora_decode_attention_workspace_bytes(int32_t sequences, int3
 extern "C" int mlora_prompt_attention(const MloraAttentionArgs* a) {
   const int rc = check_attention(a, "mlora_prompt_attention", false);
   if (rc) return rc == kNothing ? 0 : rc;
+  if (prompt_supported(a)) return launch_prompt(a);
   return launch_attend_rows(a);
 }

@@ -126,7 +126,7 @@ __device__ __forceinline__ Workspace workspace_of(const MloraAttentionArgs& a, i
 }
 
 template <typename T, int D>
-__global__ __launch_bounds__(kWaves * 64) void paged_kernel(MloraAttentionArgs a, int target, int page_shift) {
+__global__ __launch_bounds__(kWaves * 64, 2) void paged_kernel(MloraAttentionArgs a, int target, int page_shift) {
   using S = Shape<T, D>;
   constexpr int kKeys = S::kKeys, kSteps = S::kChunks / 4, kBlocks = D / 16;
   extern __shared__ __align__(16) char lds[];
@@ -214,7 +214,8 @@ __global__ __launch_bounds__(kWaves * 64) void paged_kernel(MloraAttentionArgs a
       float s[kKeys / 4];
 #pragma unroll
       for (int b = 0; b < kKeys / 16; ++b) {
-        f32x4 c{0, 0, 0, 0};
+        f32x4 products[1] = {{0, 0, 0, 0}};
+        f32x4& c = products[0];
         const int r = 16 * b + column;
 #pragma unroll
         for (int st = 0; st < kSteps; ++st) {
@@ -222,6 +223,7 @@ __global__ __launch_bounds__(kWaves * 64) void paged_kernel(MloraAttentionArgs a
           key.raw = load128(k_tile + r * S::kRow + 16 * S::k_place(r, g + 4 * st));
           c = Mma<T>::run(key, query[st], c);
         }
+        if constexpr (sizeof(T) == 4) mfma_settle(products);  // (the branch over the masks below)
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[4 * b + j] = c[j] * scale;
       }

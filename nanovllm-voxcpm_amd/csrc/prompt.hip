@@ -1,0 +1,434 @@
+// Attention of packed prompts over packed or paged keys, head sizes 64 and 128 (mlora_prompt_attention).
+//
+// One workgroup per (128 query rows of a sequence, head): four wavefronts of 32 rows each.  Tiles of 64 keys and their values are
+// staged in LDS by direct loads, two stages deep: one barrier a tile, behind which the next tile is asked for.  The scores come out of the first product with the
+// keys along the registers and the query rows along the lanes (K Q^T, 32 x 32 tiles), which is how the second one (V^T P^T) wants its
+// weights: they never leave the registers, a row's maximum and sum are a lane's own but for one exchange between the halves of the
+// wave, and V^T is read through the transposing LDS read.  The running maximum moves only when a tile's exceeds it by more than 2^8
+// (any base serves a softmax as long as its weights stay finite), so the outputs are hardly ever rescaled.
+//
+// Bound by the vector ALU at head size 64: a score costs a fused multiply-add (4 cycles for 64 of them), an exponential (16), parts of a maximum, a sum and a
+// conversion (4, 4 and 2), against 16 cycles of matrix core for its two products; at 128 by both alike.
+//
+// A row whose result is not finite is computed again by the kernel that never touches a hidden key (attend_row): 0 times NaN or infinity is what a product
+// over a tile makes of a hidden one's values.
+#include "attention.h"
+#include "common.h"
+#include "dma.h"
+#include "launch.h"
+#include "lds.h"
+
+namespace mlora {
+
+namespace {
+
+constexpr int kWaves = 4, kRows = 32 * kWaves, kKeys = 64;
+// 2^-kMoves: how far below a row's largest weight the base may lie; the weights are then at most 2^kMoves times 2^shift.
+constexpr float kMoves = 8.0f;
+
+template <typename T> struct Mma32;
+template <> struct Mma32<__bf16> {
+  static __device__ __forceinline__ f32x16 run(const Pack8& a, const Pack8& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a.bf, b.bf, c, 0, 0, 0); }
+};
+template <> struct Mma32<_Float16> {
+  static __device__ __forceinline__ f32x16 run(const Pack8& a, const Pack8& b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a.hf, b.hf, c, 0, 0, 0); }
+};
+template <> struct Mma32<float> {  // four 32x32x2 products, product j taking element j of every lane's piece
+  static __device__ __forceinline__ f32x16 run(const Pack8& a, const Pack8& b, f32x16 c) {
+    f32x4 x, y;
+    __builtin_memcpy(&x, &a, 16);
+    __builtin_memcpy(&y, &b, 16);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(x[j], y[j], c, 0, 0, 0);
+    return c;
+  }
+};
+
+template <typename T, int D> struct Shape {
+  static constexpr int kRow = D * static_cast<int>(sizeof(T)), kChunks = kRow / 16;
+  static constexpr int kBytes = kKeys * kRow;             // K or V of a tile
+  static constexpr int kLoads = kBytes / 1024 / kWaves;   // a wavefront's share of it
+  static constexpr int kRowsPerLoad = 1024 / kRow;
+  static constexpr int kLds = 2 * 2 * kBytes;
+  // A read of K takes the same piece of 32 rows, one of V^T 64 bytes of four rows (in fp32 128 of rows four apart).
+  static __device__ __forceinline__ int k_place(int row, int chunk) { return chunk ^ (kRow == 128 ? (row >> 1) & 7 : row & 15); }
+  static __device__ __forceinline__ int v_place(int row, int chunk) {
+    return chunk ^ (sizeof(T) == 4 ? ((row >> 2) & 1) << 3 : kRow == 128 ? ((row >> 1) & 1) << 2 : (row & 3) << 2);
+  }
+};
+
+typedef __attribute__((address_space(3))) s16x4 LdsS16x4;
+
+__device__ __forceinline__ float other_half(float v, float* both) {  // lanes l and l + 32
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  *both = __uint_as_float(r[1]);
+  return __uint_as_float(r[0]);
+}
+
+struct RowTile {
+  int sequence, start, rows;  // first query row (of q) and how many
+  int position;               // of the first
+  int total, key_start;
+};
+
+// The item-th tile of the batch, the last of every batch first (the later rows of a prompt see the most keys).  By one wavefront.
+__device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int item, int lane, RowTile* t) {
+  int tiles = 0, begin = 0, end = 0;
+  for (int s = lane; s < a.sequences; s += 64) {
+    begin = clamped(a.starts[s], a.num_rows);
+    end = clamped(a.starts[s + 1], a.num_rows);
+    tiles += end > begin ? (end - begin + kRows - 1) / kRows : 0;
+  }
+  for (int o = 32; o >= 1; o >>= 1) tiles += __shfl_xor(tiles, o, kWave);
+  if (item >= tiles) return false;
+  item = tiles - 1 - item;
+  int before = 0;
+  for (int base = 0; base < a.sequences; base += 64) {
+    const int s = base + lane;
+    if (a.sequences > 64) {
+      begin = s < a.sequences ? clamped(a.starts[s], a.num_rows) : 0;
+      end = s < a.sequences ? clamped(a.starts[s + 1], a.num_rows) : 0;
+    } else if (s >= a.sequences) {
+      begin = end = 0;
+    }
+    const int mine = end > begin ? (end - begin + kRows - 1) / kRows : 0;
+    int upto = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int other = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += other;
+    }
+    const unsigned long long behind = __ballot(before + upto > item);
+    if (behind) {
+      const int at = __builtin_ctzll(behind);
+      const int index = item - (before + __shfl(upto, at, kWave) - __shfl(mine, at, kWave));
+      const int first = __shfl(begin, at, kWave), last = __shfl(end, at, kWave);
+      t->sequence = base + at;
+      t->start = first + index * kRows;
+      t->rows = last - t->start < kRows ? last - t->start : kRows;
+      t->total = keys_of(a, t->sequence, &t->key_start);
+      t->position = t->total - (last - t->start);
+      return true;
+    }
+    before += __shfl(upto, 63, kWave);
+  }
+  return false;
+}
+
+// Where keys lie: packed, in pages that hold whole tiles, in any pages.
+constexpr int kPacked = 0, kWholePages = 1, kAnyPages = 2;
+
+template <typename T, int D, int kWhere>
+__global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionArgs a) {
+  using S = Shape<T, D>;
+  constexpr int kSteps = S::kChunks / 2, kBlocks = D / 32;
+  // fp16: weights are held 2^7 times as large, so that those of 2^-21 are still normal numbers and the largest (2^15) finite
+  constexpr float kShift = __is_same(T, _Float16) ? 7.0f : 0.0f;
+  extern __shared__ __align__(16) char lds[];
+  const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = a.heads / a.kv_heads;
+  // (workgroups of one key-value head go to the same XCDs: workgroup i runs on XCD i % 8)
+  const int item = blockIdx.x / a.heads, rank = blockIdx.x - item * a.heads;
+  const int kv_head = rank % a.kv_heads, head = kv_head * group + rank / a.kv_heads;
+  RowTile tile;
+  if (!find_tile(a, item, lane, &tile)) return;
+  const int sequence = __builtin_amdgcn_readfirstlane(tile.sequence), start = __builtin_amdgcn_readfirstlane(tile.start);
+  const int rows = __builtin_amdgcn_readfirstlane(tile.rows), position = __builtin_amdgcn_readfirstlane(tile.position);
+  const int total = __builtin_amdgcn_readfirstlane(tile.total), key_begin = __builtin_amdgcn_readfirstlane(tile.key_start);
+
+  // The keys that some row of the tile sees: [0, first) and [low, high), both from whole tiles of keys on.
+  const Visible of_first = visible_keys(a, position, total), of_last = visible_keys(a, position + rows - 1, total);
+  const int high = of_last.high, low = of_first.low / kKeys * kKeys;
+  const int first_tiles = ((a.sinks < low ? a.sinks : low) + kKeys - 1) / kKeys;
+  const int tiles = first_tiles + (high > low ? (high - low + kKeys - 1) / kKeys : 0);
+
+  // This lane's query row; rows behind the last repeat it and are not written.
+  const int mine = 32 * wave + column;
+  const int row = start + (mine < rows ? mine : rows - 1);
+  const int place = position + (mine < rows ? mine : rows - 1);
+  const int wave_rows = rows - 32 * wave < 32 ? rows - 32 * wave : 32;  // (may be negative)
+  const int wave_first = position + 32 * wave, wave_last = wave_first + wave_rows - 1;
+  const float scale = __builtin_fabsf(a.scale) * kLog2e;
+
+  Pack8 query[kSteps];
+  {
+    const char* q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head);
+    const uint32_t turn = a.scale < 0 ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) {
+      query[s].raw = load128(q + 16 * (half + 2 * s));
+#pragma unroll
+      for (int d = 0; d < 4; ++d) query[s].u[d] ^= turn;
+    }
+  }
+
+  f32x16 o[kBlocks];
+#pragma unroll
+  for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[d][j] = 0.0f;
+  float m = -__builtin_inff(), l = 0.0f;
+
+  const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(lds));
+  const int32_t* table = a.block_tables + (kWhere == kPacked ? 0 : sequence * a.table_row);
+  int batch = -64, ids = 0;  // page ids batch .. batch + 63, one a lane
+  auto key_of = [&](int t) { return t < first_tiles ? t * kKeys : low + (t - first_tiles) * kKeys; };
+
+  // Asks for this wavefront's quarter of tile t; returns which of the tile's keys there are.
+  auto request = [&](int t, int stage) -> unsigned long long {
+    const int key0 = key_of(t), there = high - key0 < kKeys ? high - key0 : kKeys;
+    unsigned long long valid = there == kKeys ? ~0ull : (1ull << there) - 1;
+    const uint32_t to = ring_at + stage * 2 * S::kBytes + wave * S::kLoads * 1024;
+    if constexpr (kWhere != kAnyPages) {
+      const char *k, *v;
+      if constexpr (kWhere == kPacked) {
+        k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (static_cast<int64_t>(key_begin) + key0) * a.k_row + kv_head * a.k_head);
+        v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + (static_cast<int64_t>(key_begin) + key0) * a.v_row + kv_head * a.v_head);
+      } else {
+        const int page = key0 / a.page, in_page = key0 - page * a.page;
+        if (page < batch || page >= batch + 64) {
+          batch = page;
+          const int p = batch + lane;
+          ids = table[p < a.table_width ? p : a.table_width - 1];
+        }
+        const int id = __builtin_amdgcn_readlane(ids, page - batch);
+        if (id < 0 || id >= a.num_blocks) return 0;  // (the stage keeps what it held; nobody sees it)
+        k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + id * a.k_block + in_page * a.k_row + kv_head * a.k_head);
+        v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + id * a.v_block + in_page * a.v_row + kv_head * a.v_head);
+      }
+      k = uniform(k);
+      v = uniform(v);
+      const uint32_t k_row = static_cast<uint32_t>(a.k_row * sizeof(T)), v_row = static_cast<uint32_t>(a.v_row * sizeof(T));
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks, piece = lane % S::kChunks;
+        const uint32_t from = r < there ? r : there - 1;  // (a place behind the last key repeats it)
+        dma16(k, from * k_row + 16 * S::k_place(r, piece), to + i * 1024);
+        dma16(v, from * v_row + 16 * S::v_place(r, piece), to + S::kBytes + i * 1024);
+      }
+    } else {
+      const int key = key0 + (lane < there ? lane : there - 1), page0 = key0 / a.page, page = key / a.page;
+      if (page0 < batch || (key0 + there - 1) / a.page >= batch + 64) {
+        batch = page0;
+        const int p = batch + lane;
+        ids = table[p < a.table_width ? p : a.table_width - 1];
+      }
+      const int id = __shfl(ids, page - batch, kWave), in_page = key - page * a.page;
+      const bool known = id >= 0 && id < a.num_blocks;
+      valid &= __ballot(known);
+      const T *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
+      if (known) {  // (else the first row of the cache)
+        k += id * a.k_block + in_page * a.k_row;
+        v += id * a.v_block + in_page * a.v_row;
+      }
+      const uint64_t ka = reinterpret_cast<uintptr_t>(k + kv_head * a.k_head), va = reinterpret_cast<uintptr_t>(v + kv_head * a.v_head);
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks, piece = lane % S::kChunks;
+        const uint64_t kr = __shfl(static_cast<unsigned long long>(ka), r, kWave), vr = __shfl(static_cast<unsigned long long>(va), r, kWave);
+        dma16v(reinterpret_cast<const char*>(kr) + 16 * S::k_place(r, piece), to + i * 1024);
+        dma16v(reinterpret_cast<const char*>(vr) + 16 * S::v_place(r, piece), to + S::kBytes + i * 1024);
+      }
+    }
+    return valid;
+  };
+
+  unsigned long long next_valid = tiles > 0 ? request(0, 0) : 0;
+  for (int t = 0; t < tiles; ++t) {
+    const int stage = t & 1, key0 = key_of(t);
+    const unsigned long long valid = next_valid;
+    wait_loads<0>();
+    stage_barrier();  // this tile is there, and the one before it has been read
+    if (t + 1 < tiles) next_valid = request(t + 1, stage ^ 1);
+    // (nothing of the tile is visible to this wavefront's rows)
+    const bool near = !a.window || key0 + kKeys - 1 > wave_first - a.window || key0 < a.sinks;
+    if (wave_rows <= 0 || valid == 0 || (a.causal && key0 > wave_last) || !near) continue;
+
+    const char* const k_tile = lds + stage * 2 * S::kBytes;
+    const char* const v_tile = k_tile + S::kBytes;
+    f32x16 s[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[b][j] = 0.0f;
+#pragma unroll
+      for (int st = 0; st < kSteps; ++st) {
+        Pack8 key;
+        key.raw = load128(k_tile + (32 * b + column) * S::kRow + 16 * S::k_place(32 * b + column, half + 2 * st));
+        s[b] = Mma32<T>::run(key, query[st], s[b]);
+      }
+    }
+    const bool all_behind = !a.causal || key0 + kKeys - 1 <= wave_first;
+    const bool all_near = !a.window || key0 > wave_last - a.window || key0 + kKeys <= a.sinks;
+    if (!(all_behind && all_near && valid == ~0ull)) {
+      // key 32 b + 8 (j / 4) + 4 half + j % 4 of the tile
+      const int behind = (a.causal ? place : INT32_MAX / 2) - key0 - 4 * half;
+      const int far = a.window ? place - a.window - key0 - 4 * half : INT32_MIN / 2;
+      const int sinks = a.window ? a.sinks - key0 - 4 * half : 0;
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint32_t known = static_cast<uint32_t>(valid >> (32 * b)) >> (4 * half);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int of_block = 8 * (j >> 2) + (j & 3), e = 32 * b + of_block;
+          if (!(e <= behind && (e > far || e < sinks) && (known >> of_block & 1))) s[b][j] = -__builtin_inff();
+        }
+      }
+    }
+    float top = fmaxf(s[0][0], s[1][0]);
+#pragma unroll
+    for (int j = 1; j < 16; ++j) top = fmaxf(fmaxf(top, s[0][j]), s[1][j]);
+    float upper;
+    const float lower = other_half(top, &upper);
+    top = fmaxf(lower, upper) * scale;
+    if (__any(top > m + kMoves)) {
+      const float moved = fmaxf(m, top);
+      const float alpha = moved == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m - moved);
+      m = moved;
+      l *= alpha;
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[d][j] *= alpha;
+    }
+    const float base = (m == -__builtin_inff() ? 0.0f : m) - kShift;
+    float sum = 0.0f;
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        s[b][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j], scale, -base));
+        sum += s[b][j];
+      }
+    l += sum;
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      if constexpr (sizeof(T) == 2) {
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float w8[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w8[j] = s[b][8 * c + j];
+          Pack8 weights;
+          pack8<T>(w8, weights);
+          const int i = lane & 15;
+#pragma unroll
+          for (int d = 0; d < kBlocks; ++d) {
+            union { s16x4 part[2]; Pack8 all; } v;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int r = 32 * b + 16 * c + 8 * e + 4 * half + (i >> 2);
+              const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+              v.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(v_tile + r * S::kRow + 16 * S::v_place(r, chunk) + 8 * (i & 1)));
+            }
+            o[d] = Mma32<T>::run(v.all, weights, o[d]);
+          }
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int r = 32 * b + 8 * (j >> 2) + 4 * half + (j & 3);
+#pragma unroll
+          for (int d = 0; d < kBlocks; ++d) {
+            const float v = *reinterpret_cast<const float*>(v_tile + r * S::kRow + 16 * S::v_place(r, 8 * d + (column >> 2)) + 4 * (column & 3));
+            o[d] = __builtin_amdgcn_mfma_f32_32x32x2f32(v, s[b][j], o[d], 0, 0, 0);
+          }
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int d = 0; d < kBlocks; ++d) asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(o[d]));  // (the loop may end right behind a product)
+  {
+    float upper;
+    const float lower = other_half(l, &upper);
+    l = lower + upper;
+  }
+  // (also a row without a visible key, 0 / 0)
+  const float inverse = 1.0f / l;
+  bool finite = true;
+#pragma unroll
+  for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      o[d][j] *= inverse;
+      finite &= __builtin_fabsf(o[d][j]) < __builtin_inff();
+    }
+  unsigned long long again = __ballot(!finite && mine < rows);
+  again = (again | again >> 32) & 0xffffffffull;
+  if (mine < rows && !(again >> column & 1)) {
+    T* out = static_cast<T*>(a.out) + row * a.out_row + head * a.out_head;
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d) {
+      if constexpr (sizeof(T) == 2) {
+        // halves exchange so that a lane has eight elements side by side: of group 2 p the lower, of 2 p + 1 the upper
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          float w8[8];
+#pragma unroll
+          for (int j = 0; j < 8; ++j) w8[j] = o[d][8 * p + j];
+          Pack8 w, x;
+          pack8<T>(w8, w);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const auto r = __builtin_amdgcn_permlane32_swap(w.u[j], w.u[2 + j], false, false);
+            x.u[j] = r[0];
+            x.u[2 + j] = r[1];
+          }
+          store128(out + 32 * d + 16 * p + 8 * half, x.raw);
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) *reinterpret_cast<f32x4*>(out + 32 * d + 8 * p + 4 * half) = f32x4{o[d][4 * p], o[d][4 * p + 1], o[d][4 * p + 2], o[d][4 * p + 3]};
+      }
+    }
+  }
+  __syncthreads();  // (the stages have been read)
+  while (again) {
+    const int c = __builtin_ctzll(again);
+    again &= again - 1;
+    const Place at{sequence, total, key_begin, wave_first + c};
+    attend_row<T>(a, at, start + 32 * wave + c, head, lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
+  }
+}
+
+template <typename T, int D> int launch(const MloraAttentionArgs& a) {
+  const int where = !a.block_tables ? kPacked : a.page % kKeys == 0 ? kWholePages : kAnyPages;
+  const long long items = a.num_rows / kRows + a.sequences;  // at most that many tiles of rows
+  const unsigned grid = static_cast<unsigned>(items * a.heads);
+  constexpr int kLds = Shape<T, D>::kLds;
+  const hipStream_t stream = static_cast<hipStream_t>(a.stream);
+  if (where == kPacked) {
+    allow_lds<prompt_kernel<T, D, kPacked>>(kLds);
+    prompt_kernel<T, D, kPacked><<<grid, kWaves * 64, kLds, stream>>>(a);
+  } else if (where == kWholePages) {
+    allow_lds<prompt_kernel<T, D, kWholePages>>(kLds);
+    prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a);
+  } else {
+    allow_lds<prompt_kernel<T, D, kAnyPages>>(kLds);
+    prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a);
+  }
+  return check_launch("mlora_prompt_attention");
+}
+
+}  // namespace
+
+bool prompt_supported(const MloraAttentionArgs* a) {
+  if ((a->dim != 64 && a->dim != 128) || !attention_vectors_ok(a)) return false;
+  if (a->block_tables ? a->table_width < 1 || a->num_blocks < 1 : a->num_keys < 1) return false;
+  // a tile's rows are reached by 32-bit offsets from its first
+  const int64_t most = INT32_MAX / (kKeys * 4);
+  if (a->k_row < 0 || a->v_row < 0 || a->k_row > most || a->v_row > most) return false;
+  return (static_cast<int64_t>(a->num_rows / kRows) + a->sequences) * a->heads <= INT32_MAX;
+}
+
+int launch_prompt(const MloraAttentionArgs* a) {
+  if (a->dim == 64) {
+    if (a->dtype == MLORA_DTYPE_BF16) return launch<__bf16, 64>(*a);
+    return a->dtype == MLORA_DTYPE_F16 ? launch<_Float16, 64>(*a) : launch<float, 64>(*a);
+  }
+  if (a->dtype == MLORA_DTYPE_BF16) return launch<__bf16, 128>(*a);
+  return a->dtype == MLORA_DTYPE_F16 ? launch<_Float16, 128>(*a) : launch<float, 128>(*a);
+}
+
+}  // namespace mlora
