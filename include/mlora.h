@@ -402,8 +402,8 @@ typedef struct MloraAttentionArgs {
   int32_t dtype;                /* of q, k, v and out */
   int32_t causal, window, sinks;
   float scale;
-  void* workspace;              /* decode only: 16-byte aligned scratch of mlora_decode_attention_workspace_bytes, needed only
-                                   while the call's work is under way; without it a sequence is not split */
+  void* workspace;              /* 16-byte aligned scratch of mlora_*_attention_workspace_bytes (0: none is used), needed only
+                                   while the call's work is under way; without it the length of a sequence is not split */
   int64_t workspace_bytes;
 } MloraAttentionArgs;
 
@@ -412,6 +412,7 @@ int mlora_decode_attention(const MloraAttentionArgs* args);
 size_t mlora_decode_attention_workspace_bytes(int32_t sequences, int32_t heads, int32_t kv_heads, int32_t dim);
 /* Any number of query rows per sequence, packed one sequence behind the other. */
 int mlora_prompt_attention(const MloraAttentionArgs* args);
+size_t mlora_prompt_attention_workspace_bytes(const MloraAttentionArgs* args); /* of a filled block; reads its sizes, strides and pointers' alignment */
 
 /* Identifier of the graph capture in progress on `stream`, 0 when the stream is not
  * capturing.  No counterpart in the reference: lets a host-side cache tell work recorded

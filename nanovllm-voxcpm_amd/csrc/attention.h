@@ -16,6 +16,7 @@ int launch_paged(const MloraAttentionArgs* a);
 
 // prompt.hip: packed rows, head sizes 64 and 128
 bool prompt_supported(const MloraAttentionArgs* a);
+size_t prompt_workspace_bytes(const MloraAttentionArgs* a);
 int launch_prompt(const MloraAttentionArgs* a);
 
 namespace {

@@ -114,3 +114,8 @@ extern "C" int mlora_prompt_attention(const MloraAttentionArgs* a) {
   if (prompt_supported(a)) return launch_prompt(a);
   return launch_attend_rows(a);
 }
+
+extern "C" size_t mlora_prompt_attention_workspace_bytes(const MloraAttentionArgs* a) {
+  if (!a || a->num_rows <= 0 || a->num_keys < 0 || a->sequences <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->table_width < 0) return 0;
+  return prompt_workspace_bytes(a);
+}

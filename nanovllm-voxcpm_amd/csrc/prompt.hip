@@ -50,6 +50,7 @@ template <typename T, int D> struct Shape {
   static constexpr int kLoads = kBytes / 1024 / kWaves;   // a wavefront's share of it
   static constexpr int kRowsPerLoad = 1024 / kRow;
   static constexpr int kLds = 2 * 2 * kBytes;
+
   // A read of K takes the same piece of 32 rows, one of V^T 64 bytes of four rows (in fp32 128 of rows four apart).
   static __device__ __forceinline__ int k_place(int row, int chunk) { return chunk ^ (kRow == 128 ? (row >> 1) & 7 : row & 15); }
   static __device__ __forceinline__ int v_place(int row, int chunk) {
@@ -58,7 +59,6 @@ template <typename T, int D> struct Shape {
 };
 
 typedef __attribute__((address_space(3))) s16x4 LdsS16x4;
-
 __device__ __forceinline__ float other_half(float v, float* both) {  // lanes l and l + 32
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   *both = __uint_as_float(r[1]);
@@ -114,11 +114,113 @@ __device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int item,
   return false;
 }
 
+// How many tiles of keys the rows of a tile see: [0, first) and [low, high), both from whole tiles of keys on.
+struct KeyTiles {
+  int high, low, first_tiles, count;
+  __device__ __forceinline__ KeyTiles(const MloraAttentionArgs& a, int position, int rows, int total) {
+    const Visible of_first = visible_keys(a, position, total), of_last = visible_keys(a, position + rows - 1, total);
+    high = of_last.high;
+    low = of_first.low / kKeys * kKeys;
+    first_tiles = ((a.sinks < low ? a.sinks : low) + kKeys - 1) / kKeys;
+    count = first_tiles + (high > low ? (high - low + kKeys - 1) / kKeys : 0);
+  }
+};
+
+// Few tiles of rows with many keys (a chunk of a prompt behind a long cache) leave compute units idle, or busy for a second round that few take part
+// in.  Their work is then one list: the tiles of keys of the first tile of rows, of the second and so on.  Every workgroup takes an equal share of the list, whatever rows it falls on.
+// A tile of rows that lies in several shares is joined by a second launch from what each of them left in the workspace.
+constexpr int kLeastShare = 32;  // tiles of keys: below it what is left and joined costs more than the balance gives
+
+// The tiles of rows of a batch of at most 64 sequences, one a lane.
+struct RowTiles {
+  int begin, end, total, key_start, upto;  // of this lane's sequence; upto: tiles of rows up to its end
+  int tiles;                               // of rows, all of them
+  __device__ __forceinline__ RowTile tile(int r) const {  // r may differ from lane to lane
+    int at = 0;  // the first sequence that ends behind r
+#pragma unroll
+    for (int step = 32; step >= 1; step >>= 1)
+      if (__shfl(upto, at + step - 1, kWave) <= r) at += step;
+    const int first = __shfl(begin, at, kWave), last = __shfl(end, at, kWave), seq_upto = __shfl(upto, at, kWave);
+    RowTile t;
+    t.sequence = at;
+    t.total = __shfl(total, at, kWave);
+    t.key_start = __shfl(key_start, at, kWave);
+    t.start = first + (r - seq_upto + (last - first + kRows - 1) / kRows) * kRows;
+    t.rows = last - t.start < kRows ? last - t.start : kRows;
+    t.position = t.total - (last - t.start);
+    return t;
+  }
+  __device__ __forceinline__ long long units_of(const MloraAttentionArgs& a, int r) const {
+    const RowTile t = tile(r < tiles ? r : tiles - 1);
+    return r < tiles ? KeyTiles(a, t.position, t.rows, t.total).count : 0;
+  }
+  __device__ __forceinline__ RowTiles(const MloraAttentionArgs& a, int lane) {
+    begin = end = total = key_start = 0;
+    if (lane < a.sequences) {
+      begin = clamped(a.starts[lane], a.num_rows);
+      end = clamped(a.starts[lane + 1], a.num_rows);
+      total = keys_of(a, lane, &key_start);
+    }
+    upto = end > begin ? (end - begin + kRows - 1) / kRows : 0;
+    for (int o = 1; o < 64; o <<= 1) {
+      const int other = __shfl_up(upto, o, kWave);
+      if (lane >= o) upto += other;
+    }
+    tiles = __shfl(upto, 63, kWave);
+  }
+};
+
+struct Shares : RowTiles {
+  long long units, per;  // tiles of keys, all of them and a share's; per = 0: not shared out
+  __device__ __forceinline__ Shares(const MloraAttentionArgs& a, int shares, int lane) : RowTiles(a, lane) {
+    units = per = 0;
+    if (tiles == 0) return;
+    for (int base = 0; base < tiles; base += 64) units += units_of(a, base + lane);
+    for (int o = 32; o >= 1; o >>= 1) units += __shfl_xor(units, o, kWave);
+    per = tiles < 4 * shares && units >= static_cast<long long>(kLeastShare) * shares ? (units + shares - 1) / shares : 0;
+  }
+  // The tile of rows that holds `unit` and the unit that it starts with.
+  __device__ __forceinline__ int find(const MloraAttentionArgs& a, long long unit, int lane, long long* first) const {
+    long long before = 0;
+    for (int base = 0; base < tiles; base += 64) {
+      const long long mine = units_of(a, base + lane);
+      long long last = mine;
+      for (int o = 1; o < 64; o <<= 1) {
+        const long long other = __shfl_up(last, o, kWave);
+        if (lane >= o) last += other;
+      }
+      const unsigned long long behind = __ballot(before + last > unit);
+      if (behind) {
+        const int at = __builtin_ctzll(behind);
+        *first = before + __shfl(last - mine, at, kWave);
+        return base + at;
+      }
+      before += __shfl(last, 63, kWave);
+    }
+    return -1;
+  }
+};
+
+// Workspace: of every (share, which end of it, head) its rows' (m, l), then their o.  A share has two unfinished tiles of rows at most: place 0 for
+// one that began in front of it, place 1 for one that begins in it.
+struct Unfinished {
+  float2* sums;
+  float* outputs;
+};
+__device__ __forceinline__ Unfinished unfinished(const MloraAttentionArgs& a, int shares, int share, int place, int head, int dim) {
+  const int64_t at = (static_cast<int64_t>(share) * 2 + place) * a.heads + head, all = static_cast<int64_t>(shares) * 2 * a.heads;
+  float2* const sums = static_cast<float2*>(a.workspace);
+  return {sums + at * kRows, reinterpret_cast<float*>(sums + all * kRows) + at * kRows * dim};
+}
+
+// Workgroups that a compute unit holds at once, by the bytes of a head.
+constexpr int per_unit(int row) { return row == 128 ? 3 : row == 256 ? 2 : 1; }
+
 // Where keys lie: packed, in pages that hold whole tiles, in any pages.
 constexpr int kPacked = 0, kWholePages = 1, kAnyPages = 2;
 
 template <typename T, int D, int kWhere>
-__global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionArgs a) {
+__global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_kernel(MloraAttentionArgs a, int shares) {
   using S = Shape<T, D>;
   constexpr int kSteps = S::kChunks / 2, kBlocks = D / 32;
   // fp16: weights are held 2^7 times as large, so that those of 2^-21 are still normal numbers and the largest (2^15) finite
@@ -130,17 +232,33 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
   // (workgroups of one key-value head go to the same XCDs: workgroup i runs on XCD i % 8)
   const int item = blockIdx.x / a.heads, rank = blockIdx.x - item * a.heads;
   const int kv_head = rank % a.kv_heads, head = kv_head * group + rank / a.kv_heads;
+  bool shared = false;
+  // Of a share: tiles of keys that are left of it, and the first of them in its tile of rows.
+  int left = 0, from = 0, tile_number = 0;
+  if (shares) {
+    const Shares s(a, shares, lane);
+    if (s.per) {
+      shared = true;
+      const long long unit = item * s.per;
+      if (item >= shares || unit >= s.units) return;
+      long long first;
+      tile_number = __builtin_amdgcn_readfirstlane(s.find(a, unit, lane, &first));
+      from = __builtin_amdgcn_readfirstlane(static_cast<int>(unit - first));
+      left = __builtin_amdgcn_readfirstlane(static_cast<int>(unit + s.per < s.units ? s.per : s.units - unit));
+    }
+  }
+  shared = __builtin_amdgcn_readfirstlane(shared);
+  for (;;) {
   RowTile tile;
-  if (!find_tile(a, item, lane, &tile)) return;
+  if (shared) tile = RowTiles(a, lane).tile(tile_number);
+  else if (!find_tile(a, item, lane, &tile)) return;
   const int sequence = __builtin_amdgcn_readfirstlane(tile.sequence), start = __builtin_amdgcn_readfirstlane(tile.start);
   const int rows = __builtin_amdgcn_readfirstlane(tile.rows), position = __builtin_amdgcn_readfirstlane(tile.position);
   const int total = __builtin_amdgcn_readfirstlane(tile.total), key_begin = __builtin_amdgcn_readfirstlane(tile.key_start);
-
-  // The keys that some row of the tile sees: [0, first) and [low, high), both from whole tiles of keys on.
-  const Visible of_first = visible_keys(a, position, total), of_last = visible_keys(a, position + rows - 1, total);
-  const int high = of_last.high, low = of_first.low / kKeys * kKeys;
-  const int first_tiles = ((a.sinks < low ? a.sinks : low) + kKeys - 1) / kKeys;
-  const int tiles = first_tiles + (high > low ? (high - low + kKeys - 1) / kKeys : 0);
+  const KeyTiles of_rows(a, position, rows, total);
+  const int high = of_rows.high, low = of_rows.low, first_tiles = of_rows.first_tiles;
+  // the tiles of keys from .. to of them are this workgroup's
+  const int to = shared && left < of_rows.count - from ? from + left : of_rows.count;
 
   // This lane's query row; rows behind the last repeat it and are not written.
   const int mine = 32 * wave + column;
@@ -173,12 +291,23 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
   const int32_t* table = a.block_tables + (kWhere == kPacked ? 0 : sequence * a.table_row);
   int batch = -64, ids = 0;  // page ids batch .. batch + 63, one a lane
   auto key_of = [&](int t) { return t < first_tiles ? t * kKeys : low + (t - first_tiles) * kKeys; };
+  auto stage_of = [&](int t) { return (t & 1) * 2 * S::kBytes; };
+
+  // Byte offsets of what a lane asks for in a whole tile.
+  uint32_t k_offset[S::kLoads], v_offset[S::kLoads];
+  const uint32_t k_row = static_cast<uint32_t>(a.k_row * sizeof(T)), v_row = static_cast<uint32_t>(a.v_row * sizeof(T));
+#pragma unroll
+  for (int i = 0; i < S::kLoads; ++i) {
+    const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks, piece = lane % S::kChunks;
+    k_offset[i] = r * k_row + 16 * S::k_place(r, piece);
+    v_offset[i] = r * v_row + 16 * S::v_place(r, piece);
+  }
 
   // Asks for this wavefront's quarter of tile t; returns which of the tile's keys there are.
-  auto request = [&](int t, int stage) -> unsigned long long {
+  auto request = [&](int t) -> unsigned long long {
     const int key0 = key_of(t), there = high - key0 < kKeys ? high - key0 : kKeys;
     unsigned long long valid = there == kKeys ? ~0ull : (1ull << there) - 1;
-    const uint32_t to = ring_at + stage * 2 * S::kBytes + wave * S::kLoads * 1024;
+    const uint32_t k_to = ring_at + stage_of(t) + wave * S::kLoads * 1024, v_to = k_to + S::kBytes;
     if constexpr (kWhere != kAnyPages) {
       const char *k, *v;
       if constexpr (kWhere == kPacked) {
@@ -192,19 +321,26 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
           ids = table[p < a.table_width ? p : a.table_width - 1];
         }
         const int id = __builtin_amdgcn_readlane(ids, page - batch);
-        if (id < 0 || id >= a.num_blocks) return 0;  // (the stage keeps what it held; nobody sees it)
+        if (id < 0 || id >= a.num_blocks) return 0;  // (the stage keeps what it held: every key of it is masked)
         k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + id * a.k_block + in_page * a.k_row + kv_head * a.k_head);
         v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + id * a.v_block + in_page * a.v_row + kv_head * a.v_head);
       }
       k = uniform(k);
       v = uniform(v);
-      const uint32_t k_row = static_cast<uint32_t>(a.k_row * sizeof(T)), v_row = static_cast<uint32_t>(a.v_row * sizeof(T));
+      if (there == kKeys) {
 #pragma unroll
-      for (int i = 0; i < S::kLoads; ++i) {
-        const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks, piece = lane % S::kChunks;
-        const uint32_t from = r < there ? r : there - 1;  // (a place behind the last key repeats it)
-        dma16(k, from * k_row + 16 * S::k_place(r, piece), to + i * 1024);
-        dma16(v, from * v_row + 16 * S::v_place(r, piece), to + S::kBytes + i * 1024);
+        for (int i = 0; i < S::kLoads; ++i) {
+          dma16(k, k_offset[i], k_to + i * 1024);
+          dma16(v, v_offset[i], v_to + i * 1024);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i) {
+          const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks;
+          const uint32_t back = r < there ? 0 : r - there + 1;  // (a place behind the last key repeats it)
+          dma16(k, k_offset[i] - back * k_row, k_to + i * 1024);
+          dma16(v, v_offset[i] - back * v_row, v_to + i * 1024);
+        }
       }
     } else {
       const int key = key0 + (lane < there ? lane : there - 1), page0 = key0 / a.page, page = key / a.page;
@@ -226,25 +362,29 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
       for (int i = 0; i < S::kLoads; ++i) {
         const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks, piece = lane % S::kChunks;
         const uint64_t kr = __shfl(static_cast<unsigned long long>(ka), r, kWave), vr = __shfl(static_cast<unsigned long long>(va), r, kWave);
-        dma16v(reinterpret_cast<const char*>(kr) + 16 * S::k_place(r, piece), to + i * 1024);
-        dma16v(reinterpret_cast<const char*>(vr) + 16 * S::v_place(r, piece), to + S::kBytes + i * 1024);
+        dma16v(reinterpret_cast<const char*>(kr) + 16 * S::k_place(r, piece), k_to + i * 1024);
+        dma16v(reinterpret_cast<const char*>(vr) + 16 * S::v_place(r, piece), v_to + i * 1024);
       }
     }
     return valid;
   };
 
-  unsigned long long next_valid = tiles > 0 ? request(0, 0) : 0;
-  for (int t = 0; t < tiles; ++t) {
-    const int stage = t & 1, key0 = key_of(t);
+  // The tiles that this wavefront's rows see end here; the others are only asked for.
+  const int seen_end = a.causal ? (wave_last < high - 1 ? wave_last : high - 1) : high - 1;  // their last key
+  int own = wave_rows <= 0 || seen_end < 0 ? 0 : seen_end < low ? first_tiles : first_tiles + (seen_end - low) / kKeys + 1;
+  own = own < to ? own : to;
+
+  const int i16 = lane & 15;
+  unsigned long long next_valid = from < to ? request(from) : 0;
+  for (int t = from; t < to; ++t) {
+    const int key0 = key_of(t);
     const unsigned long long valid = next_valid;
     wait_loads<0>();
     stage_barrier();  // this tile is there, and the one before it has been read
-    if (t + 1 < tiles) next_valid = request(t + 1, stage ^ 1);
-    // (nothing of the tile is visible to this wavefront's rows)
-    const bool near = !a.window || key0 + kKeys - 1 > wave_first - a.window || key0 < a.sinks;
-    if (wave_rows <= 0 || valid == 0 || (a.causal && key0 > wave_last) || !near) continue;
+    if (t + 1 < to) next_valid = request(t + 1);
+    if (t >= own) continue;
 
-    const char* const k_tile = lds + stage * 2 * S::kBytes;
+    const char* const k_tile = lds + stage_of(t);
     const char* const v_tile = k_tile + S::kBytes;
     f32x16 s[2];
 #pragma unroll
@@ -258,6 +398,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
         s[b] = Mma32<T>::run(key, query[st], s[b]);
       }
     }
+    if constexpr (sizeof(T) == 4) asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));  // (the branch over the masks below)
     const bool all_behind = !a.causal || key0 + kKeys - 1 <= wave_first;
     const bool all_near = !a.window || key0 > wave_last - a.window || key0 + kKeys <= a.sinks;
     if (!(all_behind && all_near && valid == ~0ull)) {
@@ -271,7 +412,8 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           const int of_block = 8 * (j >> 2) + (j & 3), e = 32 * b + of_block;
-          if (!(e <= behind && (e > far || e < sinks) && (known >> of_block & 1))) s[b][j] = -__builtin_inff();
+          const bool seen = (e <= behind) & ((e > far) | (e < sinks)) & ((known >> of_block & 1) != 0);
+          s[b][j] = seen ? s[b][j] : -__builtin_inff();
         }
       }
     }
@@ -292,18 +434,14 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
         for (int j = 0; j < 16; ++j) o[d][j] *= alpha;
     }
     const float base = (m == -__builtin_inff() ? 0.0f : m) - kShift;
-    float sum = 0.0f;
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        s[b][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j], scale, -base));
-        sum += s[b][j];
-      }
-    l += sum;
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[b][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j], scale, -base));
       if constexpr (sizeof(T) == 2) {
+        Pack8 ones;
+        const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
+        pack8<T>(one, ones);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
           float w8[8];
@@ -311,15 +449,15 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
           for (int j = 0; j < 8; ++j) w8[j] = s[b][8 * c + j];
           Pack8 weights;
           pack8<T>(w8, weights);
-          const int i = lane & 15;
+          l = dot8<T>(weights, ones, l);  // (the rounded weights' sum is what the outputs are divided by)
 #pragma unroll
           for (int d = 0; d < kBlocks; ++d) {
             union { s16x4 part[2]; Pack8 all; } v;
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-              const int r = 32 * b + 16 * c + 8 * e + 4 * half + (i >> 2);
-              const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-              v.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(v_tile + r * S::kRow + 16 * S::v_place(r, chunk) + 8 * (i & 1)));
+              const int r = 32 * b + 16 * c + 8 * e + 4 * half + (i16 >> 2);
+              const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+              v.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(v_tile + r * S::kRow + 16 * S::v_place(r, chunk) + 8 * (i16 & 1)));
             }
             o[d] = Mma32<T>::run(v.all, weights, o[d]);
           }
@@ -327,6 +465,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
       } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
+          l += s[b][j];
           const int r = 32 * b + 8 * (j >> 2) + 4 * half + (j & 3);
 #pragma unroll
           for (int d = 0; d < kBlocks; ++d) {
@@ -344,6 +483,16 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
     const float lower = other_half(l, &upper);
     l = lower + upper;
   }
+  if (shared && to - from < of_rows.count) {  // for the join
+    const Unfinished u = unfinished(a, shares, item, from ? 0 : 1, head, D);
+    if (half == 0) u.sums[mine] = make_float2(m, l);
+#pragma unroll
+    for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        *reinterpret_cast<f32x4*>(u.outputs + mine * D + 32 * d + 8 * p + 4 * half) = f32x4{o[d][4 * p], o[d][4 * p + 1], o[d][4 * p + 2], o[d][4 * p + 3]};
+    __syncthreads();  // (the stages have been read)
+  } else {
   // (also a row without a visible key, 0 / 0)
   const float inverse = 1.0f / l;
   bool finite = true;
@@ -390,25 +539,90 @@ __global__ __launch_bounds__(kWaves * 64, 2) void prompt_kernel(MloraAttentionAr
     const Place at{sequence, total, key_begin, wave_first + c};
     attend_row<T>(a, at, start + 32 * wave + c, head, lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
   }
+  if (shared) __syncthreads();
+  }
+  left -= to - from;
+  if (!shared || left <= 0) return;
+  from = 0;
+  ++tile_number;
+  }
+}
+
+// Joins the parts of 32 rows of a tile that lies in several shares.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, int shares) {
+  constexpr int kPer = D / 64;
+  __shared__ float scratch[kWaves][MLORA_MAX_HEAD_DIM];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.y, number = blockIdx.x >> 2;
+  const Shares batch(a, shares, lane);
+  if (number >= batch.tiles || !batch.per) return;
+  long long first = 0;
+  for (int base = 0; base < number; base += 64) {
+    const long long units = batch.units_of(a, base + lane);
+    first += base + lane < number ? units : 0;
+  }
+  for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, kWave);
+  const RowTile t = batch.tile(number);
+  const int count = KeyTiles(a, t.position, t.rows, t.total).count;
+  if (!count) return;  // (written: it is whole)
+  const int share = static_cast<int>(first / batch.per), parts = static_cast<int>((first + count - 1) / batch.per) - share + 1;
+  if (parts < 2) return;
+  for (int i = 0; i < 8; ++i) {
+    const int r = 32 * (blockIdx.x & 3) + 8 * wave + i;
+    if (r >= t.rows) break;
+    float most = -__builtin_inff(), sum = 0.0f, x[kPer] = {};
+    for (int p = 0; p < parts; ++p) most = fmaxf(most, unfinished(a, shares, share + p, p ? 0 : 1, head, D).sums[r].x);
+    for (int p = 0; p < parts; ++p) {
+      const Unfinished u = unfinished(a, shares, share + p, p ? 0 : 1, head, D);
+      const float2 ml = u.sums[r];
+      const float factor = ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
+      sum += factor * ml.y;
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[e] += factor * u.outputs[r * D + 64 * e + lane];
+    }
+    const int row = t.start + r;
+    bool finite = true;
+#pragma unroll
+    for (int e = 0; e < kPer; ++e) {
+      x[e] /= sum;
+      finite &= __builtin_fabsf(x[e]) < __builtin_inff();
+    }
+    if (__all(finite)) {
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) static_cast<T*>(a.out)[row * a.out_row + head * a.out_head + 64 * e + lane] = from_f32<T>(x[e]);
+    } else {
+      attend_row<T>(a, Place{t.sequence, t.total, t.key_start, t.position + r}, row, head, lane, scratch[wave]);
+    }
+  }
+}
+
+// Shares of a head: as many workgroups as the chip holds at once.
+int shares_of(const MloraAttentionArgs& a) {
+  const int resident = 256 * per_unit(a.dim * (a.dtype == MLORA_DTYPE_F32 ? 4 : 2)) / a.heads;
+  return resident > 1 ? resident : 1;
 }
 
 template <typename T, int D> int launch(const MloraAttentionArgs& a) {
   const int where = !a.block_tables ? kPacked : a.page % kKeys == 0 ? kWholePages : kAnyPages;
   const long long items = a.num_rows / kRows + a.sequences;  // at most that many tiles of rows
-  const unsigned grid = static_cast<unsigned>(items * a.heads);
+  const int shares = prompt_workspace_bytes(&a) && a.workspace && a.workspace_bytes >= static_cast<int64_t>(prompt_workspace_bytes(&a)) ? shares_of(a) : 0;
+  const unsigned grid = static_cast<unsigned>((items > shares ? items : shares) * a.heads);
   constexpr int kLds = Shape<T, D>::kLds;
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
   if (where == kPacked) {
     allow_lds<prompt_kernel<T, D, kPacked>>(kLds);
-    prompt_kernel<T, D, kPacked><<<grid, kWaves * 64, kLds, stream>>>(a);
+    prompt_kernel<T, D, kPacked><<<grid, kWaves * 64, kLds, stream>>>(a, shares);
   } else if (where == kWholePages) {
     allow_lds<prompt_kernel<T, D, kWholePages>>(kLds);
-    prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a);
+    prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a, shares);
   } else {
     allow_lds<prompt_kernel<T, D, kAnyPages>>(kLds);
-    prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a);
+    prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a, shares);
   }
-  return check_launch("mlora_prompt_attention");
+  const int rc = check_launch("mlora_prompt_attention");
+  if (rc || !shares) return rc;
+  prompt_join_kernel<T, D><<<dim3(static_cast<unsigned>(4 * items), a.heads), 256, 0, stream>>>(a, shares);
+  return check_launch("mlora_prompt_attention (join)");
 }
 
 }  // namespace
@@ -420,6 +634,15 @@ bool prompt_supported(const MloraAttentionArgs* a) {
   const int64_t most = INT32_MAX / (kKeys * 4);
   if (a->k_row < 0 || a->v_row < 0 || a->k_row > most || a->v_row > most) return false;
   return (static_cast<int64_t>(a->num_rows / kRows) + a->sequences) * a->heads <= INT32_MAX;
+}
+
+// Scratch of the shares where the work may be shared out: few tiles of rows for the chip, and enough keys to share.
+size_t prompt_workspace_bytes(const MloraAttentionArgs* a) {
+  if (!prompt_supported(a) || a->sequences > 64 || a->heads > 512) return 0;
+  const int64_t shares = shares_of(*a), tiles = a->num_rows / kRows + a->sequences;
+  const int64_t keys = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys;
+  if (tiles >= 2 * shares || tiles * ((keys + kKeys - 1) / kKeys) < kLeastShare * shares) return 0;
+  return static_cast<size_t>(shares * 2 * a->heads * kRows * (8 + 4 * a->dim));
 }
 
 int launch_prompt(const MloraAttentionArgs* a) {

@@ -72,6 +72,7 @@ EXPORTS = (
     "mlora_decode_attention",
     "mlora_decode_attention_workspace_bytes",
     "mlora_prompt_attention",
+    "mlora_prompt_attention_workspace_bytes",
     "mlora_stream_capture_id",
     "mlora_abi_version",
     "mlora_last_error",
@@ -285,6 +286,8 @@ def load() -> C.CDLL:
     lib.mlora_workspace_init.restype = C.c_int
     lib.mlora_decode_attention_workspace_bytes.argtypes = [C.c_int32] * 4
     lib.mlora_decode_attention_workspace_bytes.restype = C.c_size_t
+    lib.mlora_prompt_attention_workspace_bytes.argtypes = [C.POINTER(MloraAttentionArgs)]
+    lib.mlora_prompt_attention_workspace_bytes.restype = C.c_size_t
     lib.mlora_stream_capture_id.argtypes = [C.c_void_p]
     lib.mlora_stream_capture_id.restype = C.c_uint64
     _declare_diag(lib)
@@ -816,15 +819,22 @@ def _attention_args(q, out, k, v, block_tables, context_lens, causal: bool, scal
     return args
 
 
+def _scratch(args: MloraAttentionArgs, nbytes: int, device: torch.device) -> torch.Tensor | None:
+    """Scratch of one call, held by the caller until the work is enqueued: the allocator hands it to nobody before the stream
+    (or the graph) is past the call."""
+    if not nbytes:
+        return None
+    workspace = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
+    return workspace
+
+
 def decode_attention(q, out, k_cache, v_cache, block_tables, context_lens, scale: float, window: int, sinks: int) -> None:
     """One query row per sequence over a paged cache; tensors checked by ``attention_ops.decode_attention``."""
     lib = load()
     args = _attention_args(q, out, k_cache, v_cache, block_tables, context_lens, True, scale, window, sinks)
     args.sequences = q.size(0)
-    nbytes = lib.mlora_decode_attention_workspace_bytes(args.sequences, args.heads, args.kv_heads, args.dim)
-    if nbytes:  # scratch of this call alone: the allocator hands it to nobody before the stream (or the graph) is past the call
-        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-        args.workspace, args.workspace_bytes = workspace.data_ptr(), nbytes
+    workspace = _scratch(args, lib.mlora_decode_attention_workspace_bytes(args.sequences, args.heads, args.kv_heads, args.dim), q.device)  # noqa: F841
     with _on(q.device):
         _check(lib.mlora_decode_attention(C.byref(args)), "mlora_decode_attention")
 
@@ -837,6 +847,7 @@ def prompt_attention(q, out, k, v, starts, key_starts, block_tables, context_len
     if key_starts is not None:
         args.key_starts = key_starts.data_ptr()
     args.sequences = starts.numel() - 1
+    workspace = _scratch(args, lib.mlora_prompt_attention_workspace_bytes(C.byref(args)), q.device)  # noqa: F841
     with _on(q.device):
         _check(lib.mlora_prompt_attention(C.byref(args)), "mlora_prompt_attention")
 
