@@ -65,6 +65,12 @@ __device__ __forceinline__ float other_half(float v, float* both) {  // lanes l 
   return __uint_as_float(r[0]);
 }
 
+// What is the same in every lane, into scalar registers.
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ long long uniform(long long v) {
+  return (static_cast<long long>(uniform(static_cast<int>(v >> 32))) << 32) | static_cast<uint32_t>(uniform(static_cast<int>(v)));
+}
+
 struct RowTile {
   int sequence, start, rows;  // first query row (of q) and how many
   int position;               // of the first
@@ -201,16 +207,30 @@ struct Shares : RowTiles {
   }
 };
 
-// Workspace: of every (share, which end of it, head) its rows' (m, l), then their o.  A share has two unfinished tiles of rows at most: place 0 for
-// one that began in front of it, place 1 for one that begins in it.
+// Workspace: how many tiles of rows are shared out, what the join has to know of each, and of every (share, which end of it, head) the
+// rows' (m, l), then their o.  A share has two unfinished tiles of rows at most: place 0 for one that began in front of it, place 1 for one that
+// begins in it.
+struct Joint {
+  int share, parts, sequence, start, rows, position, total, key_start;
+};
 struct Unfinished {
   float2* sums;
   float* outputs;
 };
+__host__ __device__ inline int64_t joints_bytes(int64_t tiles) { return 16 + tiles * static_cast<int64_t>(sizeof(Joint)); }
+__device__ __forceinline__ int32_t* shared_tiles(const MloraAttentionArgs& a) { return static_cast<int32_t*>(a.workspace); }
+__device__ __forceinline__ Joint* joint(const MloraAttentionArgs& a, int tile) { return reinterpret_cast<Joint*>(static_cast<char*>(a.workspace) + 16) + tile; }
 __device__ __forceinline__ Unfinished unfinished(const MloraAttentionArgs& a, int shares, int share, int place, int head, int dim) {
   const int64_t at = (static_cast<int64_t>(share) * 2 + place) * a.heads + head, all = static_cast<int64_t>(shares) * 2 * a.heads;
-  float2* const sums = static_cast<float2*>(a.workspace);
+  float2* const sums = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + joints_bytes(a.num_rows / kRows + a.sequences));
   return {sums + at * kRows, reinterpret_cast<float*>(sums + all * kRows) + at * kRows * dim};
+}
+
+// The kernel's first argument where the launch left it.
+__device__ __forceinline__ const MloraAttentionArgs* arguments_again() {
+  uint64_t p = (uint64_t)(__builtin_amdgcn_kernarg_segment_ptr());
+  asm volatile("" : "+s"(p));
+  return reinterpret_cast<const MloraAttentionArgs*>(p);
 }
 
 // Workgroups that a compute unit holds at once, by the bytes of a head.
@@ -232,29 +252,30 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   // (workgroups of one key-value head go to the same XCDs: workgroup i runs on XCD i % 8)
   const int item = blockIdx.x / a.heads, rank = blockIdx.x - item * a.heads;
   const int kv_head = rank % a.kv_heads, head = kv_head * group + rank / a.kv_heads;
+  RowTile tile;
   bool shared = false;
   // Of a share: tiles of keys that are left of it, and the first of them in its tile of rows.
   int left = 0, from = 0, tile_number = 0;
+  long long a_share = 0;
   if (shares) {
     const Shares s(a, shares, lane);
-    if (s.per) {
+    const long long per = uniform(s.per), units = uniform(s.units), unit = item * per;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *shared_tiles(a) = per ? s.tiles : 0;
+    if (per) {
+      a_share = per;
+      if (item >= shares || unit >= units) return;
       shared = true;
-      const long long unit = item * s.per;
-      if (item >= shares || unit >= s.units) return;
       long long first;
-      tile_number = __builtin_amdgcn_readfirstlane(s.find(a, unit, lane, &first));
-      from = __builtin_amdgcn_readfirstlane(static_cast<int>(unit - first));
-      left = __builtin_amdgcn_readfirstlane(static_cast<int>(unit + s.per < s.units ? s.per : s.units - unit));
+      tile_number = uniform(s.find(a, unit, lane, &first));
+      from = static_cast<int>(unit - uniform(first));
+      left = static_cast<int>(unit + per < units ? per : units - unit);
     }
   }
-  shared = __builtin_amdgcn_readfirstlane(shared);
+  if (!shared && !uniform(find_tile(a, item, lane, &tile))) return;
   for (;;) {
-  RowTile tile;
   if (shared) tile = RowTiles(a, lane).tile(tile_number);
-  else if (!find_tile(a, item, lane, &tile)) return;
-  const int sequence = __builtin_amdgcn_readfirstlane(tile.sequence), start = __builtin_amdgcn_readfirstlane(tile.start);
-  const int rows = __builtin_amdgcn_readfirstlane(tile.rows), position = __builtin_amdgcn_readfirstlane(tile.position);
-  const int total = __builtin_amdgcn_readfirstlane(tile.total), key_begin = __builtin_amdgcn_readfirstlane(tile.key_start);
+  const int sequence = uniform(tile.sequence), start = uniform(tile.start), rows = uniform(tile.rows), position = uniform(tile.position);
+  const int total = uniform(tile.total), key_begin = uniform(tile.key_start);
   const KeyTiles of_rows(a, position, rows, total);
   const int high = of_rows.high, low = of_rows.low, first_tiles = of_rows.first_tiles;
   // the tiles of keys from .. to of them are this workgroup's
@@ -290,6 +311,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(lds));
   const int32_t* table = a.block_tables + (kWhere == kPacked ? 0 : sequence * a.table_row);
   int batch = -64, ids = 0;  // page ids batch .. batch + 63, one a lane
+  int page = 0, in_page = 0;
   auto key_of = [&](int t) { return t < first_tiles ? t * kKeys : low + (t - first_tiles) * kKeys; };
   auto stage_of = [&](int t) { return (t & 1) * 2 * S::kBytes; };
 
@@ -314,7 +336,15 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
         k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (static_cast<int64_t>(key_begin) + key0) * a.k_row + kv_head * a.k_head);
         v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + (static_cast<int64_t>(key_begin) + key0) * a.v_row + kv_head * a.v_head);
       } else {
-        const int page = key0 / a.page, in_page = key0 - page * a.page;
+        // (a tile lies behind the one asked for before it, but where the first keys end and the last begin)
+        in_page += kKeys;
+        if (t == from || t == first_tiles) {
+          page = key0 / a.page;
+          in_page = key0 - page * a.page;
+        } else if (in_page >= a.page) {
+          ++page;
+          in_page = 0;
+        }
         if (page < batch || page >= batch + 64) {
           batch = page;
           const int p = batch + lane;
@@ -343,19 +373,19 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
         }
       }
     } else {
-      const int key = key0 + (lane < there ? lane : there - 1), page0 = key0 / a.page, page = key / a.page;
+      const int key = key0 + (lane < there ? lane : there - 1), page0 = key0 / a.page, of_page = key / a.page;
       if (page0 < batch || (key0 + there - 1) / a.page >= batch + 64) {
         batch = page0;
         const int p = batch + lane;
         ids = table[p < a.table_width ? p : a.table_width - 1];
       }
-      const int id = __shfl(ids, page - batch, kWave), in_page = key - page * a.page;
+      const int id = __shfl(ids, of_page - batch, kWave), row_of_page = key - of_page * a.page;
       const bool known = id >= 0 && id < a.num_blocks;
       valid &= __ballot(known);
       const T *k = static_cast<const T*>(a.k), *v = static_cast<const T*>(a.v);
       if (known) {  // (else the first row of the cache)
-        k += id * a.k_block + in_page * a.k_row;
-        v += id * a.v_block + in_page * a.v_row;
+        k += id * a.k_block + row_of_page * a.k_row;
+        v += id * a.v_block + row_of_page * a.v_row;
       }
       const uint64_t ka = reinterpret_cast<uintptr_t>(k + kv_head * a.k_head), va = reinterpret_cast<uintptr_t>(v + kv_head * a.v_head);
 #pragma unroll
@@ -483,8 +513,15 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
     const float lower = other_half(l, &upper);
     l = lower + upper;
   }
+  // (the arguments once more from memory: held over the loop they would take the scalar registers that it needs)
+  const MloraAttentionArgs& args = *arguments_again();
+  if (shared && head == 0 && from == 0 && threadIdx.x == 0) {
+    const long long behind = of_rows.count - left;  // tiles of keys in the shares behind this one
+    const int parts = behind > 0 ? 1 + static_cast<int>((behind + a_share - 1) / a_share) : 1;
+    *joint(args, tile_number) = {item, parts, sequence, start, rows, position, total, key_begin};
+  }
   if (shared && to - from < of_rows.count) {  // for the join
-    const Unfinished u = unfinished(a, shares, item, from ? 0 : 1, head, D);
+    const Unfinished u = unfinished(args, shares, item, from ? 0 : 1, head, D);
     if (half == 0) u.sums[mine] = make_float2(m, l);
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d)
@@ -506,7 +543,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   unsigned long long again = __ballot(!finite && mine < rows);
   again = (again | again >> 32) & 0xffffffffull;
   if (mine < rows && !(again >> column & 1)) {
-    T* out = static_cast<T*>(a.out) + row * a.out_row + head * a.out_head;
+    T* out = static_cast<T*>(args.out) + row * args.out_row + head * args.out_head;
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d) {
       if constexpr (sizeof(T) == 2) {
@@ -537,7 +574,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
     const int c = __builtin_ctzll(again);
     again &= again - 1;
     const Place at{sequence, total, key_begin, wave_first + c};
-    attend_row<T>(a, at, start + 32 * wave + c, head, lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
+    attend_row<T>(args, at, start + 32 * wave + c, head, lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
   }
   if (shared) __syncthreads();
   }
@@ -548,51 +585,53 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   }
 }
 
-// Joins the parts of 32 rows of a tile that lies in several shares.
+// Joins the parts of 32 rows of a tile that lies in several shares, eight rows a wavefront.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, int shares) {
-  constexpr int kPer = D / 64;
+  constexpr int kPer = D / 64, kOwn = 8;
   __shared__ float scratch[kWaves][MLORA_MAX_HEAD_DIM];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.y, number = blockIdx.x >> 2;
-  const Shares batch(a, shares, lane);
-  if (number >= batch.tiles || !batch.per) return;
-  long long first = 0;
-  for (int base = 0; base < number; base += 64) {
-    const long long units = batch.units_of(a, base + lane);
-    first += base + lane < number ? units : 0;
-  }
-  for (int o = 32; o >= 1; o >>= 1) first += __shfl_xor(first, o, kWave);
-  const RowTile t = batch.tile(number);
-  const int count = KeyTiles(a, t.position, t.rows, t.total).count;
-  if (!count) return;  // (written: it is whole)
-  const int share = static_cast<int>(first / batch.per), parts = static_cast<int>((first + count - 1) / batch.per) - share + 1;
-  if (parts < 2) return;
-  for (int i = 0; i < 8; ++i) {
-    const int r = 32 * (blockIdx.x & 3) + 8 * wave + i;
-    if (r >= t.rows) break;
-    float most = -__builtin_inff(), sum = 0.0f, x[kPer] = {};
-    for (int p = 0; p < parts; ++p) most = fmaxf(most, unfinished(a, shares, share + p, p ? 0 : 1, head, D).sums[r].x);
-    for (int p = 0; p < parts; ++p) {
-      const Unfinished u = unfinished(a, shares, share + p, p ? 0 : 1, head, D);
-      const float2 ml = u.sums[r];
-      const float factor = ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
-      sum += factor * ml.y;
+  if (number >= *shared_tiles(a)) return;
+  const Joint t = *joint(a, number);
+  const int first = 32 * (blockIdx.x & 3) + kOwn * wave;
+  if (t.parts < 2 || first >= t.rows) return;
+  const int own = first + (lane & (kOwn - 1));  // the row whose (m, l) this lane looks after
+  float most = -__builtin_inff(), sum = 0.0f, x[kOwn][kPer] = {};
+  for (int p = 0; p < t.parts; ++p) most = fmaxf(most, unfinished(a, shares, t.share + p, p ? 0 : 1, head, D).sums[own].x);
+  for (int p = 0; p < t.parts; ++p) {
+    const Unfinished u = unfinished(a, shares, t.share + p, p ? 0 : 1, head, D);
+    const float2 ml = u.sums[own];
+    const float factor = ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
+    sum += factor * ml.y;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) x[e] += factor * u.outputs[r * D + 64 * e + lane];
+    for (int i = 0; i < kOwn; ++i) {
+      const float f = __shfl(factor, i, kWave);
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) x[i][e] += f * u.outputs[(first + i) * D + 64 * e + lane];
     }
-    const int row = t.start + r;
+  }
+  unsigned again = 0;
+#pragma unroll
+  for (int i = 0; i < kOwn; ++i) {
+    const int row = t.start + first + i;
+    const float l = __shfl(sum, i, kWave);
     bool finite = true;
 #pragma unroll
     for (int e = 0; e < kPer; ++e) {
-      x[e] /= sum;
-      finite &= __builtin_fabsf(x[e]) < __builtin_inff();
+      x[i][e] /= l;
+      finite &= __builtin_fabsf(x[i][e]) < __builtin_inff();
     }
-    if (__all(finite)) {
+    if (first + i >= t.rows) continue;
+    if (!__all(finite)) {
+      again |= 1u << i;
+      continue;
+    }
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) static_cast<T*>(a.out)[row * a.out_row + head * a.out_head + 64 * e + lane] = from_f32<T>(x[e]);
-    } else {
-      attend_row<T>(a, Place{t.sequence, t.total, t.key_start, t.position + r}, row, head, lane, scratch[wave]);
-    }
+    for (int e = 0; e < kPer; ++e) static_cast<T*>(a.out)[row * a.out_row + head * a.out_head + 64 * e + lane] = from_f32<T>(x[i][e]);
+  }
+  for (; again; again &= again - 1) {
+    const int r = first + __builtin_ctz(again);
+    attend_row<T>(a, Place{t.sequence, t.total, t.key_start, t.position + r}, t.start + r, head, lane, scratch[wave]);
   }
 }
 
@@ -641,8 +680,9 @@ size_t prompt_workspace_bytes(const MloraAttentionArgs* a) {
   if (!prompt_supported(a) || a->sequences > 64 || a->heads > 512) return 0;
   const int64_t shares = shares_of(*a), tiles = a->num_rows / kRows + a->sequences;
   const int64_t keys = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys;
-  if (tiles >= 2 * shares || tiles * ((keys + kKeys - 1) / kKeys) < kLeastShare * shares) return 0;
-  return static_cast<size_t>(shares * 2 * a->heads * kRows * (8 + 4 * a->dim));
+  // (keys that lie packed are mostly the rows' own: prompts by themselves, which seldom have enough of them)
+  if (tiles >= (a->block_tables ? 2 : 1) * shares || tiles * ((keys + kKeys - 1) / kKeys) < kLeastShare * shares) return 0;
+  return static_cast<size_t>(joints_bytes(tiles) + shares * 2 * a->heads * kRows * (8 + 4 * a->dim));
 }
 
 int launch_prompt(const MloraAttentionArgs* a) {
