@@ -183,7 +183,9 @@ struct Shares : RowTiles {
     if (tiles == 0) return;
     for (int base = 0; base < tiles; base += 64) units += units_of(a, base + lane);
     for (int o = 32; o >= 1; o >>= 1) units += __shfl_xor(units, o, kWave);
-    per = tiles < 4 * shares && units >= static_cast<long long>(kLeastShare) * shares ? (units + shares - 1) / shares : 0;
+    per = (units + shares - 1) / shares;
+    if (per < kLeastShare) per = units > static_cast<long long>(kLeastShare) * tiles ? kLeastShare : 0;
+    if (tiles >= 4 * shares) per = 0;
   }
   // The tile of rows that holds `unit` and the unit that it starts with.
   __device__ __forceinline__ int find(const MloraAttentionArgs& a, long long unit, int lane, long long* first) const {
@@ -429,6 +431,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
       }
     }
     if constexpr (sizeof(T) == 4) asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" : "+v"(s[0]), "+v"(s[1]));  // (the branch over the masks below)
+    __builtin_amdgcn_s_setprio(0);
     const bool all_behind = !a.causal || key0 + kKeys - 1 <= wave_first;
     const bool all_near = !a.window || key0 > wave_last - a.window || key0 + kKeys <= a.sinks;
     if (!(all_behind && all_near && valid == ~0ull)) {
@@ -465,9 +468,13 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
     }
     const float base = (m == -__builtin_inff() ? 0.0f : m) - kShift;
 #pragma unroll
-    for (int b = 0; b < 2; ++b) {
+    for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[b][j] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][j], scale, -base));
+    __builtin_amdgcn_sched_barrier(0);
+    __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
       if constexpr (sizeof(T) == 2) {
         Pack8 ones;
         const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
@@ -681,7 +688,7 @@ size_t prompt_workspace_bytes(const MloraAttentionArgs* a) {
   const int64_t shares = shares_of(*a), tiles = a->num_rows / kRows + a->sequences;
   const int64_t keys = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys;
   // (keys that lie packed are mostly the rows' own: prompts by themselves, which seldom have enough of them)
-  if (tiles >= (a->block_tables ? 2 : 1) * shares || tiles * ((keys + kKeys - 1) / kKeys) < kLeastShare * shares) return 0;
+  if (tiles >= (a->block_tables ? 2 : 1) * shares || keys <= kLeastShare * kKeys) return 0;
   return static_cast<size_t>(joints_bytes(tiles) + shares * 2 * a->heads * kRows * (8 + 4 * a->dim));
 }
 

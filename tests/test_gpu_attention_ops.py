@@ -107,6 +107,20 @@ def test_rotation_in_place_with_other_strides_and_off_alignment():
         assert got[0].data_ptr() == q.data_ptr() and torch.equal(q, want[0]) and torch.equal(k, want[1])
 
 
+@pytest.mark.parametrize("t,heads,kv_heads", [(5, 1, 0), (5, 0, 2), (70000, 2, 0), (9001, 5, 3)])
+def test_rotation_of_query_heads_or_key_heads_alone_and_of_many_tokens(t, heads, kv_heads):
+    from nanovllm_voxcpm_amd.attention_ops import rotary_table, rotate_qk
+
+    g = _gen(20)
+    q, k = (torch.randn(t, h, 64, generator=g).to(torch.float16) for h in (heads, kv_heads))
+    positions, table = torch.randint(0, 500, (t,), generator=g), rotary_table(64, 500)
+    got_q, got_k = rotate_qk(q.cuda(), k.cuda(), positions.cuda(), table.cuda())
+    some = torch.randperm(t, generator=g)[:40].sort().values
+    for got, x in ((got_q, q), (got_k, k)):
+        want, bound = oracle.rotate(x[some], positions[some], table)
+        _close(got[some.cuda()], want, bound + want.abs() * 2.0**-11 * (1 + 2**-7) + 2.0**-25)
+
+
 def test_rotation_by_a_position_outside_the_table_is_nan_and_far_positions_are_right():
     from nanovllm_voxcpm_amd.attention_ops import rotary_table, rotate_qk
 
@@ -261,6 +275,47 @@ def test_decode_behind_the_first_4_gb_of_a_cache():
     got = decode_attention(q[-1:].cuda(), k, v, table.cuda(), torch.tensor([n], dtype=torch.int32, device="cuda"))
     want, bound = oracle.attend(q[-1:], kk, vv, dtype=torch.bfloat16)
     _close(got, want, bound)
+
+
+# ---- prompts that are shared out over the chip --------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim,page", [(torch.bfloat16, 2, 1, 64, 64), (torch.float16, 16, 2, 64, 256), (torch.float16, 1, 1, 128, 16),
+                                                            (torch.float32, 4, 4, 64, 128), (torch.float32, 8, 1, 128, 0), (torch.bfloat16, 4, 2, 128, 0)])
+@pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 20000, 5), (False, 0, 0)])
+def test_chunks_behind_long_caches(dtype, heads, kv_heads, dim, page, causal, window, sinks):
+    """Few tiles of rows with many keys: their work is cut anywhere and joined.  Rows at the ends and borders of tiles are compared."""
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    if window and not causal:
+        pytest.skip("a window needs causal order")
+    print(dtype, heads, kv_heads, dim, page, causal, window, sinks, flush=True)
+    g = _gen(21)
+    new, totals = [130, 1, 300, 4, 257], [40000, 33001, 55013, 3, 257]
+    dense, k, v, table = _paged(totals, kv_heads, dim, page or 64, dtype, g, spare=0)
+    q = (1.5 * torch.randn(sum(new), heads, dim, generator=g)).to(dtype)
+    dense[2][1][54900] = NAN  # seen by some rows only
+    if page:
+        bad = 54900 // page
+        v[table[2, bad], 54900 % page] = NAN
+        got = prompt_attention(q.cuda(), k, v, _starts(new).cuda(), block_tables=table.cuda(), context_lens=torch.tensor(totals, dtype=torch.int32, device="cuda"),
+                               causal=causal, window=window, sinks=sinks)
+    else:
+        packed = [torch.cat([d[i] for d in dense]).cuda() for i in range(2)]
+        got = prompt_attention(q.cuda(), *packed, _starts(new).cuda(), cu_seqlens_k=_starts(totals).cuda(), causal=causal, window=window, sinks=sinks)
+    at = 0
+    for s, n in enumerate(new):
+        for i in sorted({0, 1, 127, 128, 129, 186, 187, 255, 256, n - 2, n - 1} & set(range(n))):
+            place = totals[s] - n + i
+            upto = place + 1 if causal else totals[s]
+            if upto <= 0:
+                assert not got[at + i].any()
+                continue
+            first = max(0, place + 1 - window) if window else 0
+            keys = [*range(min(sinks, first)), *range(first, upto)]
+            want, bound = oracle.attend(q[at + i : at + i + 1], dense[s][0][keys], dense[s][1][keys], False, dtype=dtype)
+            _close(got[at + i : at + i + 1], want, bound, (s, i))
+        at += n
 
 
 # ---- prompts ---------------------------------------------------------------------------------------------------------
