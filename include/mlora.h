@@ -409,10 +409,10 @@ typedef struct MloraAttentionArgs {
 
 /* One query row per sequence over a paged cache (num_rows == sequences). */
 int mlora_decode_attention(const MloraAttentionArgs* args);
-size_t mlora_decode_attention_workspace_bytes(int32_t sequences, int32_t heads, int32_t kv_heads, int32_t dim);
+size_t mlora_decode_attention_workspace_bytes(const MloraAttentionArgs* args); /* of a filled block; reads its sizes, strides and pointers' alignment */
 /* Any number of query rows per sequence, packed one sequence behind the other. */
 int mlora_prompt_attention(const MloraAttentionArgs* args);
-size_t mlora_prompt_attention_workspace_bytes(const MloraAttentionArgs* args); /* of a filled block; reads its sizes, strides and pointers' alignment */
+size_t mlora_prompt_attention_workspace_bytes(const MloraAttentionArgs* args);
 
 /* Identifier of the graph capture in progress on `stream`, 0 when the stream is not
  * capturing.  No counterpart in the reference: lets a host-side cache tell work recorded

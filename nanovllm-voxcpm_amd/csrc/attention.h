@@ -11,7 +11,7 @@ int launch_attend_rows(const MloraAttentionArgs* a);     // any head size, strid
 
 // paged.hip: one row per sequence over pages, head sizes 64 and 128
 bool paged_supported(const MloraAttentionArgs* a);
-size_t paged_workspace_bytes(int sequences, int heads, int kv_heads, int dim);
+size_t paged_workspace_bytes(const MloraAttentionArgs* a);
 int launch_paged(const MloraAttentionArgs* a);
 
 // prompt.hip: packed rows, head sizes 64 and 128

@@ -83,7 +83,7 @@ int check_attention(const MloraAttentionArgs* a, const char* what, bool decode) 
   }
   if (a->block_tables) {
     if (!a->context_lens || a->page < 1) { set_error("%s: pages need context_lens and a page of at least one row", what); return MLORA_E_INVALID; }
-    if (static_cast<int64_t>(a->table_width) * a->page > INT32_MAX / 2) { set_error("%s: %d pages of %d rows are more positions than 2^30", what, a->table_width, a->page); return MLORA_E_TOO_LARGE; }
+    if (static_cast<int64_t>(a->table_width) * a->page > INT32_MAX / 4) { set_error("%s: %d pages of %d rows are more positions than 2^29", what, a->table_width, a->page); return MLORA_E_TOO_LARGE; }
   }
   if (reinterpret_cast<uintptr_t>(a->workspace) & 15) { set_error("%s: workspace is not 16-byte aligned", what); return MLORA_E_INVALID; }
   const bool keys = a->block_tables ? a->num_blocks > 0 && a->table_width > 0 : a->num_keys > 0;
@@ -103,9 +103,14 @@ extern "C" int mlora_decode_attention(const MloraAttentionArgs* a) {
   return launch_attend_rows(&b);
 }
 
-extern "C" size_t mlora_decode_attention_workspace_bytes(int32_t sequences, int32_t heads, int32_t kv_heads, int32_t dim) {
-  if (sequences <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || (dim != 64 && dim != 128)) return 0;
-  return paged_workspace_bytes(sequences, heads, kv_heads, dim);
+// Blocks that the entry points would refuse need none.
+static bool sized(const MloraAttentionArgs* a) {
+  return a && a->num_rows > 0 && a->num_keys >= 0 && a->sequences > 0 && a->heads > 0 && a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->dim > 0 &&
+         a->table_width >= 0 && a->num_blocks >= 0 && a->page >= 0 && a->window >= 0 && a->sinks >= 0;
+}
+
+extern "C" size_t mlora_decode_attention_workspace_bytes(const MloraAttentionArgs* a) {
+  return sized(a) && a->block_tables && a->page > 0 && paged_supported(a) ? paged_workspace_bytes(a) : 0;
 }
 
 extern "C" int mlora_prompt_attention(const MloraAttentionArgs* a) {
@@ -115,7 +120,4 @@ extern "C" int mlora_prompt_attention(const MloraAttentionArgs* a) {
   return launch_attend_rows(a);
 }
 
-extern "C" size_t mlora_prompt_attention_workspace_bytes(const MloraAttentionArgs* a) {
-  if (!a || a->num_rows <= 0 || a->num_keys < 0 || a->sequences <= 0 || a->heads <= 0 || a->kv_heads <= 0 || a->table_width < 0) return 0;
-  return prompt_workspace_bytes(a);
-}
+extern "C" size_t mlora_prompt_attention_workspace_bytes(const MloraAttentionArgs* a) { return sized(a) ? prompt_workspace_bytes(a) : 0; }

@@ -18,12 +18,19 @@ __device__ __forceinline__ const char* uniform(const char* p) {
   return reinterpret_cast<const char*>((static_cast<uint64_t>(hi) << 32) | lo);
 }
 
+// The same load from a base that a vector instruction wrote (readfirstlane, readlane): five wait states have to lie between such a write of a
+// scalar register and a load that reads it, and the compiler keeps them in front of its own loads only.  Short of them the load goes to whatever
+// address the register held before.
+__device__ __forceinline__ void dma16_from(const void* base, uint32_t voff, uint32_t lds) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(voff), "s"(base) : "memory");
+}
+
 // One 1 KB direct load: lane i's 16 bytes at base + voff go to LDS byte lds + 16 i.  The load takes the LDS address from
 // m0, which the compiler itself puts there for the asm (an asm that wrote it could not say so: m0 is a reserved
 // register and has no place among the clobbers); between that write and the load lies one wait state.
 __device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t lds) {
 #ifdef MLORA_TRACE
-  base = uniform(static_cast<const char*>(base));  // (the branches around the stamps cost the compiler its proof of that)
+  return dma16_from(uniform(static_cast<const char*>(base)), voff, lds);  // (the branches around the stamps cost the compiler its proof of that)
 #endif
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(lds), "v"(voff), "s"(base) : "memory");
 }
@@ -31,7 +38,7 @@ __device__ __forceinline__ void dma16(const void* base, uint32_t voff, uint32_t 
 // The same with the non-temporal hint, for lines that no other workgroup asks for.
 __device__ __forceinline__ void dma16_once(const void* base, uint32_t voff, uint32_t lds) {
 #ifdef MLORA_TRACE
-  base = uniform(static_cast<const char*>(base));
+  return dma16_from(uniform(static_cast<const char*>(base)), voff, lds);
 #endif
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, %2 nt" ::"{m0}"(lds), "v"(voff), "s"(base) : "memory");
 }

@@ -2,15 +2,17 @@
 //
 // Bound by memory: every visible key and value is read once, and 16 heads of a group meet it on the matrix cores at a
 // thousandth of their rate.  So the kernel is laid out for bytes in flight.  A workgroup takes a run of tiles of one
-// sequence and key-value head, its four wavefronts a quarter of the run each; a wavefront asks for its tiles' rows by direct loads into a ring
-// of its own in LDS, two stages deep, and waits for nobody else.  Rows lie in the ring with their 16-byte pieces exchanged (piece ^ f(row)), so that the
+// sequence and key-value head, its wavefronts equal pieces of the run; a wavefront asks for its tiles' rows by direct loads into a ring
+// of its own in LDS and waits for nobody else until the sums meet.  Rows lie in the ring with their 16-byte pieces exchanged (piece ^ f(row)), so that the
 // reads below meet every bank once.  Scores come out of the first product with the keys along the registers and the heads along the lanes (K Q^T),
 // which is how the second one (V^T P^T) wants its weights: they pass from one to the other in registers.  V^T is read through the
 // transposing LDS read.
 //
-// The length is split: the tiles of the whole batch are shared out in parts of one size, as many as fill the chip, whatever sequence
+// Few long sequences are split: the tiles of the whole batch are shared out in parts of one size, as many as fill the chip, whatever sequence
 // they belong to.  Workgroups find their part from context_lens alone.  A sequence of one part is written straight away; the others leave (m, l, o) per
 // head in the workspace, and a second launch joins them: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m), in the order of the parts.
+// 3 sequences of up to 131072 keys, 32 heads, 8 of 128, bf16: 231 us, 5.1 TB/s (a copy of that size 5.2); 208 sequences, window 1024, 16 heads,
+// 2 of 64: 23 us, 4.5 TB/s; 64 of up to 2048: 15.2 us, 2.3 TB/s (the longest sequence by itself takes 12 of them).
 #include "attention.h"
 #include "common.h"
 #include "dma.h"
@@ -21,18 +23,20 @@ namespace mlora {
 
 namespace {
 
-constexpr int kWaves = 4, kStages = 2, kBlockHeads = 16;
-// Parts that a batch is cut into: workgroups of about two rounds over the chip, two workgroups a compute unit.
-constexpr int kWorkgroups = 1024;
+constexpr int kBlockHeads = 16;
+constexpr int kWorkgroups = 512;  // that a batch is cut into: two a compute unit
+constexpr int kLongWhole = 128;   // tiles of a sequence that four wavefronts take by themselves
 
 // What a hidden key's row is read from.
 __device__ __align__(16) uint32_t zero_row[MLORA_MAX_HEAD_DIM];
 
-template <typename T, int D> struct Shape {
+template <typename T, int D, int W> struct Shape {
+  static constexpr int kWaves = W, kStages = W == 4 ? 2 : 1;
   static constexpr int kRow = D * static_cast<int>(sizeof(T)), kChunks = kRow / 16;
   static constexpr int kKeys = sizeof(T) == 2 ? 32 : 16;  // one contraction of the second product
   static constexpr int kBytes = kKeys * kRow, kLoads = kBytes / 1024, kRowsPerLoad = 1024 / kRow;
-  static constexpr int kLds = kWaves * kStages * 2 * kBytes;
+  static constexpr int kRing = kWaves * kStages * 2 * kBytes, kLds = kRing + kWaves * kBlockHeads * 8 + kBlockHeads * 8 + kWaves * 4;
+  static_assert(kWaves * kBlockHeads * (D + 4) * 4 <= kRing, "the outputs meet where the rings were");
   // (K: 16 rows' piece of the same number in one read; V: 8 rows' pairs of pieces, in fp32 4 rows' four)
   static __device__ __forceinline__ int k_place(int row, int chunk) { return chunk ^ (kRow == 128 ? (row >> 1) & 7 : row & 15); }
   static __device__ __forceinline__ int v_place(int row, int chunk) {
@@ -42,14 +46,15 @@ template <typename T, int D> struct Shape {
 
 typedef __attribute__((address_space(3))) s16x4 LdsS16x4;
 
-__device__ __forceinline__ float group_max(float v) {  // over the lanes of the same number modulo 16
-  v = fmaxf(v, __shfl_xor(v, 16, kWave));
-  return fmaxf(v, __shfl_xor(v, 32, kWave));
+// Over the lanes of the same number modulo 16.
+template <typename F> __device__ __forceinline__ float over_groups(float v, F f) {
+  const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  v = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+  const auto h = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return f(__uint_as_float(h[0]), __uint_as_float(h[1]));
 }
-__device__ __forceinline__ float group_sum(float v) {
-  v += __shfl_xor(v, 16, kWave);
-  return v + __shfl_xor(v, 32, kWave);
-}
+__device__ __forceinline__ float group_max(float v) { return over_groups(v, [](float x, float y) { return fmaxf(x, y); }); }
+__device__ __forceinline__ float group_sum(float v) { return over_groups(v, [](float x, float y) { return x + y; }); }
 
 // The tiles of a sequence: those of the first keys, then those of the last.
 template <int KEYS> struct Tiles {
@@ -62,6 +67,9 @@ template <int KEYS> struct Tiles {
     count = first_tiles + (seen.high > seen.low ? (seen.high + KEYS - 1) / KEYS - low_tile : 0);
   }
   __device__ __forceinline__ int key(int tile) const { return (tile < first_tiles ? tile : tile - first_tiles + low_tile) * KEYS; }
+  __device__ __forceinline__ bool sees_all(int tile, int key0) const {
+    return tile < first_tiles ? key0 + KEYS <= seen.first : key0 >= seen.low && key0 + KEYS <= seen.high;
+  }
   __device__ __forceinline__ bool sees(int tile, int key) const { return tile < first_tiles ? key < seen.first : key >= seen.low && key < seen.high; }
 };
 
@@ -69,42 +77,51 @@ struct Part {
   int sequence, index, parts, tiles_per_part;
 };
 
+// Inclusive sums over the lanes: within rows of 16 by shifts, then the rows' last lanes to the rows behind them.
+template <int kControl, int kRows> __device__ __forceinline__ uint32_t plus_moved(uint32_t v) {
+  return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), kControl, kRows, 0xf, false));
+}
+__device__ __forceinline__ uint32_t wave_scan(uint32_t v) {
+  v = plus_moved<0x111, 0xf>(v);
+  v = plus_moved<0x112, 0xf>(v);
+  v = plus_moved<0x114, 0xf>(v);
+  v = plus_moved<0x118, 0xf>(v);
+  v = plus_moved<0x142, 0xa>(v);
+  return plus_moved<0x143, 0xc>(v);
+}
+__device__ __forceinline__ uint32_t lane_value(uint32_t v, int lane) { return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane)); }
+
 // Part number `item` of the batch; `target`: parts to cut the batch's tiles into (0: one a sequence).  By one wavefront.
-template <int KEYS> __device__ __forceinline__ bool find_part(const MloraAttentionArgs& a, int item, int target, int lane, Part* p) {
+template <int KEYS, int kWaves> __device__ __forceinline__ bool find_part(const MloraAttentionArgs& a, int item, int target, int lane, Part* p) {
   if (!target) {
     *p = {item, 0, 1, INT32_MAX};
     return item < a.sequences;
   }
-  int key_start, mine = 0;
-  long long tiles = 0;
-  for (int s = lane; s < a.sequences; s += 64) {
-    mine = Tiles<KEYS>(a, keys_of(a, s, &key_start)).count;
-    tiles += mine;
+  int key_start;
+  uint32_t mine = 0;
+  uint64_t tiles = 0;
+  for (int base = 0; base < a.sequences; base += 64) {
+    mine = base + lane < a.sequences ? Tiles<KEYS>(a, keys_of(a, base + lane, &key_start)).count : 0;
+    tiles += lane_value(wave_scan(mine), 63);
   }
-  for (int o = 32; o >= 1; o >>= 1) tiles += __shfl_xor(tiles, o, kWave);
-  // (never fewer than a tile a wavefront)
-  int per = static_cast<int>((tiles + target - 1) / target);
-  per = per < kWaves ? kWaves : per;
-  int before = 0;
+  // (whole rounds of the wavefronts)
+  const uint64_t least = (tiles + target - 1) / target;
+  const uint32_t per = static_cast<uint32_t>(least + kWaves - 1) / kWaves * kWaves + (least == 0 ? kWaves : 0);
+  uint32_t before = 0;
   for (int base = 0; base < a.sequences; base += 64) {
     const int s = base + lane;
     if (a.sequences > 64) mine = s < a.sequences ? Tiles<KEYS>(a, keys_of(a, s, &key_start)).count : 0;
-    const int parts = s < a.sequences ? (mine + per - 1) / per + (mine == 0) : 0;
-    int upto = parts;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int other = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += other;
-    }
-    const unsigned long long behind = __ballot(before + upto > item);
+    const uint32_t parts = s < a.sequences ? (mine + per - 1) / per + (mine == 0) : 0, upto = wave_scan(parts);
+    const unsigned long long behind = __ballot(before + upto > static_cast<uint32_t>(item));
     if (behind) {
       const int at = __builtin_ctzll(behind);
       p->sequence = base + at;
-      p->parts = __shfl(parts, at, kWave);
-      p->index = item - (before + __shfl(upto, at, kWave) - p->parts);
+      p->parts = lane_value(parts, at);
+      p->index = item - (before + lane_value(upto, at) - p->parts);
       p->tiles_per_part = per;
       return true;
     }
-    before += __shfl(upto, 63, kWave);
+    before += lane_value(upto, 63);
   }
   return false;
 }
@@ -125,17 +142,40 @@ __device__ __forceinline__ Workspace workspace_of(const MloraAttentionArgs& a, i
   return w;
 }
 
-template <typename T, int D>
-__global__ __launch_bounds__(kWaves * 64, 2) void paged_kernel(MloraAttentionArgs a, int target, int page_shift) {
-  using S = Shape<T, D>;
+// `pages`: log2 of the page where it is a power of two of 8 rows or more and rows lie near enough for 32-bit offsets, else -1.
+template <typename T, int D, int W>
+__global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAttentionArgs a, int target, int pages) {
+  using S = Shape<T, D, W>;
+  constexpr int kWaves = W, kStages = S::kStages;
   constexpr int kKeys = S::kKeys, kSteps = S::kChunks / 4, kBlocks = D / 16;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = a.heads / a.kv_heads, head_blocks = (group + kBlockHeads - 1) / kBlockHeads;
   const int kv_head = blockIdx.y / head_blocks, head_block = blockIdx.y - kv_head * head_blocks;
+  const int head_in_group = head_block * kBlockHeads + column;
+  const bool real = head_in_group < group;
+  const int head = kv_head * group + (real ? head_in_group : 0);
+
+  // What the first trip to memory can bring: lengths and, where the sequence is known without them, its queries and first page ids.
+  Pack8 query[kSteps];
+  int batch = 0, ids = 0;  // page ids batch .. batch + 63, one a lane
+  auto load_query = [&](int sequence) {
+    const char* q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + sequence * a.q_row + head * a.q_head);
+#pragma unroll
+    for (int s = 0; s < kSteps; ++s) query[s].raw = load128(q + 16 * (g + 4 * s));
+  };
+  auto load_ids = [&](int sequence, int page) {
+    batch = page;
+    const int p = batch + lane;
+    ids = a.block_tables[sequence * a.table_row + (p < a.table_width ? p : a.table_width - 1)];
+  };
+  if (!target) {
+    load_ids(blockIdx.x, 0);
+    load_query(blockIdx.x);
+  }
   Part part;
-  if (!find_part<kKeys>(a, blockIdx.x, target, lane, &part)) return;
+  if (!__builtin_amdgcn_readfirstlane(find_part<kKeys, kWaves>(a, blockIdx.x, target, lane, &part))) return;
   const int sequence = __builtin_amdgcn_readfirstlane(part.sequence);
   int key_start;
   const Tiles<kKeys> tiles(a, __builtin_amdgcn_readfirstlane(keys_of(a, sequence, &key_start)));
@@ -145,10 +185,7 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_kernel(MloraAttentionArg
   // this wavefront's run
   const int share = (end - begin + kWaves - 1) / kWaves;
   const int from = begin + wave * share, to = from + share < end ? from + share : end;
-
-  const int head_in_group = head_block * kBlockHeads + column;
-  const bool real = head_in_group < group;
-  const int head = kv_head * group + (real ? head_in_group : 0);
+  const int working = share ? (end - begin + share - 1) / share : 0;  // wavefronts that have one
   const float scale = a.scale * kLog2e;
 
   f32x4 o[kBlocks];
@@ -158,27 +195,47 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_kernel(MloraAttentionArg
   bool any = false;
 
   if (from < to) {
-    Pack8 query[kSteps];
-    const T* q = static_cast<const T*>(a.q) + sequence * a.q_row + head * a.q_head;
+    auto page_of = [&](int key) { return pages >= 0 ? key >> pages : key / a.page; };
+    if (target) {
+      load_ids(sequence, page_of(tiles.key(from)));
+      load_query(sequence);
+    }
+    if (!real) {
 #pragma unroll
-    for (int s = 0; s < kSteps; ++s) query[s].raw = real ? load128(reinterpret_cast<const char*>(q) + 16 * (g + 4 * s)) : i32x4{0, 0, 0, 0};
-
+      for (int s = 0; s < kSteps; ++s) query[s].raw = i32x4{0, 0, 0, 0};
+    }
+    unsigned long long known = __ballot(ids >= 0 && ids < a.num_blocks);
     char* const ring = lds + wave * (kStages * 2 * S::kBytes);
     const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(ring));
-    const int32_t* table = a.block_tables + sequence * a.table_row;
-    int batch = -64, ids = 0;  // page ids batch .. batch + 63, one a lane
     uint32_t masks[kStages];
+    const int own_row = lane / S::kChunks, piece = lane % S::kChunks;
+    const uint32_t k_from = own_row * static_cast<uint32_t>(a.k_row * sizeof(T)), v_from = own_row * static_cast<uint32_t>(a.v_row * sizeof(T));
 
     // Asks for the rows of tile t.
     auto request = [&](int t, int stage) {
-      const int key0 = tiles.key(t), key = key0 + (lane & 31);
-      const int page0 = page_shift >= 0 ? key0 >> page_shift : key0 / a.page, page = page_shift >= 0 ? key >> page_shift : key / a.page;
-      const int last = page_shift >= 0 ? (key0 + kKeys - 1) >> page_shift : (key0 + kKeys - 1) / a.page;
+      const int key0 = tiles.key(t), page0 = page_of(key0), last = page_of(key0 + kKeys - 1);
       if (page0 < batch || last >= batch + 64) {
-        batch = page0;
-        const int p = batch + lane;
-        ids = table[p < a.table_width ? p : a.table_width - 1];
+        load_ids(sequence, page0);
+        known = __ballot(ids >= 0 && ids < a.num_blocks);
       }
+      const unsigned long long wanted = ((last - page0 == 63 ? 0ull : 1ull << (last - page0 + 1)) - 1) << (page0 - batch);
+      const uint32_t to_k = ring_at + stage * 2 * S::kBytes, to_v = to_k + S::kBytes;
+      if (pages >= 0 && tiles.sees_all(t, key0) && (known & wanted) == wanted) {
+        // the rows of one load lie in one page
+        masks[stage] = kKeys == 32 ? 0xffffffffu : 0xffffu;
+#pragma unroll
+        for (int i = 0; i < S::kLoads; ++i) {
+          const int key = key0 + i * S::kRowsPerLoad, id = __builtin_amdgcn_readlane(ids, (key >> pages) - batch), in_page = key & ((1 << pages) - 1);
+          const char* k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + id * a.k_block + in_page * a.k_row + kv_head * a.k_head);
+          const char* v = reinterpret_cast<const char*>(static_cast<const T*>(a.v) + id * a.v_block + in_page * a.v_row + kv_head * a.v_head);
+          const int r = i * S::kRowsPerLoad + own_row;
+          dma16_from(uniform(k), k_from + 16 * S::k_place(r, piece), to_k + i * 1024);
+          dma16_from(uniform(v), v_from + 16 * S::v_place(r, piece), to_v + i * 1024);
+        }
+        return;
+      }
+      // Row by row: lanes 0 .. 31 find the keys', lanes 32 .. 63 the values'.
+      const int key = key0 + (lane & 31), page = page_of(key);
       const int id = __shfl(ids, page - batch, kWave);
       const bool valid = (lane & 31) < kKeys && tiles.sees(t, key) && id >= 0 && id < a.num_blocks;
       masks[stage] = static_cast<uint32_t>(__ballot(valid));
@@ -193,24 +250,24 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_kernel(MloraAttentionArg
       for (int kv = 0; kv < 2; ++kv) {
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i) {
-          const int r = i * S::kRowsPerLoad + lane / S::kChunks, piece = lane % S::kChunks;
-          const int chunk = kv ? S::v_place(r, piece) : S::k_place(r, piece);
+          const int r = i * S::kRowsPerLoad + own_row, chunk = kv ? S::v_place(r, piece) : S::k_place(r, piece);
           const uint32_t l32 = __shfl(lo, 32 * kv + r, kWave), h32 = __shfl(hi, 32 * kv + r, kWave);
           const char* p = reinterpret_cast<const char*>((static_cast<uint64_t>(h32) << 32) | l32) + 16 * chunk;
-          dma16v(p, ring_at + (stage * 2 + kv) * S::kBytes + i * 1024);
+          dma16v(p, (kv ? to_v : to_k) + i * 1024);
         }
       }
     };
 
-    request(from, 0);
-    if (from + 1 < to) request(from + 1, 1);
+#pragma unroll
+    for (int i = 0; i < kStages; ++i)
+      if (from + i < to) request(from + i, i);
     for (int t = from; t < to; ++t) {
-      const int stage = (t - from) & 1;
-      if (t + 1 < to) wait_loads<2 * S::kLoads>();
+      const int stage = kStages == 1 ? 0 : (t - from) & 1;
+      if (kStages == 2 && t + 1 < to) wait_loads<2 * S::kLoads>();
       else wait_loads<0>();
       const char* const k_tile = ring + stage * 2 * S::kBytes;
       const char* const v_tile = k_tile + S::kBytes;
-      const uint32_t mask = stage ? masks[1] : masks[0];
+      const uint32_t mask = masks[stage];
       float s[kKeys / 4];
 #pragma unroll
       for (int b = 0; b < kKeys / 16; ++b) {
@@ -291,125 +348,175 @@ __global__ __launch_bounds__(kWaves * 64, 2) void paged_kernel(MloraAttentionArg
     for (int d = 0; d < kBlocks; d += 4) mfma_settle(*reinterpret_cast<f32x4(*)[4]>(&o[d]));
   }
 
-  // The four wavefronts' sums: weights to the common maximum first, then element by element.
+  // The wavefronts' sums meet: every one weighs its own to the common maximum, then the outputs are added up element by element.
+  float2* const shared_ml = reinterpret_cast<float2*>(lds + S::kRing);  // [wave][head]
+  float2* const shared_sum = shared_ml + kWaves * kBlockHeads;          // [head]
+  int* const shared_any = reinterpret_cast<int*>(shared_sum + kBlockHeads);
   l = group_sum(l);
-  __syncthreads();  // (the rings have been read)
+  if (g == 0) shared_ml[wave * kBlockHeads + column] = make_float2(m, l);
+  if (lane == 0) shared_any[wave] = any;
+  __syncthreads();  // (the rings have been read, too)
   float* const shared_o = reinterpret_cast<float*>(lds);  // [wave][head][D + 4]
-  float* const shared_m = shared_o + kWaves * kBlockHeads * (D + 4);
-  float* const shared_l = shared_m + kWaves * kBlockHeads;
-  if (g == 0) {
-    shared_m[wave * kBlockHeads + column] = m;
-    shared_l[wave * kBlockHeads + column] = any ? l : -1.0f;  // (a wavefront that saw no key)
-  }
+  if (wave < working) {
+    // (each group of lanes looks at a quarter of the wavefronts)
+    float most = -__builtin_inff(), sum = 0.0f;
+    float2 ml[kWaves / 4];
 #pragma unroll
-  for (int d = 0; d < kBlocks; ++d) *reinterpret_cast<f32x4*>(shared_o + (wave * kBlockHeads + column) * (D + 4) + 16 * d + 4 * g) = o[d];
+    for (int i = 0; i < kWaves / 4; ++i) {
+      const int v = 4 * i + g;
+      ml[i] = v < working ? shared_ml[v * kBlockHeads + column] : make_float2(-__builtin_inff(), 0.0f);
+      most = fmaxf(most, ml[i].x);
+    }
+    most = group_max(most);
+#pragma unroll
+    for (int i = 0; i < kWaves / 4; ++i) sum += ml[i].y * (ml[i].x == most ? 1.0f : __builtin_amdgcn_exp2f(ml[i].x - most));
+    sum = group_sum(sum);
+    const float factor = m == most ? 1.0f : __builtin_amdgcn_exp2f(m - most);
+    if (real) {
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d) *reinterpret_cast<f32x4*>(shared_o + (wave * kBlockHeads + column) * (D + 4) + 16 * d + 4 * g) = o[d] * factor;
+    }
+    if (wave == 0 && g == 0) shared_sum[column] = make_float2(most, sum);
+  }
+  const bool some = __any(lane < working && shared_any[lane < kWaves ? lane : 0]);
   __syncthreads();
 
   const int items = gridDim.x;
   const bool whole = part.parts == 1;
-  Workspace w = workspace_of(a, items);
+  const Workspace w = workspace_of(a, items);
   if (target && threadIdx.x == 0 && blockIdx.y == 0 && index == 0) {
     w.rows[2 * sequence] = blockIdx.x;
     w.rows[2 * sequence + 1] = part.parts;
   }
-  constexpr int kPer = D / 16;  // elements of a thread: 16 threads a head
-  const int row = threadIdx.x >> 4, e0 = (threadIdx.x & 15) * kPer;
-  const int out_in_group = head_block * kBlockHeads + row;
-  if (out_in_group >= group) return;
-  const int out_head = kv_head * group + out_in_group;
-  float most = -__builtin_inff();
-  bool some = false;
 #pragma unroll
-  for (int v = 0; v < kWaves; ++v) {
-    if (shared_l[v * kBlockHeads + row] < 0) continue;
-    some = true;
-    most = fmaxf(most, shared_m[v * kBlockHeads + row]);
-  }
-  float sum = 0, x[kPer] = {};
+  for (int i = threadIdx.x; i < kBlockHeads * D; i += kWaves * 64) {
+    const int row = i / D, e = i % D, out_in_group = head_block * kBlockHeads + row;
+    if (out_in_group >= group) break;
+    const int out_head = kv_head * group + out_in_group;
+    float x = 0.0f;
 #pragma unroll
-  for (int v = 0; v < kWaves; ++v) {
-    if (shared_l[v * kBlockHeads + row] < 0) continue;
-    const float mv = shared_m[v * kBlockHeads + row], factor = mv == most ? 1.0f : __builtin_amdgcn_exp2f(mv - most);
-    sum += factor * shared_l[v * kBlockHeads + row];
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) x[e] += factor * shared_o[(v * kBlockHeads + row) * (D + 4) + e0 + e];
-  }
-  if (whole) {
-    T* out = static_cast<T*>(a.out) + sequence * a.out_row + out_head * a.out_head + e0;
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) out[e] = from_f32<T>(some ? x[e] / sum : 0.0f);
-  } else {
-    const int64_t at = static_cast<int64_t>(blockIdx.x) * a.heads + out_head;
-    if ((threadIdx.x & 15) == 0) w.sums[at] = make_float2(most, some ? sum : -1.0f);
-#pragma unroll
-    for (int e = 0; e < kPer; ++e) w.outputs[at * D + e0 + e] = x[e];
+    for (int v = 0; v < kWaves; ++v)
+      if (v < working) x += shared_o[(v * kBlockHeads + row) * (D + 4) + e];
+    const float2 ml = some ? shared_sum[row] : make_float2(-__builtin_inff(), -1.0f);
+    if (whole) {
+      static_cast<T*>(a.out)[sequence * a.out_row + out_head * a.out_head + e] = from_f32<T>(some ? x / ml.y : 0.0f);
+    } else {
+      const int64_t at = static_cast<int64_t>(blockIdx.x) * a.heads + out_head;
+      if (e == 0) w.sums[at] = ml;
+      w.outputs[at * D + e] = x;
+    }
   }
 }
 
-// Joins the parts of a (sequence, head).
+// Joins the parts of a (sequence, head): their weights to the common maximum first, kJoinParts of them at a time.
+constexpr int kJoinParts = 256;
 template <typename T, int D>
 __global__ __launch_bounds__(256) void join_kernel(MloraAttentionArgs a, int items) {
   constexpr int kRuns = 256 / D;  // threads of an element, each with every kRuns-th part
-  __shared__ float tops[4], sums[kRuns], values[kRuns][D];
-  const int sequence = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63;
+  __shared__ float tops[4], sums[4], factors[kJoinParts], values[kRuns][D];
+  const int sequence = blockIdx.x, head = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const Workspace w = workspace_of(a, items);
   const int first = w.rows[2 * sequence], parts = w.rows[2 * sequence + 1];
   if (parts < 2) return;
   const float2* const at = w.sums + static_cast<int64_t>(first) * a.heads + head;
+  const float* const from = w.outputs + (static_cast<int64_t>(first) * a.heads + head) * D;
+  const int64_t stride = static_cast<int64_t>(a.heads) * D;
   float most = -__builtin_inff();
   for (int i = threadIdx.x; i < parts; i += 256) {
     const float2 ml = at[static_cast<int64_t>(i) * a.heads];
-    if (ml.y >= 0 || ml.y != ml.y) most = fmaxf(most, ml.x);
+    if (!(ml.y < 0)) most = fmaxf(most, ml.x);
   }
   most = wave_max(most);
-  if (lane == 0) tops[threadIdx.x >> 6] = most;
+  if (lane == 0) tops[wave] = most;
   __syncthreads();
   most = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
   const int run = threadIdx.x / D, e = threadIdx.x - run * D;
   float sum = 0, x = 0;
   bool some = false;
-  for (int i = run; i < parts; i += kRuns) {
-    const float2 ml = at[static_cast<int64_t>(i) * a.heads];
-    if (ml.y < 0) continue;
-    some = true;
-    const float factor = ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
-    sum += factor * ml.y;
-    x += factor * w.outputs[(static_cast<int64_t>(first + i) * a.heads + head) * D + e];
+  for (int base = 0; base < parts; base += kJoinParts) {
+    const int n = parts - base < kJoinParts ? parts - base : kJoinParts;
+    float factor = 0.0f;
+    if (static_cast<int>(threadIdx.x) < n) {
+      const float2 ml = at[static_cast<int64_t>(base + threadIdx.x) * a.heads];
+      if (!(ml.y < 0)) {  // (a part that saw no key counts for nothing)
+        some = true;
+        factor = ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
+        sum += factor * ml.y;
+      }
+    }
+    if (base) __syncthreads();
+    factors[threadIdx.x] = factor;
+    __syncthreads();
+    int i = run;
+    for (; i + 7 * kRuns < n; i += 8 * kRuns) {
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = from[(base + i + j * kRuns) * stride + e];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x += factors[i + j * kRuns] * v[j];
+    }
+    for (; i < n; i += kRuns) x += factors[i] * from[(base + i) * stride + e];
   }
   values[run][e] = x;
-  if (e == 0) sums[run] = some ? sum : -1.0f;
+  sum = wave_sum(sum);
+  some = __any(some);
+  if (lane == 0) sums[wave] = some ? sum : -1.0f;
   __syncthreads();
   if (run) return;
   sum = 0, x = 0, some = false;
 #pragma unroll
-  for (int i = 0; i < kRuns; ++i) {
+  for (int i = 0; i < 4; ++i) {
     if (sums[i] < 0) continue;
     some = true;
     sum += sums[i];
-    x += values[i][e];
   }
+#pragma unroll
+  for (int i = 0; i < kRuns; ++i) x += values[i][e];
   static_cast<T*>(a.out)[sequence * a.out_row + head * a.out_head + e] = from_f32<T>(some ? x / sum : 0.0f);
 }
 
 int units_of_part(int heads, int kv_heads) { return kv_heads * ((heads / kv_heads + kBlockHeads - 1) / kBlockHeads); }
-int parts_wanted(int heads, int kv_heads) { return (kWorkgroups + units_of_part(heads, kv_heads) - 1) / units_of_part(heads, kv_heads); }
+// Wavefronts of a workgroup where a few of them have to take a whole sequence.
+constexpr int wide(int dim) { return dim == 64 ? 16 : 8; }
 
-template <typename T, int D> int launch(const MloraAttentionArgs& a) {
-  const bool split = a.workspace && a.workspace_bytes >= static_cast<int64_t>(paged_workspace_bytes(a.sequences, a.heads, a.kv_heads, a.dim));
-  const int target = split ? parts_wanted(a.heads, a.kv_heads) : 0;
+// How a call is cut.  Every way is right for every length; the lengths themselves only the device knows.
+//   Many sequences and heads (or a window, which bounds what a sequence costs): a workgroup of four wavefronts each, no join.
+//   Few, and none longer than four tiles a wavefront of the wide workgroups: one of these each, no join.
+//   Else the batch's tiles are shared out in parts of four wavefronts and joined.
+// us by the device's clock, four wavefronts whole / wide workgroups / parts: 208 sequences, 2 heads of 64, window 1024: 23 / 28 / 31; 64 of up to 2048 keys, 2 heads
+// of 64: 20.5 / 15.2 / 17.0; one of 900: 12.0 / 10.1 / 9.8 (the call's second launch costs the host more than that); 3 of up to 131072, 8 heads
+// of 128: 2150 / 1440 / 224.
+struct Way {
+  int waves, target;  // target: parts wanted, 0: none
+};
+Way cut_of(const MloraAttentionArgs& a) {
+  const int units = units_of_part(a.heads, a.kv_heads);
+  const int64_t keys = a.dtype == MLORA_DTYPE_F32 ? 16 : 32, most_keys = static_cast<int64_t>(a.table_width) * a.page;
+  const int64_t seen = a.window ? static_cast<int64_t>(a.window) + a.sinks + 2 * keys : INT64_MAX, tiles = ((most_keys < seen ? most_keys : seen) + keys - 1) / keys;
+  if (static_cast<int64_t>(a.sequences) * units >= 192 && tiles <= kLongWhole) return {4, 0};
+  if (tiles <= 4 * wide(a.dim)) return {wide(a.dim), 0};
+  return {4, (kWorkgroups + units - 1) / units};
+}
+
+template <typename T, int D, int W> int launch(const MloraAttentionArgs& a, int target, int pages) {
+  using S = Shape<T, D, W>;
   const int items = a.sequences + target;
-  int shift = 0;
-  while ((1 << shift) < a.page && shift < 30) ++shift;
-  if ((1 << shift) != a.page) shift = -1;
-  constexpr int kJoin = (kWaves * kBlockHeads * (D + 4) + 2 * kWaves * kBlockHeads) * 4;
-  constexpr int kLds = Shape<T, D>::kLds > kJoin ? Shape<T, D>::kLds : kJoin;
-  allow_lds<paged_kernel<T, D>>(kLds);
+  allow_lds<paged_kernel<T, D, W>>(S::kLds);
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
-  paged_kernel<T, D><<<dim3(items, units_of_part(a.heads, a.kv_heads)), kWaves * 64, kLds, stream>>>(a, target, shift);
+  paged_kernel<T, D, W><<<dim3(items, units_of_part(a.heads, a.kv_heads)), W * 64, S::kLds, stream>>>(a, target, pages);
   if (const int rc = check_launch("mlora_decode_attention")) return rc;
-  if (!split) return 0;
+  if (!target) return 0;
   join_kernel<T, D><<<dim3(a.sequences, a.heads), 256, 0, stream>>>(a, items);
   return check_launch("mlora_decode_attention (join)");
+}
+
+template <typename T, int D> int launch_shape(const MloraAttentionArgs& a) {
+  Way cut = cut_of(a);
+  if (!a.workspace || a.workspace_bytes < static_cast<int64_t>(paged_workspace_bytes(&a))) cut.target = 0;
+  int pages = -1;
+  const int64_t most = INT32_MAX / (8 * 4);
+  if (a.page >= 8 && (a.page & (a.page - 1)) == 0 && a.k_row >= 0 && a.v_row >= 0 && a.k_row <= most && a.v_row <= most) pages = __builtin_ctz(a.page);
+  return cut.waves == 4 ? launch<T, D, 4>(a, cut.target, pages) : launch<T, D, wide(D)>(a, cut.target, pages);
 }
 
 }  // namespace
@@ -418,18 +525,20 @@ bool paged_supported(const MloraAttentionArgs* a) {
   return (a->dim == 64 || a->dim == 128) && attention_vectors_ok(a) && a->table_width > 0 && units_of_part(a->heads, a->kv_heads) <= 65535 && a->heads <= 65535;
 }
 
-size_t paged_workspace_bytes(int sequences, int heads, int kv_heads, int dim) {
-  const int64_t items = static_cast<int64_t>(sequences) + parts_wanted(heads, kv_heads);
-  return static_cast<size_t>(workspace_rows_bytes(sequences) + ((items * heads + 1) & ~1ll) * 8 + items * heads * dim * 4);
+size_t paged_workspace_bytes(const MloraAttentionArgs* a) {
+  const Way cut = cut_of(*a);
+  if (!cut.target) return 0;
+  const int64_t items = static_cast<int64_t>(a->sequences) + cut.target;
+  return static_cast<size_t>(workspace_rows_bytes(a->sequences) + ((items * a->heads + 1) & ~1ll) * 8 + items * a->heads * a->dim * 4);
 }
 
 int launch_paged(const MloraAttentionArgs* a) {
   if (a->dim == 64) {
-    if (a->dtype == MLORA_DTYPE_BF16) return launch<__bf16, 64>(*a);
-    return a->dtype == MLORA_DTYPE_F16 ? launch<_Float16, 64>(*a) : launch<float, 64>(*a);
+    if (a->dtype == MLORA_DTYPE_BF16) return launch_shape<__bf16, 64>(*a);
+    return a->dtype == MLORA_DTYPE_F16 ? launch_shape<_Float16, 64>(*a) : launch_shape<float, 64>(*a);
   }
-  if (a->dtype == MLORA_DTYPE_BF16) return launch<__bf16, 128>(*a);
-  return a->dtype == MLORA_DTYPE_F16 ? launch<_Float16, 128>(*a) : launch<float, 128>(*a);
+  if (a->dtype == MLORA_DTYPE_BF16) return launch_shape<__bf16, 128>(*a);
+  return a->dtype == MLORA_DTYPE_F16 ? launch_shape<_Float16, 128>(*a) : launch_shape<float, 128>(*a);
 }
 
 }  // namespace mlora

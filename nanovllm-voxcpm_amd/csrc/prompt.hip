@@ -362,16 +362,16 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
       if (there == kKeys) {
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i) {
-          dma16(k, k_offset[i], k_to + i * 1024);
-          dma16(v, v_offset[i], v_to + i * 1024);
+          dma16_from(k, k_offset[i], k_to + i * 1024);
+          dma16_from(v, v_offset[i], v_to + i * 1024);
         }
       } else {
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i) {
           const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks;
           const uint32_t back = r < there ? 0 : r - there + 1;  // (a place behind the last key repeats it)
-          dma16(k, k_offset[i] - back * k_row, k_to + i * 1024);
-          dma16(v, v_offset[i] - back * v_row, v_to + i * 1024);
+          dma16_from(k, k_offset[i] - back * k_row, k_to + i * 1024);
+          dma16_from(v, v_offset[i] - back * v_row, v_to + i * 1024);
         }
       }
     } else {

@@ -284,7 +284,7 @@ def load() -> C.CDLL:
     lib.mlora_add_workspace_bytes.restype = C.c_size_t
     lib.mlora_workspace_init.argtypes = [C.c_void_p, C.c_int64, C.c_void_p]
     lib.mlora_workspace_init.restype = C.c_int
-    lib.mlora_decode_attention_workspace_bytes.argtypes = [C.c_int32] * 4
+    lib.mlora_decode_attention_workspace_bytes.argtypes = [C.POINTER(MloraAttentionArgs)]
     lib.mlora_decode_attention_workspace_bytes.restype = C.c_size_t
     lib.mlora_prompt_attention_workspace_bytes.argtypes = [C.POINTER(MloraAttentionArgs)]
     lib.mlora_prompt_attention_workspace_bytes.restype = C.c_size_t
@@ -834,7 +834,7 @@ def decode_attention(q, out, k_cache, v_cache, block_tables, context_lens, scale
     lib = load()
     args = _attention_args(q, out, k_cache, v_cache, block_tables, context_lens, True, scale, window, sinks)
     args.sequences = q.size(0)
-    workspace = _scratch(args, lib.mlora_decode_attention_workspace_bytes(args.sequences, args.heads, args.kv_heads, args.dim), q.device)  # noqa: F841
+    workspace = _scratch(args, lib.mlora_decode_attention_workspace_bytes(C.byref(args)), q.device)  # noqa: F841
     with _on(q.device):
         _check(lib.mlora_decode_attention(C.byref(args)), "mlora_decode_attention")
 
