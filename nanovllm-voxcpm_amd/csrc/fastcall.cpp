@@ -17,6 +17,8 @@
 #include <Python.h>
 
 #include <ATen/core/Tensor.h>
+#include <ATen/ops/empty.h>
+#include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
@@ -577,6 +579,222 @@ template <typename F> PyObject* run_op(F f, PyObject* const* args, Py_ssize_t na
 PyObject* py_shrink(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_op(op_shrink, args, nargs, 6); }
 PyObject* py_expand(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_op(op_expand, args, nargs, 7); }
 
+// ---- the attention block -------------------------------------------------------------------------------
+// rotate(address of mlora_rotate_qk, q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, v, k_cache, v_cache, slot_mapping) -> (q, k or None),
+// decode(addresses of mlora_decode_attention and its workspace_bytes, q, k_cache, v_cache, block_tables, context_lens, scale, window, sinks) -> out,
+// prompt(addresses of mlora_prompt_attention and its workspace_bytes, q, k, v, cu_seqlens, cu_seqlens_k, block_tables, context_lens, causal, scale, window,
+// sinks) -> out: the usual calls of attention_ops, checked and enqueued, with new tensors for results; None for anything that has to raise, that names its
+// outputs, or that lives on another device than the current one.
+
+// A tensor argument; nullptr for None, `ok` cleared for anything else.
+const at::Tensor* optional_tensor(PyObject* o, bool* ok) {
+  if (o == Py_None) return nullptr;
+  if (!THPVariable_Check(o)) {
+    *ok = false;
+    return nullptr;
+  }
+  return &THPVariable_Unpack(o);
+}
+
+bool learns(const at::Tensor* t) { return t && t->requires_grad(); }
+
+// `dims` dimensions with the last side by side, of the element type and on the device of q.
+bool rows_like(const at::Tensor& t, int64_t dims, const at::Tensor& q) {
+  return t.dim() == dims && t.device() == q.device() && t.scalar_type() == q.scalar_type() && (t.numel() == 0 || t.size(dims - 1) == 1 || t.stride(dims - 1) == 1);
+}
+
+bool index_vector(const at::Tensor& t, const at::Tensor& q, int64_t least, bool* is64) {
+  const bool wide = t.scalar_type() == c10::ScalarType::Long;
+  if (is64) *is64 = wide;
+  return (t.scalar_type() == c10::ScalarType::Int || (is64 && wide)) && t.dim() == 1 && t.is_contiguous() && t.device() == q.device() && t.numel() >= least;
+}
+
+bool head_rows(const at::Tensor& q) {
+  return q.is_cuda() && c10::hip::current_device() == q.device().index() && rows_like(q, 3, q) && code_of(q.scalar_type()) >= 0 && q.size(0) <= INT32_MAX &&
+         q.size(1) <= INT32_MAX && q.size(2) <= INT32_MAX;
+}
+
+void* stream_of(const at::Tensor& q) { return c10::hip::getCurrentHIPStream(q.device().index()).stream(); }
+
+bool shares_memory(const at::Tensor& t) {
+  for (int64_t i = 0; i < t.dim(); ++i)
+    if (t.stride(i) == 0 && t.size(i) > 1) return true;
+  return false;
+}
+
+bool cache_like(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) {
+  return rows_like(k, 4, q) && rows_like(v, 4, q) && k.sizes() == v.sizes() && k.size(0) <= INT32_MAX && k.size(1) >= 1 && k.size(1) <= INT32_MAX && k.size(3) == q.size(2);
+}
+
+PyObject* op_rotate(PyObject* const* args) {
+  bool ok = true;
+  const at::Tensor *q = optional_tensor(args[1], &ok), *k = optional_tensor(args[2], &ok), *positions = optional_tensor(args[3], &ok), *table = optional_tensor(args[4], &ok);
+  const at::Tensor *weights[2] = {optional_tensor(args[5], &ok), optional_tensor(args[6], &ok)};
+  const at::Tensor *v = optional_tensor(args[9], &ok), *k_cache = optional_tensor(args[10], &ok), *v_cache = optional_tensor(args[11], &ok), *slots = optional_tensor(args[12], &ok);
+  if (!ok || !q || !k || !positions || !table || !head_rows(*q) || !rows_like(*k, 3, *q)) return nullptr;
+  if (c10::GradMode::is_enabled() && (learns(q) || learns(k) || learns(v) || learns(weights[0]) || learns(weights[1]))) return nullptr;
+  const int64_t rows = q->size(0), dim = q->size(2);
+  MloraRotateArgs a = {};
+  bool is64 = false;
+  if (k->size(0) != rows || k->size(2) != dim || k->size(1) > INT32_MAX || !index_vector(*positions, *q, rows, &is64)) return nullptr;
+  a.positions64 = is64;
+  if (table->dim() != 2 || table->scalar_type() != c10::ScalarType::Float || (table->numel() && table->stride(1) != 1) || table->device() != q->device() || table->size(1) > INT32_MAX)
+    return nullptr;
+  for (const at::Tensor* w : weights) {
+    if (!w) continue;
+    const bool wide = w->scalar_type() == c10::ScalarType::Float;
+    if (w->device() != q->device() || !(wide || w->scalar_type() == q->scalar_type()) || w->dim() != 1 || w->size(0) != dim || !w->is_contiguous()) return nullptr;
+    a.weights32 = wide;
+  }
+  if (weights[0] && weights[1] && weights[0]->scalar_type() != weights[1]->scalar_type()) return nullptr;
+  const bool cached = v != nullptr;
+  if (cached != (k_cache != nullptr) || cached != (v_cache != nullptr) || cached != (slots != nullptr)) return nullptr;
+  if (cached) {
+    if (!rows_like(*v, 3, *q) || v->sizes() != k->sizes() || !cache_like(*k_cache, *v_cache, *q) || k_cache->size(2) != k->size(1) || shares_memory(*k_cache) ||
+        shares_memory(*v_cache) || !index_vector(*slots, *q, rows, &is64))
+      return nullptr;
+    a.slots64 = is64;
+    a.v = v->data_ptr(); a.v_row = v->stride(0); a.v_head = v->stride(1);
+    a.k_cache = k_cache->data_ptr(); a.k_block = k_cache->stride(0); a.k_cache_row = k_cache->stride(1); a.k_cache_head = k_cache->stride(2);
+    a.v_cache = v_cache->data_ptr(); a.v_block = v_cache->stride(0); a.v_cache_row = v_cache->stride(1); a.v_cache_head = v_cache->stride(2);
+    a.slots = slots->data_ptr();
+    a.num_blocks = static_cast<int32_t>(k_cache->size(0)); a.page = static_cast<int32_t>(k_cache->size(1));
+  }
+  a.eps = static_cast<float>(PyFloat_AsDouble(args[7]));
+  a.interleaved = PyObject_IsTrue(args[8]) == 1;
+  const auto fn = reinterpret_cast<int (*)(const MloraRotateArgs*)>(PyLong_AsSize_t(args[0]));
+  if (PyErr_Occurred()) return nullptr;
+  a.stream = stream_of(*q);
+  a.q = q->data_ptr(); a.q_row = q->stride(0); a.q_head = q->stride(1);
+  a.k = k->data_ptr(); a.k_row = k->stride(0); a.k_head = k->stride(1);
+  a.positions = positions->data_ptr();
+  a.cos_sin = static_cast<const float*>(table->data_ptr()); a.table_row = table->stride(0); a.num_positions = table->size(0);
+  a.q_weight = weights[0] ? weights[0]->data_ptr() : nullptr;
+  a.k_weight = weights[1] ? weights[1]->data_ptr() : nullptr;
+  a.num_tokens = static_cast<int32_t>(rows); a.heads = static_cast<int32_t>(q->size(1)); a.kv_heads = static_cast<int32_t>(k->size(1));
+  a.dim = static_cast<int32_t>(dim); a.rotary = static_cast<int32_t>(table->size(1)); a.dtype = code_of(q->scalar_type());
+  at::Tensor q_out = at::empty(q->sizes(), q->options().requires_grad(false)), k_out;
+  a.q_out = q_out.data_ptr(); a.q_out_row = q_out.stride(0); a.q_out_head = q_out.stride(1);
+  if (!cached) {
+    k_out = at::empty(k->sizes(), k->options().requires_grad(false));
+    a.k_out = k_out.data_ptr(); a.k_out_row = k_out.stride(0); a.k_out_head = k_out.stride(1);
+  }
+  if (fn(&a) != 0) return nullptr;
+  PyObject* first = THPVariable_Wrap(std::move(q_out));
+  PyObject* second = nullptr;
+  if (cached) {
+    second = Py_None;
+    Py_INCREF(second);
+  } else {
+    second = THPVariable_Wrap(std::move(k_out));
+  }
+  PyObject* both = first && second ? PyTuple_Pack(2, first, second) : nullptr;
+  Py_XDECREF(first);
+  Py_XDECREF(second);
+  return both;
+}
+
+bool small_number(PyObject* o, int32_t* out) {
+  const long v = PyLong_AsLong(o);
+  if (PyErr_Occurred() || v < 0) return false;
+  *out = v > INT32_MAX ? INT32_MAX : static_cast<int32_t>(v);
+  return true;
+}
+
+// Fills in q, the keys and the pages of a call; false for what the Python path has to see to.
+bool fill_attention(MloraAttentionArgs* a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor* tables, const at::Tensor* lens, int64_t sequences) {
+  if (!head_rows(q) || sequences < 0 || sequences > INT32_MAX) return false;
+  if (c10::GradMode::is_enabled() && (learns(&q) || learns(&k) || learns(&v))) return false;
+  int64_t kv_heads;
+  if (tables) {
+    if (!lens || !cache_like(k, v, q) || tables->dim() != 2 || tables->scalar_type() != c10::ScalarType::Int || tables->device() != q.device() || tables->size(0) < sequences ||
+        tables->size(1) > INT32_MAX || (tables->numel() && tables->size(1) > 1 && tables->stride(1) != 1) || !index_vector(*lens, q, sequences, nullptr))
+      return false;
+    kv_heads = k.size(2);
+    a->k_block = k.stride(0); a->k_row = k.stride(1); a->k_head = k.stride(2);
+    a->v_block = v.stride(0); a->v_row = v.stride(1); a->v_head = v.stride(2);
+    // (a table without pages has no memory of its own, and none is read)
+    a->block_tables = static_cast<const int32_t*>(tables->numel() ? tables->data_ptr() : lens->data_ptr()); a->context_lens = static_cast<const int32_t*>(lens->data_ptr());
+    a->table_row = tables->stride(0); a->table_width = static_cast<int32_t>(tables->size(1));
+    a->num_blocks = static_cast<int32_t>(k.size(0)); a->page = static_cast<int32_t>(k.size(1));
+  } else {
+    if (lens || !rows_like(k, 3, q) || !rows_like(v, 3, q) || k.sizes() != v.sizes() || k.size(2) != q.size(2) || k.size(0) > INT32_MAX) return false;
+    kv_heads = k.size(1);
+    a->k_row = k.stride(0); a->k_head = k.stride(1);
+    a->v_row = v.stride(0); a->v_head = v.stride(1);
+    a->num_keys = static_cast<int32_t>(k.size(0));
+  }
+  if (q.size(1) && (kv_heads < 1 || kv_heads > INT32_MAX || q.size(1) % kv_heads)) return false;
+  a->q = q.data_ptr(); a->q_row = q.stride(0); a->q_head = q.stride(1);
+  a->k = k.data_ptr(); a->v = v.data_ptr();
+  a->num_rows = static_cast<int32_t>(q.size(0)); a->heads = static_cast<int32_t>(q.size(1)); a->dim = static_cast<int32_t>(q.size(2));
+  a->kv_heads = static_cast<int32_t>(kv_heads); a->sequences = static_cast<int32_t>(sequences); a->dtype = code_of(q.scalar_type());
+  return true;
+}
+
+PyObject* run_attention(MloraAttentionArgs* a, const at::Tensor& q, PyObject* entry, PyObject* sizing, PyObject* scale) {
+  const auto fn = reinterpret_cast<int (*)(const MloraAttentionArgs*)>(PyLong_AsSize_t(entry));
+  const auto bytes = reinterpret_cast<size_t (*)(const MloraAttentionArgs*)>(PyLong_AsSize_t(sizing));
+  a->scale = static_cast<float>(scale == Py_None ? 1.0 / std::sqrt(static_cast<double>(q.size(2))) : PyFloat_AsDouble(scale));
+  if (PyErr_Occurred()) return nullptr;
+  at::Tensor out = at::empty(q.sizes(), q.options().requires_grad(false)), workspace;
+  a->out = out.data_ptr(); a->out_row = out.stride(0); a->out_head = out.stride(1);
+  a->stream = stream_of(q);
+  if (const size_t n = bytes(a)) {  // (given back when the call is enqueued: the allocator hands it to nobody before the stream is past it)
+    workspace = at::empty({static_cast<int64_t>(n)}, q.options().dtype(c10::ScalarType::Byte).requires_grad(false));
+    a->workspace = workspace.data_ptr();
+    a->workspace_bytes = static_cast<int64_t>(n);
+  }
+  if (fn(a) != 0) return nullptr;
+  return THPVariable_Wrap(std::move(out));
+}
+
+PyObject* op_decode(PyObject* const* args) {
+  bool ok = true;
+  const at::Tensor *q = optional_tensor(args[2], &ok), *k = optional_tensor(args[3], &ok), *v = optional_tensor(args[4], &ok), *tables = optional_tensor(args[5], &ok),
+                   *lens = optional_tensor(args[6], &ok);
+  if (!ok || !q || !k || !v || !tables || !lens || q->dim() != 3) return nullptr;
+  MloraAttentionArgs a = {};
+  a.causal = 1;
+  if (!fill_attention(&a, *q, *k, *v, tables, lens, q->size(0)) || !small_number(args[8], &a.window) || !small_number(args[9], &a.sinks)) return nullptr;
+  return run_attention(&a, *q, args[0], args[1], args[7]);
+}
+
+PyObject* op_prompt(PyObject* const* args) {
+  bool ok = true;
+  const at::Tensor *q = optional_tensor(args[2], &ok), *k = optional_tensor(args[3], &ok), *v = optional_tensor(args[4], &ok), *starts = optional_tensor(args[5], &ok),
+                   *key_starts = optional_tensor(args[6], &ok), *tables = optional_tensor(args[7], &ok), *lens = optional_tensor(args[8], &ok);
+  if (!ok || !q || !k || !v || !starts || q->dim() != 3 || !index_vector(*starts, *q, 1, nullptr)) return nullptr;
+  const int64_t sequences = starts->numel() - 1;
+  MloraAttentionArgs a = {};
+  a.causal = PyObject_IsTrue(args[9]) == 1;
+  if (!fill_attention(&a, *q, *k, *v, tables, lens, sequences) || !small_number(args[11], &a.window) || !small_number(args[12], &a.sinks)) return nullptr;
+  if (!a.causal && (a.window || a.sinks)) return nullptr;
+  if (key_starts && (tables || !index_vector(*key_starts, *q, sequences + 1, nullptr))) return nullptr;
+  a.starts = static_cast<const int32_t*>(starts->data_ptr());
+  a.key_starts = key_starts ? static_cast<const int32_t*>(key_starts->data_ptr()) : nullptr;
+  return run_attention(&a, *q, args[0], args[1], args[10]);
+}
+
+template <typename F> PyObject* run_result(F f, PyObject* const* args, Py_ssize_t nargs, Py_ssize_t want) {
+  if (nargs != want) {
+    PyErr_Format(PyExc_TypeError, "expected %zd arguments", want);
+    return nullptr;
+  }
+  PyObject* result = nullptr;
+  try {
+    result = f(args);
+  } catch (...) {
+    result = nullptr;
+  }
+  if (result) return result;
+  if (PyErr_Occurred()) PyErr_Clear();
+  Py_RETURN_NONE;
+}
+PyObject* py_rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_rotate, args, nargs, 13); }
+PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_decode, args, nargs, 10); }
+PyObject* py_prompt(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_prompt, args, nargs, 13); }
+
 // ---- batch contexts --------------------------------------------------------------------------------------
 // The runs of a batch (slot ids and token counts as Python lists) as arrays.
 bool read_runs(PyObject* slots, PyObject* counts, std::vector<int32_t>* s, std::vector<int32_t>* c) {
@@ -797,6 +1015,9 @@ PyMethodDef kMethods[] = {
      "call_stacked(state, target, x, A, Bs, indices, metadata, scaling, effective_rank) -> 0, a library error code, or NOT_HANDLED"},
     {"shrink", method(py_shrink), METH_FASTCALL, "shrink(address of mlora_shrink, inputs, weights, output, slots, scaling) -> 0, a library error code, or NOT_HANDLED"},
     {"expand", method(py_expand), METH_FASTCALL, "expand(address of mlora_expand, inputs, weights, output, slots, offset, add) -> 0, a library error code, or NOT_HANDLED"},
+    {"rotate", method(py_rotate), METH_FASTCALL, "rotate(address of mlora_rotate_qk, q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, v, k_cache, v_cache, slot_mapping) -> (q, k) or None"},
+    {"decode", method(py_decode), METH_FASTCALL, "decode(address of mlora_decode_attention, of its workspace_bytes, q, k_cache, v_cache, block_tables, context_lens, scale, window, sinks) -> out or None"},
+    {"prompt", method(py_prompt), METH_FASTCALL, "prompt(address of mlora_prompt_attention, of its workspace_bytes, q, k, v, cu_seqlens, cu_seqlens_k, block_tables, context_lens, causal, scale, window, sinks) -> out or None"},
     {"run_totals", py_run_totals, METH_VARARGS, "run_totals(slots, counts) -> (tokens, with a slot, active slots, largest slot) or None"},
     {"build_context", py_build_context, METH_VARARGS, "build_context(address of mlora_meta_build_runs, slots, counts, device, max_slots, capacity, six addresses) -> rc"},
     {"install_batch", py_install_batch, METH_NOARGS, "install_batch() -> an empty batch of slot installs"},

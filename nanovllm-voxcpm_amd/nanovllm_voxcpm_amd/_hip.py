@@ -805,7 +805,8 @@ def _attention_args(q, out, k, v, block_tables, context_lens, causal: bool, scal
     if block_tables is not None:
         _strides(args, ("k_block", "k_row", "k_head"), k)
         _strides(args, ("v_block", "v_row", "v_head"), v)
-        args.block_tables, args.context_lens = block_tables.data_ptr(), context_lens.data_ptr()
+        # (a table without pages has no memory of its own, and none is read)
+        args.block_tables, args.context_lens = (block_tables if block_tables.numel() else context_lens).data_ptr(), context_lens.data_ptr()
         args.table_row, args.table_width = block_tables.stride(0), block_tables.size(1)
         args.num_blocks, args.page = k.size(0), k.size(1)
     else:

@@ -144,6 +144,11 @@ def rotate_qk(
     Returns (q, k): in ``q_out`` and ``k_out`` where given (an input itself is fine), else new tensors; k is None with a cache
     and without ``k_out``, since the cache has it.
     """
+    fast = _hip.load_fastcall()
+    if fast is not None and q_out is None and k_out is None:  # the usual call, checked and enqueued in C++
+        result = fast.rotate(_hip.entry_point("mlora_rotate_qk"), q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, v, k_cache, v_cache, slot_mapping)
+        if result is not None:
+            return result
     _heads(q, "q")
     _heads(k, "k", q)
     _no_grad(q, k, v, q_weight, k_weight)
@@ -235,6 +240,12 @@ def decode_attention(
     first ``sinks`` beside them.  A sequence of no rows (padding) gives 0.  Lengths beyond the table's pages end there; the rows of a page
     id outside the cache are not seen.  What lies in rows that are not seen does not matter.
     """
+    fast = _hip.load_fastcall()
+    if fast is not None and out is None:
+        result = fast.decode(_hip.entry_point("mlora_decode_attention"), _hip.entry_point("mlora_decode_attention_workspace_bytes"), q, k_cache, v_cache,
+                             block_tables, context_lens, scale, window, sinks)
+        if result is not None:
+            return result
     _heads(q, "q")
     _cache(k_cache, v_cache, None, q)
     _no_grad(q, k_cache, v_cache)
@@ -269,6 +280,12 @@ def prompt_attention(
     them and the first ``sinks`` keys; without ``causal`` every row sees the whole sequence.  Rows that see nothing are 0, rows of
     ``out`` behind the last sequence are left as they are (a new ``out`` holds anything there).
     """
+    fast = _hip.load_fastcall()
+    if fast is not None and out is None:
+        result = fast.prompt(_hip.entry_point("mlora_prompt_attention"), _hip.entry_point("mlora_prompt_attention_workspace_bytes"), q, k, v, cu_seqlens,
+                             cu_seqlens_k, block_tables, context_lens, causal, scale, window, sinks)
+        if result is not None:
+            return result
     _heads(q, "q")
     _masks(window, sinks)
     if not causal and (window or sinks):

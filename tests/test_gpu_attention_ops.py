@@ -413,3 +413,124 @@ def test_prompts_with_other_strides_and_off_alignment():
         out = torch.empty(heads, n, dim, dtype=dtype, device="cuda").transpose(0, 1)
         prompt_attention(*turned, starts, out=out)
         _close(out, want, bound)
+
+
+# ---- host paths, streams and graphs ----------------------------------------------------------------------------------------
+
+
+def _everything(seed, dtype, out=None):
+    """One call of every kind: the step of a batch of prompts and the step behind it."""
+    from nanovllm_voxcpm_amd.attention_ops import decode_attention, prompt_attention, rotary_table, rotate_qk
+
+    g = _gen(seed)
+    t, heads, kv_heads, dim, page = 93, 8, 2, 64, 16
+    q, k, v, weights, _ = _rotation(t, heads, kv_heads, dim, dtype, seed)
+    caches = [torch.zeros(12, page, kv_heads, dim, dtype=dtype, device="cuda") for _ in range(2)]
+    slots = torch.arange(t, dtype=torch.int32, device="cuda")
+    tables = torch.arange(12, dtype=torch.int32, device="cuda").view(2, 6)[:1].contiguous()
+    results = list(rotate_qk(q, k, slots, rotary_table(dim, 128).cuda(), q_weight=weights[0], k_weight=weights[1]))
+    turned, _ = rotate_qk(q, k, slots, rotary_table(dim, 128).cuda(), interleaved=True, v=v, k_cache=caches[0], v_cache=caches[1], slot_mapping=slots)
+    starts = _starts([40, t - 40]).cuda()
+    results += [turned, *caches, prompt_attention(turned, results[1], v, starts, window=30, sinks=2), prompt_attention(turned, results[1], v, starts, causal=False, scale=0.3),
+                prompt_attention(turned, *caches, _starts([t]).cuda(), block_tables=tables, context_lens=torch.tensor([t], dtype=torch.int32, device="cuda")),
+                decode_attention(turned[-1:], *caches, tables, torch.tensor([t], dtype=torch.int32, device="cuda"), sinks=3, window=50)]
+    return results
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_both_host_paths_make_the_same_calls(dtype, monkeypatch):
+    from nanovllm_voxcpm_amd import _hip
+
+    if _hip.load_fastcall() is None:
+        pytest.skip("the C++ host path is not built (make -C nanovllm-voxcpm_amd/csrc fastcall)")
+    quick = _everything(30, dtype)
+    monkeypatch.setenv("MLORA_NO_FASTCALL", "1")
+    _hip.reload_knobs()
+    assert _hip.load_fastcall() is None
+    slow = _everything(30, dtype)
+    assert len(quick) == len(slow) and all(torch.equal(a, b) for a, b in zip(quick, slow))
+
+
+def test_the_quick_host_path_leaves_what_it_does_not_know_to_the_other():
+    from nanovllm_voxcpm_amd.attention_ops import decode_attention, prompt_attention, rotate_qk
+
+    q, k = torch.zeros(3, 4, 64, device="cuda"), torch.zeros(3, 2, 64, device="cuda")
+    table = torch.zeros(4, 64, device="cuda")
+    positions = torch.zeros(3, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="differ"):
+        rotate_qk(q, k[:2], positions, table)
+    with pytest.raises(ValueError, match="positions lives on cpu"):
+        rotate_qk(q, k, positions.cpu(), table)
+    with pytest.raises(RuntimeError, match="no backward"):
+        rotate_qk(q.clone().requires_grad_(), k, positions, table)
+    with torch.no_grad():
+        rotate_qk(q.clone().requires_grad_(), k, positions, table)
+    with pytest.raises(RuntimeError, match="rotary = 24"):
+        rotate_qk(q, k, positions, table[:, :24])
+    with pytest.raises(ValueError, match="evenly"):
+        prompt_attention(q, k[:, :1].expand(3, 3, 64).contiguous(), k[:, :1].expand(3, 3, 64).contiguous(), positions)
+    cache = torch.zeros(2, 16, 2, 64, device="cuda")
+    with pytest.raises(ValueError, match="negative"):
+        decode_attention(q, cache, cache, torch.zeros(3, 1, dtype=torch.int32, device="cuda"), positions, window=-1)
+    with pytest.raises(ValueError, match="context_lens"):
+        decode_attention(q, cache, cache, torch.zeros(3, 1, dtype=torch.int32, device="cuda"), positions.long())
+    assert decode_attention(q[:0], cache, cache, torch.zeros(0, 1, dtype=torch.int32, device="cuda"), positions[:0]).shape == (0, 4, 64)
+    assert prompt_attention(q[:0], k[:0], k[:0], positions[:1]).shape == (0, 4, 64)
+    assert not decode_attention(q + 1, cache, cache, torch.zeros(3, 0, dtype=torch.int32, device="cuda"), positions + 5).any()  # a table without pages
+
+
+def test_calls_on_another_stream_and_two_at_once():
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    want = [[t.clone() for t in _everything(40 + i, torch.bfloat16)] for i in range(3)]
+    torch.cuda.synchronize()
+    got = []
+    for i, stream in enumerate(streams):
+        with torch.cuda.stream(stream):
+            got.append(_everything(40 + i, torch.bfloat16))
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("longest,dim", [(700, 64), (30000, 64), (9000, 128)])
+def test_graphs_of_decode_and_chunks_replayed(longest, dim):
+    """Two graphs, replayed in turn with eager work between the replays; lengths, pages and values change in place."""
+    from nanovllm_voxcpm_amd.attention_ops import decode_attention, prompt_attention, rotary_table, rotate_qk
+
+    g = _gen(50)
+    page, heads, kv_heads, sequences, chunk = 64, 8, 2, 3, 70
+    pages = -(-longest // page)
+    caches = [torch.randn(sequences * pages, page, kv_heads, dim, generator=g).to(torch.bfloat16).cuda() for _ in range(2)]
+    tables = torch.arange(sequences * pages, dtype=torch.int32, device="cuda").view(sequences, pages).contiguous()
+    lens = torch.tensor([longest, 5, longest // 2], dtype=torch.int32, device="cuda")
+    rows = torch.randn(sequences + chunk, heads + 2 * kv_heads, dim, generator=g).to(torch.bfloat16).cuda()
+    starts, chunk_lens = _starts([chunk]).cuda(), torch.tensor([longest], dtype=torch.int32, device="cuda")
+    slots = torch.full((sequences + chunk,), -1, dtype=torch.int32, device="cuda")
+    slots[:3] = torch.tensor([longest - 1, pages * page + 4, 2 * pages * page + longest // 2 - 1], dtype=torch.int32)
+    table = rotary_table(dim, 64).cuda()
+    positions = torch.zeros(sequences + chunk, dtype=torch.int32, device="cuda")
+
+    def step():
+        q, k, v = rows.split([heads, kv_heads, kv_heads], dim=1)
+        q, _ = rotate_qk(q, k, positions, table, v=v, k_cache=caches[0], v_cache=caches[1], slot_mapping=slots)
+        return [decode_attention(q[:sequences], *caches, tables, lens, window=0), decode_attention(q[:sequences], *caches, tables, lens, window=333, sinks=4),
+                prompt_attention(q[sequences:], *caches, starts, block_tables=tables, context_lens=chunk_lens)]
+
+    step()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            held = step()
+        graphs.append((graph, held))
+    for i in range(5):
+        rows.copy_(torch.randn(rows.shape, generator=g).to(torch.bfloat16))
+        positions.fill_(7 * i % 64)
+        lens.copy_(torch.tensor([longest - i, 5 + i, longest // 2 + 3 * i], dtype=torch.int32))
+        graph, held = graphs[i % 2]
+        graph.replay()
+        got = [t.clone() for t in held]
+        want = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
