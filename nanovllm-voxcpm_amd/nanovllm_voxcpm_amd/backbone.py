@@ -2,7 +2,8 @@
 
 Not a served model: random-init weights, plain torch for everything that is not LoRA (RMSNorm,
 rotary embedding, attention over a dense padded KV cache, SwiGLU), and this package's LoRA
-linears for the four stacked projections of every layer.  The shape follows the end-to-end
+linears for the four stacked projections of every layer.  ``forward_paged`` runs the same layers over a
+paged cache with this package's attention (``layers.attention``): prompts, chunks of them, and decode steps.  The shape follows the end-to-end
 benchmark configuration: 24 layers, hidden 1024, 16 query heads / 2 KV heads of 64, SwiGLU
 intermediate 4096, RMSNorm; decode streams with one new token each.
 """
@@ -13,6 +14,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
+from .layers.attention import AttentionBatch, PagedAttention
 from .layers.lora import LoRAMergedColumnParallelLinear, LoRAQKVParallelLinear, LoRARowParallelLinear
 
 
@@ -39,12 +41,13 @@ def _rotary(t: torch.Tensor, positions: torch.Tensor, base: float = 10000.0) -> 
 
 
 class DecoderLayer(nn.Module):
-    def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, inter: int, max_loras: int, rank: int):
+    def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, inter: int, max_loras: int, rank: int, **attention):
         super().__init__()
         self.heads, self.kv_heads, self.head_dim = heads, kv_heads, head_dim
         kw = dict(max_loras=max_loras, max_lora_rank=rank)
         self.input_norm = RMSNorm(hidden)
         self.qkv = LoRAQKVParallelLinear(hidden, head_dim, heads, kv_heads, **kw)
+        self.attention = PagedAttention(heads, kv_heads, head_dim, **attention)
         self.o = LoRARowParallelLinear(heads * head_dim, hidden, **kw)
         self.post_norm = RMSNorm(hidden)
         self.gate_up = LoRAMergedColumnParallelLinear(hidden, [inter, inter], **kw)
@@ -73,12 +76,22 @@ class DecoderLayer(nn.Module):
         return x + self.down(F.silu(gate) * up)
 
 
+    def forward_paged(self, x, k_cache, v_cache, batch: AttentionBatch):
+        """x [rows, hidden]; caches [blocks, block size, kv_heads, head_dim]."""
+        x = x + self.o(self.attention(self.qkv(self.input_norm(x)), k_cache, v_cache, batch))
+        gate, up = self.gate_up(self.post_norm(x)).chunk(2, dim=-1)
+        return x + self.down(F.silu(gate) * up)
+
+
 class MiniDecoder(nn.Module):
+    """``attention``: options of ``PagedAttention`` (norms of the heads, window, first tokens) that ``forward_paged`` has and
+    ``forward``, which knows none of them, has not."""
+
     def __init__(self, layers: int = 24, hidden: int = 1024, heads: int = 16, kv_heads: int = 2, head_dim: int = 64,
-                 inter: int = 4096, max_loras: int = 32, rank: int = 32):
+                 inter: int = 4096, max_loras: int = 32, rank: int = 32, **attention):
         super().__init__()
         self.hidden, self.kv_heads, self.head_dim = hidden, kv_heads, head_dim
-        self.layers = nn.ModuleList(DecoderLayer(hidden, heads, kv_heads, head_dim, inter, max_loras, rank) for _ in range(layers))
+        self.layers = nn.ModuleList(DecoderLayer(hidden, heads, kv_heads, head_dim, inter, max_loras, rank, **attention) for _ in range(layers))
         self.norm = RMSNorm(hidden)
 
     @torch.no_grad()
@@ -118,4 +131,17 @@ class MiniDecoder(nn.Module):
         mask = (torch.arange(s, device=x.device)[None, :] <= positions[:, None])[:, None, None, :]
         for layer, (k_cache, v_cache) in zip(self.layers, caches):
             x = layer(x, k_cache, v_cache, positions, mask)
+        return self.norm(x)
+
+    def make_paged_cache(self, blocks: int, block_size: int, dtype, device):
+        """Zeroed caches [layers][2] of shape [blocks, block_size, kv_heads, head_dim]; the layers share one rotary table."""
+        table = None
+        for layer in self.layers:
+            table = layer.attention.prepare(device, table)
+        shape = (blocks, block_size, self.kv_heads, self.head_dim)
+        return [(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)) for _ in self.layers]
+
+    def forward_paged(self, x, caches, batch: AttentionBatch):
+        for layer, (k_cache, v_cache) in zip(self.layers, caches):
+            x = layer.forward_paged(x, k_cache, v_cache, batch)
         return self.norm(x)
