@@ -1,6 +1,6 @@
 // Attention of packed prompts over packed or paged keys, head sizes 64 and 128 (mlora_prompt_attention).
 //
-// One workgroup per (128 query rows of a sequence, head): four wavefronts of 32 rows each.  Tiles of 64 keys and their values are
+// One workgroup per 128 rows of queries that share a key-value head: four wavefronts of 32 rows each, of one head or of two or four.  Tiles of 64 keys and their values are
 // staged in LDS by direct loads, two stages deep: one barrier a tile, behind which the next tile is asked for.  The scores come out of the first product with the
 // keys along the registers and the query rows along the lanes (K Q^T, 32 x 32 tiles), which is how the second one (V^T P^T) wants its
 // weights: they never leave the registers, a row's maximum and sum are a lane's own but for one exchange between the halves of the
@@ -71,6 +71,23 @@ __device__ __forceinline__ long long uniform(long long v) {
   return (static_cast<long long>(uniform(static_cast<int>(v >> 32))) << 32) | static_cast<uint32_t>(uniform(static_cast<int>(v)));
 }
 
+// A workgroup's four wavefronts take 32 rows of the same head each, or 1 << together heads of one key-value head with 128 >> together rows of each:
+// the same products either way, but rows that see the same keys, and few of them left over where sequences are short.  16 heads of 2: 16 prompts of 587
+// tokens 37.4 us against 40.5 with a head each, 64 sequences of 13 in fp32 15.7 against 26.7, two chunks of 2048 behind 28001 the same to a hundredth.
+__host__ __device__ constexpr int tile_rows(int together) { return kRows >> together; }
+__host__ __device__ constexpr int row_tiles(int rows, int together) { return rows > 0 ? (rows + tile_rows(together) - 1) >> (7 - together) : 0; }
+
+// Of lane l the sum of lanes 0 .. l, by moves between lanes (a trip through LDS for each of the six steps costs a short prompt a microsecond).
+__device__ __forceinline__ int upto_lane(int v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4 and 8 lanes below in its row of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // a row's last lane to all of rows 1 and 3
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // lane 31 to rows 2 and 3
+  return v;
+}
+
 struct RowTile {
   int sequence, start, rows;  // first query row (of q) and how many
   int position;               // of the first
@@ -78,44 +95,33 @@ struct RowTile {
 };
 
 // The item-th tile of the batch, the last of every batch first (the later rows of a prompt see the most keys).  By one wavefront.
-__device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int item, int lane, RowTile* t) {
+__device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int together, int item, int lane, RowTile* t) {
   int tiles = 0, begin = 0, end = 0;
-  for (int s = lane; s < a.sequences; s += 64) {
-    begin = clamped(a.starts[s], a.num_rows);
-    end = clamped(a.starts[s + 1], a.num_rows);
-    tiles += end > begin ? (end - begin + kRows - 1) / kRows : 0;
+  if (a.sequences > 64) {
+    for (int s = lane; s < a.sequences; s += 64) tiles += row_tiles(clamped(a.starts[s + 1], a.num_rows) - clamped(a.starts[s], a.num_rows), together);
+    tiles = __builtin_amdgcn_readlane(upto_lane(tiles), 63);
   }
-  for (int o = 32; o >= 1; o >>= 1) tiles += __shfl_xor(tiles, o, kWave);
-  if (item >= tiles) return false;
-  item = tiles - 1 - item;
   int before = 0;
   for (int base = 0; base < a.sequences; base += 64) {
     const int s = base + lane;
-    if (a.sequences > 64) {
-      begin = s < a.sequences ? clamped(a.starts[s], a.num_rows) : 0;
-      end = s < a.sequences ? clamped(a.starts[s + 1], a.num_rows) : 0;
-    } else if (s >= a.sequences) {
-      begin = end = 0;
-    }
-    const int mine = end > begin ? (end - begin + kRows - 1) / kRows : 0;
-    int upto = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int other = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += other;
-    }
-    const unsigned long long behind = __ballot(before + upto > item);
+    begin = s < a.sequences ? clamped(a.starts[s], a.num_rows) : 0;
+    end = s < a.sequences ? clamped(a.starts[s + 1], a.num_rows) : 0;
+    const int mine = row_tiles(end - begin, together), upto = upto_lane(mine);
+    if (a.sequences <= 64) tiles = __builtin_amdgcn_readlane(upto, 63);
+    if (item >= tiles) return false;
+    const unsigned long long behind = __ballot(before + upto > tiles - 1 - item);
     if (behind) {
       const int at = __builtin_ctzll(behind);
-      const int index = item - (before + __shfl(upto, at, kWave) - __shfl(mine, at, kWave));
-      const int first = __shfl(begin, at, kWave), last = __shfl(end, at, kWave);
+      const int index = tiles - 1 - item - (before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at));
+      const int first = __builtin_amdgcn_readlane(begin, at), last = __builtin_amdgcn_readlane(end, at);
       t->sequence = base + at;
-      t->start = first + index * kRows;
-      t->rows = last - t->start < kRows ? last - t->start : kRows;
+      t->start = first + index * tile_rows(together);
+      t->rows = last - t->start < tile_rows(together) ? last - t->start : tile_rows(together);
       t->total = keys_of(a, t->sequence, &t->key_start);
       t->position = t->total - (last - t->start);
       return true;
     }
-    before += __shfl(upto, 63, kWave);
+    before += __builtin_amdgcn_readlane(upto, 63);
   }
   return false;
 }
@@ -141,6 +147,7 @@ constexpr int kLeastShare = 32;  // tiles of keys: below it what is left and joi
 struct RowTiles {
   int begin, end, total, key_start, upto;  // of this lane's sequence; upto: tiles of rows up to its end
   int tiles;                               // of rows, all of them
+  int together;
   __device__ __forceinline__ RowTile tile(int r) const {  // r may differ from lane to lane
     int at = 0;  // the first sequence that ends behind r
 #pragma unroll
@@ -151,8 +158,8 @@ struct RowTiles {
     t.sequence = at;
     t.total = __shfl(total, at, kWave);
     t.key_start = __shfl(key_start, at, kWave);
-    t.start = first + (r - seq_upto + (last - first + kRows - 1) / kRows) * kRows;
-    t.rows = last - t.start < kRows ? last - t.start : kRows;
+    t.start = first + (r - seq_upto + row_tiles(last - first, together)) * tile_rows(together);
+    t.rows = last - t.start < tile_rows(together) ? last - t.start : tile_rows(together);
     t.position = t.total - (last - t.start);
     return t;
   }
@@ -160,25 +167,21 @@ struct RowTiles {
     const RowTile t = tile(r < tiles ? r : tiles - 1);
     return r < tiles ? KeyTiles(a, t.position, t.rows, t.total).count : 0;
   }
-  __device__ __forceinline__ RowTiles(const MloraAttentionArgs& a, int lane) {
+  __device__ __forceinline__ RowTiles(const MloraAttentionArgs& a, int heads_together, int lane) : together(heads_together) {
     begin = end = total = key_start = 0;
     if (lane < a.sequences) {
       begin = clamped(a.starts[lane], a.num_rows);
       end = clamped(a.starts[lane + 1], a.num_rows);
       total = keys_of(a, lane, &key_start);
     }
-    upto = end > begin ? (end - begin + kRows - 1) / kRows : 0;
-    for (int o = 1; o < 64; o <<= 1) {
-      const int other = __shfl_up(upto, o, kWave);
-      if (lane >= o) upto += other;
-    }
-    tiles = __shfl(upto, 63, kWave);
+    upto = upto_lane(row_tiles(end - begin, together));
+    tiles = __builtin_amdgcn_readlane(upto, 63);
   }
 };
 
 struct Shares : RowTiles {
   long long units, per;  // tiles of keys, all of them and a share's; per = 0: not shared out
-  __device__ __forceinline__ Shares(const MloraAttentionArgs& a, int shares, int lane) : RowTiles(a, lane) {
+  __device__ __forceinline__ Shares(const MloraAttentionArgs& a, int shares, int together, int lane) : RowTiles(a, together, lane) {
     units = per = 0;
     if (tiles == 0) return;
     for (int base = 0; base < tiles; base += 64) units += units_of(a, base + lane);
@@ -222,9 +225,10 @@ struct Unfinished {
 __host__ __device__ inline int64_t joints_bytes(int64_t tiles) { return 16 + tiles * static_cast<int64_t>(sizeof(Joint)); }
 __device__ __forceinline__ int32_t* shared_tiles(const MloraAttentionArgs& a) { return static_cast<int32_t*>(a.workspace); }
 __device__ __forceinline__ Joint* joint(const MloraAttentionArgs& a, int tile) { return reinterpret_cast<Joint*>(static_cast<char*>(a.workspace) + 16) + tile; }
-__device__ __forceinline__ Unfinished unfinished(const MloraAttentionArgs& a, int shares, int share, int place, int head, int dim) {
-  const int64_t at = (static_cast<int64_t>(share) * 2 + place) * a.heads + head, all = static_cast<int64_t>(shares) * 2 * a.heads;
-  float2* const sums = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + joints_bytes(a.num_rows / kRows + a.sequences));
+__device__ __forceinline__ Unfinished unfinished(const MloraAttentionArgs& a, int shares, int together, int share, int place, int rank, int dim) {
+  const int ranks = a.heads >> together;
+  const int64_t at = (static_cast<int64_t>(share) * 2 + place) * ranks + rank, all = static_cast<int64_t>(shares) * 2 * ranks;
+  float2* const sums = reinterpret_cast<float2*>(static_cast<char*>(a.workspace) + joints_bytes(a.num_rows / tile_rows(together) + a.sequences));
   return {sums + at * kRows, reinterpret_cast<float*>(sums + all * kRows) + at * kRows * dim};
 }
 
@@ -242,7 +246,7 @@ constexpr int per_unit(int row) { return row == 128 ? 3 : row == 256 ? 2 : 1; }
 constexpr int kPacked = 0, kWholePages = 1, kAnyPages = 2;
 
 template <typename T, int D, int kWhere>
-__global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_kernel(MloraAttentionArgs a, int shares) {
+__global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_kernel(MloraAttentionArgs a, int shares, int together) {
   using S = Shape<T, D>;
   constexpr int kSteps = S::kChunks / 2, kBlocks = D / 32;
   // fp16: weights are held 2^7 times as large, so that those of 2^-21 are still normal numbers and the largest (2^15) finite
@@ -252,15 +256,16 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int group = a.heads / a.kv_heads;
   // (workgroups of one key-value head go to the same XCDs: workgroup i runs on XCD i % 8)
-  const int item = blockIdx.x / a.heads, rank = blockIdx.x - item * a.heads;
-  const int kv_head = rank % a.kv_heads, head = kv_head * group + rank / a.kv_heads;
+  const int ranks = a.heads >> together, item = blockIdx.x / ranks, rank = blockIdx.x - item * ranks;
+  const int kv_head = rank % a.kv_heads, head = kv_head * group + ((rank / a.kv_heads) << together) + (wave & ((1 << together) - 1));
+  const int row_of_wave = 32 * (wave >> together);
   RowTile tile;
   bool shared = false;
   // Of a share: tiles of keys that are left of it, and the first of them in its tile of rows.
   int left = 0, from = 0, tile_number = 0;
   long long a_share = 0;
   if (shares) {
-    const Shares s(a, shares, lane);
+    const Shares s(a, shares, together, lane);
     const long long per = uniform(s.per), units = uniform(s.units), unit = item * per;
     if (blockIdx.x == 0 && threadIdx.x == 0) *shared_tiles(a) = per ? s.tiles : 0;
     if (per) {
@@ -273,9 +278,9 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
       left = static_cast<int>(unit + per < units ? per : units - unit);
     }
   }
-  if (!shared && !uniform(find_tile(a, item, lane, &tile))) return;
+  if (!shared && !uniform(find_tile(a, together, item, lane, &tile))) return;
   for (;;) {
-  if (shared) tile = RowTiles(a, lane).tile(tile_number);
+  if (shared) tile = RowTiles(a, together, lane).tile(tile_number);
   const int sequence = uniform(tile.sequence), start = uniform(tile.start), rows = uniform(tile.rows), position = uniform(tile.position);
   const int total = uniform(tile.total), key_begin = uniform(tile.key_start);
   const KeyTiles of_rows(a, position, rows, total);
@@ -284,11 +289,11 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   const int to = shared && left < of_rows.count - from ? from + left : of_rows.count;
 
   // This lane's query row; rows behind the last repeat it and are not written.
-  const int mine = 32 * wave + column;
+  const int mine = row_of_wave + column;
   const int row = start + (mine < rows ? mine : rows - 1);
   const int place = position + (mine < rows ? mine : rows - 1);
-  const int wave_rows = rows - 32 * wave < 32 ? rows - 32 * wave : 32;  // (may be negative)
-  const int wave_first = position + 32 * wave, wave_last = wave_first + wave_rows - 1;
+  const int wave_rows = rows - row_of_wave < 32 ? rows - row_of_wave : 32;  // (may be negative)
+  const int wave_first = position + row_of_wave, wave_last = wave_first + wave_rows - 1;
   const float scale = __builtin_fabsf(a.scale) * kLog2e;
 
   Pack8 query[kSteps];
@@ -419,10 +424,12 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
     const char* const k_tile = lds + stage_of(t);
     const char* const v_tile = k_tile + S::kBytes;
     f32x16 s[2];
+    const bool second = key0 + 32 <= seen_end;  // (fp32, where a block of 32 keys costs 2048 cycles for each product: 64 sequences of 13 tokens 13.9 us, 15.7 without)
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
 #pragma unroll
       for (int j = 0; j < 16; ++j) s[b][j] = 0.0f;
+      if (sizeof(T) == 4 && b == 1 && !second) continue;
 #pragma unroll
       for (int st = 0; st < kSteps; ++st) {
         Pack8 key;
@@ -467,6 +474,22 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
         for (int j = 0; j < 16; ++j) o[d][j] *= alpha;
     }
     const float base = (m == -__builtin_inff() ? 0.0f : m) - kShift;
+    // V^T of 16 keys, at head size 128 read one step ahead of its product: a transposing read takes some 400 cycles when every wavefront reads, and two
+    // wavefronts a SIMD hide less of it than three (16384 tokens of 32 heads 567 us against 586; at head size 64, 2 x 2048 tokens behind 28001, 574 against 568).
+    constexpr bool kAhead = D == 128;
+    union Piece { s16x4 part[2]; Pack8 all; };
+    Piece v[2][kBlocks];
+    auto read_v = [&](int step, Piece* to) {
+#pragma unroll
+      for (int d = 0; d < kBlocks; ++d)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int r = 16 * step + 8 * e + 4 * half + (i16 >> 2);
+          const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
+          to[d].part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(v_tile + r * S::kRow + 16 * S::v_place(r, chunk) + 8 * (i16 & 1)));
+        }
+    };
+    if constexpr (sizeof(T) == 2 && kAhead) read_v(0, v[0]);
 #pragma unroll
     for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -481,6 +504,8 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
         pack8<T>(one, ones);
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
+          if (!kAhead) read_v(2 * b + c, v[c]);
+          else if (2 * b + c < 3) read_v(2 * b + c + 1, v[1 - c]);
           float w8[8];
 #pragma unroll
           for (int j = 0; j < 8; ++j) w8[j] = s[b][8 * c + j];
@@ -488,18 +513,10 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
           pack8<T>(w8, weights);
           l = dot8<T>(weights, ones, l);  // (the rounded weights' sum is what the outputs are divided by)
 #pragma unroll
-          for (int d = 0; d < kBlocks; ++d) {
-            union { s16x4 part[2]; Pack8 all; } v;
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int r = 32 * b + 16 * c + 8 * e + 4 * half + (i16 >> 2);
-              const int chunk = 4 * d + 2 * ((lane >> 4) & 1) + ((i16 & 3) >> 1);
-              v.part[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsS16x4*)(v_tile + r * S::kRow + 16 * S::v_place(r, chunk) + 8 * (i16 & 1)));
-            }
-            o[d] = Mma32<T>::run(v.all, weights, o[d]);
-          }
+          for (int d = 0; d < kBlocks; ++d) o[d] = Mma32<T>::run(v[c][d].all, weights, o[d]);
         }
       } else {
+        if (b == 1 && !second) continue;
 #pragma unroll
         for (int j = 0; j < 16; ++j) {
           l += s[b][j];
@@ -522,19 +539,20 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   }
   // (the arguments once more from memory: held over the loop they would take the scalar registers that it needs)
   const MloraAttentionArgs& args = *arguments_again();
-  if (shared && head == 0 && from == 0 && threadIdx.x == 0) {
+  if (shared && rank == 0 && from == 0 && threadIdx.x == 0) {
     const long long behind = of_rows.count - left;  // tiles of keys in the shares behind this one
     const int parts = behind > 0 ? 1 + static_cast<int>((behind + a_share - 1) / a_share) : 1;
     *joint(args, tile_number) = {item, parts, sequence, start, rows, position, total, key_begin};
   }
   if (shared && to - from < of_rows.count) {  // for the join
-    const Unfinished u = unfinished(args, shares, item, from ? 0 : 1, head, D);
-    if (half == 0) u.sums[mine] = make_float2(m, l);
+    const Unfinished u = unfinished(args, shares, together, item, from ? 0 : 1, rank, D);
+    const int at = 32 * wave + column;
+    if (half == 0) u.sums[at] = make_float2(m, l);
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d)
 #pragma unroll
       for (int p = 0; p < 4; ++p)
-        *reinterpret_cast<f32x4*>(u.outputs + mine * D + 32 * d + 8 * p + 4 * half) = f32x4{o[d][4 * p], o[d][4 * p + 1], o[d][4 * p + 2], o[d][4 * p + 3]};
+        *reinterpret_cast<f32x4*>(u.outputs + at * D + 32 * d + 8 * p + 4 * half) = f32x4{o[d][4 * p], o[d][4 * p + 1], o[d][4 * p + 2], o[d][4 * p + 3]};
     __syncthreads();  // (the stages have been read)
   } else {
   // (also a row without a visible key, 0 / 0)
@@ -581,7 +599,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
     const int c = __builtin_ctzll(again);
     again &= again - 1;
     const Place at{sequence, total, key_begin, wave_first + c};
-    attend_row<T>(args, at, start + 32 * wave + c, head, lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
+    attend_row<T>(args, at, start + row_of_wave + c, head, lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
   }
   if (shared) __syncthreads();
   }
@@ -594,19 +612,21 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
 
 // Joins the parts of 32 rows of a tile that lies in several shares, eight rows a wavefront.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, int shares) {
+__global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, int shares, int together) {
   constexpr int kPer = D / 64, kOwn = 8;
   __shared__ float scratch[kWaves][MLORA_MAX_HEAD_DIM];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, head = blockIdx.y, number = blockIdx.x >> 2;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, rank = blockIdx.y, number = blockIdx.x >> 2;
   if (number >= *shared_tiles(a)) return;
   const Joint t = *joint(a, number);
-  const int first = 32 * (blockIdx.x & 3) + kOwn * wave;
+  const int of_wave = blockIdx.x & 3, group = a.heads / a.kv_heads;  // (the wavefront that had them)
+  const int head = rank % a.kv_heads * group + ((rank / a.kv_heads) << together) + (of_wave & ((1 << together) - 1));
+  const int first = 32 * (of_wave >> together) + kOwn * wave, first_left = 32 * of_wave + kOwn * wave;  // of the tile, of what was left
   if (t.parts < 2 || first >= t.rows) return;
-  const int own = first + (lane & (kOwn - 1));  // the row whose (m, l) this lane looks after
+  const int own = first_left + (lane & (kOwn - 1));  // the row whose (m, l) this lane looks after
   float most = -__builtin_inff(), sum = 0.0f, x[kOwn][kPer] = {};
-  for (int p = 0; p < t.parts; ++p) most = fmaxf(most, unfinished(a, shares, t.share + p, p ? 0 : 1, head, D).sums[own].x);
+  for (int p = 0; p < t.parts; ++p) most = fmaxf(most, unfinished(a, shares, together, t.share + p, p ? 0 : 1, rank, D).sums[own].x);
   for (int p = 0; p < t.parts; ++p) {
-    const Unfinished u = unfinished(a, shares, t.share + p, p ? 0 : 1, head, D);
+    const Unfinished u = unfinished(a, shares, together, t.share + p, p ? 0 : 1, rank, D);
     const float2 ml = u.sums[own];
     const float factor = ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
     sum += factor * ml.y;
@@ -614,7 +634,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, 
     for (int i = 0; i < kOwn; ++i) {
       const float f = __shfl(factor, i, kWave);
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) x[i][e] += f * u.outputs[(first + i) * D + 64 * e + lane];
+      for (int e = 0; e < kPer; ++e) x[i][e] += f * u.outputs[(first_left + i) * D + 64 * e + lane];
     }
   }
   unsigned again = 0;
@@ -642,32 +662,40 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, 
   }
 }
 
-// Shares of a head: as many workgroups as the chip holds at once.
+// At least four lists of shares are left, so that a list is not long for those who look for their place in it.
+int heads_together(const MloraAttentionArgs& a) {
+  const int group = a.heads / a.kv_heads;
+  if (group % 4 == 0 && a.heads >= 16) return 2;
+  return group % 2 == 0 && a.heads >= 8 ? 1 : 0;
+}
+
+// Shares of a list: as many workgroups as the chip holds at once.
 int shares_of(const MloraAttentionArgs& a) {
-  const int resident = 256 * per_unit(a.dim * (a.dtype == MLORA_DTYPE_F32 ? 4 : 2)) / a.heads;
+  const int resident = 256 * per_unit(a.dim * (a.dtype == MLORA_DTYPE_F32 ? 4 : 2)) / (a.heads >> heads_together(a));
   return resident > 1 ? resident : 1;
 }
 
 template <typename T, int D> int launch(const MloraAttentionArgs& a) {
   const int where = !a.block_tables ? kPacked : a.page % kKeys == 0 ? kWholePages : kAnyPages;
-  const long long items = a.num_rows / kRows + a.sequences;  // at most that many tiles of rows
+  const int together = heads_together(a);
+  const long long items = a.num_rows / tile_rows(together) + a.sequences;  // at most that many tiles of rows
   const int shares = prompt_workspace_bytes(&a) && a.workspace && a.workspace_bytes >= static_cast<int64_t>(prompt_workspace_bytes(&a)) ? shares_of(a) : 0;
-  const unsigned grid = static_cast<unsigned>((items > shares ? items : shares) * a.heads);
+  const unsigned grid = static_cast<unsigned>((items > shares ? items : shares) * (a.heads >> together));
   constexpr int kLds = Shape<T, D>::kLds;
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
   if (where == kPacked) {
     allow_lds<prompt_kernel<T, D, kPacked>>(kLds);
-    prompt_kernel<T, D, kPacked><<<grid, kWaves * 64, kLds, stream>>>(a, shares);
+    prompt_kernel<T, D, kPacked><<<grid, kWaves * 64, kLds, stream>>>(a, shares, together);
   } else if (where == kWholePages) {
     allow_lds<prompt_kernel<T, D, kWholePages>>(kLds);
-    prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a, shares);
+    prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a, shares, together);
   } else {
     allow_lds<prompt_kernel<T, D, kAnyPages>>(kLds);
-    prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a, shares);
+    prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a, shares, together);
   }
   const int rc = check_launch("mlora_prompt_attention");
   if (rc || !shares) return rc;
-  prompt_join_kernel<T, D><<<dim3(static_cast<unsigned>(4 * items), a.heads), 256, 0, stream>>>(a, shares);
+  prompt_join_kernel<T, D><<<dim3(static_cast<unsigned>(4 * items), a.heads >> together), 256, 0, stream>>>(a, shares, together);
   return check_launch("mlora_prompt_attention (join)");
 }
 
@@ -679,17 +707,18 @@ bool prompt_supported(const MloraAttentionArgs* a) {
   // a tile's rows are reached by 32-bit offsets from its first
   const int64_t most = INT32_MAX / (kKeys * 4);
   if (a->k_row < 0 || a->v_row < 0 || a->k_row > most || a->v_row > most) return false;
-  return (static_cast<int64_t>(a->num_rows / kRows) + a->sequences) * a->heads <= INT32_MAX;
+  const int together = heads_together(*a);
+  return (static_cast<int64_t>(a->num_rows / tile_rows(together)) + a->sequences) * (a->heads >> together) <= INT32_MAX;
 }
 
 // Scratch of the shares where the work may be shared out: few tiles of rows for the chip, and enough keys to share.
 size_t prompt_workspace_bytes(const MloraAttentionArgs* a) {
   if (!prompt_supported(a) || a->sequences > 64 || a->heads > 512) return 0;
-  const int64_t shares = shares_of(*a), tiles = a->num_rows / kRows + a->sequences;
+  const int64_t shares = shares_of(*a), tiles = a->num_rows / tile_rows(heads_together(*a)) + a->sequences;
   const int64_t keys = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys;
   // (keys that lie packed are mostly the rows' own: prompts by themselves, which seldom have enough of them)
   if (tiles >= (a->block_tables ? 2 : 1) * shares || keys <= kLeastShare * kKeys) return 0;
-  return static_cast<size_t>(joints_bytes(tiles) + shares * 2 * a->heads * kRows * (8 + 4 * a->dim));
+  return static_cast<size_t>(joints_bytes(tiles) + shares * 2 * (a->heads >> heads_together(*a)) * kRows * (8 + 4 * a->dim));
 }
 
 int launch_prompt(const MloraAttentionArgs* a) {

@@ -281,7 +281,8 @@ def test_decode_behind_the_first_4_gb_of_a_cache():
 
 
 @pytest.mark.parametrize("dtype,heads,kv_heads,dim,page", [(torch.bfloat16, 2, 1, 64, 64), (torch.float16, 16, 2, 64, 256), (torch.float16, 1, 1, 128, 16),
-                                                            (torch.float32, 4, 4, 64, 128), (torch.float32, 8, 1, 128, 0), (torch.bfloat16, 4, 2, 128, 0)])
+                                                            (torch.float32, 4, 4, 64, 128), (torch.float32, 8, 1, 128, 0), (torch.bfloat16, 4, 2, 128, 0), (torch.bfloat16, 12, 2, 64, 256),
+                                                            (torch.bfloat16, 16, 4, 128, 64)])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 20000, 5), (False, 0, 0)])
 def test_chunks_behind_long_caches(dtype, heads, kv_heads, dim, page, causal, window, sinks):
     """Few tiles of rows with many keys: their work is cut anywhere and joined.  Rows at the ends and borders of tiles are compared."""
@@ -326,7 +327,7 @@ def _starts(lens):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (2, 2, 128), (7, 1, 64), (2, 1, 96)])
+@pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (2, 2, 128), (7, 1, 64), (2, 1, 96), (16, 4, 64), (12, 2, 64), (16, 1, 128)])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 33, 0), (True, 70, 4), (True, 1, 130), (False, 0, 0)])
 def test_prompts_of_every_length(dtype, heads, kv_heads, dim, causal, window, sinks):
     from nanovllm_voxcpm_amd.attention_ops import prompt_attention
@@ -348,7 +349,7 @@ def test_prompts_of_every_length(dtype, heads, kv_heads, dim, causal, window, si
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (3, 1, 128, 256), (2, 2, 64, 48), (2, 1, 64, 9)])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (3, 1, 128, 256), (2, 2, 64, 48), (2, 1, 64, 9), (16, 4, 64, 64), (8, 4, 128, 16)])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 100, 3), (False, 0, 0)])
 def test_chunks_behind_cached_rows(dtype, heads, kv_heads, dim, page, causal, window, sinks):
     """New rows behind what is cached, a row without any, more rows than keys (the first of them see nothing)."""
@@ -370,6 +371,25 @@ def test_chunks_behind_cached_rows(dtype, heads, kv_heads, dim, page, causal, wi
         want, bound = oracle.attend(q[at], *dense[s], causal, window, sinks, dtype=dtype)
         _close(got[at], want, bound, ("pages", s))
         _close(other[at], want, bound, ("packed", s))
+
+
+@pytest.mark.parametrize("heads,kv_heads", [(2, 1), (16, 4)])
+@pytest.mark.parametrize("sequences", [63, 64, 65, 200])
+def test_many_short_prompts(sequences, heads, kv_heads):
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    print(sequences, heads, kv_heads, flush=True)
+    g = _gen(22)
+    lens = torch.randint(0, 40, (sequences,), generator=g).tolist()
+    lens[0], lens[-1], lens[sequences // 2] = 0, 33, 150
+    starts = _starts(lens)
+    q = (1.5 * torch.randn(sum(lens), heads, 64, generator=g)).to(torch.bfloat16)
+    k, v = (torch.randn(sum(lens), kv_heads, 64, generator=g).to(torch.bfloat16) for _ in range(2))
+    got = prompt_attention(q.cuda(), k.cuda(), v.cuda(), starts.cuda())
+    for s in range(sequences):
+        at = slice(int(starts[s]), int(starts[s + 1]))
+        want, bound = oracle.attend(q[at], k[at], v[at], True, dtype=torch.bfloat16)
+        _close(got[at], want, bound, (s, lens[s]))
 
 
 @pytest.mark.parametrize("dim", [64, 128, 96])
