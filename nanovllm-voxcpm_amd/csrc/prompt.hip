@@ -94,31 +94,62 @@ struct RowTile {
   int total, key_start;
 };
 
-// The item-th tile of the batch, the last of every batch first (the later rows of a prompt see the most keys).  By one wavefront.
-__device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int together, int item, int lane, RowTile* t) {
-  int tiles = 0, begin = 0, end = 0;
+// Tile `index` of sequence `s`, whose rows are first .. last - 1.
+__device__ __forceinline__ RowTile tile_of(const MloraAttentionArgs& a, int together, int s, int first, int last, int index) {
+  RowTile t;
+  t.sequence = s;
+  t.start = first + index * tile_rows(together);
+  t.rows = last - t.start < tile_rows(together) ? last - t.start : tile_rows(together);
+  t.total = keys_of(a, s, &t.key_start);
+  t.position = t.total - (last - t.start);
+  return t;
+}
+
+// The item-th tile of the batch, of which the chip holds `at_once` at a time.  By one wavefront.  The later rows of a prompt see the most keys: the last
+// first.  Of more tiles than start at once those with the largest indexes start first, whatever their sequence (up to 64 of them), so that the short ones fill
+// the gaps at the end: 16 prompts of 587 tokens 32.4 us, 35.0 in the order of the rows.
+__device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int together, int at_once, int item, int lane, RowTile* t) {
+  int begin = lane < a.sequences ? clamped(a.starts[lane], a.num_rows) : 0, end = lane < a.sequences ? clamped(a.starts[lane + 1], a.num_rows) : 0;
+  int mine = row_tiles(end - begin, together), upto = upto_lane(mine), tiles = __builtin_amdgcn_readlane(upto, 63);
   if (a.sequences > 64) {
-    for (int s = lane; s < a.sequences; s += 64) tiles += row_tiles(clamped(a.starts[s + 1], a.num_rows) - clamped(a.starts[s], a.num_rows), together);
-    tiles = __builtin_amdgcn_readlane(upto_lane(tiles), 63);
+    int all = mine;
+    for (int s = lane + 64; s < a.sequences; s += 64) all += row_tiles(clamped(a.starts[s + 1], a.num_rows) - clamped(a.starts[s], a.num_rows), together);
+    tiles = __builtin_amdgcn_readlane(upto_lane(all), 63);
   }
+  if (item >= tiles) return false;
+  if (tiles > at_once && a.sequences > 1 && a.sequences <= 64) {
+    // the largest index that more than `item` tiles reach: `reached` of them lie behind it
+    int index = 0, over = 1, reached = 0;
+    while (__any(mine > over)) over *= 2;
+    while (over - index > 1) {
+      const int middle = (index + over) >> 1, of_lane = mine > middle ? mine - middle : 0, count = __builtin_amdgcn_readlane(upto_lane(of_lane), 63);
+      if (count > item) {
+        index = middle;
+      } else {
+        over = middle;
+        reached = count;
+      }
+    }
+    const unsigned long long have = __ballot(mine > index);
+    const int rank = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(have >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(have), 0));
+    const int at = __builtin_ctzll(__ballot((have >> lane & 1) && rank == item - reached));
+    *t = tile_of(a, together, at, __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at), index);
+    return true;
+  }
+  item = tiles - 1 - item;
   int before = 0;
   for (int base = 0; base < a.sequences; base += 64) {
-    const int s = base + lane;
-    begin = s < a.sequences ? clamped(a.starts[s], a.num_rows) : 0;
-    end = s < a.sequences ? clamped(a.starts[s + 1], a.num_rows) : 0;
-    const int mine = row_tiles(end - begin, together), upto = upto_lane(mine);
-    if (a.sequences <= 64) tiles = __builtin_amdgcn_readlane(upto, 63);
-    if (item >= tiles) return false;
-    const unsigned long long behind = __ballot(before + upto > tiles - 1 - item);
+    if (base) {
+      const int s = base + lane;
+      begin = s < a.sequences ? clamped(a.starts[s], a.num_rows) : 0;
+      end = s < a.sequences ? clamped(a.starts[s + 1], a.num_rows) : 0;
+      mine = row_tiles(end - begin, together);
+      upto = upto_lane(mine);
+    }
+    const unsigned long long behind = __ballot(before + upto > item);
     if (behind) {
-      const int at = __builtin_ctzll(behind);
-      const int index = tiles - 1 - item - (before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at));
-      const int first = __builtin_amdgcn_readlane(begin, at), last = __builtin_amdgcn_readlane(end, at);
-      t->sequence = base + at;
-      t->start = first + index * tile_rows(together);
-      t->rows = last - t->start < tile_rows(together) ? last - t->start : tile_rows(together);
-      t->total = keys_of(a, t->sequence, &t->key_start);
-      t->position = t->total - (last - t->start);
+      const int at = __builtin_ctzll(behind), index = item - (before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at));
+      *t = tile_of(a, together, base + at, __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at), index);
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
@@ -278,7 +309,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
       left = static_cast<int>(unit + per < units ? per : units - unit);
     }
   }
-  if (!shared && !uniform(find_tile(a, together, item, lane, &tile))) return;
+  if (!shared && !uniform(find_tile(a, together, 256 * per_unit(sizeof(T) * D) / ranks, item, lane, &tile))) return;
   for (;;) {
   if (shared) tile = RowTiles(a, together, lane).tile(tile_number);
   const int sequence = uniform(tile.sequence), start = uniform(tile.start), rows = uniform(tile.rows), position = uniform(tile.position);

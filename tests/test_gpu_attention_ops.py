@@ -392,6 +392,31 @@ def test_many_short_prompts(sequences, heads, kv_heads):
         _close(got[at], want, bound, (s, lens[s]))
 
 
+@pytest.mark.parametrize("sequences,behind", [(40, 0), (2, 0), (64, 20)])
+def test_more_tiles_than_the_chip_holds_at_once(sequences, behind):
+    """They start in the order of what they cost; `behind`: keys of every sequence in front of its rows."""
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    print(sequences, behind, flush=True)
+    g = _gen(23)
+    heads, kv_heads, dim = 16, 4, 128
+    lens = torch.randint(0, 300 if sequences > 2 else 3000, (sequences,), generator=g).tolist()
+    lens[-1] = 2500 if sequences == 2 else 1
+    lens[sequences // 2] += 2048
+    totals = [n + behind for n in lens]
+    starts, key_starts = _starts(lens), _starts(totals)
+    assert sum((n + 31) // 32 for n in lens) > 128
+    q = (1.5 * torch.randn(sum(lens), heads, dim, generator=g)).to(torch.float16)
+    k, v = (torch.randn(sum(totals), kv_heads, dim, generator=g).to(torch.float16) for _ in range(2))
+    got = prompt_attention(q.cuda(), k.cuda(), v.cuda(), starts.cuda(), cu_seqlens_k=key_starts.cuda()).cpu()
+    assert torch.isfinite(got).all()
+    for s, n in enumerate(lens):
+        for i in sorted({0, 31, 32, 63, 64, 100, n // 2, n - 1} & set(range(n))):
+            row, keys = slice(int(starts[s]) + i, int(starts[s]) + i + 1), slice(int(key_starts[s]), int(key_starts[s]) + behind + i + 1)
+            want, bound = oracle.attend(q[row], k[keys], v[keys], False, dtype=torch.float16)
+            _close(got[row], want, bound, (s, n, i))
+
+
 @pytest.mark.parametrize("dim", [64, 128, 96])
 @pytest.mark.parametrize("dtype", DTYPES)
 def test_what_a_row_does_not_see_does_not_reach_it(dtype, dim):
