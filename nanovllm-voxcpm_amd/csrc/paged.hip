@@ -11,8 +11,8 @@
 // Few long sequences are split: the tiles of the whole batch are shared out in parts of one size, as many as fill the chip, whatever sequence
 // they belong to.  Workgroups find their part from context_lens alone.  A sequence of one part is written straight away; the others leave (m, l, o) per
 // head in the workspace, and a second launch joins them: o = sum o_i 2^(m_i - m) / sum l_i 2^(m_i - m), in the order of the parts.
-// 3 sequences of up to 131072 keys, 32 heads, 8 of 128, bf16: 231 us, 5.1 TB/s (a copy of that size 5.2); 208 sequences, window 1024, 16 heads,
-// 2 of 64: 23 us, 4.5 TB/s; 64 of up to 2048: 15.2 us, 2.3 TB/s (the longest sequence by itself takes 12 of them).
+// 3 sequences of up to 131072 keys, 32 heads, 8 of 128, bf16: 225 us, 5.3 TB/s (a large copy 5.2); 208 sequences, window 1024, 16 heads,
+// 2 of 64: 23 us, 4.5 TB/s; 64 of up to 2048: 13.3 us, 2.6 TB/s (bound by the trips to memory that the longest one's wavefronts make one behind the other).
 #include "attention.h"
 #include "common.h"
 #include "dma.h"
@@ -142,17 +142,16 @@ __device__ __forceinline__ Workspace workspace_of(const MloraAttentionArgs& a, i
   return w;
 }
 
-// `pages`: log2 of the page where it is a power of two of 8 rows or more and rows lie near enough for 32-bit offsets, else -1.
+// `group`: heads of a key-value head; `pages`: log2 of the page where it is a power of two of 8 rows or more and rows lie near enough for 32-bit offsets, else -1.
 template <typename T, int D, int W>
-__global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAttentionArgs a, int target, int pages) {
+__global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAttentionArgs a, int target, int pages, int group) {
   using S = Shape<T, D, W>;
   constexpr int kWaves = W, kStages = S::kStages;
   constexpr int kKeys = S::kKeys, kSteps = S::kChunks / 4, kBlocks = D / 16;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = a.heads / a.kv_heads, head_blocks = (group + kBlockHeads - 1) / kBlockHeads;
-  const int kv_head = blockIdx.y / head_blocks, head_block = blockIdx.y - kv_head * head_blocks;
+  const int kv_head = blockIdx.y, head_block = blockIdx.z;
   const int head_in_group = head_block * kBlockHeads + column;
   const bool real = head_in_group < group;
   const int head = kv_head * group + (real ? head_in_group : 0);
@@ -210,6 +209,13 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
     uint32_t masks[kStages];
     const int own_row = lane / S::kChunks, piece = lane % S::kChunks;
     const uint32_t k_from = own_row * static_cast<uint32_t>(a.k_row * sizeof(T)), v_from = own_row * static_cast<uint32_t>(a.v_row * sizeof(T));
+    uint32_t k_offset[S::kLoads], v_offset[S::kLoads];  // of a lane's pieces in a tile that lies in one page
+#pragma unroll
+    for (int i = 0; i < S::kLoads; ++i) {
+      const int r = i * S::kRowsPerLoad + own_row;
+      k_offset[i] = r * static_cast<uint32_t>(a.k_row * sizeof(T)) + 16 * S::k_place(r, piece);
+      v_offset[i] = r * static_cast<uint32_t>(a.v_row * sizeof(T)) + 16 * S::v_place(r, piece);
+    }
 
     // Asks for the rows of tile t.
     auto request = [&](int t, int stage) {
@@ -221,8 +227,19 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
       const unsigned long long wanted = ((last - page0 == 63 ? 0ull : 1ull << (last - page0 + 1)) - 1) << (page0 - batch);
       const uint32_t to_k = ring_at + stage * 2 * S::kBytes, to_v = to_k + S::kBytes;
       if (pages >= 0 && tiles.sees_all(t, key0) && (known & wanted) == wanted) {
-        // the rows of one load lie in one page
         masks[stage] = kKeys == 32 ? 0xffffffffu : 0xffffu;
+        if ((1 << pages) >= kKeys) {  // all rows lie in one page (an address each instead of one a load: 64 streams of up to 2048 keys 13.3 us, 15.2 before)
+          const int id = __builtin_amdgcn_readlane(ids, page0 - batch), in_page = key0 & ((1 << pages) - 1);
+          const char* const k = uniform(reinterpret_cast<const char*>(static_cast<const T*>(a.k) + id * a.k_block + in_page * a.k_row + kv_head * a.k_head));
+          const char* const v = uniform(reinterpret_cast<const char*>(static_cast<const T*>(a.v) + id * a.v_block + in_page * a.v_row + kv_head * a.v_head));
+#pragma unroll
+          for (int i = 0; i < S::kLoads; ++i) {
+            dma16_from(k, k_offset[i], to_k + i * 1024);
+            dma16_from(v, v_offset[i], to_v + i * 1024);
+          }
+          return;
+        }
+        // the rows of one load lie in one page
 #pragma unroll
         for (int i = 0; i < S::kLoads; ++i) {
           const int key = key0 + i * S::kRowsPerLoad, id = __builtin_amdgcn_readlane(ids, (key >> pages) - batch), in_page = key & ((1 << pages) - 1);
@@ -384,7 +401,7 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
   const int items = gridDim.x;
   const bool whole = part.parts == 1;
   const Workspace w = workspace_of(a, items);
-  if (target && threadIdx.x == 0 && blockIdx.y == 0 && index == 0) {
+  if (target && threadIdx.x == 0 && blockIdx.y == 0 && blockIdx.z == 0 && index == 0) {
     w.rows[2 * sequence] = blockIdx.x;
     w.rows[2 * sequence + 1] = part.parts;
   }
@@ -483,9 +500,8 @@ constexpr int wide(int dim) { return dim == 64 ? 16 : 8; }
 //   Many sequences and heads (or a window, which bounds what a sequence costs): a workgroup of four wavefronts each, no join.
 //   Few, and none longer than four tiles a wavefront of the wide workgroups: one of these each, no join.
 //   Else the batch's tiles are shared out in parts of four wavefronts and joined.
-// us by the device's clock, four wavefronts whole / wide workgroups / parts: 208 sequences, 2 heads of 64, window 1024: 23 / 28 / 31; 64 of up to 2048 keys, 2 heads
-// of 64: 20.5 / 15.2 / 17.0; one of 900: 12.0 / 10.1 / 9.8 (the call's second launch costs the host more than that); 3 of up to 131072, 8 heads
-// of 128: 2150 / 1440 / 224.
+// us by the device's clock, four wavefronts whole / wide workgroups / parts: 208 sequences, 2 heads of 64, window 1024: 23 / 27 / 40; 64 of up to 2048 keys, 2 heads
+// of 64: 17.1 / 13.3 / 16.5; one of 900: 10.3 / 8.2 / 10.1; 3 of up to 131072, 8 heads of 128: 1475 / 1400 / 224.
 struct Way {
   int waves, target;  // target: parts wanted, 0: none
 };
@@ -503,7 +519,8 @@ template <typename T, int D, int W> int launch(const MloraAttentionArgs& a, int 
   const int items = a.sequences + target;
   allow_lds<paged_kernel<T, D, W>>(S::kLds);
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
-  paged_kernel<T, D, W><<<dim3(items, units_of_part(a.heads, a.kv_heads)), W * 64, S::kLds, stream>>>(a, target, pages);
+  const int group = a.heads / a.kv_heads;
+  paged_kernel<T, D, W><<<dim3(items, a.kv_heads, (group + kBlockHeads - 1) / kBlockHeads), W * 64, S::kLds, stream>>>(a, target, pages, group);
   if (const int rc = check_launch("mlora_decode_attention")) return rc;
   if (!target) return 0;
   join_kernel<T, D><<<dim3(a.sequences, a.heads), 256, 0, stream>>>(a, items);
@@ -514,7 +531,7 @@ template <typename T, int D> int launch_shape(const MloraAttentionArgs& a) {
   Way cut = cut_of(a);
   if (!a.workspace || a.workspace_bytes < static_cast<int64_t>(paged_workspace_bytes(&a))) cut.target = 0;
   int pages = -1;
-  const int64_t most = INT32_MAX / (8 * 4);
+  const int64_t most = INT32_MAX / (32 * 4);
   if (a.page >= 8 && (a.page & (a.page - 1)) == 0 && a.k_row >= 0 && a.v_row >= 0 && a.k_row <= most && a.v_row <= most) pages = __builtin_ctz(a.page);
   return cut.waves == 4 ? launch<T, D, 4>(a, cut.target, pages) : launch<T, D, wide(D)>(a, cut.target, pages);
 }
