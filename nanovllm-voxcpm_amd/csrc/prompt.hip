@@ -7,8 +7,12 @@
 // wave, and V^T is read through the transposing LDS read.  The running maximum moves only when a tile's exceeds it by more than 2^8
 // (any base serves a softmax as long as its weights stay finite), so the outputs are hardly ever rescaled.
 //
-// Bound by the vector ALU at head size 64: a score costs a fused multiply-add (4 cycles for 64 of them), an exponential (16), parts of a maximum, a sum and a
-// conversion (4, 4 and 2), against 16 cycles of matrix core for its two products; at 128 by both alike.
+// Bound by the matrix cores and what stands between their two products.  At head size 64 a tile of 64 keys costs a wavefront 512 cycles of matrix core, 256 of
+// exponentials (32 of 8 cycles) and 250 of the other vector instructions (two cycles each where wavefronts share a SIMD); three wavefronts a SIMD overlap them, and the
+// matrix cores are busy for 45 % of the cycles.  The chip's power leaves it 1.5 to 1.8 GHz meanwhile.  Two chunks of 2048 behind 28001 keys, 16 heads of 64, fp16:
+// 557 us, 818 TFLOP/s (a plain product of 8192 x 8192 x 8192 1140); 16384 tokens, window 2048, 32 heads of 128, bf16: 552 us, 935 TFLOP/s (1180); 16 prompts of 587:
+// 32 us (1216 workgroups, 768 of them at once).  Slower were: eight wavefronts of two heads whose products and exponentials take turns
+// (727 us and 782 for the chunks and the window), halves of a tile with the next one's scores computed ahead (630 and 720), four wavefronts a SIMD (634 for the chunks).
 //
 // A row whose result is not finite is computed again by the kernel that never touches a hidden key (attend_row): 0 times NaN or infinity is what a product
 // over a tile makes of a hidden one's values.
@@ -105,10 +109,10 @@ __device__ __forceinline__ RowTile tile_of(const MloraAttentionArgs& a, int toge
   return t;
 }
 
-// The item-th tile of the batch, of which the chip holds `at_once` at a time.  By one wavefront.  The later rows of a prompt see the most keys: the last
+// The item-th tile of the batch, of which there are `ranks`, one a list of heads; the chip holds `at_once` of all of them at a time.  By one wavefront.  The later rows of a prompt see the most keys: the last
 // first.  Of more tiles than start at once those with the largest indexes start first, whatever their sequence (up to 64 of them), so that the short ones fill
 // the gaps at the end: 16 prompts of 587 tokens 32.4 us, 35.0 in the order of the rows.
-__device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int together, int at_once, int item, int lane, RowTile* t) {
+__device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int together, int ranks, int at_once, int item, int lane, RowTile* t) {
   int begin = lane < a.sequences ? clamped(a.starts[lane], a.num_rows) : 0, end = lane < a.sequences ? clamped(a.starts[lane + 1], a.num_rows) : 0;
   int mine = row_tiles(end - begin, together), upto = upto_lane(mine), tiles = __builtin_amdgcn_readlane(upto, 63);
   if (a.sequences > 64) {
@@ -117,7 +121,7 @@ __device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int toget
     tiles = __builtin_amdgcn_readlane(upto_lane(all), 63);
   }
   if (item >= tiles) return false;
-  if (tiles > at_once && a.sequences > 1 && a.sequences <= 64) {
+  if (static_cast<long long>(tiles) * ranks > at_once && a.sequences > 1 && a.sequences <= 64) {
     // the largest index that more than `item` tiles reach: `reached` of them lie behind it
     int index = 0, over = 1, reached = 0;
     while (__any(mine > over)) over *= 2;
@@ -273,11 +277,18 @@ __device__ __forceinline__ const MloraAttentionArgs* arguments_again() {
 // Workgroups that a compute unit holds at once, by the bytes of a head.
 constexpr int per_unit(int row) { return row == 128 ? 3 : row == 256 ? 2 : 1; }
 
+// What the host works out for the workgroups, which would divide for it one by one in front of their first load.
+struct Grid {
+  int shares, together, group;
+  uint32_t kv_heads_inverse;  // 2^31 / kv_heads rounded up: right for ranks up to 2^15
+};
+constexpr int kMostHeads = 1 << 15, kItemsPerPlane = 1 << 15;
+
 // Where keys lie: packed, in pages that hold whole tiles, in any pages.
 constexpr int kPacked = 0, kWholePages = 1, kAnyPages = 2;
 
 template <typename T, int D, int kWhere>
-__global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_kernel(MloraAttentionArgs a, int shares, int together) {
+__global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_kernel(MloraAttentionArgs a, Grid grid) {
   using S = Shape<T, D>;
   constexpr int kSteps = S::kChunks / 2, kBlocks = D / 32;
   // fp16: weights are held 2^7 times as large, so that those of 2^-21 are still normal numbers and the largest (2^15) finite
@@ -285,10 +296,11 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, column = lane & 31, half = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int group = a.heads / a.kv_heads;
+  const int shares = grid.shares, together = grid.together;
   // (workgroups of one key-value head go to the same XCDs: workgroup i runs on XCD i % 8)
-  const int ranks = a.heads >> together, item = blockIdx.x / ranks, rank = blockIdx.x - item * ranks;
-  const int kv_head = rank % a.kv_heads, head = kv_head * group + ((rank / a.kv_heads) << together) + (wave & ((1 << together) - 1));
+  const int ranks = gridDim.x, rank = blockIdx.x, item = blockIdx.y + kItemsPerPlane * blockIdx.z;
+  const int of_group = static_cast<int>(__umulhi(2u * rank, grid.kv_heads_inverse)), kv_head = rank - of_group * a.kv_heads;
+  const int head = kv_head * grid.group + (of_group << together) + (wave & ((1 << together) - 1));
   const int row_of_wave = 32 * (wave >> together);
   RowTile tile;
   bool shared = false;
@@ -298,7 +310,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   if (shares) {
     const Shares s(a, shares, together, lane);
     const long long per = uniform(s.per), units = uniform(s.units), unit = item * per;
-    if (blockIdx.x == 0 && threadIdx.x == 0) *shared_tiles(a) = per ? s.tiles : 0;
+    if (rank == 0 && item == 0 && threadIdx.x == 0) *shared_tiles(a) = per ? s.tiles : 0;
     if (per) {
       a_share = per;
       if (item >= shares || unit >= units) return;
@@ -309,7 +321,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
       left = static_cast<int>(unit + per < units ? per : units - unit);
     }
   }
-  if (!shared && !uniform(find_tile(a, together, 256 * per_unit(sizeof(T) * D) / ranks, item, lane, &tile))) return;
+  if (!shared && !uniform(find_tile(a, together, ranks, 256 * per_unit(sizeof(T) * D), item, lane, &tile))) return;
   for (;;) {
   if (shared) tile = RowTiles(a, together, lane).tile(tile_number);
   const int sequence = uniform(tile.sequence), start = uniform(tile.start), rows = uniform(tile.rows), position = uniform(tile.position);
@@ -711,18 +723,20 @@ template <typename T, int D> int launch(const MloraAttentionArgs& a) {
   const int together = heads_together(a);
   const long long items = a.num_rows / tile_rows(together) + a.sequences;  // at most that many tiles of rows
   const int shares = prompt_workspace_bytes(&a) && a.workspace && a.workspace_bytes >= static_cast<int64_t>(prompt_workspace_bytes(&a)) ? shares_of(a) : 0;
-  const unsigned grid = static_cast<unsigned>((items > shares ? items : shares) * (a.heads >> together));
+  const long long all = items > shares ? items : shares;
+  const dim3 grid(a.heads >> together, static_cast<unsigned>(all < kItemsPerPlane ? all : kItemsPerPlane), static_cast<unsigned>((all + kItemsPerPlane - 1) / kItemsPerPlane));
+  const Grid given{shares, together, a.heads / a.kv_heads, static_cast<uint32_t>(((1ll << 31) + a.kv_heads - 1) / a.kv_heads)};
   constexpr int kLds = Shape<T, D>::kLds;
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
   if (where == kPacked) {
     allow_lds<prompt_kernel<T, D, kPacked>>(kLds);
-    prompt_kernel<T, D, kPacked><<<grid, kWaves * 64, kLds, stream>>>(a, shares, together);
+    prompt_kernel<T, D, kPacked><<<grid, kWaves * 64, kLds, stream>>>(a, given);
   } else if (where == kWholePages) {
     allow_lds<prompt_kernel<T, D, kWholePages>>(kLds);
-    prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a, shares, together);
+    prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a, given);
   } else {
     allow_lds<prompt_kernel<T, D, kAnyPages>>(kLds);
-    prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a, shares, together);
+    prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a, given);
   }
   const int rc = check_launch("mlora_prompt_attention");
   if (rc || !shares) return rc;
@@ -738,8 +752,8 @@ bool prompt_supported(const MloraAttentionArgs* a) {
   // a tile's rows are reached by 32-bit offsets from its first
   const int64_t most = INT32_MAX / (kKeys * 4);
   if (a->k_row < 0 || a->v_row < 0 || a->k_row > most || a->v_row > most) return false;
-  const int together = heads_together(*a);
-  return (static_cast<int64_t>(a->num_rows / tile_rows(together)) + a->sequences) * (a->heads >> together) <= INT32_MAX;
+  const int64_t items = static_cast<int64_t>(a->num_rows / tile_rows(heads_together(*a))) + a->sequences;
+  return a->heads <= kMostHeads && items <= static_cast<int64_t>(kItemsPerPlane) * 65535 && 4 * items <= INT32_MAX;
 }
 
 // Scratch of the shares where the work may be shared out: few tiles of rows for the chip, and enough keys to share.

@@ -1,5 +1,5 @@
-// Norm, rotation and cache store of a batch's query, key and value heads (mlora_rotate_qk); stands where the reference runs its
-// rotary embedding and its store_kvcache_kernel (nanovllm_voxcpm/layers/rotary_embedding.py, layers/attention.py:10-50).
+// Norm, rotation and cache store of a batch's query, key and value heads (mlora_rotate_qk); stands where the reference turns them and
+// stores keys and values in its cache (nanovllm_voxcpm/layers/rotary_embedding.py, layers/attention.py:10-50).
 //
 // A head is W lanes of 16 bytes each (W = dim / 8, in fp32 dim / 4, up to the next power of two): its mean square is a butterfly over
 // those lanes, and what an element is paired with comes from the lane W / 2 on (or, in neighbouring pairs, from the lane itself).  With the weights taken into the

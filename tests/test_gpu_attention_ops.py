@@ -392,6 +392,19 @@ def test_many_short_prompts(sequences, heads, kv_heads):
         _close(got[at], want, bound, (s, lens[s]))
 
 
+def test_tens_of_thousands_of_prompts_of_a_token_or_none():
+    """A single token's output is its value."""
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    g = _gen(24)
+    lens = torch.randint(0, 2, (70000,), generator=g)
+    n = int(lens.sum())
+    starts = torch.cat([torch.zeros(1, dtype=torch.int64), lens.cumsum(0)]).to(torch.int32).cuda()
+    q, k, v = (torch.randn(n, h, 64, generator=g).to(torch.bfloat16).cuda() for h in (6, 3, 3))
+    got = prompt_attention(q, k, v, starts)
+    assert torch.equal(got, v.repeat_interleave(2, dim=1))
+
+
 @pytest.mark.parametrize("sequences,behind", [(40, 0), (2, 0), (64, 20)])
 def test_more_tiles_than_the_chip_holds_at_once(sequences, behind):
     """They start in the order of what they cost; `behind`: keys of every sequence in front of its rows."""
