@@ -11,7 +11,7 @@
 // exponentials (32 of 8 cycles) and 250 of the other vector instructions (two cycles each where wavefronts share a SIMD); three wavefronts a SIMD overlap them, and the
 // matrix cores are busy for 45 % of the cycles.  The chip's power leaves it 1.5 to 1.8 GHz meanwhile.  Two chunks of 2048 behind 28001 keys, 16 heads of 64, fp16:
 // 557 us, 818 TFLOP/s (a plain product of 8192 x 8192 x 8192 1140); 16384 tokens, window 2048, 32 heads of 128, bf16: 552 us, 935 TFLOP/s (1180); 16 prompts of 587:
-// 32 us (1216 workgroups, 768 of them at once).  Slower were: eight wavefronts of two heads whose products and exponentials take turns
+// 31 us (1216 workgroups, 768 of them at once).  Slower were: eight wavefronts of two heads whose products and exponentials take turns
 // (727 us and 782 for the chunks and the window), halves of a tile with the next one's scores computed ahead (630 and 720), four wavefronts a SIMD (634 for the chunks).
 //
 // A row whose result is not finite is computed again by the kernel that never touches a hidden key (attend_row): 0 times NaN or infinity is what a product
@@ -98,23 +98,35 @@ struct RowTile {
   int total, key_start;
 };
 
-// Tile `index` of sequence `s`, whose rows are first .. last - 1.
-__device__ __forceinline__ RowTile tile_of(const MloraAttentionArgs& a, int together, int s, int first, int last, int index) {
-  RowTile t;
-  t.sequence = s;
-  t.start = first + index * tile_rows(together);
-  t.rows = last - t.start < tile_rows(together) ? last - t.start : tile_rows(together);
-  t.total = keys_of(a, s, &t.key_start);
-  t.position = t.total - (last - t.start);
-  return t;
-}
+// A sequence of each lane: its rows begin .. end - 1 and its keys, in one trip to memory.
+struct Lengths {
+  int begin = 0, end = 0, total = 0, key_start = 0;
+  __device__ __forceinline__ Lengths(const MloraAttentionArgs& a, int s) {
+    if (s >= a.sequences) return;
+    begin = clamped(a.starts[s], a.num_rows);
+    end = clamped(a.starts[s + 1], a.num_rows);
+    total = keys_of(a, s, &key_start);
+  }
+  // Tile `index` of lane `at`'s sequence `s`.
+  __device__ __forceinline__ RowTile tile(int together, int at, int s, int index) const {
+    const int first = __builtin_amdgcn_readlane(begin, at), last = __builtin_amdgcn_readlane(end, at);
+    RowTile t;
+    t.sequence = s;
+    t.start = first + index * tile_rows(together);
+    t.rows = last - t.start < tile_rows(together) ? last - t.start : tile_rows(together);
+    t.total = __builtin_amdgcn_readlane(total, at);
+    t.key_start = __builtin_amdgcn_readlane(key_start, at);
+    t.position = t.total - (last - t.start);
+    return t;
+  }
+};
 
 // The item-th tile of the batch, of which there are `ranks`, one a list of heads; the chip holds `at_once` of all of them at a time.  By one wavefront.  The later rows of a prompt see the most keys: the last
 // first.  Of more tiles than start at once those with the largest indexes start first, whatever their sequence (up to 64 of them), so that the short ones fill
 // the gaps at the end: 16 prompts of 587 tokens 32.4 us, 35.0 in the order of the rows.
 __device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int together, int ranks, int at_once, int item, int lane, RowTile* t) {
-  int begin = lane < a.sequences ? clamped(a.starts[lane], a.num_rows) : 0, end = lane < a.sequences ? clamped(a.starts[lane + 1], a.num_rows) : 0;
-  int mine = row_tiles(end - begin, together), upto = upto_lane(mine), tiles = __builtin_amdgcn_readlane(upto, 63);
+  Lengths of(a, lane);
+  int mine = row_tiles(of.end - of.begin, together), upto = upto_lane(mine), tiles = __builtin_amdgcn_readlane(upto, 63);
   if (a.sequences > 64) {
     int all = mine;
     for (int s = lane + 64; s < a.sequences; s += 64) all += row_tiles(clamped(a.starts[s + 1], a.num_rows) - clamped(a.starts[s], a.num_rows), together);
@@ -137,23 +149,21 @@ __device__ __forceinline__ bool find_tile(const MloraAttentionArgs& a, int toget
     const unsigned long long have = __ballot(mine > index);
     const int rank = __builtin_amdgcn_mbcnt_hi(static_cast<uint32_t>(have >> 32), __builtin_amdgcn_mbcnt_lo(static_cast<uint32_t>(have), 0));
     const int at = __builtin_ctzll(__ballot((have >> lane & 1) && rank == item - reached));
-    *t = tile_of(a, together, at, __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at), index);
+    *t = of.tile(together, at, at, index);
     return true;
   }
   item = tiles - 1 - item;
   int before = 0;
   for (int base = 0; base < a.sequences; base += 64) {
     if (base) {
-      const int s = base + lane;
-      begin = s < a.sequences ? clamped(a.starts[s], a.num_rows) : 0;
-      end = s < a.sequences ? clamped(a.starts[s + 1], a.num_rows) : 0;
-      mine = row_tiles(end - begin, together);
+      of = Lengths(a, base + lane);
+      mine = row_tiles(of.end - of.begin, together);
       upto = upto_lane(mine);
     }
     const unsigned long long behind = __ballot(before + upto > item);
     if (behind) {
       const int at = __builtin_ctzll(behind), index = item - (before + __builtin_amdgcn_readlane(upto, at) - __builtin_amdgcn_readlane(mine, at));
-      *t = tile_of(a, together, base + at, __builtin_amdgcn_readlane(begin, at), __builtin_amdgcn_readlane(end, at), index);
+      *t = of.tile(together, at, base + at, index);
       return true;
     }
     before += __builtin_amdgcn_readlane(upto, 63);
