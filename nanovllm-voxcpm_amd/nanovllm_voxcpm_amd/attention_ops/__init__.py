@@ -92,6 +92,22 @@ def _memory(t: torch.Tensor) -> tuple[int, int]:
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
 
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two [rows, heads, head size] tensors share memory; those that are columns of one buffer, rows as far apart in both, may lie
+    between one another without."""
+    if not a.numel() or not b.numel():
+        return False
+    (a0, a1), (b0, b1) = _memory(a), _memory(b)
+    if a1 <= b0 or b1 <= a0:
+        return False
+    size, row = a.element_size(), a.stride(0)
+    if a.dim() != b.dim() or row != b.stride(0) or row <= 0 or (b0 - a0) % size:
+        return True
+    width = [1 + sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])) for t in (a, b)]
+    apart = (b0 - a0) // size % row
+    return not (width[0] <= apart and apart + width[1] <= row)
+
+
 def _rows_apart(t: torch.Tensor, name: str) -> None:
     """An output's elements must not lie on one another (an expanded view)."""
     if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
@@ -106,10 +122,8 @@ def _result(out: torch.Tensor | None, source: torch.Tensor, name: str) -> torch.
         raise ValueError(f"{name} has shape {tuple(out.shape)}, {tuple(source.shape)} is needed")
     _heads(out, name, source)
     _rows_apart(out, name)
-    if out.numel() and not (out.data_ptr() == source.data_ptr() and out.stride() == source.stride()):
-        (a, b), (c, d) = _memory(out), _memory(source)
-        if a < d and c < b and not (out.untyped_storage().data_ptr() == source.untyped_storage().data_ptr() and out.stride(0) == source.stride(0)):
-            raise ValueError(f"{name} overlaps its input")
+    if not (out.data_ptr() == source.data_ptr() and out.stride() == source.stride()) and _overlap(out, source):
+        raise ValueError(f"{name} overlaps its input")
     return out
 
 
@@ -183,6 +197,9 @@ def rotate_qk(
     q_out = _result(q_out, q, "q_out")
     if k_out is not None or not all(cached):
         k_out = _result(k_out, k, "k_out")
+    for out, name, others in ((q_out, "q_out", (k, v, k_out)), (k_out, "k_out", (q, v))):
+        if out is not None and any(t is not None and _overlap(out, t) for t in others):
+            raise ValueError(f"{name} overlaps another of the tensors")
     _hip.rotate_qk(q, k, v, q_out, k_out, k_cache, v_cache, positions, slot_mapping, cos_sin, q_weight, k_weight, float(eps), bool(interleaved))
     return q_out, k_out
 
@@ -202,17 +219,16 @@ def _table(block_tables: torch.Tensor, context_lens: torch.Tensor, sequences: in
     _index(context_lens, "context_lens", device, sequences)
 
 
-def _output(out: torch.Tensor | None, q: torch.Tensor) -> torch.Tensor:
+def _output(out: torch.Tensor | None, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor) -> torch.Tensor:
     if out is None:
         return torch.empty(q.shape, dtype=q.dtype, device=q.device)
     if out.shape != q.shape:
         raise ValueError(f"out has shape {tuple(out.shape)}, {tuple(q.shape)} is needed")
     _heads(out, "out", q)
     _rows_apart(out, "out")
-    if out.numel():
-        (a, b), (c, d) = _memory(out), _memory(q)
-        if a < d and c < b:
-            raise ValueError("out overlaps q")
+    for t, name in ((q, "q"), (k, "k"), (v, "v")):
+        if _overlap(out, t):
+            raise ValueError(f"out overlaps {name}")
     return out
 
 
@@ -252,7 +268,7 @@ def decode_attention(
     _shared_heads(q.size(1), k_cache.size(2))
     _masks(window, sinks)
     _table(block_tables, context_lens, q.size(0), q.device)
-    out = _output(out, q)
+    out = _output(out, q, k_cache, v_cache)
     _hip.decode_attention(q, out, k_cache, v_cache, block_tables, context_lens, q.size(2) ** -0.5 if scale is None else float(scale), window, sinks)
     return out
 
@@ -309,7 +325,7 @@ def prompt_attention(
         if cu_seqlens_k is not None:
             _index(cu_seqlens_k, "cu_seqlens_k", q.device, sequences + 1)
     _no_grad(q, k, v)
-    out = _output(out, q)
+    out = _output(out, q, k, v)
     _hip.prompt_attention(q, out, k, v, cu_seqlens, cu_seqlens_k, block_tables, context_lens, bool(causal),
                           q.size(2) ** -0.5 if scale is None else float(scale), window, sinks)
     return out

@@ -148,6 +148,33 @@ def test_outputs_may_not_overlap_their_inputs():
         decode_attention(**_decode(q=memory[:3], out=memory[:3]))
 
 
+def _refused(call, arguments, text):
+    """A call that passes its checks ends at the missing GPU."""
+    with pytest.raises(ValueError if text else RuntimeError, match=text or "GPU"):
+        call(**arguments)
+
+
+def test_results_may_lie_between_their_inputs_but_not_on_them():
+    qkv = torch.zeros(5, 8, 64)
+    q, k, v = qkv.split([4, 2, 2], dim=1)
+    rotation = _rotation(q=q, k=k)
+    _refused(rotate_qk, {**rotation, "q_out": q, "k_out": k}, None)
+    _refused(rotate_qk, {**rotation, "q_out": q, "k_out": v}, None)  # (v takes no part in a call without a cache)
+    _refused(rotate_qk, {**rotation, "q_out": qkv[:, 1:5]}, "q_out overlaps")
+    _refused(rotate_qk, {**rotation, "k_out": qkv[:, 5:7]}, "k_out overlaps")
+    _refused(rotate_qk, {**rotation, "k_out": q[:, 2:]}, "k_out overlaps another")
+    _refused(rotate_qk, {**rotation, "q_out": qkv[:, 4:]}, "q_out overlaps another")
+    room = torch.zeros(5, 4, 64)
+    _refused(rotate_qk, {**rotation, "q_out": room, "k_out": room[:, 1:3]}, "q_out overlaps another")
+    _refused(rotate_qk, {**_rotation(cached=True, q=q, k=k, v=v), "k_out": v}, "k_out overlaps another")
+    wide = torch.zeros(7, 10, 64)
+    for out, text in ((wide[:, 6:], None), (wide[:, 5:9], "out overlaps v"), (wide[:, :4], "out overlaps k")):
+        _refused(prompt_attention, _prompt(k=wide[:, 2:4], v=wide[:, 4:6], out=out), text)
+    _refused(prompt_attention, _prompt(q=torch.zeros(7, 2, 64), k=wide[:, 2:4], v=wide[:, 4:6], out=wide[:, 4:6]), "out overlaps v")
+    pages = torch.zeros(5, 16, 2, 64)
+    _refused(decode_attention, _decode(k_cache=pages, out=pages.view(-1, 4, 64)[6:9]), "out overlaps k")
+
+
 def _prompt(**change):
     return {**dict(q=torch.zeros(7, 4, 64), k=torch.zeros(7, 2, 64), v=torch.zeros(7, 2, 64), cu_seqlens=torch.tensor([0, 3, 7], dtype=torch.int32)), **change}
 
