@@ -233,7 +233,8 @@ struct Shares : RowTiles {
     for (int o = 32; o >= 1; o >>= 1) units += __shfl_xor(units, o, kWave);
     per = (units + shares - 1) / shares;
     if (per < kLeastShare) per = units > static_cast<long long>(kLeastShare) * tiles ? kLeastShare : 0;
-    if (tiles >= 4 * shares) per = 0;
+    // (more tiles than the workspace has places for: starts that run backwards, whose sequences lie on one another)
+    if (tiles >= 4 * shares || tiles > a.num_rows / tile_rows(together) + a.sequences) per = 0;
   }
   // The tile of rows that holds `unit` and the unit that it starts with.
   __device__ __forceinline__ int find(const MloraAttentionArgs& a, long long unit, int lane, long long* first) const {

@@ -289,6 +289,7 @@ def prompt_attention(
     out: torch.Tensor | None = None,
 ) -> torch.Tensor:
     """Attention of packed sequences: rows ``cu_seqlens[s] : cu_seqlens[s + 1]`` of ``q [T, heads, D]`` are the last rows of sequence s.
+    (Starts that decrease are read as they are: nothing outside the tensors is touched, but not every row need be written.)
 
     Keys and values lie packed, ``k``, ``v [rows, kv_heads, D]`` with sequence s at ``cu_seqlens_k[s] : cu_seqlens_k[s + 1]`` (``cu_seqlens`` by
     default), or, with ``block_tables`` and ``context_lens``, in the pages of a cache, ``[blocks, rows of a block, kv_heads, D]``, as in

@@ -392,6 +392,23 @@ def test_many_short_prompts(sequences, heads, kv_heads):
         _close(got[at], want, bound, (s, lens[s]))
 
 
+def test_starts_that_run_backwards_stay_inside_the_workspace():
+    """Sequences that lie on one another, 3 x 94 tiles of 32 rows where the rows make room for 98.  The launch has places for 192 of them and takes the last
+    of each sequence first: the rows of tiles 30 to 93, whose answer is one since all three sequences have the same keys."""
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    g, n, total, page = _gen(25), 3000, 6000, 64
+    dense, k, v, table = _paged([total], 2, 64, page, torch.bfloat16, g)
+    q = (1.5 * torch.randn(n, 16, 64, generator=g)).to(torch.bfloat16)
+    starts = torch.tensor([0, n, 0, n, 0, n], dtype=torch.int32, device="cuda")
+    lens = torch.full((5,), total, dtype=torch.int32, device="cuda")
+    got = prompt_attention(q.cuda(), k, v, starts, block_tables=table.cuda().expand(5, -1).contiguous(), context_lens=lens)
+    for i in (960, 991, 992, 1500, n - 1):
+        upto = total - n + i + 1
+        want, bound = oracle.attend(q[i : i + 1], dense[0][0][:upto], dense[0][1][:upto], False, dtype=torch.bfloat16)
+        _close(got[i : i + 1], want, bound, i)
+
+
 def test_tens_of_thousands_of_prompts_of_a_token_or_none():
     """A single token's output is its value."""
     from nanovllm_voxcpm_amd.attention_ops import prompt_attention
