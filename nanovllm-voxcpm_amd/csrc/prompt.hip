@@ -186,7 +186,15 @@ struct KeyTiles {
 // Few tiles of rows with many keys (a chunk of a prompt behind a long cache) leave compute units idle, or busy for a second round that few take part
 // in.  Their work is then one list: the tiles of keys of the first tile of rows, of the second and so on.  Every workgroup takes an equal share of the list, whatever rows it falls on.
 // A tile of rows that lies in several shares is joined by a second launch from what each of them left in the workspace.
-constexpr int kLeastShare = 32;  // tiles of keys: below it what is left and joined costs more than the balance gives
+// A share is 32 tiles of keys at least: below it what is left and joined costs more than the balance gives.  Where so few tiles of rows are there that they leave most compute
+// units idle, shares go down to `least`, if the longest tile of rows is longer than that by what the second launch costs (`join`): in 16 bits a tile of keys takes
+// two thirds of a microsecond, in fp32 four to eight.  16 tokens of 4 prompts behind 2000 each 28 us (51 with shares of 32), 173 in fp32 behind 8450, 8 heads of 128, 83 (288);
+// 2000 tokens by themselves would take 44, without shares 35.
+constexpr int kLeastShare = 32;
+struct ShareCosts {
+  int few, least, join;  // few: workgroups without shares
+};
+__host__ __device__ constexpr ShareCosts share_costs(int dtype) { return dtype == MLORA_DTYPE_F32 ? ShareCosts{512, 2, 4} : ShareCosts{128, 8, 16}; }
 
 // The tiles of rows of a batch of at most 64 sequences, one a lane.
 struct RowTiles {
@@ -208,9 +216,11 @@ struct RowTiles {
     t.position = t.total - (last - t.start);
     return t;
   }
+  // (rows without a key count for one, so that somebody comes by and writes them)
   __device__ __forceinline__ long long units_of(const MloraAttentionArgs& a, int r) const {
     const RowTile t = tile(r < tiles ? r : tiles - 1);
-    return r < tiles ? KeyTiles(a, t.position, t.rows, t.total).count : 0;
+    const int count = KeyTiles(a, t.position, t.rows, t.total).count;
+    return r >= tiles ? 0 : count > 0 ? count : 1;
   }
   __device__ __forceinline__ RowTiles(const MloraAttentionArgs& a, int heads_together, int lane) : together(heads_together) {
     begin = end = total = key_start = 0;
@@ -226,13 +236,28 @@ struct RowTiles {
 
 struct Shares : RowTiles {
   long long units, per;  // tiles of keys, all of them and a share's; per = 0: not shared out
-  __device__ __forceinline__ Shares(const MloraAttentionArgs& a, int shares, int together, int lane) : RowTiles(a, together, lane) {
+  __device__ __forceinline__ Shares(const MloraAttentionArgs& a, int shares, int together, int ranks, int lane) : RowTiles(a, together, lane) {
     units = per = 0;
     if (tiles == 0) return;
-    for (int base = 0; base < tiles; base += 64) units += units_of(a, base + lane);
-    for (int o = 32; o >= 1; o >>= 1) units += __shfl_xor(units, o, kWave);
+    int longest = 0;
+    for (int base = 0; base < tiles; base += 64) {
+      const int mine = static_cast<int>(units_of(a, base + lane));
+      units += mine;
+      longest = mine > longest ? mine : longest;
+    }
+    for (int o = 32; o >= 1; o >>= 1) {
+      units += __shfl_xor(units, o, kWave);
+      const int other = __shfl_xor(longest, o, kWave);
+      longest = other > longest ? other : longest;
+    }
     per = (units + shares - 1) / shares;
-    if (per < kLeastShare) per = units > static_cast<long long>(kLeastShare) * tiles ? kLeastShare : 0;
+    const ShareCosts costs = share_costs(a.dtype);
+    if (static_cast<long long>(tiles) * ranks <= costs.few) {
+      if (per < costs.least) per = costs.least;
+      if (longest < per + costs.join) per = 0;
+    } else if (per < kLeastShare) {
+      per = units > static_cast<long long>(kLeastShare) * tiles ? kLeastShare : 0;
+    }
     // (more tiles than the workspace has places for: starts that run backwards, whose sequences lie on one another)
     if (tiles >= 4 * shares || tiles > a.num_rows / tile_rows(together) + a.sequences) per = 0;
   }
@@ -319,7 +344,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   int left = 0, from = 0, tile_number = 0;
   long long a_share = 0;
   if (shares) {
-    const Shares s(a, shares, together, lane);
+    const Shares s(a, shares, together, ranks, lane);
     const long long per = uniform(s.per), units = uniform(s.units), unit = item * per;
     if (rank == 0 && item == 0 && threadIdx.x == 0) *shared_tiles(a) = per ? s.tiles : 0;
     if (per) {
@@ -657,7 +682,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   }
   if (shared) __syncthreads();
   }
-  left -= to - from;
+  left -= of_rows.count ? to - from : 1;
   if (!shared || left <= 0) return;
   from = 0;
   ++tile_number;
@@ -678,17 +703,32 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, 
   if (t.parts < 2 || first >= t.rows) return;
   const int own = first_left + (lane & (kOwn - 1));  // the row whose (m, l) this lane looks after
   float most = -__builtin_inff(), sum = 0.0f, x[kOwn][kPer] = {};
+#pragma unroll 4
   for (int p = 0; p < t.parts; ++p) most = fmaxf(most, unfinished(a, shares, together, t.share + p, p ? 0 : 1, rank, D).sums[own].x);
-  for (int p = 0; p < t.parts; ++p) {
-    const Unfinished u = unfinished(a, shares, together, t.share + p, p ? 0 : 1, rank, D);
-    const float2 ml = u.sums[own];
-    const float factor = ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
-    sum += factor * ml.y;
+  constexpr int kAtOnce = 4;  // parts whose outputs are on their way together
+  for (int base = 0; base < t.parts; base += kAtOnce) {
+    float factor[kAtOnce], v[kAtOnce][kOwn][kPer];
 #pragma unroll
-    for (int i = 0; i < kOwn; ++i) {
-      const float f = __shfl(factor, i, kWave);
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int p = base + j < t.parts ? base + j : t.parts - 1;
+      const Unfinished u = unfinished(a, shares, together, t.share + p, p ? 0 : 1, rank, D);
+      const float2 ml = u.sums[own];
+      factor[j] = base + j >= t.parts ? 0.0f : ml.x == most ? 1.0f : __builtin_amdgcn_exp2f(ml.x - most);
+      sum += base + j >= t.parts ? 0.0f : factor[j] * ml.y;
 #pragma unroll
-      for (int e = 0; e < kPer; ++e) x[i][e] += f * u.outputs[(first_left + i) * D + 64 * e + lane];
+      for (int i = 0; i < kOwn; ++i)
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) v[j][i][e] = u.outputs[(first_left + i) * D + 64 * e + lane];
+    }
+#pragma unroll
+    for (int j = 0; j < kAtOnce; ++j) {
+      if (base + j >= t.parts) break;
+#pragma unroll
+      for (int i = 0; i < kOwn; ++i) {
+        const float f = __shfl(factor[j], i, kWave);
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) x[i][e] += f * v[j][i][e];
+      }
     }
   }
   unsigned again = 0;
@@ -770,10 +810,14 @@ bool prompt_supported(const MloraAttentionArgs* a) {
 // Scratch of the shares where the work may be shared out: few tiles of rows for the chip, and enough keys to share.
 size_t prompt_workspace_bytes(const MloraAttentionArgs* a) {
   if (!prompt_supported(a) || a->sequences > 64 || a->heads > 512) return 0;
+  const ShareCosts costs = share_costs(a->dtype);
   const int64_t shares = shares_of(*a), tiles = a->num_rows / tile_rows(heads_together(*a)) + a->sequences;
-  const int64_t keys = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys;
-  // (keys that lie packed are mostly the rows' own: prompts by themselves, which seldom have enough of them)
-  if (tiles >= (a->block_tables ? 2 : 1) * shares || keys <= kLeastShare * kKeys) return 0;
+  // As the device will decide, with the longest that a sequence may be, or of packed keys the average (the rows of a prompt by itself see half of its keys each): the
+  // launch that joins costs one also where it finds nothing to do.
+  const int64_t keys = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys / a->sequences;
+  const bool by_itself = !a->block_tables && !a->key_starts && a->causal;
+  const int64_t least = tiles * (a->heads >> heads_together(*a)) <= costs.few ? costs.least + costs.join : by_itself ? 2 * kLeastShare : kLeastShare;
+  if (tiles >= (a->block_tables ? 2 : 1) * shares || keys <= least * kKeys) return 0;
   return static_cast<size_t>(joints_bytes(tiles) + shares * 2 * (a->heads >> heads_together(*a)) * kRows * (8 + 4 * a->dim));
 }
 

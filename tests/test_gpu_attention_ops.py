@@ -326,6 +326,31 @@ def _starts(lens):
     return torch.tensor([0, *torch.tensor(lens).cumsum(0).tolist()], dtype=torch.int32)
 
 
+@pytest.mark.parametrize("dtype,heads,kv_heads,dim", [(torch.bfloat16, 16, 2, 64), (torch.float16, 2, 1, 128), (torch.float32, 2, 2, 64)])
+@pytest.mark.parametrize("totals", [[0, 30000, 0, 0, 28000, 0], [0, 0, 33000], [25000, 0]])
+def test_rows_without_keys_among_long_caches(dtype, heads, kv_heads, dim, totals):
+    """They have no part in the list of tiles of keys that is shared out, and are written all the same."""
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    print(dtype, heads, kv_heads, dim, totals, flush=True)
+    g = _gen(26)
+    new = [70 + 5 * s for s in range(len(totals))]
+    dense, k, v, table = _paged(totals, kv_heads, dim, 64, dtype, g, spare=0)
+    q = (1.5 * torch.randn(sum(new), heads, dim, generator=g)).to(dtype)
+    out = torch.full(q.shape, 7.0, dtype=dtype, device="cuda")
+    prompt_attention(q.cuda(), k, v, _starts(new).cuda(), block_tables=table.cuda(), context_lens=torch.tensor(totals, dtype=torch.int32, device="cuda"), out=out)
+    at = 0
+    for s, n in enumerate(new):
+        if totals[s] == 0:
+            assert not out[at : at + n].any(), s
+        else:
+            for i in (0, 31, 32, n - 1):
+                upto = totals[s] - n + i + 1
+                want, bound = oracle.attend(q[at + i : at + i + 1], dense[s][0][:upto], dense[s][1][:upto], False, dtype=dtype)
+                _close(out[at + i : at + i + 1], want, bound, (s, i))
+        at += n
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim", [(4, 2, 64), (2, 2, 128), (7, 1, 64), (2, 1, 96), (16, 4, 64), (12, 2, 64), (16, 1, 128)])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 33, 0), (True, 70, 4), (True, 1, 130), (False, 0, 0)])
