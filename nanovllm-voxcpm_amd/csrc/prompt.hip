@@ -317,11 +317,14 @@ constexpr int per_unit(int row) { return row == 128 ? 3 : row == 256 ? 2 : 1; }
 struct Grid {
   int shares, together, group;
   uint32_t kv_heads_inverse;  // 2^31 / kv_heads rounded up: right for ranks up to 2^15
+  uint32_t page_inverse;      // 2^(31 + page_shift) / page rounded up, 2^page_shift <= page: key / page is (2 key page_inverse >> 32) >> page_shift for keys up to 2^29
+  int page_shift;
 };
 constexpr int kMostHeads = 1 << 15, kItemsPerPlane = 1 << 15;
 
-// Where keys lie: packed, in pages that hold whole tiles, in any pages.
-constexpr int kPacked = 0, kWholePages = 1, kAnyPages = 2;
+// Where keys lie: packed, in pages that hold whole tiles, in pages that hold the rows of whole loads (two chunks of 2048 behind 28001 keys in pages of 16: 613 us,
+// 663 as in any pages, 575 in pages of 256 on the same machine), in any pages.
+constexpr int kPacked = 0, kWholePages = 1, kLoadPages = 2, kAnyPages = 3;
 
 template <typename T, int D, int kWhere>
 __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_kernel(MloraAttentionArgs a, Grid grid) {
@@ -397,6 +400,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   const uint32_t ring_at = __builtin_amdgcn_readfirstlane(lds_address(lds));
   const int32_t* table = a.block_tables + (kWhere == kPacked ? 0 : sequence * a.table_row);
   int batch = -64, ids = 0;  // page ids batch .. batch + 63, one a lane
+  unsigned long long known_pages = 0;  // which of them are pages of the cache
   int page = 0, in_page = 0;
   auto key_of = [&](int t) { return t < first_tiles ? t * kKeys : low + (t - first_tiles) * kKeys; };
   auto stage_of = [&](int t) { return (t & 1) * 2 * S::kBytes; };
@@ -407,8 +411,9 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
 #pragma unroll
   for (int i = 0; i < S::kLoads; ++i) {
     const int r = (wave * S::kLoads + i) * S::kRowsPerLoad + lane / S::kChunks, piece = lane % S::kChunks;
-    k_offset[i] = r * k_row + 16 * S::k_place(r, piece);
-    v_offset[i] = r * v_row + 16 * S::v_place(r, piece);
+    const int from_base = kWhere == kLoadPages ? lane / S::kChunks : r;
+    k_offset[i] = from_base * k_row + 16 * S::k_place(r, piece);
+    v_offset[i] = from_base * v_row + 16 * S::v_place(r, piece);
   }
 
   // Asks for this wavefront's quarter of tile t; returns which of the tile's keys there are.
@@ -416,7 +421,30 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
     const int key0 = key_of(t), there = high - key0 < kKeys ? high - key0 : kKeys;
     unsigned long long valid = there == kKeys ? ~0ull : (1ull << there) - 1;
     const uint32_t k_to = ring_at + stage_of(t) + wave * S::kLoads * 1024, v_to = k_to + S::kBytes;
-    if constexpr (kWhere != kAnyPages) {
+    if constexpr (kWhere == kLoadPages) {
+      auto page_of = [&](int key) { return static_cast<int>(__umulhi(2u * static_cast<uint32_t>(key), grid.page_inverse) >> grid.page_shift); };
+      const int first = page_of(key0), last = page_of(key0 + there - 1);
+      if (first < batch || last >= batch + 64) {
+        batch = first;
+        const int p = batch + lane;
+        ids = table[p < a.table_width ? p : a.table_width - 1];
+        known_pages = __ballot(ids >= 0 && ids < a.num_blocks);
+      }
+      const unsigned long long wanted = ((1ull << (last - first + 1)) - 1) << (first - batch);  // (nine pages at most)
+      if ((known_pages & wanted) != wanted) valid &= __ballot(known_pages >> (page_of(key0 + (lane < there ? lane : there - 1)) - batch) & 1);
+#pragma unroll
+      for (int i = 0; i < S::kLoads; ++i) {
+        const int r = (wave * S::kLoads + i) * S::kRowsPerLoad, end = (there - 1) / S::kRowsPerLoad * S::kRowsPerLoad, row = r < end ? r : end;
+        const int page = page_of(key0 + row), in_page = key0 + row - page * a.page;
+        const int64_t block = known_pages >> (page - batch) & 1 ? __builtin_amdgcn_readlane(ids, page - batch) : 0;  // (what lies in a page of no cache is masked)
+        const char* const k = uniform(reinterpret_cast<const char*>(static_cast<const T*>(a.k) + block * a.k_block + in_page * a.k_row + kv_head * a.k_head));
+        const char* const v = uniform(reinterpret_cast<const char*>(static_cast<const T*>(a.v) + block * a.v_block + in_page * a.v_row + kv_head * a.v_head));
+        const int behind = row + lane / S::kChunks - (there - 1);
+        const uint32_t back = behind > 0 ? behind : 0;  // (a place behind the last key repeats it)
+        dma16_from(k, k_offset[i] - back * k_row, k_to + i * 1024);
+        dma16_from(v, v_offset[i] - back * v_row, v_to + i * 1024);
+      }
+    } else if constexpr (kWhere != kAnyPages) {
       const char *k, *v;
       if constexpr (kWhere == kPacked) {
         k = reinterpret_cast<const char*>(static_cast<const T*>(a.k) + (static_cast<int64_t>(key_begin) + key0) * a.k_row + kv_head * a.k_head);
@@ -770,13 +798,15 @@ int shares_of(const MloraAttentionArgs& a) {
 }
 
 template <typename T, int D> int launch(const MloraAttentionArgs& a) {
-  const int where = !a.block_tables ? kPacked : a.page % kKeys == 0 ? kWholePages : kAnyPages;
+  const int where = !a.block_tables ? kPacked : a.page % kKeys == 0 ? kWholePages : a.page % Shape<T, D>::kRowsPerLoad == 0 && a.page >= 8 ? kLoadPages : kAnyPages;
   const int together = heads_together(a);
   const long long items = a.num_rows / tile_rows(together) + a.sequences;  // at most that many tiles of rows
   const int shares = prompt_workspace_bytes(&a) && a.workspace && a.workspace_bytes >= static_cast<int64_t>(prompt_workspace_bytes(&a)) ? shares_of(a) : 0;
   const long long all = items > shares ? items : shares;
   const dim3 grid(a.heads >> together, static_cast<unsigned>(all < kItemsPerPlane ? all : kItemsPerPlane), static_cast<unsigned>((all + kItemsPerPlane - 1) / kItemsPerPlane));
-  const Grid given{shares, together, a.heads / a.kv_heads, static_cast<uint32_t>(((1ll << 31) + a.kv_heads - 1) / a.kv_heads)};
+  const int page = a.block_tables ? a.page : 1, page_shift = 31 - __builtin_clz(static_cast<uint32_t>(page));
+  const Grid given{shares, together, a.heads / a.kv_heads, static_cast<uint32_t>(((1ll << 31) + a.kv_heads - 1) / a.kv_heads),
+                   static_cast<uint32_t>(((1ull << (31 + page_shift)) + page - 1) / page), page_shift};
   constexpr int kLds = Shape<T, D>::kLds;
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
   if (where == kPacked) {
@@ -785,6 +815,9 @@ template <typename T, int D> int launch(const MloraAttentionArgs& a) {
   } else if (where == kWholePages) {
     allow_lds<prompt_kernel<T, D, kWholePages>>(kLds);
     prompt_kernel<T, D, kWholePages><<<grid, kWaves * 64, kLds, stream>>>(a, given);
+  } else if (where == kLoadPages) {
+    allow_lds<prompt_kernel<T, D, kLoadPages>>(kLds);
+    prompt_kernel<T, D, kLoadPages><<<grid, kWaves * 64, kLds, stream>>>(a, given);
   } else {
     allow_lds<prompt_kernel<T, D, kAnyPages>>(kLds);
     prompt_kernel<T, D, kAnyPages><<<grid, kWaves * 64, kLds, stream>>>(a, given);

@@ -282,7 +282,7 @@ def test_decode_behind_the_first_4_gb_of_a_cache():
 
 @pytest.mark.parametrize("dtype,heads,kv_heads,dim,page", [(torch.bfloat16, 2, 1, 64, 64), (torch.float16, 16, 2, 64, 256), (torch.float16, 1, 1, 128, 16),
                                                             (torch.float32, 4, 4, 64, 128), (torch.float32, 8, 1, 128, 0), (torch.bfloat16, 4, 2, 128, 0), (torch.bfloat16, 12, 2, 64, 256),
-                                                            (torch.bfloat16, 16, 4, 128, 64)])
+                                                            (torch.bfloat16, 16, 4, 128, 64), (torch.float16, 16, 4, 64, 16), (torch.bfloat16, 2, 1, 64, 24)])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 20000, 5), (False, 0, 0)])
 def test_chunks_behind_long_caches(dtype, heads, kv_heads, dim, page, causal, window, sinks):
     """Few tiles of rows with many keys: their work is cut anywhere and joined.  Rows at the ends and borders of tiles are compared."""
@@ -374,7 +374,8 @@ def test_prompts_of_every_length(dtype, heads, kv_heads, dim, causal, window, si
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (3, 1, 128, 256), (2, 2, 64, 48), (2, 1, 64, 9), (16, 4, 64, 64), (8, 4, 128, 16)])
+@pytest.mark.parametrize("heads,kv_heads,dim,page", [(4, 2, 64, 16), (3, 1, 128, 256), (2, 2, 64, 48), (2, 1, 64, 9), (16, 4, 64, 64), (8, 4, 128, 16),
+                                                     (2, 1, 128, 24), (16, 2, 64, 8)])
 @pytest.mark.parametrize("causal,window,sinks", [(True, 0, 0), (True, 100, 3), (False, 0, 0)])
 def test_chunks_behind_cached_rows(dtype, heads, kv_heads, dim, page, causal, window, sinks):
     """New rows behind what is cached, a row without any, more rows than keys (the first of them see nothing)."""
@@ -396,6 +397,35 @@ def test_chunks_behind_cached_rows(dtype, heads, kv_heads, dim, page, causal, wi
         want, bound = oracle.attend(q[at], *dense[s], causal, window, sinks, dtype=dtype)
         _close(got[at], want, bound, ("pages", s))
         _close(other[at], want, bound, ("packed", s))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [1, 5, 8, 9, 16, 24, 48, 64, 256])
+def test_prompts_leave_pages_outside_the_cache_unread(page, dim, dtype):
+    """Their keys are hidden, in the middle, at the end and where all of them are; pages that end inside tiles of 64 keys."""
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    print(page, dim, dtype, flush=True)
+    g = _gen(27)
+    new, totals = [40, 70, 3, 33], [200, 333, 90, 600]
+    dense, k, v, table = _paged(totals, 2, dim, page, dtype, g)
+    q = (1.5 * torch.randn(sum(new), 4, dim, generator=g)).to(dtype)
+    bad = {0: [0], 1: [(totals[1] - 1) // page], 2: list(range(-(-totals[2] // page))), 3: [i for i in range(-(-totals[3] // page)) if 100 <= i * page <= 140]}
+    for s, pages in bad.items():
+        for i, n in enumerate(pages):
+            table[s, n] = -1 if i % 2 == 0 else k.size(0)
+    got = prompt_attention(q.cuda(), k, v, _starts(new).cuda(), block_tables=table.cuda(), context_lens=torch.tensor(totals, dtype=torch.int32, device="cuda"))
+    at = 0
+    for s, n in enumerate(new):
+        for i in range(n):
+            keys = [j for j in range(totals[s] - n + i + 1) if j // page not in bad[s]]
+            if not keys:
+                assert not got[at + i].any()
+                continue
+            want, bound = oracle.attend(q[at + i : at + i + 1], dense[s][0][keys], dense[s][1][keys], False, dtype=dtype)
+            _close(got[at + i : at + i + 1], want, bound, (s, i))
+        at += n
 
 
 @pytest.mark.parametrize("heads,kv_heads", [(2, 1), (16, 4)])
