@@ -120,36 +120,42 @@ template <int kDistance, typename T, int N> __device__ __forceinline__ void all_
   for (int i = 0; i < N; ++i) other[i].raw = across<kDistance>(x[i].raw);
 }
 
-// Groups of a token: of query heads, of key heads, of value heads.
+// Groups of a token and how a number is divided by them: n / d = (n magic >> 32) >> shift for n below 2^31, with magic = 2^(31 + L) / d + 1, L = the
+// bits of d - 1 and shift = L - 1; d of one has no such number.
 struct Groups {
-  int q, kv, all;
-};
-__host__ __device__ inline Groups groups_of(const MloraRotateArgs& a, int per) {
-  const int q = (a.heads + per - 1) / per, kv = (a.kv_heads + per - 1) / per;
-  return {q, kv, q + kv + (a.v ? kv : 0)};
-}
-
-// Lanes of a head, a division by the number of groups (n / d = (n magic >> 32) >> shift for n below 2^31, with magic = 2^(31 + L) / d + 1, L = the
-// bits of d - 1 and shift = L - 1; d of one has no such number), and 1 / dim.
-struct Layout {
-  int log_width, shift;
+  int count, shift;
   uint32_t magic;
-  float inverse_dim;
+  Groups(int heads, int per) : count((heads + per - 1) / per) {
+    int bits = 1;
+    while ((1u << bits) < static_cast<unsigned>(count)) ++bits;
+    shift = bits - 1;
+    magic = count ? static_cast<uint32_t>((1ull << (31 + bits)) / count + 1) : 0;
+  }
+};
+
+// A workgroup has heads of one kind, which so costs its wavefronts no choice lane by lane: the first `q_blocks` those of q, the next `kv_blocks` those
+// of k, the rest those of v.
+struct Layout {
+  int log_width;  // lanes of a head
+  unsigned q_blocks, kv_blocks;
+  Groups q, kv;
+  float inverse_dim;  // 1 / dim
 };
 
 // kPer: heads of a group.
 template <typename T, bool kAligned, int kPer, bool kInterleaved>
 __global__ __launch_bounds__(kThreads) void rotate_kernel(MloraRotateArgs a, Layout layout) {
   constexpr int C = 16 / sizeof(T);
-  const Groups groups = groups_of(a, kPer);
   const int lane = threadIdx.x & 63, c = lane & ((1 << layout.log_width) - 1);
-  const unsigned unit = (blockIdx.x * kThreads + threadIdx.x) >> layout.log_width;
-  const int t = groups.all == 1 ? unit : __umulhi(unit, layout.magic) >> layout.shift, group = unit - t * groups.all;
+  const bool is_q = blockIdx.x < layout.q_blocks, is_v = blockIdx.x >= layout.q_blocks + layout.kv_blocks;
+  const unsigned block_of_kind = blockIdx.x - (is_q ? 0 : layout.q_blocks + (is_v ? layout.kv_blocks : 0));
+  const Groups& groups = is_q ? layout.q : layout.kv;
+  const unsigned unit = (block_of_kind * kThreads + threadIdx.x) >> layout.log_width;
+  const int t = groups.count == 1 ? unit : __umulhi(unit, groups.magic) >> groups.shift, group = unit - t * groups.count;
   if (t >= a.num_tokens) return;
   const int e0 = c * C, half = a.rotary >> 1;
   const bool mine = e0 < a.dim;
-  const bool is_q = group < groups.q, is_v = group >= groups.q + groups.kv;
-  const int first = (is_q ? group : group - groups.q - (is_v ? groups.kv : 0)) * kPer, heads = is_q ? a.heads : a.kv_heads;
+  const int first = group * kPer, heads = is_q ? a.heads : a.kv_heads;
   const bool turned = e0 < a.rotary && !is_v;
   const int partner = e0 < half ? e0 + half : e0 - half;  // first element of the other halves of this lane's pairs
   const int64_t head_stride = is_q ? a.q_head : is_v ? a.v_head : a.k_head, row_stride = is_q ? a.q_row : is_v ? a.v_row : a.k_row;
@@ -272,12 +278,10 @@ bool aligned(const void* p, int64_t row, int64_t head, int64_t block, int size) 
 }
 
 template <typename T, bool kAligned, int kPer> void launch_heads(const MloraRotateArgs& a, int log_width) {
-  const unsigned groups = groups_of(a, kPer).all;
-  const long long threads = (static_cast<long long>(a.num_tokens) * groups) << log_width;
-  const unsigned grid = static_cast<unsigned>((threads + kThreads - 1) / kThreads);
-  int bits = 1;
-  while ((1u << bits) < groups) ++bits;
-  const Layout layout = {log_width, bits - 1, static_cast<uint32_t>((1ull << (31 + bits)) / groups + 1), 1.0f / a.dim};
+  const Groups q(a.heads, kPer), kv(a.kv_heads, kPer);
+  auto blocks = [&](int groups) { return static_cast<unsigned>((((static_cast<long long>(a.num_tokens) * groups) << log_width) + kThreads - 1) / kThreads); };
+  const Layout layout{log_width, blocks(q.count), blocks(kv.count), q, kv, 1.0f / a.dim};
+  const unsigned grid = layout.q_blocks + layout.kv_blocks * (a.v ? 2 : 1);
   const hipStream_t stream = static_cast<hipStream_t>(a.stream);
   if (a.interleaved) rotate_kernel<T, kAligned, kPer, true><<<grid, kThreads, 0, stream>>>(a, layout);
   else rotate_kernel<T, kAligned, kPer, false><<<grid, kThreads, 0, stream>>>(a, layout);
