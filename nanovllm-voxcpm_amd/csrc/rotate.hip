@@ -5,9 +5,10 @@
 // those lanes, and what an element is paired with comes from the lane W / 2 on (or, in neighbouring pairs, from the lane itself).  With the weights taken into the
 // cosines and sines an element is inverse * (own * x + paired * other): all of it in fp32, one rounding at the end.
 //
-// Bound by memory: a batch's heads are read once and written once.  A group of W lanes takes two heads of one token, for which it holds the coefficients in
-// registers: read anew for every head they would be as many bytes as the head again.  9392 tokens, 16 + 2 heads of 64, bf16, norms and cache: 15.4 us,
-// 3.1 TB/s (a copy of as many bytes 9.3 us); 8381 tokens, 32 + 8 heads of 128, fp16: 43.1 us, 4.8 TB/s (a copy: 40).
+// Bound by memory: a batch's heads are read once and written once.  A group of W lanes takes four heads of one token, for which it holds the coefficients in
+// registers: read anew for every head they would be as many bytes as the head again.  9392 tokens, 16 + 2 heads of 64, bf16, norms and cache: 13.0 us,
+// 3.7 TB/s (an elementwise operation over as many bytes 9.2 us: what is more here is the trip from positions to the table and the arithmetic of norm and rotation);
+// 8381 tokens, 32 + 8 heads of 128, fp16: 41.9 us, 4.9 TB/s (39).
 #include "common.h"
 #include "launch.h"
 
@@ -296,11 +297,11 @@ template <typename T> void launch(const MloraRotateArgs& a) {
                        aligned(a.q_out, a.q_out_row, a.q_out_head, 0, size) && aligned(a.k_out, a.k_out_row, a.k_out_head, 0, size) &&
                        aligned(a.k_cache, a.k_cache_row, a.k_cache_head, a.k_block, size) && aligned(a.v_cache, a.v_cache_row, a.v_cache_head, a.v_block, size) &&
                        aligned(a.cos_sin, a.table_row, 0, 0, 4) && aligned(a.q_weight, 0, 0, 0, 1) && aligned(a.k_weight, 0, 0, 0, 1);
-  // Two heads a group read the table and the weights half as often as one (9392 tokens, 16 + 2 heads of 64, bf16, norms: 15.4 us against 17.4; 8381, 32 + 8
-  // of 128, fp16: 43.1 / 52.3; four 15.0 / 44.9); with few tokens one, so that every compute unit has some.
+  // Four heads a group read the table and the weights a fourth as often as one (9392 tokens, 16 + 2 heads of 64, bf16, norms: 1, 2, 4, 8 heads 15.7, 14.1,
+  // 13.0, 14.2 us; 8381, 32 + 8 of 128, fp16: 52.0, 42.4, 41.9, 42.8); with few tokens one, so that every compute unit has some.
   const bool many = (static_cast<long long>(a.num_tokens) * all << log_width) >= kManyThreads;
   if (!vectors) launch_heads<T, false, 1>(a, log_width);
-  else if (many) launch_heads<T, true, 2>(a, log_width);
+  else if (many) launch_heads<T, true, 4>(a, log_width);
   else launch_heads<T, true, 1>(a, log_width);
 }
 
