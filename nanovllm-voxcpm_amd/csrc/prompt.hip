@@ -188,13 +188,13 @@ struct KeyTiles {
 // A tile of rows that lies in several shares is joined by a second launch from what each of them left in the workspace.
 // A share is 32 tiles of keys at least: below it what is left and joined costs more than the balance gives.  Where so few tiles of rows are there that they leave most compute
 // units idle, shares go down to `least`, if the longest tile of rows is longer than that by what the second launch costs (`join`): in 16 bits a tile of keys takes
-// two thirds of a microsecond, in fp32 four to eight.  16 tokens of 4 prompts behind 2000 each 28 us (51 with shares of 32), 173 in fp32 behind 8450, 8 heads of 128, 83 (288);
+// two thirds of a microsecond, in fp32 four to eight.  16 tokens of 4 prompts behind 2000 each 28 us (51 with shares of 32), 300 behind 1700 27 (34), 173 in fp32 behind 8450, 8 heads of 128, 83 (288);
 // 2000 tokens by themselves would take 44, without shares 35.
 constexpr int kLeastShare = 32;
 struct ShareCosts {
   int few, least, join;  // few: workgroups without shares
 };
-__host__ __device__ constexpr ShareCosts share_costs(int dtype) { return dtype == MLORA_DTYPE_F32 ? ShareCosts{512, 2, 4} : ShareCosts{128, 8, 16}; }
+__host__ __device__ constexpr ShareCosts share_costs(int dtype) { return dtype == MLORA_DTYPE_F32 ? ShareCosts{512, 2, 4} : ShareCosts{128, 4, 16}; }
 
 // The tiles of rows of a batch of at most 64 sequences, one a lane.
 struct RowTiles {
@@ -847,7 +847,8 @@ size_t prompt_workspace_bytes(const MloraAttentionArgs* a) {
   const int64_t shares = shares_of(*a), tiles = a->num_rows / tile_rows(heads_together(*a)) + a->sequences;
   // As the device will decide, with the longest that a sequence may be, or of packed keys the average (the rows of a prompt by itself see half of its keys each): the
   // launch that joins costs one also where it finds nothing to do.
-  const int64_t keys = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys / a->sequences;
+  const int64_t there = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys / a->sequences;
+  const int64_t near = a->window ? static_cast<int64_t>(a->window) + a->sinks + kRows + 2 * kKeys : INT64_MAX, keys = there < near ? there : near;
   const bool by_itself = !a->block_tables && !a->key_starts && a->causal;
   const int64_t least = tiles * (a->heads >> heads_together(*a)) <= costs.few ? costs.least + costs.join : by_itself ? 2 * kLeastShare : kLeastShare;
   if (tiles >= (a->block_tables ? 2 : 1) * shares || keys <= least * kKeys) return 0;
