@@ -1,6 +1,6 @@
 // Attention of packed prompts over packed or paged keys, head sizes 64 and 128 (mlora_prompt_attention).
 //
-// One workgroup per 128 rows of queries that share a key-value head: four wavefronts of 32 rows each, of one head or of two or four.  Tiles of 64 keys and their values are
+// One workgroup per 128 rows of queries that share a key-value head: four wavefronts of 32 rows each, of one head or of several.  Tiles of 64 keys and their values are
 // staged in LDS by direct loads, two stages deep: one barrier a tile, behind which the next tile is asked for.  The scores come out of the first product with the
 // keys along the registers and the query rows along the lanes (K Q^T, 32 x 32 tiles), which is how the second one (V^T P^T) wants its
 // weights: they never leave the registers, a row's maximum and sum are a lane's own but for one exchange between the halves of the
@@ -75,7 +75,8 @@ __device__ __forceinline__ long long uniform(long long v) {
   return (static_cast<long long>(uniform(static_cast<int>(v >> 32))) << 32) | static_cast<uint32_t>(uniform(static_cast<int>(v)));
 }
 
-// A workgroup's four wavefronts take 32 rows of the same head each, or 1 << together heads of one key-value head with 128 >> together rows of each:
+// A workgroup's four wavefronts take 32 rows of the same head each, or 1 << together heads of one key-value head with 128 >> together rows of each (above
+// four heads a wavefront's 32 columns are several heads of fewer rows):
 // the same products either way, but rows that see the same keys, and few of them left over where sequences are short.  16 heads of 2: 16 prompts of 587
 // tokens 37.4 us against 40.5 with a head each, 64 sequences of 13 in fp32 15.7 against 26.7, two chunks of 2048 behind 28001 the same to a hundredth.
 __host__ __device__ constexpr int tile_rows(int together) { return kRows >> together; }
@@ -339,7 +340,9 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   // (workgroups of one key-value head go to the same XCDs: workgroup i runs on XCD i % 8)
   const int ranks = gridDim.x, rank = blockIdx.x, item = blockIdx.y + kItemsPerPlane * blockIdx.z;
   const int of_group = static_cast<int>(__umulhi(2u * rank, grid.kv_heads_inverse)), kv_head = rank - of_group * a.kv_heads;
-  const int head = kv_head * grid.group + (of_group << together) + (wave & ((1 << together) - 1));
+  // a wavefront's columns: rows row_of_wave .. + row_mask of 32 / (row_mask + 1) heads from first_head on
+  const int heads_of_wave = together > 2 ? together - 2 : 0, row_mask = 31 >> heads_of_wave;
+  const int first_head = kv_head * grid.group + (of_group << together) + ((wave & ((1 << together) - 1)) << heads_of_wave);
   const int row_of_wave = 32 * (wave >> together);
   RowTile tile;
   bool shared = false;
@@ -371,16 +374,16 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   const int to = shared && left < of_rows.count - from ? from + left : of_rows.count;
 
   // This lane's query row; rows behind the last repeat it and are not written.
-  const int mine = row_of_wave + column;
+  const int mine = row_of_wave + (column & row_mask);
   const int row = start + (mine < rows ? mine : rows - 1);
   const int place = position + (mine < rows ? mine : rows - 1);
-  const int wave_rows = rows - row_of_wave < 32 ? rows - row_of_wave : 32;  // (may be negative)
+  const int wave_rows = rows - row_of_wave < row_mask + 1 ? rows - row_of_wave : row_mask + 1;  // (may be negative)
   const int wave_first = position + row_of_wave, wave_last = wave_first + wave_rows - 1;
   const float scale = __builtin_fabsf(a.scale) * kLog2e;
 
   Pack8 query[kSteps];
   {
-    const char* q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + row * a.q_row + head * a.q_head);
+    const char* q = reinterpret_cast<const char*>(static_cast<const T*>(a.q) + row * a.q_row + (first_head + (column >> (5 - heads_of_wave))) * a.q_head);
     const uint32_t turn = a.scale < 0 ? (sizeof(T) == 2 ? 0x80008000u : 0x80000000u) : 0u;
 #pragma unroll
     for (int s = 0; s < kSteps; ++s) {
@@ -675,7 +678,7 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   unsigned long long again = __ballot(!finite && mine < rows);
   again = (again | again >> 32) & 0xffffffffull;
   if (mine < rows && !(again >> column & 1)) {
-    T* out = static_cast<T*>(args.out) + row * args.out_row + head * args.out_head;
+    T* out = static_cast<T*>(args.out) + row * args.out_row + (first_head + (column >> (5 - heads_of_wave))) * args.out_head;
 #pragma unroll
     for (int d = 0; d < kBlocks; ++d) {
       if constexpr (sizeof(T) == 2) {
@@ -705,8 +708,9 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
   while (again) {
     const int c = __builtin_ctzll(again);
     again &= again - 1;
-    const Place at{sequence, total, key_begin, wave_first + c};
-    attend_row<T>(args, at, start + row_of_wave + c, head, lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
+    const int r = c & row_mask;
+    const Place at{sequence, total, key_begin, wave_first + r};
+    attend_row<T>(args, at, start + row_of_wave + r, first_head + (c >> (5 - heads_of_wave)), lane, reinterpret_cast<float*>(lds) + wave * MLORA_MAX_HEAD_DIM);
   }
   if (shared) __syncthreads();
   }
@@ -726,9 +730,10 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, 
   if (number >= *shared_tiles(a)) return;
   const Joint t = *joint(a, number);
   const int of_wave = blockIdx.x & 3, group = a.heads / a.kv_heads;  // (the wavefront that had them)
-  const int head = rank % a.kv_heads * group + ((rank / a.kv_heads) << together) + (of_wave & ((1 << together) - 1));
-  const int first = 32 * (of_wave >> together) + kOwn * wave, first_left = 32 * of_wave + kOwn * wave;  // of the tile, of what was left
-  if (t.parts < 2 || first >= t.rows) return;
+  const int heads_of_wave = together > 2 ? together - 2 : 0, row_mask = 31 >> heads_of_wave;
+  const int first_head = rank % a.kv_heads * group + ((rank / a.kv_heads) << together) + ((of_wave & ((1 << together) - 1)) << heads_of_wave);
+  const int column = kOwn * wave, row_of_wave = 32 * (of_wave >> together), first_left = 32 * of_wave + column;  // columns from `column` on
+  if (t.parts < 2 || row_of_wave + (column & row_mask) >= t.rows) return;
   const int own = first_left + (lane & (kOwn - 1));  // the row whose (m, l) this lane looks after
   float most = -__builtin_inff(), sum = 0.0f, x[kOwn][kPer] = {};
 #pragma unroll 4
@@ -762,7 +767,7 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, 
   unsigned again = 0;
 #pragma unroll
   for (int i = 0; i < kOwn; ++i) {
-    const int row = t.start + first + i;
+    const int r = row_of_wave + ((column + i) & row_mask), head = first_head + ((column + i) >> (5 - heads_of_wave));
     const float l = __shfl(sum, i, kWave);
     bool finite = true;
 #pragma unroll
@@ -770,25 +775,29 @@ __global__ __launch_bounds__(256) void prompt_join_kernel(MloraAttentionArgs a, 
       x[i][e] /= l;
       finite &= __builtin_fabsf(x[i][e]) < __builtin_inff();
     }
-    if (first + i >= t.rows) continue;
+    if (r >= t.rows) continue;
     if (!__all(finite)) {
       again |= 1u << i;
       continue;
     }
 #pragma unroll
-    for (int e = 0; e < kPer; ++e) static_cast<T*>(a.out)[row * a.out_row + head * a.out_head + 64 * e + lane] = from_f32<T>(x[i][e]);
+    for (int e = 0; e < kPer; ++e) static_cast<T*>(a.out)[(t.start + r) * a.out_row + head * a.out_head + 64 * e + lane] = from_f32<T>(x[i][e]);
   }
   for (; again; again &= again - 1) {
-    const int r = first + __builtin_ctz(again);
-    attend_row<T>(a, Place{t.sequence, t.total, t.key_start, t.position + r}, t.start + r, head, lane, scratch[wave]);
+    const int c = column + __builtin_ctz(again), r = row_of_wave + (c & row_mask);
+    attend_row<T>(a, Place{t.sequence, t.total, t.key_start, t.position + r}, t.start + r, first_head + (c >> (5 - heads_of_wave)), lane, scratch[wave]);
   }
 }
 
-// At least four lists of shares are left, so that a list is not long for those who look for their place in it.
+// At least four lists of shares are left where there are many rows, so that a list is not long for those who look for their place in it.
 int heads_together(const MloraAttentionArgs& a) {
-  const int group = a.heads / a.kv_heads;
-  if (group % 4 == 0 && a.heads >= 16) return 2;
-  return group % 2 == 0 && a.heads >= 8 ? 1 : 0;
+  const int group = a.heads / a.kv_heads, rows = a.num_rows / a.sequences;
+  int together = group % 4 == 0 && a.heads >= 16 ? 2 : group % 2 == 0 && a.heads >= 8 ? 1 : 0;
+  // Sequences of few rows fill a tile with as many heads as there are, up to 32, and so read their keys once: 233 rows of 42 sequences behind 63560 keys each,
+  // 8 heads of one of 64, 183 us, 393 in tiles of two heads; 64 sequences of 13 tokens in fp32 12.1 us, 13.9 in tiles of four.
+  for (int more = together + 1; more <= 5 && group % (1 << more) == 0; ++more)
+    if (rows <= tile_rows(more)) together = more;
+  return together;
 }
 
 // Shares of a list: as many workgroups as the chip holds at once.

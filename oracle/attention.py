@@ -61,7 +61,8 @@ def attend(q, k, v, causal=True, window=0, sinks=0, scale=None, dtype=torch.floa
             rows_of = slice(g * (heads // kv_heads), (g + 1) * (heads // kv_heads))
             out[i, rows_of] = o
             # (fp16: the weights below its least normal number are off by 2^-25 each, of a largest of one)
-            tiny = len(seen) * 2.0**-25 * vv.abs().amax() if dtype == torch.float16 else 0.0
+            # (element by element of v: sum_j 2^-25 |v_je| <= n 2^-25 max_j |v_je|, and a NaN in one element is no bound of another's)
+            tiny = len(seen) * 2.0**-25 * vv.abs().amax(0) if dtype == torch.float16 else 0.0
             # sum l may be of the rounded weights: o = (sum p (1 + e) v) / (sum p (1 + e)) with |e| <= step, off by at most step (a + |o|) to
             # first order, and by that times 2 step beyond it; then the result's own rounding
             bound[i, rows_of] = (wrong + step * (1 + 2 * step)) * a + tiny + step * o.abs() * (2 + 3 * step)

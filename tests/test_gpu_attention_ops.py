@@ -400,6 +400,39 @@ def test_chunks_behind_cached_rows(dtype, heads, kv_heads, dim, page, causal, wi
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 64), (32, 1, 128), (8, 1, 64), (64, 2, 64), (24, 3, 128), (4, 1, 64), (6, 3, 64)])
+@pytest.mark.parametrize("new,longest", [([1, 0, 3, 2, 40, 1, 5, 16, 17, 33, 4, 1], 300), ([2, 1, 1], 300), ([1, 3, 1, 9], 12000), ([5, 1, 7, 30], 9000)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (150, 3)])
+def test_few_rows_of_many_heads(dtype, heads, kv_heads, dim, new, longest, window, sinks):
+    """A tile holds several heads of few rows, in wavefronts of two, four and eight heads; a value that some rows see is NaN."""
+    from nanovllm_voxcpm_amd.attention_ops import prompt_attention
+
+    print(dtype, heads, kv_heads, dim, new, longest, window, sinks, flush=True)
+    g = _gen(28)
+    totals = [min(longest, n + longest * (s + 1) // len(new)) if s != 1 else new[1] for s, n in enumerate(new)]
+    dense, k, v, table = _paged(totals, kv_heads, dim, 64, dtype, g)
+    q = (1.5 * torch.randn(sum(new), heads, dim, generator=g)).to(dtype)
+    last = len(new) - 1
+    at = totals[last] - 1
+    dense[last][1][at, 0, 5] = NAN
+    v[table[last, at // 64], at % 64, 0, 5] = NAN
+    got = prompt_attention(q.cuda(), k, v, _starts(new).cuda(), block_tables=table.cuda(), context_lens=torch.tensor(totals, dtype=torch.int32, device="cuda"),
+                           window=window, sinks=sinks)
+    packed = [torch.cat([d[i] for d in dense]).cuda() for i in range(2)]
+    other = prompt_attention(q.cuda(), *packed, _starts(new).cuda(), cu_seqlens_k=_starts(totals).cuda(), window=window, sinks=sinks)
+    row = 0
+    for s, n in enumerate(new):
+        for i in range(n):
+            upto = totals[s] - n + i + 1
+            first = max(0, upto - window) if window else 0
+            keys = [*range(min(sinks, first)), *range(first, upto)]
+            want, bound = oracle.attend(q[row : row + 1], dense[s][0][keys], dense[s][1][keys], False, dtype=dtype)
+            _close(got[row : row + 1], want, bound, ("pages", s, i))
+            _close(other[row : row + 1], want, bound, ("packed", s, i))
+            row += 1
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("page", [1, 5, 8, 9, 16, 24, 48, 64, 256])
 def test_prompts_leave_pages_outside_the_cache_unread(page, dim, dtype):
