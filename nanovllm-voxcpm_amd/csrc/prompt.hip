@@ -188,7 +188,7 @@ struct KeyTiles {
 // in.  Their work is then one list: the tiles of keys of the first tile of rows, of the second and so on.  Every workgroup takes an equal share of the list, whatever rows it falls on.
 // A tile of rows that lies in several shares is joined by a second launch from what each of them left in the workspace.
 // A share is 32 tiles of keys at least: below it what is left and joined costs more than the balance gives.  Where so few tiles of rows are there that they leave most compute
-// units idle, shares go down to `least`, if the longest tile of rows is longer than that by what the second launch costs (`join`): in 16 bits a tile of keys takes
+// units idle, shares go down to `least`, if the longest tile of rows (or, of up to twice as many, the average) is longer than that by what the second launch costs (`join`): in 16 bits a tile of keys takes
 // two thirds of a microsecond, in fp32 four to eight.  16 tokens of 4 prompts behind 2000 each 28 us (51 with shares of 32), 300 behind 1700 27 (34), 173 in fp32 behind 8450, 8 heads of 128, 83 (288);
 // 2000 tokens by themselves would take 44, without shares 35.
 constexpr int kLeastShare = 32;
@@ -253,12 +253,10 @@ struct Shares : RowTiles {
     }
     per = (units + shares - 1) / shares;
     const ShareCosts costs = share_costs(a.dtype);
-    if (static_cast<long long>(tiles) * ranks <= costs.few) {
-      if (per < costs.least) per = costs.least;
-      if (longest < per + costs.join) per = 0;
-    } else if (per < kLeastShare) {
-      per = units > static_cast<long long>(kLeastShare) * tiles ? kLeastShare : 0;
-    }
+    const long long alone = static_cast<long long>(tiles) * ranks, short_share = per < costs.least ? costs.least : per;  // alone: workgroups without shares
+    if (alone <= costs.few ? longest >= short_share + costs.join : alone <= 2 * costs.few && units >= (short_share + costs.join) * tiles) per = short_share;
+    else if (alone <= costs.few) per = 0;
+    else if (per < kLeastShare) per = units > static_cast<long long>(kLeastShare) * tiles ? kLeastShare : 0;
     // (more tiles than the workspace has places for: starts that run backwards, whose sequences lie on one another)
     if (tiles >= 4 * shares || tiles > a.num_rows / tile_rows(together) + a.sequences) per = 0;
   }
@@ -859,7 +857,7 @@ size_t prompt_workspace_bytes(const MloraAttentionArgs* a) {
   const int64_t there = a->block_tables ? static_cast<int64_t>(a->table_width) * a->page : a->num_keys / a->sequences;
   const int64_t near = a->window ? static_cast<int64_t>(a->window) + a->sinks + kRows + 2 * kKeys : INT64_MAX, keys = there < near ? there : near;
   const bool by_itself = !a->block_tables && !a->key_starts && a->causal;
-  const int64_t least = tiles * (a->heads >> heads_together(*a)) <= costs.few ? costs.least + costs.join : by_itself ? 2 * kLeastShare : kLeastShare;
+  const int64_t least = tiles * (a->heads >> heads_together(*a)) <= costs.few * (by_itself ? 1 : 2) ? costs.least + costs.join : by_itself ? 2 * kLeastShare : kLeastShare;
   if (tiles >= (a->block_tables ? 2 : 1) * shares || keys <= least * kKeys) return 0;
   return static_cast<size_t>(joints_bytes(tiles) + shares * 2 * (a->heads >> heads_together(*a)) * kRows * (8 + 4 * a->dim));
 }
