@@ -148,6 +148,8 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
   using S = Shape<T, D, W>;
   constexpr int kWaves = W, kStages = S::kStages;
   constexpr int kKeys = S::kKeys, kSteps = S::kChunks / 4, kBlocks = D / 16;
+  // fp16: weights, at most 1, are held 2^15 times as large: the largest is finite, those of 2^-29 are still normal numbers
+  constexpr float kShift = __is_same(T, _Float16) ? 15.0f : 0.0f;
   extern __shared__ __align__(16) char lds[];
   const int lane = threadIdx.x & 63, column = lane & 15, g = lane >> 4;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -313,8 +315,8 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
 #pragma unroll
       for (int j = 1; j < kKeys / 4; ++j) top = fmaxf(top, s[j]);
       top = fmaxf(m, group_max(top));
-      const float base = top == -__builtin_inff() ? 0.0f : top;
-      const float alpha = __builtin_amdgcn_exp2f(m - base);
+      const float bottom = top == -__builtin_inff() ? 0.0f : top, base = bottom - kShift;
+      const float alpha = __builtin_amdgcn_exp2f(m - bottom);
       m = top;
       l *= alpha;
 #pragma unroll
@@ -322,16 +324,18 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[d][j] *= alpha;
 #pragma unroll
-      for (int j = 0; j < kKeys / 4; ++j) {
-        s[j] = __builtin_amdgcn_exp2f(s[j] - base);
-        l += s[j];
-      }
+      for (int j = 0; j < kKeys / 4; ++j) s[j] = __builtin_amdgcn_exp2f(s[j] - base);
       if constexpr (sizeof(T) == 2) {
+        // The matrix cores take weights of the element type (half a step of it each; in fp32 this product would cost eight times as much).  The sum is of
+        // the rounded ones, so that what is left out of the numerator is left out of the denominator too: equal values come out as they are.
         float p8[8];
+        const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
         for (int j = 0; j < 8; ++j) p8[j] = s[j];
-        Pack8 weights;
+        Pack8 weights, ones;
         pack8<T>(p8, weights);
+        pack8<T>(one, ones);
+        l = dot8<T>(weights, ones, l);
         const int i = column;
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) {
@@ -346,6 +350,8 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
         }
       } else {
         const int i = column;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) l += s[j];
 #pragma unroll
         for (int d = 0; d < kBlocks; ++d) {
 #pragma unroll
