@@ -13,10 +13,13 @@ import re
 import sys
 
 NEED = 5
+READS_ONLY = ("s_cmp", "s_bitcmp", "s_setpc", "s_setreg", "s_setvskip", "s_set_gpr_idx", "s_branch", "s_cbranch")  # their first operand is no destination
 
 
 def sgprs(text):
     out = set()
+    text = re.sub(r"\bvcc\b", "vcc_lo vcc_hi", text)
+    out.update(name for name in ("vcc_lo", "vcc_hi") if name in text)
     for m in re.finditer(r"\bs\[(\d+):(\d+)\]", text):
         out.update(range(int(m.group(1)), int(m.group(2)) + 1))
     for m in re.finditer(r"\bs(\d+)\b", text):
@@ -48,7 +51,7 @@ def scan(path):
         if op.startswith("v_"):
             for r in sgprs(first):
                 written[r] = states + 1
-        elif op.startswith("s_"):
+        elif op.startswith("s_") and not op.startswith(READS_ONLY):
             for r in sgprs(first):
                 written.pop(r, None)
         states += 1
