@@ -14,14 +14,15 @@ namespace mlora {
 namespace {
 
 constexpr int kWaves = 4;
+constexpr long long kLine = 1 << 20;  // workgroups along a launch's first dimension
 
 template <typename T>
 __global__ __launch_bounds__(kWaves * 64) void attend_rows_kernel(MloraAttentionArgs a) {
   __shared__ float queries[kWaves][MLORA_MAX_HEAD_DIM];
   const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const long long unit = static_cast<long long>(blockIdx.x) * kWaves + wave;
+  const long long unit = (static_cast<long long>(blockIdx.y) * gridDim.x + blockIdx.x) * kWaves + wave;
   const int row = static_cast<int>(unit / a.heads), head = static_cast<int>(unit - static_cast<long long>(row) * a.heads);
-  if (row >= a.num_rows) return;
+  if (unit >= static_cast<long long>(a.num_rows) * a.heads) return;
   Place at;
   if (!place_of_row(a, row, &at)) return;
   attend_row<T>(a, at, row, head, lane, queries[wave]);
@@ -39,7 +40,9 @@ bool attention_vectors_ok(const MloraAttentionArgs* a) {
 
 int launch_attend_rows(const MloraAttentionArgs* a) {
   const long long units = static_cast<long long>(a->num_rows) * a->heads;
-  const unsigned grid = static_cast<unsigned>((units + kWaves - 1) / kWaves);
+  // (a dimension of a launch has fewer than 2^32 threads: what is more goes along the second)
+  const long long blocks = (units + kWaves - 1) / kWaves, line = blocks < kLine ? blocks : kLine;
+  const dim3 grid(static_cast<unsigned>(line), static_cast<unsigned>((blocks + line - 1) / line));
   const hipStream_t stream = static_cast<hipStream_t>(a->stream);
   if (a->dtype == MLORA_DTYPE_BF16) attend_rows_kernel<__bf16><<<grid, kWaves * 64, 0, stream>>>(*a);
   else if (a->dtype == MLORA_DTYPE_F16) attend_rows_kernel<_Float16><<<grid, kWaves * 64, 0, stream>>>(*a);

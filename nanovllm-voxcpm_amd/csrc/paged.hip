@@ -545,7 +545,10 @@ template <typename T, int D> int launch_shape(const MloraAttentionArgs& a) {
 }  // namespace
 
 bool paged_supported(const MloraAttentionArgs* a) {
-  return (a->dim == 64 || a->dim == 128) && attention_vectors_ok(a) && a->table_width > 0 && units_of_part(a->heads, a->kv_heads) <= 65535 && a->heads <= 65535;
+  if ((a->dim != 64 && a->dim != 128) || !attention_vectors_ok(a) || a->table_width < 1 || units_of_part(a->heads, a->kv_heads) > 65535 || a->heads > 65535) return false;
+  // a dimension of a launch has fewer than 2^32 threads
+  const Way cut = cut_of(*a);
+  return (static_cast<int64_t>(a->sequences) + cut.target) * cut.waves * 64 <= UINT32_MAX;
 }
 
 size_t paged_workspace_bytes(const MloraAttentionArgs* a) {
