@@ -86,26 +86,53 @@ def _no_grad(*tensors: torch.Tensor | None) -> None:
         raise RuntimeError("the attention ops have no backward: call them under torch.no_grad() or torch.inference_mode()")
 
 
-def _memory(t: torch.Tensor) -> tuple[int, int]:
-    """First byte of a strided tensor and the one behind its last."""
-    last = sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
-    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+def _memory(t: torch.Tensor) -> tuple[int, int, int, int]:
+    """First byte of a strided tensor and the one behind its last; bytes from row to row and of a row's extent."""
+    size, shape, strides = t.element_size(), t.shape, t.stride()
+    if 0 in shape:
+        return 0, 0, 0, 0
+    width = 1 + sum((n - 1) * s for n, s in zip(shape[1:], strides[1:]))
+    start = t.data_ptr()
+    return start, start + size * ((shape[0] - 1) * strides[0] + width), size * strides[0], size * width
+
+
+def _beside(a: tuple[int, int, int, int], b: tuple[int, int, int, int]) -> bool:
+    """Whether two tensors' memory is plainly apart: one behind the other, or columns of one buffer, rows as far apart in both."""
+    if a[1] <= b[0] or b[1] <= a[0]:
+        return True
+    row = a[2]
+    if row != b[2] or row <= 0:
+        return False
+    apart = (b[0] - a[0]) % row
+    return a[3] <= apart and apart + b[3] <= row
+
+
+def _reaches(terms: list[tuple[int, int, int]], target: int, tries: list[int]) -> bool:
+    """Whether sum c x = target for some whole numbers x, terms (c, least x, largest x) of falling c > 0.  Strides nest as a rule, so that one or
+    two x are possible at every term; after ``tries[0]`` of them the answer is yes."""
+    if not terms:
+        return target == 0
+    (c, lo, hi), rest = terms[0], terms[1:]
+    least, most = sum(r * x for r, x, _ in rest), sum(r * x for r, _, x in rest)
+    for x in range(max(lo, -((most - target) // c)), min(hi, (target - least) // c) + 1):
+        tries[0] -= 1
+        if tries[0] < 0 or _reaches(rest, target - c * x, tries):
+            return True
+    return False
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """Whether two [rows, heads, head size] tensors share memory; those that are columns of one buffer, rows as far apart in both, may lie
-    between one another without."""
-    if not a.numel() or not b.numel():
+    """Whether an element of one tensor lies on one of the other.  (Views may lie between one another without: heads of the packed rows of a linear.)"""
+    at, bt = _memory(a), _memory(b)
+    if _beside(at, bt):
         return False
-    (a0, a1), (b0, b1) = _memory(a), _memory(b)
-    if a1 <= b0 or b1 <= a0:
-        return False
-    size, row = a.element_size(), a.stride(0)
-    if a.dim() != b.dim() or row != b.stride(0) or row <= 0 or (b0 - a0) % size:
-        return True
-    width = [1 + sum((n - 1) * s for n, s in zip(t.shape[1:], t.stride()[1:])) for t in (a, b)]
-    apart = (b0 - a0) // size % row
-    return not (width[0] <= apart and apart + width[1] <= row)
+    # an address of a less one of b, by bytes
+    terms = {1: [1 - b.element_size(), a.element_size() - 1]}
+    for t, end, sign in ((a, 1, 1), (b, 0, -1)):
+        for n, s in zip(t.shape, t.stride()):
+            if n > 1 and s:
+                terms.setdefault(s * t.element_size(), [0, 0])[end] += sign * (n - 1)
+    return _reaches([(c, *terms[c]) for c in sorted(terms, reverse=True)], bt[0] - at[0], [10000])
 
 
 def _rows_apart(t: torch.Tensor, name: str) -> None:
@@ -155,8 +182,8 @@ def rotate_qk(
     ``slot_mapping[t]`` of the cache, counted over all blocks; a negative slot (padding) or one behind the last block is
     not stored.  No two tokens may share a slot.
 
-    Returns (q, k): in ``q_out`` and ``k_out`` where given (an input itself is fine), else new tensors; k is None with a cache
-    and without ``k_out``, since the cache has it.
+    Returns (q, k): in ``q_out`` and ``k_out`` where given (an input itself is fine; the caches and the other tensors are not), else new
+    tensors; k is None with a cache and without ``k_out``, since the cache has it.
     """
     fast = _hip.load_fastcall()
     if fast is not None and q_out is None and k_out is None:  # the usual call, checked and enqueued in C++
@@ -197,9 +224,13 @@ def rotate_qk(
     q_out = _result(q_out, q, "q_out")
     if k_out is not None or not all(cached):
         k_out = _result(k_out, k, "k_out")
+    lies = {id(t): _memory(t) for t in (q, k, v, q_out, k_out, k_cache, v_cache) if t is not None}
     for out, name, others in ((q_out, "q_out", (k, v, k_out)), (k_out, "k_out", (q, v))):
-        if out is not None and any(t is not None and _overlap(out, t) for t in others):
-            raise ValueError(f"{name} overlaps another of the tensors")
+        if out is None:
+            continue
+        for t, of in (*((t, "another of the tensors") for t in others), (k_cache, "k_cache"), (v_cache, "v_cache")):
+            if t is not None and not _beside(lies[id(out)], lies[id(t)]) and _overlap(out, t):
+                raise ValueError(f"{name} overlaps {of}")
     _hip.rotate_qk(q, k, v, q_out, k_out, k_cache, v_cache, positions, slot_mapping, cos_sin, q_weight, k_weight, float(eps), bool(interleaved))
     return q_out, k_out
 
