@@ -616,10 +616,36 @@ bool head_rows(const at::Tensor& q) {
 
 void* stream_of(const at::Tensor& q) { return c10::hip::getCurrentHIPStream(q.device().index()).stream(); }
 
-bool shares_memory(const at::Tensor& t) {
-  for (int64_t i = 0; i < t.dim(); ++i)
-    if (t.stride(i) == 0 && t.size(i) > 1) return true;
+// Elements of a tensor of up to four dimensions may lie on one another: strides that do not nest (the Python path tells exactly).
+bool may_share_memory(const at::Tensor& t) {
+  if (t.is_contiguous() || t.numel() == 0) return false;
+  int64_t reach = 0;  // of the dimensions of smaller strides, which are taken in their order
+  bool taken[4] = {};
+  for (int64_t i = 0; i < t.dim(); ++i) {
+    int64_t next = -1;
+    for (int64_t d = 0; d < t.dim(); ++d)
+      if (!taken[d] && (next < 0 || t.stride(d) < t.stride(next))) next = d;
+    taken[next] = true;
+    if (t.size(next) == 1) continue;
+    if (t.stride(next) <= reach) return true;
+    reach += t.stride(next) * (t.size(next) - 1);
+  }
   return false;
+}
+
+// Two tensors alike in sizes may meet: their memory is not one behind the other, nor columns of one buffer.
+bool may_meet(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0) return false;
+  int64_t width[2] = {1, 1};
+  const at::Tensor* const both[2] = {&a, &b};
+  for (int i = 0; i < 2; ++i)
+    for (int64_t d = 1; d < a.dim(); ++d) width[i] += (a.size(d) - 1) * both[i]->stride(d);
+  const int64_t size = static_cast<int64_t>(a.element_size()), row = a.stride(0);
+  const int64_t apart = static_cast<const char*>(b.data_ptr()) - static_cast<const char*>(a.data_ptr());
+  if (apart >= size * ((a.size(0) - 1) * row + width[0]) || -apart >= size * ((a.size(0) - 1) * b.stride(0) + width[1])) return false;
+  if (row != b.stride(0) || row <= 0 || apart % size) return true;
+  const int64_t column = (apart / size % row + row) % row;
+  return column < width[0] || column + width[1] > row;
 }
 
 bool cache_like(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) {
@@ -650,8 +676,8 @@ PyObject* op_rotate(PyObject* const* args) {
   const bool cached = v != nullptr;
   if (cached != (k_cache != nullptr) || cached != (v_cache != nullptr) || cached != (slots != nullptr)) return nullptr;
   if (cached) {
-    if (!rows_like(*v, 3, *q) || v->sizes() != k->sizes() || !cache_like(*k_cache, *v_cache, *q) || k_cache->size(2) != k->size(1) || shares_memory(*k_cache) ||
-        shares_memory(*v_cache) || !index_vector(*slots, *q, rows, &is64))
+    if (!rows_like(*v, 3, *q) || v->sizes() != k->sizes() || !cache_like(*k_cache, *v_cache, *q) || k_cache->size(2) != k->size(1) || may_share_memory(*k_cache) ||
+        may_share_memory(*v_cache) || may_meet(*k_cache, *v_cache) || !index_vector(*slots, *q, rows, &is64))
       return nullptr;
     a.slots64 = is64;
     a.v = v->data_ptr(); a.v_row = v->stride(0); a.v_head = v->stride(1);

@@ -136,9 +136,21 @@ def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _rows_apart(t: torch.Tensor, name: str) -> None:
-    """An output's elements must not lie on one another (an expanded view)."""
-    if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
-        raise ValueError(f"rows or heads of {name} share memory")
+    """A written tensor's elements must not lie on one another (an expanded view, rows closer than they are long)."""
+    if t.is_contiguous() or not t.numel():
+        return
+    terms = sorted(((s, n - 1) for n, s in zip(t.shape, t.stride()) if n > 1), reverse=True)
+    reach = 0  # of the dimensions of smaller strides
+    for i in range(len(terms) - 1, -1, -1):
+        stride, most = terms[i]
+        # (where strides do not nest: a step along some dimension that the others take back)
+        if stride <= reach or stride == 0:
+            for j in range(len(terms)):
+                one = [(s, 1 if n == j else -m, m) for n, (s, m) in enumerate(terms) if s]
+                if terms[j][0] == 0 or _reaches(one, 0, [10000]):
+                    raise ValueError(f"rows or heads of {name} share memory")
+            return
+        reach += stride * most
 
 
 def _result(out: torch.Tensor | None, source: torch.Tensor, name: str) -> torch.Tensor:
@@ -180,7 +192,7 @@ def rotate_qk(
 
     With ``k_cache``, ``v_cache [blocks, rows of a block, kv_heads, D]``, ``v`` and ``slot_mapping [T]`` the new k and v of token t go to row
     ``slot_mapping[t]`` of the cache, counted over all blocks; a negative slot (padding) or one behind the last block is
-    not stored.  No two tokens may share a slot.
+    not stored.  No two tokens may share a slot, and no two rows of the caches memory.
 
     Returns (q, k): in ``q_out`` and ``k_out`` where given (an input itself is fine; the caches and the other tensors are not), else new
     tensors; k is None with a cache and without ``k_out``, since the cache has it.
@@ -220,6 +232,8 @@ def rotate_qk(
         _cache(k_cache, v_cache, k.size(1), q)
         for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
             _rows_apart(t, name)
+        if _overlap(k_cache, v_cache):
+            raise ValueError("k_cache overlaps v_cache")
         _index(slot_mapping, "slot_mapping", q.device, rows, (torch.int32, torch.int64))
     q_out = _result(q_out, q, "q_out")
     if k_out is not None or not all(cached):

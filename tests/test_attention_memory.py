@@ -56,3 +56,38 @@ def test_overlap_against_all_places():
         seen[meet] += 1
         assert attention_ops._overlap(*views) == meet, [(v.shape, v.stride(), v.storage_offset()) for v in views]
     assert min(seen.values()) > 300
+
+
+def test_caches_on_one_another_are_refused():
+    pages = torch.zeros(4, 16, 2, 64)
+    _ends("k_cache overlaps v_cache", k_cache=pages, v_cache=pages)
+    _ends("k_cache overlaps v_cache", k_cache=pages[:3], v_cache=pages[1:])
+    both = torch.zeros(3, 2, 16, 2, 64)
+    _ends(None, k_cache=both[:, 0], v_cache=both[:, 1])
+    _ends(None, k_cache=pages.new_zeros(3, 16, 2, 128)[..., :64], v_cache=pages.new_zeros(3, 16, 2, 128)[..., 64:])
+
+
+def test_written_tensors_whose_rows_lie_on_one_another_are_refused():
+    row = torch.zeros(4000)
+    _ends("q_out share memory", q_out=row.as_strided((5, 4, 64), (128, 64, 1)))
+    _ends("k_out share memory", k_out=row.as_strided((5, 2, 64), (64, 64, 1)))
+    _ends("rows or heads of k_cache", k_cache=row.as_strided((3, 16, 2, 64), (64, 64, 64, 1)))
+    _ends("rows or heads of v_cache", v_cache=torch.zeros(7000).as_strided((3, 16, 2, 64), (2047, 128, 64, 1)))
+    _ends(None, q_out=torch.zeros(4, 5, 64).transpose(0, 1))  # (heads outside rows)
+    _ends(None, k_cache=torch.zeros(3, 2, 16, 64).transpose(1, 2), v_cache=torch.zeros(16, 3, 2, 64).transpose(0, 1))
+
+
+def test_own_overlap_against_all_places():
+    pick, seen = random.Random(4), {True: 0, False: 0}
+    memory = torch.zeros(400, dtype=torch.float16)
+    for _ in range(2000):
+        shape = [pick.randint(1, 4) for _ in range(4)]
+        t = torch.as_strided(memory, shape, [pick.choice([1, 2, 3, 4, 5, 8, 12, 16, 24, 30]) for _ in range(4)])
+        on_itself = len(_places(t)) < t.numel() * t.element_size()
+        seen[on_itself] += 1
+        if on_itself:
+            with pytest.raises(ValueError, match="share memory"):
+                attention_ops._rows_apart(t, "t")
+        else:
+            attention_ops._rows_apart(t, "t")
+    assert min(seen.values()) > 300
