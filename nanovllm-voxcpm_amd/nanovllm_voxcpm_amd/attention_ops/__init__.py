@@ -232,8 +232,6 @@ def rotate_qk(
         _cache(k_cache, v_cache, k.size(1), q)
         for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
             _rows_apart(t, name)
-        if _overlap(k_cache, v_cache):
-            raise ValueError("k_cache overlaps v_cache")
         _index(slot_mapping, "slot_mapping", q.device, rows, (torch.int32, torch.int64))
     q_out = _result(q_out, q, "q_out")
     if k_out is not None or not all(cached):
@@ -245,6 +243,8 @@ def rotate_qk(
         for t, of in (*((t, "another of the tensors") for t in others), (k_cache, "k_cache"), (v_cache, "v_cache")):
             if t is not None and not _beside(lies[id(out)], lies[id(t)]) and _overlap(out, t):
                 raise ValueError(f"{name} overlaps {of}")
+    if all(cached) and q.is_cuda and not _beside(lies[id(k_cache)], lies[id(v_cache)]) and _overlap(k_cache, v_cache):  # (of host tensors nothing is written)
+        raise ValueError("k_cache overlaps v_cache")
     _hip.rotate_qk(q, k, v, q_out, k_out, k_cache, v_cache, positions, slot_mapping, cos_sin, q_weight, k_weight, float(eps), bool(interleaved))
     return q_out, k_out
 

@@ -58,13 +58,12 @@ def test_overlap_against_all_places():
     assert min(seen.values()) > 300
 
 
-def test_caches_on_one_another_are_refused():
-    pages = torch.zeros(4, 16, 2, 64)
-    _ends("k_cache overlaps v_cache", k_cache=pages, v_cache=pages)
-    _ends("k_cache overlaps v_cache", k_cache=pages[:3], v_cache=pages[1:])
-    both = torch.zeros(3, 2, 16, 2, 64)
-    _ends(None, k_cache=both[:, 0], v_cache=both[:, 1])
-    _ends(None, k_cache=pages.new_zeros(3, 16, 2, 128)[..., :64], v_cache=pages.new_zeros(3, 16, 2, 128)[..., 64:])
+def test_which_caches_lie_on_one_another():
+    pages, both, side = torch.zeros(4, 16, 2, 64), torch.zeros(3, 2, 16, 2, 64), torch.zeros(3, 16, 2, 128)
+    for k_cache, v_cache, meet in ((pages, pages, True), (pages[:3], pages[1:], True), (both[:, 0], both[:, 1], False), (side[..., :64], side[..., 64:], False),
+                                   (side[..., :64], side[..., 63:127], True), (pages[:2], pages[2:], False)):
+        assert attention_ops._overlap(k_cache, v_cache) == meet
+        _ends(None, k_cache=k_cache, v_cache=v_cache)  # (on the host nothing is written)
 
 
 def test_written_tensors_whose_rows_lie_on_one_another_are_refused():
