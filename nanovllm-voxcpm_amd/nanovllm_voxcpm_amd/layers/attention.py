@@ -79,7 +79,8 @@ def build_attention_batch(new_tokens: list[int], cached_tokens: list[int], block
 class PagedAttention(nn.Module):
     """Rotation (with per-head norms of queries and keys where ``qk_norm``), cache store and attention of one layer.
 
-    ``window``, ``sinks``: a row sees the last ``window`` keys and the first ``sinks`` (0: all).  The rotary table is fp32 whatever
+    ``window``, ``sinks``: a row sees the last ``window`` keys and the first ``sinks`` (0: all).  ``rotary_dim``: elements of a head that
+    are turned, all of them by default, 0 for none.  The rotary table is fp32 whatever
     the module's type and is made once per device by ``prepare``, which the first call does too if nobody did (outside
     a graph capture, then)."""
 
@@ -90,7 +91,8 @@ class PagedAttention(nn.Module):
             raise ValueError(f"{num_heads} query heads do not share {num_kv_heads} key-value heads evenly")
         self.num_heads, self.num_kv_heads, self.head_size = num_heads, num_kv_heads, head_size
         self.eps, self.window, self.sinks, self.scale = eps, window, sinks, scale
-        self.rotary_dim, self.max_position, self.base, self.interleaved = rotary_dim or head_size, max_position, base, interleaved
+        self.rotary_dim = head_size if rotary_dim is None else rotary_dim
+        self.max_position, self.base, self.interleaved = max_position, base, interleaved
         self.q_norm = nn.Parameter(torch.ones(head_size)) if qk_norm else None
         self.k_norm = nn.Parameter(torch.ones(head_size)) if qk_norm else None
         self._tables: dict[torch.device, torch.Tensor] = {}
@@ -103,7 +105,10 @@ class PagedAttention(nn.Module):
         if table is None:
             table = self._tables.get(device)
         if table is None:
-            table = rotary_table(self.rotary_dim, self.max_position, base=self.base, device=device)
+            if self.rotary_dim:
+                table = rotary_table(self.rotary_dim, self.max_position, base=self.base, device=device)
+            else:
+                table = torch.zeros(self.max_position, 0, device=device)
         self._tables[device] = table
         return table
 
