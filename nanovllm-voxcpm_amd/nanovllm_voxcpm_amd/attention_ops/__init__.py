@@ -8,7 +8,7 @@ token per sequence to such a cache, ``prompt_attention`` with any number of rows
 All three enqueue work on torch's current stream and neither synchronise nor read device data on the host, so they may be
 captured into a graph.  They have no backward: call them under ``torch.no_grad()`` or ``torch.inference_mode()``.
 Element types are fp32, fp16 and bf16, head sizes multiples of 8 up to 256; index vectors are int32 (positions and slots may
-be int64).  Tensors may be strided views as long as a head's elements lie side by side.
+be int64).  The rotary size, columns of the table of ``rotate_qk``, is a multiple of 16 up to the head size, or 0.  Tensors may be strided views as long as a head's elements lie side by side.
 """
 
 from __future__ import annotations
@@ -23,7 +23,7 @@ __all__ = ["decode_attention", "prompt_attention", "rotary_table", "rotate_qk"]
 def rotary_table(rotary_dim: int, num_positions: int, *, base: float = 10000.0, factors: torch.Tensor | list[float] | None = None,
                  scale: float = 1.0, device: torch.device | str | None = None) -> torch.Tensor:
     """The fp32 table ``[num_positions, rotary_dim]`` of ``rotate_qk``: cosines, then sines, of position * base ** (-2 i / rotary_dim) /
-    factors[i] (``factors``: one per pair, for long-context models), times ``scale``.  Angles are computed in 64 bits: in 32
+    factors[i] (``factors``: one per pair, for long-context models), times ``scale``.  ``rotate_qk`` takes sizes that are multiples of 16.  Angles are computed in 64 bits: in 32
     those of far positions are off by thousandths."""
     if rotary_dim < 2 or rotary_dim % 2:
         raise ValueError(f"rotary_dim must be an even number, got {rotary_dim}")

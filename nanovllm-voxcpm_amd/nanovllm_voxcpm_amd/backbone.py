@@ -14,7 +14,7 @@ import torch
 import torch.nn as nn
 import torch.nn.functional as F
 
-from .layers.attention import AttentionBatch, PagedAttention
+from .layers.attention import AttentionBatch, PagedAttention, unserved_sizes
 from .layers.lora import LoRAMergedColumnParallelLinear, LoRAQKVParallelLinear, LoRARowParallelLinear
 
 
@@ -47,7 +47,8 @@ class DecoderLayer(nn.Module):
         kw = dict(max_loras=max_loras, max_lora_rank=rank)
         self.input_norm = RMSNorm(hidden)
         self.qkv = LoRAQKVParallelLinear(hidden, head_dim, heads, kv_heads, **kw)
-        self.attention = PagedAttention(heads, kv_heads, head_dim, **attention)
+        # (heads that the attention calls do not serve have the dense form only)
+        self.attention = PagedAttention(heads, kv_heads, head_dim, **attention) if attention or not unserved_sizes(head_dim) else None
         self.o = LoRARowParallelLinear(heads * head_dim, hidden, **kw)
         self.post_norm = RMSNorm(hidden)
         self.gate_up = LoRAMergedColumnParallelLinear(hidden, [inter, inter], **kw)
@@ -137,6 +138,8 @@ class MiniDecoder(nn.Module):
         """Zeroed caches [layers][2] of shape [blocks, block_size, kv_heads, head_dim]; the layers share one rotary table."""
         table = None
         for layer in self.layers:
+            if layer.attention is None:
+                raise ValueError(unserved_sizes(layer.head_dim))
             table = layer.attention.prepare(device, table)
         shape = (blocks, block_size, self.kv_heads, self.head_dim)
         return [(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)) for _ in self.layers]

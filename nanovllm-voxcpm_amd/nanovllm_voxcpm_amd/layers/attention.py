@@ -76,11 +76,21 @@ def build_attention_batch(new_tokens: list[int], cached_tokens: list[int], block
     return AttentionBatch(views[0], views[1], views[4].view(entries, blocks), views[2], None if decode else views[3])
 
 
+def unserved_sizes(head_size: int, rotary_dim: int | None = None) -> str:
+    """What keeps the attention calls from serving these head and rotary sizes; empty where nothing does."""
+    if head_size < 8 or head_size % 8 or head_size > 256:
+        return f"head_size = {head_size} is not a multiple of 8 up to 256"
+    rotary_dim = head_size if rotary_dim is None else rotary_dim
+    if rotary_dim < 0 or rotary_dim % 16 or rotary_dim > head_size:
+        return f"rotary_dim = {rotary_dim} is not a multiple of 16 up to the head size {head_size}"
+    return ""
+
+
 class PagedAttention(nn.Module):
     """Rotation (with per-head norms of queries and keys where ``qk_norm``), cache store and attention of one layer.
 
     ``window``, ``sinks``: a row sees the last ``window`` keys and the first ``sinks`` (0: all).  ``rotary_dim``: elements of a head that
-    are turned, all of them by default, 0 for none.  The rotary table is fp32 whatever
+    are turned, all of them by default, 0 for none; a multiple of 16, as ``head_size`` is one of 8, up to 256.  The rotary table is fp32 whatever
     the module's type and is made once per device by ``prepare``, which the first call does too if nobody did (outside
     a graph capture, then)."""
 
@@ -89,6 +99,8 @@ class PagedAttention(nn.Module):
         super().__init__()
         if num_kv_heads < 1 or num_heads % num_kv_heads:
             raise ValueError(f"{num_heads} query heads do not share {num_kv_heads} key-value heads evenly")
+        if unserved := unserved_sizes(head_size, rotary_dim):
+            raise ValueError(unserved)
         self.num_heads, self.num_kv_heads, self.head_size = num_heads, num_kv_heads, head_size
         self.eps, self.window, self.sinks, self.scale = eps, window, sinks, scale
         self.rotary_dim = head_size if rotary_dim is None else rotary_dim
