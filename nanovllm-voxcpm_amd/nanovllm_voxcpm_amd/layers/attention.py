@@ -22,7 +22,9 @@ class AttentionBatch:
 
     ``positions``, ``slot_mapping``: per row, its position in its sequence and its row in the cache counted over all blocks (-1:
     not stored, for padding).  ``block_tables``, ``context_lens``: per sequence, its blocks and its keys, the batch's rows among them.
-    ``cu_seqlens``: first row of every sequence and the end of the last; None when every sequence has one row (decode).
+    ``cu_seqlens``: first row of every sequence and the end of the last; None when every sequence has one row (decode).  ``end_position``: one more
+    than the largest position, where the host knows it; a layer refuses a batch beyond its rotary table by it.  (A position that it does not
+    speak of, copied into the tensors of a captured batch, say, turns by NaN there.)
     """
 
     positions: torch.Tensor
@@ -30,6 +32,7 @@ class AttentionBatch:
     block_tables: torch.Tensor
     context_lens: torch.Tensor
     cu_seqlens: torch.Tensor | None = None
+    end_position: int | None = None
 
 
 def build_attention_batch(new_tokens: list[int], cached_tokens: list[int], block_tables: list[list[int]], block_size: int, *,
@@ -73,7 +76,8 @@ def build_attention_batch(new_tokens: list[int], cached_tokens: list[int], block
     for part in parts:
         views.append(packed[at : at + len(part)])
         at += len(part)
-    return AttentionBatch(views[0], views[1], views[4].view(entries, blocks), views[2], None if decode else views[3])
+    return AttentionBatch(views[0], views[1], views[4].view(entries, blocks), views[2], None if decode else views[3],
+                          max([n + c for n, c in zip(new_tokens, cached_tokens) if n], default=0))
 
 
 def unserved_sizes(head_size: int, rotary_dim: int | None = None) -> str:
@@ -130,6 +134,8 @@ class PagedAttention(nn.Module):
         table = self._tables.get(qkv.device)
         if table is None:
             table = self.prepare(qkv.device)
+        if batch.end_position is not None and batch.end_position > table.size(0) and self.rotary_dim:
+            raise ValueError(f"position {batch.end_position - 1} of the batch lies behind the {table.size(0)} positions of the layer's rotary table (max_position)")
         heads = qkv.view(rows, self.num_heads + 2 * self.num_kv_heads, size)
         q, k, v = heads.split([self.num_heads, self.num_kv_heads, self.num_kv_heads], dim=1)
         q, _ = rotate_qk(q, k, batch.positions, table, q_weight=self.q_norm, k_weight=self.k_norm, eps=self.eps, interleaved=self.interleaved,

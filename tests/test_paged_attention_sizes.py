@@ -35,3 +35,17 @@ def test_a_decoder_of_other_head_sizes_keeps_its_dense_form():
         assert torch.isfinite(model(torch.randn(3, 64), caches, torch.zeros(3, dtype=torch.int64))).all()
     with pytest.raises(ValueError, match="rotary_dim = 24"):
         model.make_paged_cache(4, 16, torch.float32, "cpu")
+
+
+@pytest.mark.parametrize("new,cached,rotary_dim,refused", [([33], [0], None, True), ([32], [0], None, False), ([1, 1], [3, 32], None, True), ([1, 1], [3, 31], None, False),
+                                                           ([0, 2], [40, 0], None, False), ([33], [0], 0, False), ([], [], None, False)])
+def test_positions_behind_the_layers_table_are_refused(new, cached, rotary_dim, refused):
+    from nanovllm_voxcpm_amd.layers.attention import AttentionBatch, build_attention_batch
+
+    layer, cache = PagedAttention(2, 1, 64, max_position=32, rotary_dim=rotary_dim), torch.zeros(9, 16, 1, 64)
+    batch = build_attention_batch(new, cached, [[3 * s, 3 * s + 1, 3 * s + 2] for s in range(len(new))], 16, device="cpu", rows=sum(new) + 2)
+    with torch.no_grad(), pytest.raises(ValueError if refused else RuntimeError, match="position 32 .* 32 positions" if refused else "GPU"):
+        layer(torch.zeros(sum(new) + 2, 4 * 64), cache, cache, batch)
+    unknown = AttentionBatch(batch.positions, batch.slot_mapping, batch.block_tables, batch.context_lens, batch.cu_seqlens)
+    with torch.no_grad(), pytest.raises(RuntimeError, match="GPU"):  # (what the host does not know is the kernel's: NaN)
+        layer(torch.zeros(sum(new) + 2, 4 * 64), cache, cache, unknown)
