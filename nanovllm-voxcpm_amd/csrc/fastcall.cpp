@@ -18,6 +18,7 @@
 
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
@@ -596,7 +597,10 @@ const at::Tensor* optional_tensor(PyObject* o, bool* ok) {
   return &THPVariable_Unpack(o);
 }
 
-bool learns(const at::Tensor* t) { return t && t->requires_grad(); }
+// A derivative would be asked of a call with this tensor: it waits for a gradient or carries a tangent.
+bool learns(const at::Tensor* t) {
+  return t && ((c10::GradMode::is_enabled() && t->requires_grad()) || (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined()));
+}
 
 // `dims` dimensions with the last side by side, of the element type and on the device of q.
 bool rows_like(const at::Tensor& t, int64_t dims, const at::Tensor& q) {
@@ -658,7 +662,7 @@ PyObject* op_rotate(PyObject* const* args) {
   const at::Tensor *weights[2] = {optional_tensor(args[5], &ok), optional_tensor(args[6], &ok)};
   const at::Tensor *v = optional_tensor(args[9], &ok), *k_cache = optional_tensor(args[10], &ok), *v_cache = optional_tensor(args[11], &ok), *slots = optional_tensor(args[12], &ok);
   if (!ok || !q || !k || !positions || !table || !head_rows(*q) || !rows_like(*k, 3, *q)) return nullptr;
-  if (c10::GradMode::is_enabled() && (learns(q) || learns(k) || learns(v) || learns(weights[0]) || learns(weights[1]))) return nullptr;
+  if (learns(q) || learns(k) || learns(v) || learns(weights[0]) || learns(weights[1]) || learns(table)) return nullptr;
   const int64_t rows = q->size(0), dim = q->size(2);
   MloraRotateArgs a = {};
   bool is64 = false;
@@ -730,7 +734,7 @@ bool small_number(PyObject* o, int32_t* out) {
 // Fills in q, the keys and the pages of a call; false for what the Python path has to see to.
 bool fill_attention(MloraAttentionArgs* a, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor* tables, const at::Tensor* lens, int64_t sequences) {
   if (!head_rows(q) || sequences < 0 || sequences > INT32_MAX) return false;
-  if (c10::GradMode::is_enabled() && (learns(&q) || learns(&k) || learns(&v))) return false;
+  if (learns(&q) || learns(&k) || learns(&v)) return false;
   int64_t kv_heads;
   if (tables) {
     if (!lens || !cache_like(k, v, q) || tables->dim() != 2 || tables->scalar_type() != c10::ScalarType::Int || tables->device() != q.device() || tables->size(0) < sequences ||

@@ -6,7 +6,7 @@ token per sequence to such a cache, ``prompt_attention`` with any number of rows
 (reference: nanovllm_voxcpm/layers/attention.py:70-105).
 
 All three enqueue work on torch's current stream and neither synchronise nor read device data on the host, so they may be
-captured into a graph.  They have no backward: call them under ``torch.no_grad()`` or ``torch.inference_mode()``.
+captured into a graph.  They have no derivatives: call them under ``torch.no_grad()`` or ``torch.inference_mode()``.
 Element types are fp32, fp16 and bf16, head sizes multiples of 8 up to 256; index vectors are int32 (positions and slots may
 be int64).  The rotary size, columns of the table of ``rotate_qk``, is a multiple of 16 up to the head size, or 0.  Tensors may be strided views as long as a head's elements lie side by side.
 """
@@ -14,6 +14,7 @@ be int64).  The rotary size, columns of the table of ``rotate_qk``, is a multipl
 from __future__ import annotations
 
 import torch
+from torch.autograd import forward_ad
 
 from nanovllm_voxcpm_amd import _hip
 
@@ -84,6 +85,8 @@ def _cache(k: torch.Tensor, v: torch.Tensor, kv_heads: int | None, q: torch.Tens
 def _no_grad(*tensors: torch.Tensor | None) -> None:
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
         raise RuntimeError("the attention ops have no backward: call them under torch.no_grad() or torch.inference_mode()")
+    if not torch.is_inference_mode_enabled() and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError("the attention ops have no backward, nor a forward derivative: a tensor carries a tangent")
 
 
 def _memory(t: torch.Tensor) -> tuple[int, int, int, int]:
@@ -204,7 +207,7 @@ def rotate_qk(
             return result
     _heads(q, "q")
     _heads(k, "k", q)
-    _no_grad(q, k, v, q_weight, k_weight)
+    _no_grad(q, k, v, q_weight, k_weight, cos_sin)
     rows, dim = q.size(0), q.size(2)
     if k.size(0) != rows or k.size(2) != dim:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} differ in rows or head size")
