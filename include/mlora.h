@@ -377,7 +377,8 @@ int mlora_rotate_qk(const MloraRotateArgs* args);
 
 /* Attention of packed rows of queries over the keys and values of their sequences:
  * out = sum_j p_j v_j, p = softmax over the visible keys j of scale * q . k_j, softmax and sums in fp32, one rounding at the
- * end; in the 16-bit types p is rounded to the element type before it meets v.  Head h reads key-value head h / (heads / kv_heads).
+ * end; in the 16-bit types p is rounded to the element type before it meets v, and the sum that it is divided by is of the rounded
+ * ones.  Head sizes 64 and 128 with rows on 16 bytes run on the matrix cores; the others on a kernel that reads a key at a time and is many times slower.  Head h reads key-value head h / (heads / kv_heads).
  * The query row i of a sequence with Lq rows and Lk keys stands at position p = Lk - Lq + i.  In causal order it sees the keys
  * j <= p with j > p - window (window 0: all of them) or j < sinks; without it, all Lk.  A row that sees nothing is 0.  What lies in hidden
  * places (infinities and NaN too) does not reach the result.  Keys and values lie packed, [num_keys, kv_heads, dim], or in the pages of a

@@ -326,8 +326,10 @@ __global__ __launch_bounds__(W * 64, W == 4 ? 2 : 1) void paged_kernel(MloraAtte
 #pragma unroll
       for (int j = 0; j < kKeys / 4; ++j) s[j] = __builtin_amdgcn_exp2f(s[j] - base);
       if constexpr (sizeof(T) == 2) {
-        // The matrix cores take weights of the element type (half a step of it each; in fp32 this product would cost eight times as much).  The sum is of
-        // the rounded ones, so that what is left out of the numerator is left out of the denominator too: equal values come out as they are.
+        // The matrix cores take weights of the element type, half a step of it off each.  The sum is of the rounded ones, so that what is left out of the
+        // numerator is left out of the denominator too: equal values come out as they are.  (Held as two pieces of 16 bits, weights would be as good
+        // as fp32: an error against 64 bits of 0.0017 in bf16, of which the output's own rounding is 0.0016, in place of 0.0019; 1 stream 7.85 us and 64 streams 12.41,
+        // as they are 7.64 and 12.26.)
         float p8[8];
         const float one[8] = {1, 1, 1, 1, 1, 1, 1, 1};
 #pragma unroll
@@ -506,8 +508,13 @@ constexpr int wide(int dim) { return dim == 64 ? 16 : 8; }
 //   Many sequences and heads (or a window, which bounds what a sequence costs): a workgroup of four wavefronts each, no join.
 //   Few, and none longer than four tiles a wavefront of the wide workgroups: one of these each, no join.
 //   Else the batch's tiles are shared out in parts of four wavefronts and joined.
-// us by the device's clock, four wavefronts whole / wide workgroups / parts: 208 sequences, 2 heads of 64, window 1024: 23 / 27 / 40; 64 of up to 2048 keys, 2 heads
-// of 64: 17.1 / 13.3 / 16.5; one of 900: 10.3 / 8.2 / 10.1; 3 of up to 131072, 8 heads of 128: 1475 / 1400 / 224.
+// us by the device's clock, four wavefronts whole / wide workgroups / parts.  208 sequences, 2 heads of 64, window 1024: 23 / 27 / 40; 3 of up to 131072, 8 heads of 128:
+// 1475 / 1400 / 224.  On both sides of the lines, sequences of up to `longest` keys, 2 heads of 64, in tables as wide as the longest:
+//   units (sequences times heads)  128 | 160 | 192 | 256 | 384 at 1000 keys: 11.2 / 9.7 / 12.9 | 11.7 / 10.0 / 16.4 | 12.0 / 10.7 / 16.6 | 12.6 / 11.5 / 20.7 | 15.2 / 18.5 / 26.4
+//   (the wide ones would be faster by 9 to 14 % up to 256 units, and slower by a fifth at 384);
+//   64 tiles, 2000 | 4000 keys of 16 sequences 16.5 / 12.1 / 11.5 and 28 / 17.6 / 13.6, of 64 17.4 / 13.5 / 17.2 and 28 / 21 / 22, of 80 at 4000 29 / 23 / 30;
+//   kLongWhole, 4000 | 8000 keys of 128 sequences 32 / 30 / 36 and 67 / 70 / 72, of 32 28 / 18 / 16 and 50 / 31 / 22.
+// A table wider than the longest sequence is cut for its width: 64 streams of up to 2048 keys 12.9 us, 15.8 in tables of 9 pages of 256 and more.
 struct Way {
   int waves, target;  // target: parts wanted, 0: none
 };

@@ -191,6 +191,11 @@ struct KeyTiles {
 // units idle, shares go down to `least`, if the longest tile of rows (or, of up to twice as many, the average) is longer than that by what the second launch costs (`join`): in 16 bits a tile of keys takes
 // two thirds of a microsecond, in fp32 four to eight.  16 tokens of 4 prompts behind 2000 each 28 us (51 with shares of 32), 300 behind 1700 27 (34), 173 in fp32 behind 8450, 8 heads of 128, 83 (288);
 // 2000 tokens by themselves would take 44, without shares 35.
+// On both sides of the lines, one chunk of T tokens behind C, 16 heads of 2 of 64, us without shares / with the short ones / with shares of 32.
+//   bf16 (T / 8 workgroups without shares).  The join, T = 128, C = 250, 500, 1000: 16 / 22 / 55, 21 / 23 / 56, 32 / 27 / 53.  `few`, T = 1024, C = 100, 500, 1000: 27 / 33 / 80, 35 / 36 / 61,
+//   45 / 40 / 60.  Twice `few`, T = 2048, C = 100, 1000, 8000: 44 / 44 / 84, 63 / 54 / 68, 198 / 129 / 131; T = 2560: 54 / 52 / 86, 68 / 61 / 71, 182 / 136 / 137.  What the lines take is within
+//   16 % of the best of the three, and 21 % off at T = 1024, C = 250 (too early) and at T = 2560, C below 1000 (too late).
+//   fp32.  The join, T = 32, C = 100, 250, 500: 21 / 22 / 24, 34 / 24 / 38, 56 / 25 / 60 (too late by a third at C = 250).  `few`, T = 4096, C = 500: 465 / 362 / 361; T = 5000: 558 / 488 / 490.
 constexpr int kLeastShare = 32;
 struct ShareCosts {
   int few, least, join;  // few: workgroups without shares
@@ -618,8 +623,10 @@ __global__ __launch_bounds__(kWaves * 64, per_unit(sizeof(T) * D)) void prompt_k
 #pragma unroll
           for (int j = 0; j < 8; ++j) w8[j] = s[b][8 * c + j];
           Pack8 weights;
+          // (the matrix cores take weights of the element type, half a step of it off each: as two pieces of 16 bits they would cost this product, half of
+          // all of them, twice; the rounded weights' sum is what the outputs are divided by)
           pack8<T>(w8, weights);
-          l = dot8<T>(weights, ones, l);  // (the rounded weights' sum is what the outputs are divided by)
+          l = dot8<T>(weights, ones, l);
 #pragma unroll
           for (int d = 0; d < kBlocks; ++d) o[d] = Mma32<T>::run(v[c][d].all, weights, o[d]);
         }

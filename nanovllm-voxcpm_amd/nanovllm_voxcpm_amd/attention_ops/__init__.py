@@ -9,6 +9,11 @@ All three enqueue work on torch's current stream and neither synchronise nor rea
 captured into a graph.  They have no derivatives: call them under ``torch.no_grad()`` or ``torch.inference_mode()``.
 Element types are fp32, fp16 and bf16, head sizes multiples of 8 up to 256; index vectors are int32 (positions and slots may
 be int64).  The rotary size, columns of the table of ``rotate_qk``, is a multiple of 16 up to the head size, or 0.  Tensors may be strided views as long as a head's elements lie side by side.
+
+Attention is fast at head sizes 64 and 128 with rows that start on 16 bytes.  Every other call is right but runs on a kernel that reads
+its keys one at a time: short sequences do well there, long ones take longer than a product, a softmax and a product of torch's would
+(3 streams of 131072 keys, 8 heads of 96, 97 ms and 4; 64 of 2048 1.2 ms and 0.4).  A table of blocks wider than the longest sequence costs
+decode a second launch where its width alone asks for one (64 streams of up to 2048 keys 12.9 us, 15.8 in tables of twice that).
 """
 
 from __future__ import annotations
