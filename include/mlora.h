@@ -415,6 +415,62 @@ size_t mlora_decode_attention_workspace_bytes(const MloraAttentionArgs* args); /
 int mlora_prompt_attention(const MloraAttentionArgs* args);
 size_t mlora_prompt_attention_workspace_bytes(const MloraAttentionArgs* args);
 
+/* ---- a linear with weights in 8 bits, and the rows in front of it ---------------------------------- */
+
+/* Rows of z f, f a factor of the row, in the element type or in 8 bits: scale = max(max|z f| / 448, 2^-100), values = e4m3(z f / scale).
+ *   mlora_quantize_rows  z = x, f = 1 (8 bits only)
+ *   mlora_add_rms_norm   z = s * weight, f = rsqrt(mean(s^2) + eps), s = x + residual rounded to the element type and written to sum
+ *                        (without a residual s = x, and nothing is written)
+ *   mlora_silu_mul       z = g / (1 + exp(-g)) * u for a row g | u of 2 * width elements, f = 1
+ * fp32 throughout.  A NaN in a row, or an infinity, makes what comes of it NaN as the formulas say.  Rows may start anywhere; sum may be x's or the residual's own memory with the same strides.
+ * (reference: nanovllm_voxcpm/layers/layernorm.py:1-42, layers/activation.py:1-14) */
+typedef struct MloraRowsArgs {
+  void* stream;
+  const void* x;            /* [num_rows, width], mlora_silu_mul [num_rows, 2 width]; row strides in elements */
+  const void* residual;     /* [num_rows, width] or NULL */
+  void* sum;                /* [num_rows, width], with a residual */
+  const void* weight;       /* [width] of dtype, or fp32 with weight32 */
+  void* out;                /* [num_rows, width] of dtype, or e4m3 with scales */
+  float* scales;            /* [num_rows], or NULL: out is of dtype */
+  int64_t x_row, residual_row, sum_row, out_row;
+  int32_t num_rows, width;
+  int32_t dtype;            /* of x, residual, sum and out */
+  int32_t weight32;
+  float eps;
+} MloraRowsArgs;
+
+int mlora_add_rms_norm(const MloraRowsArgs* args);
+int mlora_silu_mul(const MloraRowsArgs* args);
+int mlora_quantize_rows(const MloraRowsArgs* args);
+
+/* A linear over e4m3 rows and weights, with the adapters of the batch's requests beside it:
+ *   y[t, n] = x_scales[t] w_scales[n] sum_k x[t, k] w[n, k] + bias[n]
+ *             + sum_j h[t, j] b[slot, n - y_col, j],  h[t, j] = x_scales[t] sum_k x[t, k] a[slot, j, k]
+ * for the slice that column n lies in (if any) and slot = token_to_slot[t] (an id outside [0, num_slots): no adapter).  Sums are
+ * fp32 and y is rounded once; h meets b as two bf16 numbers (2^-16 of it).  y lies on none of the inputs.
+ * (reference: nanovllm_voxcpm/layers/lora.py, the linears' forward, with weights in 16 bits there) */
+typedef struct MloraProjectArgs {
+  void* stream;
+  const void* x;            /* [num_rows, k] e4m3, k a multiple of 16, rows on 16 bytes, row strides in elements */
+  const void* w;            /* [n, k] e4m3, the same */
+  const float* x_scales;    /* [num_rows] */
+  const float* w_scales;    /* [n] */
+  const void* bias;         /* [n] of dtype, or NULL */
+  void* y;                  /* [num_rows, n] of dtype */
+  int64_t x_row, w_row, y_row;
+  int32_t num_rows, k, n;
+  int32_t dtype;            /* fp16 or bf16: of y, bias and the adapters */
+  int32_t num_slices;       /* 0: no adapters */
+  int32_t r, num_slots;
+  const int32_t* token_to_slot; /* [num_rows] */
+  MloraSlice slices[MLORA_MAX_SLICES]; /* a [num_slots, r, k], b [num_slots, n, r], each on 16 bytes; columns from y_col on, slice behind slice */
+  void* workspace;          /* 16-byte aligned scratch of mlora_project_workspace_bytes, needed only while the call's work is under way */
+  int64_t workspace_bytes;
+} MloraProjectArgs;
+
+int mlora_project(const MloraProjectArgs* args);
+size_t mlora_project_workspace_bytes(const MloraProjectArgs* args); /* of a filled block; reads its sizes */
+
 /* Identifier of the graph capture in progress on `stream`, 0 when the stream is not
  * capturing.  No counterpart in the reference: lets a host-side cache tell work recorded
  * into one capture from work run eagerly or recorded into another capture. */

@@ -1,0 +1,107 @@
+// What the kernels of the 8-bit linear share: its operands' layout over lanes, the adapters of a tile of rows, the intermediate of their first product.
+#pragma once
+#include "common.h"
+#include "mlora.h"
+
+namespace mlora {
+
+size_t project_workspace_bytes(const MloraProjectArgs* a);
+
+// shrink8.hip: the adapters' first product
+int launch_shrink8(const MloraProjectArgs* a);
+
+// project.hip: few rows
+int launch_project_rows(const MloraProjectArgs* a);
+
+namespace {
+
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// 16x16x128 e4m3 product: operand lane l holds row (or column) l % 16 and thirty-two elements of the contraction, which both operands order alike, so that it
+// does not matter which: here those of the 16-byte pieces 16 (l / 16) and 64 + 16 (l / 16) of the 128.  The result as in 16x16x32.
+union Eight {
+  i32x4 piece[2];
+  i32x8 all;
+};
+__device__ __forceinline__ f32x4 mma8(const Eight& a, const Eight& b, f32x4 c) {
+  return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.all, b.all, c, 0, 0, 0, 0, 0, 0);
+}
+
+// The intermediate h of the adapters, fp32 in value, lies in the workspace as two bf16 numbers hi + lo, [rows][slices][ranks rounded up to eight] each: the
+// second product multiplies 16-bit numbers, and with both pieces h is off by 2^-16 of itself there, not by 2^-8.
+__host__ __device__ inline int padded_ranks(int r) { return (r + 7) & ~7; }
+__device__ __forceinline__ void split(float h, __bf16* hi, __bf16* lo) {
+  *hi = static_cast<__bf16>(h);
+  const float rest = h - static_cast<float>(*hi);
+  *lo = static_cast<__bf16>((__float_as_uint(rest) & 0x7f800000u) == 0x7f800000u ? 0.0f : rest);  // (of an infinity or a NaN hi is all there is)
+}
+
+// A row's slot, -1 where it has no adapter.
+__device__ __forceinline__ int slot_of(const MloraProjectArgs& a, int row) {
+  if (row >= a.num_rows) return -1;
+  const int s = a.token_to_slot[row];
+  return s >= 0 && s < a.num_slots ? s : -1;
+}
+
+// The different slots of the sixteen rows whose slots lanes 0..15 (and again 16..31, ...) hold: lane i keeps the i-th; returns how many.
+__device__ __forceinline__ int different(int mine, int lane, int* list) {
+  unsigned long long left = __ballot(mine >= 0) & 0xffffull;
+  int count = 0;
+  *list = -1;
+  while (left) {
+    const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    left &= ~__ballot(mine == s);
+    if (lane == count) *list = s;
+    ++count;
+  }
+  return count;
+}
+
+// Whether one of eight 16-bit numbers is an infinity or a NaN.
+template <typename T> __device__ __forceinline__ bool any_beyond(const Pack8& p) {
+  constexpr uint32_t kExponent = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7f807f80u : 0x7c007c00u;
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t e = p.u[i] & kExponent;
+    any |= (e & 0xffffu) == (kExponent & 0xffffu) || (e >> 16) == (kExponent >> 16);
+  }
+  return any;
+}
+
+// Eight elements of B as bf16 numbers hi + lo (of bf16 adapters lo is nothing).
+template <typename T> struct BPiece;
+template <> struct BPiece<__bf16> {
+  static constexpr bool kTwo = false;
+  Pack8 hi;
+  __device__ __forceinline__ void from(const Pack8& raw) { hi = raw; }
+};
+template <> struct BPiece<_Float16> {
+  static constexpr bool kTwo = true;
+  Pack8 hi, lo;
+  __device__ __forceinline__ void from(const Pack8& raw) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      __bf16 h, l;
+      split(static_cast<float>(raw.hf[i]), &h, &l);  // (an fp16 number has eleven bits: hi + lo is all of it)
+      hi.bf[i] = h;
+      lo.bf[i] = l;
+    }
+  }
+};
+
+// What four columns from n on (of the slice; -3 .. columns - 1) of one row gain from `some` ranks, one number at a time: for pieces of B that hold infinities or NaN, which
+// a matrix product would carry to the rows of other slots (0 times them is NaN).
+template <typename T>
+__device__ inline void add_slowly(const T* b, int columns, int n, int r, int first, int some, const uint16_t* hi, const uint16_t* lo, f32x4& acc) {
+  for (int j = first; j < first + some && j < r; ++j) {
+    const float h = static_cast<float>(__builtin_bit_cast(__bf16, hi[j])) + static_cast<float>(__builtin_bit_cast(__bf16, lo[j]));
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (n + i >= 0 && n + i < columns) acc[i] += h * to_f32(b[static_cast<int64_t>(n + i) * r + j]);
+  }
+}
+
+}  // namespace
+
+}  // namespace mlora

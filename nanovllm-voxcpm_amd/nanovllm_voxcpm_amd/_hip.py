@@ -73,6 +73,11 @@ EXPORTS = (
     "mlora_decode_attention_workspace_bytes",
     "mlora_prompt_attention",
     "mlora_prompt_attention_workspace_bytes",
+    "mlora_add_rms_norm",
+    "mlora_silu_mul",
+    "mlora_quantize_rows",
+    "mlora_project",
+    "mlora_project_workspace_bytes",
     "mlora_stream_capture_id",
     "mlora_abi_version",
     "mlora_last_error",
@@ -226,6 +231,27 @@ class MloraAttentionArgs(C.Structure):
     ]
 
 
+class MloraRowsArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("stream", "x", "residual", "sum", "weight", "out", "scales")),
+        *((n, C.c_int64) for n in ("x_row", "residual_row", "sum_row", "out_row")),
+        *((n, C.c_int32) for n in ("num_rows", "width", "dtype", "weight32")),
+        ("eps", C.c_float),
+    ]
+
+
+class MloraProjectArgs(C.Structure):
+    _fields_ = [
+        *((n, C.c_void_p) for n in ("stream", "x", "w", "x_scales", "w_scales", "bias", "y")),
+        *((n, C.c_int64) for n in ("x_row", "w_row", "y_row")),
+        *((n, C.c_int32) for n in ("num_rows", "k", "n", "dtype", "num_slices", "r", "num_slots")),
+        ("token_to_slot", C.c_void_p),
+        ("slices", MloraSlice * MAX_SLICES),
+        ("workspace", C.c_void_p),
+        ("workspace_bytes", C.c_int64),
+    ]
+
+
 _LIB: C.CDLL | None = None
 _LOAD_ERROR: str | None = None
 
@@ -264,6 +290,10 @@ def load() -> C.CDLL:
         ("mlora_rotate_qk", MloraRotateArgs),
         ("mlora_decode_attention", MloraAttentionArgs),
         ("mlora_prompt_attention", MloraAttentionArgs),
+        ("mlora_add_rms_norm", MloraRowsArgs),
+        ("mlora_silu_mul", MloraRowsArgs),
+        ("mlora_quantize_rows", MloraRowsArgs),
+        ("mlora_project", MloraProjectArgs),
     ):
         fn = getattr(lib, name)
         fn.argtypes = [C.POINTER(args)]
@@ -288,6 +318,8 @@ def load() -> C.CDLL:
     lib.mlora_decode_attention_workspace_bytes.restype = C.c_size_t
     lib.mlora_prompt_attention_workspace_bytes.argtypes = [C.POINTER(MloraAttentionArgs)]
     lib.mlora_prompt_attention_workspace_bytes.restype = C.c_size_t
+    lib.mlora_project_workspace_bytes.argtypes = [C.POINTER(MloraProjectArgs)]
+    lib.mlora_project_workspace_bytes.restype = C.c_size_t
     lib.mlora_stream_capture_id.argtypes = [C.c_void_p]
     lib.mlora_stream_capture_id.restype = C.c_uint64
     _declare_diag(lib)
@@ -793,6 +825,49 @@ def rotate_qk(q, k, v, q_out, k_out, k_cache, v_cache, positions, slots, cos_sin
     args.interleaved, args.eps = interleaved, eps
     with _on(q.device):
         _check(lib.mlora_rotate_qk(C.byref(args)), "mlora_rotate_qk")
+
+
+def rows(entry: str, x, out, scales, width: int, *, residual=None, total=None, weight=None, eps: float = 0.0) -> None:
+    """One of the row operators (``entry``: its C entry point); tensors checked by ``quant_ops``."""
+    lib = load()
+    _require_cuda(x, "x")
+    args = MloraRowsArgs()
+    args.stream = _stream(x.device)
+    for name, t in (("x", x), ("residual", residual), ("sum", total), ("out", out)):
+        if t is not None:
+            setattr(args, name, t.data_ptr())
+            setattr(args, f"{name}_row", t.stride(0))
+    if scales is not None:
+        args.scales = scales.data_ptr()
+    if weight is not None:
+        args.weight, args.weight32 = weight.data_ptr(), weight.dtype == torch.float32
+    args.num_rows, args.width, args.dtype, args.eps = x.size(0), width, dtype_code(x.dtype), eps
+    with _on(x.device):
+        _check(getattr(lib, entry)(C.byref(args)), entry)
+
+
+def project(x, x_scales, w, w_scales, bias, y, a, b, columns, token_to_slot) -> None:
+    """A linear over 8-bit rows and weights with adapters (none: ``a`` empty); tensors checked by ``quant_ops.quantized_linear``."""
+    lib = load()
+    _require_cuda(x, "x")
+    args = MloraProjectArgs()
+    args.stream = _stream(x.device)
+    args.x, args.w, args.x_scales, args.w_scales, args.y = x.data_ptr(), w.data_ptr(), x_scales.data_ptr(), w_scales.data_ptr(), y.data_ptr()
+    if bias is not None:
+        args.bias = bias.data_ptr()
+    args.x_row, args.w_row, args.y_row = x.stride(0), w.stride(0), y.stride(0)
+    args.num_rows, args.k, args.n, args.dtype = x.size(0), x.size(1), w.size(0), dtype_code(y.dtype)
+    if a:
+        args.num_slices, args.r, args.num_slots = len(a), a[0].size(1), a[0].size(0)
+        args.token_to_slot = token_to_slot.data_ptr()
+        for slot, (a_of, b_of, column) in enumerate(zip(a, b, columns)):
+            args.slices[slot] = MloraSlice(a_of.data_ptr(), b_of.data_ptr(), b_of.size(1), column)
+    with _on(x.device):
+        size = lib.mlora_project_workspace_bytes(C.byref(args))
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+            args.workspace, args.workspace_bytes = workspace.data_ptr(), size
+        _check(lib.mlora_project(C.byref(args)), "mlora_project")
 
 
 def _attention_args(q, out, k, v, block_tables, context_lens, causal: bool, scale: float, window: int, sinks: int) -> MloraAttentionArgs:
