@@ -23,6 +23,7 @@
 #include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <hip/hip_runtime_api.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <cmath>
@@ -652,6 +653,19 @@ bool may_meet(const at::Tensor& a, const at::Tensor& b) {
   return column < width[0] || column + width[1] > row;
 }
 
+// The bytes between the first and the last element of two tensors overlap.
+bool may_reach(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const char* end[2];
+  const at::Tensor* const both[2] = {&a, &b};
+  for (int i = 0; i < 2; ++i) {
+    int64_t last = 1;
+    for (int64_t d = 0; d < both[i]->dim(); ++d) last += (both[i]->size(d) - 1) * both[i]->stride(d);
+    end[i] = static_cast<const char*>(both[i]->data_ptr()) + last * static_cast<int64_t>(both[i]->element_size());
+  }
+  return static_cast<const char*>(a.data_ptr()) < end[1] && static_cast<const char*>(b.data_ptr()) < end[0];
+}
+
 bool cache_like(const at::Tensor& k, const at::Tensor& v, const at::Tensor& q) {
   return rows_like(k, 4, q) && rows_like(v, 4, q) && k.sizes() == v.sizes() && k.size(0) <= INT32_MAX && k.size(1) >= 1 && k.size(1) <= INT32_MAX && k.size(3) == q.size(2);
 }
@@ -806,6 +820,145 @@ PyObject* op_prompt(PyObject* const* args) {
   return run_attention(&a, *q, args[0], args[1], args[10]);
 }
 
+// ---- rows in 8 bits and the linear over them -----------------------------------------------------------
+constexpr c10::ScalarType kEight = c10::ScalarType::Float8_e4m3fn;
+
+// [rows, width] with elements side by side, on the current device.
+bool plain_rows(const at::Tensor& t) {
+  return t.dim() == 2 && t.is_cuda() && c10::hip::current_device() == t.device().index() && t.size(0) <= INT32_MAX && t.size(1) >= 1 && t.size(1) <= INT32_MAX &&
+         (t.size(0) == 0 || t.size(1) == 1 || t.stride(1) == 1);
+}
+bool plain_vector(const at::Tensor& t, int64_t n, c10::ScalarType type, const at::Tensor& like) {
+  return t.dim() == 1 && t.size(0) == n && t.scalar_type() == type && t.device() == like.device() && t.is_contiguous();
+}
+
+// rows(address of a row operator's entry point, x, columns of x for one of the result, quantize, weight, residual, eps, sum_out)
+PyObject* op_rows(PyObject* const* args) {
+  bool ok = true;
+  const at::Tensor *x = optional_tensor(args[1], &ok), *weight = optional_tensor(args[4], &ok), *residual = optional_tensor(args[5], &ok), *sum_out = optional_tensor(args[7], &ok);
+  if (!ok || !x || !plain_rows(*x) || code_of(x->scalar_type()) < 0 || learns(x) || learns(weight) || learns(residual)) return nullptr;
+  const long per = PyLong_AsLong(args[2]);
+  const bool quantize = PyObject_IsTrue(args[3]) == 1;
+  if (per < 1 || x->size(1) % per) return nullptr;
+  MloraRowsArgs a = {};
+  a.num_rows = static_cast<int32_t>(x->size(0)); a.width = static_cast<int32_t>(x->size(1) / per);
+  a.dtype = code_of(x->scalar_type());
+  a.x = x->data_ptr(); a.x_row = x->stride(0);
+  if (weight) {
+    const bool wide = weight->scalar_type() == c10::ScalarType::Float;
+    if (!plain_vector(*weight, a.width, wide ? c10::ScalarType::Float : x->scalar_type(), *x)) return nullptr;
+    a.weight = weight->data_ptr();
+    a.weight32 = wide;
+    a.eps = static_cast<float>(PyFloat_AsDouble(args[6]));
+    if (!(a.eps >= 0)) return nullptr;
+  }
+  at::Tensor total, out, scales;
+  const auto options = x->options().requires_grad(false);
+  if (residual) {
+    if (!plain_rows(*residual) || residual->scalar_type() != x->scalar_type() || residual->sizes() != x->sizes() || residual->device() != x->device()) return nullptr;
+    a.residual = residual->data_ptr(); a.residual_row = residual->stride(0);
+    if (sum_out) {  // (in place of an input that lies apart from the other; the rest is the Python path's)
+      const at::Tensor* const in = sum_out->data_ptr() == x->data_ptr() ? x : residual;
+      if (in->data_ptr() != sum_out->data_ptr() || in->strides() != sum_out->strides() || in->sizes() != sum_out->sizes() || in->scalar_type() != sum_out->scalar_type() || may_share_memory(*in) ||
+          may_meet(*x, *residual) || (weight && may_reach(*in, *weight)))
+        return nullptr;
+      total = *sum_out;
+    } else {
+      total = at::empty(x->sizes(), options);
+    }
+    a.sum = total.data_ptr(); a.sum_row = total.stride(0);
+  } else if (sum_out) {
+    return nullptr;
+  }
+  const auto fn = reinterpret_cast<int (*)(const MloraRowsArgs*)>(PyLong_AsSize_t(args[0]));
+  if (PyErr_Occurred()) return nullptr;
+  out = at::empty({x->size(0), a.width}, quantize ? options.dtype(kEight) : options);
+  a.out = out.data_ptr(); a.out_row = out.stride(0);
+  if (quantize) {
+    scales = at::empty({x->size(0)}, options.dtype(c10::ScalarType::Float));
+    a.scales = static_cast<float*>(scales.data_ptr());
+  }
+  a.stream = stream_of(*x);
+  if (fn(&a) != 0) return nullptr;
+  PyObject* const result = PyTuple_New(3);
+  if (!result) return nullptr;
+  const at::Tensor* const parts[3] = {&out, &scales, residual ? &total : nullptr};
+  for (int i = 0; i < 3; ++i) {
+    PyObject* part = nullptr;
+    if (i == 2 && sum_out) part = Py_NewRef(args[7]);
+    else if (parts[i] && parts[i]->defined()) part = THPVariable_Wrap(*parts[i]);
+    else part = Py_NewRef(Py_None);
+    if (!part) {
+      Py_DECREF(result);
+      return nullptr;
+    }
+    PyTuple_SET_ITEM(result, i, part);
+  }
+  return result;
+}
+
+bool eight_rows(const at::Tensor* values, const at::Tensor* scales) {
+  return values && scales && plain_rows(*values) && values->scalar_type() == kEight && values->size(1) % 16 == 0 && reinterpret_cast<uintptr_t>(values->data_ptr()) % 16 == 0 &&
+         (values->size(0) <= 1 || values->stride(0) % 16 == 0) && plain_vector(*scales, values->size(0), c10::ScalarType::Float, *values) && !learns(values) && !learns(scales);
+}
+
+// linear8(address of mlora_project, of its workspace_bytes, x, x scales, w, w scales, bias, dtype, lora_a, lora_b, token_to_slot)
+PyObject* op_linear8(PyObject* const* args) {
+  bool ok = true;
+  const at::Tensor *x = optional_tensor(args[2], &ok), *xs = optional_tensor(args[3], &ok), *w = optional_tensor(args[4], &ok), *ws = optional_tensor(args[5], &ok),
+                   *bias = optional_tensor(args[6], &ok), *slots = optional_tensor(args[10], &ok);
+  if (!ok || !eight_rows(x, xs) || !eight_rows(w, ws) || w->size(1) != x->size(1) || !THPDtype_Check(args[7])) return nullptr;
+  const c10::ScalarType type = reinterpret_cast<THPDtype*>(args[7])->scalar_type;
+  if (type != c10::ScalarType::Half && type != c10::ScalarType::BFloat16) return nullptr;
+  if (bias && (!plain_vector(*bias, w->size(0), type, *x) || learns(bias))) return nullptr;
+  MloraProjectArgs a = {};
+  a.x = x->data_ptr(); a.x_scales = static_cast<const float*>(xs->data_ptr()); a.x_row = x->stride(0);
+  a.w = w->data_ptr(); a.w_scales = static_cast<const float*>(ws->data_ptr()); a.w_row = w->stride(0);
+  if (x->size(0) == 1) a.x_row = x->size(1);  // (a dimension of one has any stride)
+  if (w->size(0) == 1) a.w_row = w->size(1);
+  a.bias = bias ? bias->data_ptr() : nullptr;
+  a.num_rows = static_cast<int32_t>(x->size(0)); a.k = static_cast<int32_t>(x->size(1)); a.n = static_cast<int32_t>(w->size(0));
+  a.dtype = code_of(type);
+  const bool lora = args[8] != Py_None;
+  if (lora != (args[9] != Py_None) || lora != (slots != nullptr)) return nullptr;
+  if (lora) {
+    if (!(PyList_Check(args[8]) || PyTuple_Check(args[8])) || !(PyList_Check(args[9]) || PyTuple_Check(args[9]))) return nullptr;
+    const Py_ssize_t count = PySequence_Fast_GET_SIZE(args[8]);
+    if (count < 1 || count > MLORA_MAX_SLICES || PySequence_Fast_GET_SIZE(args[9]) != count || !plain_vector(*slots, x->size(0), c10::ScalarType::Int, *x)) return nullptr;
+    int64_t column = 0;
+    for (Py_ssize_t i = 0; i < count; ++i) {
+      const at::Tensor *of_a = optional_tensor(PySequence_Fast_GET_ITEM(args[8], i), &ok), *of_b = optional_tensor(PySequence_Fast_GET_ITEM(args[9], i), &ok);
+      if (!ok || !of_a || !of_b || of_a->dim() != 3 || of_b->dim() != 3 || learns(of_a) || learns(of_b)) return nullptr;
+      if (i == 0) {
+        if (of_a->size(0) < 1 || of_a->size(0) > MLORA_MAX_SLOTS || of_a->size(1) < 1 || of_a->size(1) > MLORA_MAX_RANK) return nullptr;
+        a.num_slots = static_cast<int32_t>(of_a->size(0)); a.r = static_cast<int32_t>(of_a->size(1));
+      }
+      for (const at::Tensor* t : {of_a, of_b})
+        if (t->scalar_type() != type || t->device() != x->device() || !t->is_contiguous() || reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 || t->size(0) != a.num_slots) return nullptr;
+      if (of_a->size(1) != a.r || of_a->size(2) != a.k || of_b->size(2) != a.r || of_b->size(1) < 1 || column + of_b->size(1) > a.n) return nullptr;
+      a.slices[i].a = of_a->data_ptr(); a.slices[i].b = of_b->data_ptr();
+      a.slices[i].n = static_cast<int32_t>(of_b->size(1)); a.slices[i].y_col = static_cast<int32_t>(column);
+      column += of_b->size(1);
+    }
+    a.num_slices = static_cast<int32_t>(count);
+    a.token_to_slot = static_cast<const int32_t*>(slots->data_ptr());
+  }
+  const auto fn = reinterpret_cast<int (*)(const MloraProjectArgs*)>(PyLong_AsSize_t(args[0]));
+  const auto bytes = reinterpret_cast<size_t (*)(const MloraProjectArgs*)>(PyLong_AsSize_t(args[1]));
+  if (PyErr_Occurred()) return nullptr;
+  const auto options = x->options().requires_grad(false);
+  at::Tensor y = at::empty({x->size(0), w->size(0)}, options.dtype(type)), workspace;
+  a.y = y.data_ptr(); a.y_row = y.stride(0);
+  a.stream = stream_of(*x);
+  if (const size_t n = bytes(&a)) {
+    workspace = at::empty({static_cast<int64_t>(n)}, options.dtype(c10::ScalarType::Byte));
+    a.workspace = workspace.data_ptr();
+    a.workspace_bytes = static_cast<int64_t>(n);
+  }
+  if (fn(&a) != 0) return nullptr;
+  return THPVariable_Wrap(std::move(y));
+}
+
 template <typename F> PyObject* run_result(F f, PyObject* const* args, Py_ssize_t nargs, Py_ssize_t want) {
   if (nargs != want) {
     PyErr_Format(PyExc_TypeError, "expected %zd arguments", want);
@@ -824,6 +977,8 @@ template <typename F> PyObject* run_result(F f, PyObject* const* args, Py_ssize_
 PyObject* py_rotate(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_rotate, args, nargs, 13); }
 PyObject* py_decode(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_decode, args, nargs, 10); }
 PyObject* py_prompt(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_prompt, args, nargs, 13); }
+PyObject* py_rows(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_rows, args, nargs, 8); }
+PyObject* py_linear8(PyObject*, PyObject* const* args, Py_ssize_t nargs) { return run_result(op_linear8, args, nargs, 11); }
 
 // ---- batch contexts --------------------------------------------------------------------------------------
 // The runs of a batch (slot ids and token counts as Python lists) as arrays.
@@ -1048,6 +1203,8 @@ PyMethodDef kMethods[] = {
     {"rotate", method(py_rotate), METH_FASTCALL, "rotate(address of mlora_rotate_qk, q, k, positions, cos_sin, q_weight, k_weight, eps, interleaved, v, k_cache, v_cache, slot_mapping) -> (q, k) or None"},
     {"decode", method(py_decode), METH_FASTCALL, "decode(address of mlora_decode_attention, of its workspace_bytes, q, k_cache, v_cache, block_tables, context_lens, scale, window, sinks) -> out or None"},
     {"prompt", method(py_prompt), METH_FASTCALL, "prompt(address of mlora_prompt_attention, of its workspace_bytes, q, k, v, cu_seqlens, cu_seqlens_k, block_tables, context_lens, causal, scale, window, sinks) -> out or None"},
+    {"rows", method(py_rows), METH_FASTCALL, "rows(address of a row operator, x, columns of x for one of the result, quantize, weight, residual, eps, sum_out) -> (out, scales, sum) or None"},
+    {"linear8", method(py_linear8), METH_FASTCALL, "linear8(address of mlora_project, of its workspace_bytes, x, x scales, w, w scales, bias, dtype, lora_a, lora_b, token_to_slot) -> out or None"},
     {"run_totals", py_run_totals, METH_VARARGS, "run_totals(slots, counts) -> (tokens, with a slot, active slots, largest slot) or None"},
     {"build_context", py_build_context, METH_VARARGS, "build_context(address of mlora_meta_build_runs, slots, counts, device, max_slots, capacity, six addresses) -> rc"},
     {"install_batch", py_install_batch, METH_NOARGS, "install_batch() -> an empty batch of slot installs"},

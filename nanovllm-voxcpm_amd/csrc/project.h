@@ -5,13 +5,19 @@
 
 namespace mlora {
 
-size_t project_workspace_bytes(const MloraProjectArgs* a);
+// Which kernel serves a call.  Rows by themselves where they are few, else tiles; with or without adapters the same, so that a row's base product is the same.
+enum { kRows, kTiles64, kTiles64x128, kTiles128 };
+int project_kind(const MloraProjectArgs* a);
 
-// shrink8.hip: the adapters' first product
-int launch_shrink8(const MloraProjectArgs* a);
+// shrink8.hip: the adapters' first product, and in front of tiles the rows' order by slot
+int launch_shrink8(const MloraProjectArgs* a, bool ordered);
 
 // project.hip: few rows
 int launch_project_rows(const MloraProjectArgs* a);
+
+// tiles8.hip: many rows
+bool tiles8_supported(const MloraProjectArgs* a);
+int launch_tiles8(const MloraProjectArgs* a, int kind);
 
 namespace {
 
@@ -29,7 +35,10 @@ __device__ __forceinline__ f32x4 mma8(const Eight& a, const Eight& b, f32x4 c) {
 
 // The intermediate h of the adapters, fp32 in value, lies in the workspace as two bf16 numbers hi + lo, [rows][slices][ranks rounded up to eight] each: the
 // second product multiplies 16-bit numbers, and with both pieces h is off by 2^-16 of itself there, not by 2^-8.
+// In front of it lie, for tiles, the rows by slot (their numbers, then their slots): h has their order then, else that of the rows.
 __host__ __device__ inline int padded_ranks(int r) { return (r + 7) & ~7; }
+__host__ __device__ inline int64_t order_bytes(int rows) { return (8ll * rows + 15) & ~15ll; }
+__device__ __forceinline__ uint16_t* intermediate(const MloraProjectArgs& a) { return reinterpret_cast<uint16_t*>(static_cast<char*>(a.workspace) + order_bytes(a.num_rows)); }
 __device__ __forceinline__ void split(float h, __bf16* hi, __bf16* lo) {
   *hi = static_cast<__bf16>(h);
   const float rest = h - static_cast<float>(*hi);

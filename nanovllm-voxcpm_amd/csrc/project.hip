@@ -48,15 +48,14 @@ template <typename T, int TF, int WAVES> __global__ __launch_bounds__(WAVES * 64
 #pragma unroll
   for (int i = 0; i < 4; ++i) scales[i] = n0 + 4 * g + i < a.n ? a.w_scales[n0 + 4 * g + i] : 0.0f;
   const int ranks = padded_ranks(a.r), pieces = ranks / 8, width = a.num_slices * ranks;
-  const uint16_t* hi = static_cast<const uint16_t*>(a.workspace);
+  const uint16_t* hi = intermediate(a);
   const uint16_t* lo = hi + static_cast<int64_t>(a.num_rows) * width;
   const bool words = a.r % 8 == 0;
 #pragma unroll
   for (int f = 0; f < TF; ++f) {
     const int t = t0 + 16 * f + m;
-    const float scale = t < a.num_rows ? a.x_scales[t] : 0.0f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[f][i] = acc[f][i] * scale * scales[i];
+    for (int i = 0; i < 4; ++i) acc[f][i] *= scales[i];
     if (!a.num_slices) continue;
     const int mine = slot_of(a, t);
     int list;
@@ -114,10 +113,11 @@ template <typename T, int TF, int WAVES> __global__ __launch_bounds__(WAVES * 64
     f32x4 sum = parts[0][f][lane];
 #pragma unroll
     for (int v = 1; v < WAVES; ++v) sum += parts[v][f][lane];
+    const float scale = a.x_scales[t];
     T* y = static_cast<T*>(a.y) + static_cast<int64_t>(t) * a.y_row + n;
 #pragma unroll
     for (int i = 0; i < 4; ++i)
-      if (n + i < a.n) y[i] = from_f32<T>(sum[i] + (a.bias ? to_f32(static_cast<const T*>(a.bias)[n + i]) : 0.0f));
+      if (n + i < a.n) y[i] = from_f32<T>(__builtin_fmaf(sum[i], scale, a.bias ? to_f32(static_cast<const T*>(a.bias)[n + i]) : 0.0f));
   }
 }
 
@@ -131,6 +131,10 @@ template <typename T> void launch(const MloraProjectArgs* a) {
 }
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+size_t workspace_bytes(const MloraProjectArgs* a) {
+  return static_cast<size_t>(order_bytes(a->num_rows)) + static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * 4;
+}
 
 int check_project(const MloraProjectArgs* a) {
   const char* const what = "mlora_project";
@@ -160,8 +164,8 @@ int check_project(const MloraProjectArgs* a) {
     end = slice.y_col + slice.n;
     if (!slice.a || !slice.b || !on16(slice.a) || !on16(slice.b)) { set_error("%s: a and b of slice %d must start on 16 bytes", what, s); return MLORA_E_INVALID; }
   }
-  if (!a->workspace || !on16(a->workspace) || a->workspace_bytes < static_cast<int64_t>(project_workspace_bytes(a))) {
-    set_error("%s: workspace of %lld bytes, %zu are needed, on 16 bytes", what, static_cast<long long>(a->workspace_bytes), project_workspace_bytes(a));
+  if (!a->workspace || !on16(a->workspace) || a->workspace_bytes < static_cast<int64_t>(workspace_bytes(a))) {
+    set_error("%s: workspace of %lld bytes, %zu are needed, on 16 bytes", what, static_cast<long long>(a->workspace_bytes), workspace_bytes(a));
     return MLORA_E_INVALID;
   }
   return 0;
@@ -169,7 +173,12 @@ int check_project(const MloraProjectArgs* a) {
 
 }  // namespace
 
-size_t project_workspace_bytes(const MloraProjectArgs* a) { return static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * 4; }
+int project_kind(const MloraProjectArgs* a) {
+  const int forced = env_int("MLORA_TILE8", 0);
+  if (forced) return forced - 1;
+  if (a->num_rows <= 256 || !tiles8_supported(a)) return kRows;
+  return a->num_rows > 2048 ? kTiles128 : kTiles64;
+}
 
 int launch_project_rows(const MloraProjectArgs* a) {
   if (a->dtype == MLORA_DTYPE_BF16) launch<__bf16>(a);
@@ -184,11 +193,12 @@ using namespace mlora;
 extern "C" int mlora_project(const MloraProjectArgs* a) {
   const int rc = check_project(a);
   if (rc) return rc == kNothingToDo ? 0 : rc;
+  const int kind = project_kind(a);
   if (a->num_slices)
-    if (const int failed = launch_shrink8(a)) return failed;
-  return launch_project_rows(a);
+    if (const int failed = launch_shrink8(a, kind != kRows)) return failed;
+  return kind == kRows ? launch_project_rows(a) : launch_tiles8(a, kind);
 }
 
 extern "C" size_t mlora_project_workspace_bytes(const MloraProjectArgs* a) {
-  return a && a->num_rows > 0 && a->n > 0 && a->num_slices > 0 && a->num_slices <= MLORA_MAX_SLICES && a->r > 0 && a->r <= MLORA_MAX_RANK ? project_workspace_bytes(a) : 0;
+  return a && a->num_rows > 0 && a->n > 0 && a->num_slices > 0 && a->num_slices <= MLORA_MAX_SLICES && a->r > 0 && a->r <= MLORA_MAX_RANK ? workspace_bytes(a) : 0;
 }

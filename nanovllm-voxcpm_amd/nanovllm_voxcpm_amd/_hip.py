@@ -855,7 +855,8 @@ def project(x, x_scales, w, w_scales, bias, y, a, b, columns, token_to_slot) -> 
     args.x, args.w, args.x_scales, args.w_scales, args.y = x.data_ptr(), w.data_ptr(), x_scales.data_ptr(), w_scales.data_ptr(), y.data_ptr()
     if bias is not None:
         args.bias = bias.data_ptr()
-    args.x_row, args.w_row, args.y_row = x.stride(0), w.stride(0), y.stride(0)
+    # (a dimension of one has any stride)
+    args.x_row, args.w_row, args.y_row = x.stride(0) if x.size(0) > 1 else x.size(1), w.stride(0) if w.size(0) > 1 else w.size(1), y.stride(0)
     args.num_rows, args.k, args.n, args.dtype = x.size(0), x.size(1), w.size(0), dtype_code(y.dtype)
     if a:
         args.num_slices, args.r, args.num_slots = len(a), a[0].size(1), a[0].size(0)

@@ -71,6 +71,11 @@ def quantize_rows(x: torch.Tensor) -> QuantizedRows:
 
     A row with a NaN is NaN altogether; one with an infinity has an infinite scale.  Of a weight ``[out, in]`` this makes what ``quantized_linear`` takes.
     """
+    fast = _hip.load_fastcall()
+    if fast is not None:  # the usual call, checked and enqueued in C++
+        result = fast.rows(_hip.entry_point("mlora_quantize_rows"), x, 1, True, None, None, 0.0, None)
+        if result is not None:
+            return QuantizedRows(result[0], result[1])
     _rows(x, "x")
     _no_grad(x)
     values, scales = _outputs(x, x.size(1), True)
@@ -94,6 +99,11 @@ def add_rms_norm(
     rounding.  The sum goes to ``sum_out`` where given (x or the residual itself are fine), else to a new tensor; without a residual
     it is x itself and nothing is written.
     """
+    fast = _hip.load_fastcall()
+    if fast is not None and weight is not None:
+        result = fast.rows(_hip.entry_point("mlora_add_rms_norm"), x, 1, quantize, weight, residual, eps, sum_out)
+        if result is not None:
+            return QuantizedRows(result[0], result[1]) if quantize else result[0], x if residual is None else result[2]
     _rows(x, "x")
     _no_grad(x, weight, residual)
     if weight.device != x.device:
@@ -124,6 +134,11 @@ def add_rms_norm(
 def silu_mul(gate_up: torch.Tensor, *, quantize: bool = False) -> torch.Tensor | QuantizedRows:
     """silu(gate) * up for rows gate | up of ``gate_up [rows, 2 * width]``, silu(g) = g / (1 + exp(-g)); in 8 bits with ``quantize``, else in the
     element type; fp32 in between, one rounding."""
+    fast = _hip.load_fastcall()
+    if fast is not None:
+        result = fast.rows(_hip.entry_point("mlora_silu_mul"), gate_up, 2, quantize, None, None, 0.0, None)
+        if result is not None:
+            return QuantizedRows(result[0], result[1]) if quantize else result[0]
     _rows(gate_up, "gate_up")
     _no_grad(gate_up)
     if gate_up.size(1) % 2:
@@ -192,6 +207,12 @@ def quantized_linear(
     ``token_to_slot``: int32 ``[T]``, ids outside the slots stand for rows without an adapter.  Sums are fp32, the result is rounded
     once.  ``in`` is a multiple of 16 and rows start on 16 bytes.
     """
+    fast = _hip.load_fastcall()
+    if fast is not None and out is None and lora_columns is None:
+        result = fast.linear8(_hip.entry_point("mlora_project"), _hip.entry_point("mlora_project_workspace_bytes"), rows[0], rows[1], weight[0], weight[1], bias, dtype,
+                              lora_a, lora_b, token_to_slot)
+        if result is not None:
+            return result
     _quantized(rows, "rows")
     _quantized(weight, "weight", rows.values.device)
     x, w = rows.values, weight.values
