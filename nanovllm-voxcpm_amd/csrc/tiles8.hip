@@ -29,7 +29,10 @@ __device__ __forceinline__ Tile tile_of(int id, int rows, int columns) {
   return Tile{strip * kStrip + in % high, in / high};
 }
 
-template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_bounds__(256, LORA || TT * NN > 8 ? 2 : 3) void tiles8_kernel(MloraProjectArgs a) {
+// Adapters: none, through LDS like the rest, or by loads of the lanes (ranks that are no multiple of eight, whose rows of B lie anywhere).
+enum { kNone, kStaged, kLoose };
+
+template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_bounds__(256, LORA || TT * NN > 8 ? 2 : 3) void tiles8_kernel(MloraProjectArgs a) {
   constexpr int BT = 32 * TT, BN = 32 * NN, kStage = (BT + BN) * 128;
   extern __shared__ char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
@@ -40,39 +43,128 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
   // the loads run two steps ahead of the products, over the tiles of this workgroup one behind the other
   int load_tile = blockIdx.x, load_k = 0, buffer = 0;
   const char *x_base = nullptr, *w_base = nullptr;
-  // rows in the order of their slots
-  const int32_t* const order = static_cast<const int32_t*>(a.workspace);
-  int coming[TT];  // the rows that this lane loads of the tile after the next
-  auto look_up = [&](int id) {
-    if (id >= total) return;
-    const int t0 = tile_of(id, rows, columns).t * BT;
-#pragma unroll
-    for (int i = 0; i < TT; ++i) {
-      const int at = t0 + (wave * TT + i) * 8 + (lane >> 3);
-      coming[i] = order[at < a.num_rows ? at : a.num_rows - 1];
-    }
-  };
   uint32_t x_off[TT], w_off[NN];  // eight rows a load, whole lines of 128 bytes; a row's 16-byte pieces lie exchanged in LDS
+  int load_t0 = 0, load_n0 = 0;
+
+  // With adapters: rows in the order of their slots.  What a tile's rows are lies in LDS for four tiles, the one that is multiplied, those that are loaded and the one
+  // behind them, which is written a tile ahead of its use by what was asked for a tile before that.
+  const int32_t* const order = static_cast<const int32_t*>(a.workspace);
+  struct Table {
+    int32_t rows[BT], slots[BT], list[BT];  // the last: the different slots among the tile's rows, `count` of them
+    int32_t count, unused[3];
+  };
+  Table* const tables = reinterpret_cast<Table*>(lds + 2 * kStage);
+  int coming_row = 0, coming_slot = -1, turn = 0;
+  auto look_up = [&](int id) {
+    if (id >= total || threadIdx.x >= BT) return;
+    const int at = tile_of(id, rows, columns).t * BT + static_cast<int>(threadIdx.x), within = at < a.num_rows ? at : a.num_rows - 1;
+    coming_row = order[within];
+    coming_slot = order[a.num_rows + within];
+    if (at >= a.num_rows) coming_slot = -1;
+  };
+  auto write_table = [&](int which) {
+    if (threadIdx.x >= BT) return;
+    tables[which & 3].rows[threadIdx.x] = coming_row;
+    tables[which & 3].slots[threadIdx.x] = coming_slot;
+  };
+  auto write_list = [&](Table& table) {  // (by one wavefront; equal slots lie side by side, -1 last)
+    int count = 0;
+#pragma unroll
+    for (int i = 0; i < BT; i += 64) {
+      const int mine = table.slots[i + lane], before = i + lane ? table.slots[i + lane - 1] : -1;
+      const bool first = mine >= 0 && mine != before;
+      const unsigned long long all = __ballot(first);
+      if (first) table.list[count + __builtin_popcountll(all & ((1ull << lane) - 1))] = mine;
+      count += __builtin_popcountll(all);
+    }
+    if (lane == 0) table.count = count;
+  };
+  // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 32 ranks at a time.
+  const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
+  struct Extra {
+    int left, slice, c;  // slots that are not done yet
+  };
+  auto meeting = [&](int s, int n0) {  // the first slice from s on that the columns meet; num_slices for none
+    while (s < a.num_slices && (n0 + BN <= a.slices[s].y_col || n0 >= a.slices[s].y_col + a.slices[s].n)) ++s;
+    return s;
+  };
+  auto first_extra = [&](const Table& table, int n0) {
+    const int s = meeting(0, n0);
+    return Extra{s < a.num_slices ? __builtin_amdgcn_readfirstlane(table.count) : 0, s, 0};
+  };
+  auto advance = [&](Extra& e, int n0) {
+    e.c += 32;
+    if (e.c < ranks) return;
+    e.c = 0;
+    e.slice = meeting(e.slice + 1, n0);
+    if (e.slice < a.num_slices) return;
+    e.slice = meeting(0, n0);
+    --e.left;
+  };
+  Extra load_extra = {0, 0, 0};
   auto aim = [&]() {
     const Tile tile = tile_of(load_tile, rows, columns);
-    const int t0 = tile.t * BT, n0 = tile.n * BN;
-    x_base = static_cast<const char*>(a.x) + (LORA ? 0 : static_cast<int64_t>(t0) * a.x_row);
-    w_base = static_cast<const char*>(a.w) + static_cast<int64_t>(n0) * a.w_row;
+    load_t0 = tile.t * BT;
+    load_n0 = tile.n * BN;
+    x_base = static_cast<const char*>(a.x) + (LORA ? 0 : static_cast<int64_t>(load_t0) * a.x_row);
+    w_base = static_cast<const char*>(a.w) + static_cast<int64_t>(load_n0) * a.w_row;
+    if constexpr (LORA) {
+      Table& table = tables[turn & 3];
 #pragma unroll
-    for (int i = 0; i < TT; ++i) {
-      const int row = (wave * TT + i) * 8 + (lane >> 3), most = a.num_rows - t0 - 1;
-      x_off[i] = static_cast<uint32_t>((LORA ? coming[i] : row < most ? row : most) * a.x_row);
+      for (int i = 0; i < TT; ++i) x_off[i] = static_cast<uint32_t>(table.rows[(wave * TT + i) * 8 + (lane >> 3)]) * static_cast<uint32_t>(a.x_row);
+      if (wave == 0) write_list(table);
+      ++turn;
+      write_table(turn);
+      look_up(load_tile + 2 * gridDim.x);
+    } else {
+#pragma unroll
+      for (int i = 0; i < TT; ++i) {
+        const int row = (wave * TT + i) * 8 + (lane >> 3), most = a.num_rows - load_t0 - 1;
+        x_off[i] = static_cast<uint32_t>((row < most ? row : most) * a.x_row);
+      }
     }
-    if constexpr (LORA) look_up(load_tile + gridDim.x);
 #pragma unroll
     for (int i = 0; i < NN; ++i) {
-      const int at = (wave * NN + i) * 8 + (lane >> 3), block = at >> 4, f = block % NN, r = at & 15, most = a.n - n0 - 1;
+      const int at = (wave * NN + i) * 8 + (lane >> 3), block = at >> 4, f = block % NN, r = at & 15, most = a.n - load_n0 - 1;
       const int row = block / NN * (16 * NN) + 32 * (f >> 1) + 8 * (r >> 2) + 4 * (f & 1) + (r & 3);
       w_off[i] = static_cast<uint32_t>((row < most ? row : most) * a.w_row);
     }
   };
+  // Of an adapters' step: hi and lo of the rows' h, B of the columns, each in blocks of sixteen rows as the lanes want them.
+  auto request_extra = [&]() {
+    const uint32_t to = home + buffer * kStage;
+    const Table& table = tables[(turn - 1) & 3];
+    const int slot = __builtin_amdgcn_readfirstlane(table.list[__builtin_amdgcn_readfirstlane(table.count) - load_extra.left]);
+    const int rank = load_extra.c + 8 * g, at = rank < ranks ? rank : 0;  // (behind the last rank: what is multiplied by zero)
+    const char* const hi = reinterpret_cast<const char*>(intermediate(a) + static_cast<int64_t>(load_t0) * width + load_extra.slice * ranks);
+    const char* const lo = hi + static_cast<int64_t>(a.num_rows) * width * 2;
+    const int wide = a.slices[load_extra.slice].n, column = a.slices[load_extra.slice].y_col;
+    const char* const b = static_cast<const char*>(a.slices[load_extra.slice].b) + static_cast<int64_t>(slot) * wide * a.r * 2;
+#pragma unroll
+    for (int i = 0; i < TT / 2; ++i) {
+      const int block = wave * (TT / 2) + i, row = block * 16 + m, most = a.num_rows - load_t0 - 1;
+      const uint32_t from = static_cast<uint32_t>(((row < most ? row : most) * width + at) * 2);
+      dma16_from(hi, from, to + block * 1024);
+      dma16_from(lo, from, to + (2 * TT + block) * 1024);
+    }
+#pragma unroll
+    for (int i = 0; i < NN / 2; ++i) {
+      const int block = wave * (NN / 2) + i, f = block % NN;
+      const int in = load_n0 + block / NN * (16 * NN) + 32 * (f >> 1) + 8 * (m >> 2) + 4 * (f & 1) + (m & 3) - column;
+      dma16_from(b, (static_cast<uint32_t>(in < 0 ? 0 : in < wide ? in : wide - 1) * static_cast<uint32_t>(a.r) + at) * 2, to + (4 * TT + block) * 1024);
+    }
+    buffer ^= 1;
+    advance(load_extra, load_n0);
+    if (!load_extra.left) load_tile += gridDim.x;
+  };
   auto request = [&]() {
     if (load_tile >= total) return;
+    if constexpr (LORA == kStaged) {
+      if (load_extra.left) {
+        request_extra();
+        return;
+      }
+    }
     if (load_k == 0) aim();  // (everything that was asked for is there: the rows to load as well)
     const uint32_t to = home + buffer * kStage;
     // piece c of row r lies at c ^ (r / 2 % 8): sixteen rows' same piece, which a product reads at once, in all banks
@@ -81,15 +173,23 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
       const int k = load_k + 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * odd));
       const uint32_t at = !TAIL || k < a.k ? k : 0;  // (behind the end of a row: its first bytes, which are multiplied by zero)
 #pragma unroll
-      for (int i = odd; i < TT; i += 2) dma16(x_base, x_off[i] + at, to + (wave * TT + i) * 1024);
+      for (int i = odd; i < TT; i += 2) dma16_from(x_base, x_off[i] + at, to + (wave * TT + i) * 1024);
 #pragma unroll
-      for (int i = odd; i < NN; i += 2) dma16(w_base, w_off[i] + at, to + (4 * TT + wave * NN + i) * 1024);
+      for (int i = odd; i < NN; i += 2) dma16_from(w_base, w_off[i] + at, to + (4 * TT + wave * NN + i) * 1024);
     }
     buffer ^= 1;
     load_k += 128;
     if (load_k >= a.k) {
       load_k = 0;
-      load_tile += gridDim.x;
+      // (the list of a tile of one step is another wavefront's work of this very request)
+      if constexpr (LORA == kStaged) {
+        if (a.k <= 128) {
+          wait_lds();
+          stage_barrier();
+        }
+        load_extra = first_extra(tables[(turn - 1) & 3], load_n0);
+      }
+      if (LORA != kStaged || !load_extra.left) load_tile += gridDim.x;
     }
   };
   const char* const x_home = lds + wt * (TT * 2048) + m * 128;
@@ -139,8 +239,15 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
     now ^= 1;
   };
 
-  if constexpr (LORA) look_up(load_tile);
+  if constexpr (LORA) {
+    look_up(load_tile);
+    write_table(0);
+    look_up(load_tile + gridDim.x);
+    wait_lds();
+    stage_barrier();
+  }
   request();
+  wait_lds();
   wait_loads<0>();
   stage_barrier();
   request();
@@ -152,12 +259,15 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
     for (int i = 0; i < 2; ++i) block_of(x_home + now * kStage, i, x01[0][i]);
   };
   begin();
-  for (int id = blockIdx.x; id < total; id += gridDim.x) {
+  int done = 0;
+  for (int id = blockIdx.x; id < total; id += gridDim.x, ++done) {
     if (LORA && id != blockIdx.x) begin();  // (again: the adapters want the registers)
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int n = 0; n < NN; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const Tile tile = tile_of(id, rows, columns);
+    const int t0 = tile.t * BT + wt * (16 * TT), n0 = tile.n * BN + wn * (16 * NN) + 8 * g;  // the lane's columns: n0 + 32 c + 0 .. 7
     for (k = 0; k < a.k;) {
       step(w[0], x01[0], w[1], x01[1]);
       if (k < a.k) {
@@ -169,20 +279,7 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
         for (int i = 0; i < 2; ++i) x01[0][i] = x01[1][i];
       }
     }
-
-    const Tile tile = tile_of(id, rows, columns);
-    const int t0 = tile.t * BT + wt * (16 * TT), n0 = tile.n * BN + wn * (16 * NN) + 8 * g;  // the lane's columns: n0 + 32 c + 0 .. 7
     const bool whole = (tile.n + 1) * BN <= a.n && ((reinterpret_cast<uintptr_t>(a.y) | static_cast<uintptr_t>(a.y_row * 2)) & 15) == 0;
-    int mine[TT];
-    if constexpr (LORA) {
-      const int32_t* const slots = order + a.num_rows;
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const int at = t0 + 16 * t + m;
-        mine[t] = slots[at < a.num_rows ? at : a.num_rows - 1];
-        if (at >= a.num_rows) mine[t] = -1;
-      }
-    }
     float scales[NN / 2][8];
 #pragma unroll
     for (int c = 0; c < NN / 2; ++c)
@@ -195,11 +292,62 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[t][n][i] *= scales[n / 2][n % 2 * 4 + i];
 
-    if constexpr (LORA) {  // every different slot among the wavefront's rows
-      const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
+    int mine[TT];
+    const Table& table = tables[done & 3];
+    if constexpr (LORA) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t) mine[t] = table.slots[wt * (16 * TT) + 16 * t + m];
+    }
+    if constexpr (LORA == kStaged) {
+      const int begin = tile.n * BN, count = __builtin_amdgcn_readfirstlane(table.count);
+      for (Extra e = first_extra(table, begin); e.left; advance(e, begin)) {
+        const int slot = __builtin_amdgcn_readfirstlane(table.list[count - e.left]);
+        const char* const stage = lds + now * kStage + lane * 16;
+        Pack8 h[TT][2], raw[NN];
+#pragma unroll
+        for (int n = 0; n < NN; ++n) raw[n].raw = load128(stage + (4 * TT + wn * NN + n) * 1024);
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          h[t][0].raw = load128(stage + (wt * TT + t) * 1024);
+          h[t][1].raw = load128(stage + (2 * TT + wt * TT + t) * 1024);
+        }
+        wait_lds();
+        wait_loads<0>();
+        stage_barrier();
+        request();
+        now ^= 1;
+        const bool some = e.c + 8 * g < ranks;
+        const int wide = a.slices[e.slice].n, from = begin + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - a.slices[e.slice].y_col;
+        BPiece<T> b[NN];
+#pragma unroll
+        for (int n = 0; n < NN; ++n) {
+          const int in = from + 32 * (n >> 1) + 4 * (n & 1);
+          if (!(some && in >= 0 && in < wide)) raw[n].raw = i32x4{0, 0, 0, 0};
+          b[n].from(raw[n]);
+        }
+#pragma unroll
+        for (int t = 0; t < TT; ++t) {
+          // (a lane's results are of one row, and come from that row's h alone: rows of other slots keep what they have, whatever is in this one's B)
+          const bool own = mine[t] == slot;
+          if (!__ballot(own)) continue;
+#pragma unroll
+          for (int v = 0; v < 2; ++v)
+            if (!some) h[t][v].raw = i32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int n = 0; n < NN; ++n) {
+            f32x4 next = Mma<__bf16>::run(b[n].hi, h[t][0], acc[t][n]);
+            next = Mma<__bf16>::run(b[n].hi, h[t][1], next);
+            if constexpr (BPiece<T>::kTwo) next = Mma<__bf16>::run(b[n].lo, h[t][0], next);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[t][n][i] = own ? next[i] : acc[t][n][i];
+          }
+        }
+      }
+    }
+
+    if constexpr (LORA == kLoose) {  // every different slot among the wavefront's rows
       const uint16_t* const hi = intermediate(a);
       const uint16_t* const lo = hi + static_cast<int64_t>(a.num_rows) * width;
-      const bool words = a.r % 8 == 0;
       const int begin = tile.n * BN + wn * (16 * NN);
       unsigned left[TT];
 #pragma unroll
@@ -238,15 +386,11 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
               const int in = begin + 32 * (n >> 1) + 8 * (m >> 2) + 4 * (n & 1) + (m & 3) - column;
               const bool there = some && in >= 0 && in < wide;
               const T* const from = b_slot + (there ? static_cast<int64_t>(in) * a.r + rank : 0);
-              if (words) {
-                raw[n].raw = load128(from);
-              } else {
-                T* e = reinterpret_cast<T*>(&raw[n]);
+              T* e = reinterpret_cast<T*>(&raw[n]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                  e[i] = from[there && rank + i < a.r ? i : 0];
-                  if (rank + i >= a.r) e[i] = static_cast<T>(0.0f);
-                }
+              for (int i = 0; i < 8; ++i) {
+                e[i] = from[there && rank + i < a.r ? i : 0];
+                if (rank + i >= a.r) e[i] = static_cast<T>(0.0f);
               }
               if (!there) raw[n].raw = i32x4{0, 0, 0, 0};
             }
@@ -281,7 +425,7 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
     for (int t = 0; t < TT; ++t) {
       const int at = t0 + 16 * t + m;
       if (at >= a.num_rows) continue;
-      const int row = LORA ? order[at] : at;
+      const int row = LORA ? table.rows[wt * (16 * TT) + 16 * t + m] : at;
       const float scale = a.x_scales[row];
       T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.y_row + n0;
 #pragma unroll
@@ -303,27 +447,27 @@ template <typename T, int TT, int NN, bool TAIL, bool LORA> __global__ __launch_
   }
 }
 
-template <typename T, int TT, int NN, bool TAIL, bool LORA> void launch(const MloraProjectArgs* a) {
+template <typename T, int TT, int NN, bool TAIL, int LORA> void launch(const MloraProjectArgs* a) {
   constexpr auto kernel = tiles8_kernel<T, TT, NN, TAIL, LORA>;
-  constexpr int bytes = 2 * (32 * TT + 32 * NN) * 128;
+  constexpr int bytes = 2 * (32 * TT + 32 * NN) * 128 + (LORA ? 4 * (3 * 32 * TT + 4) * 4 : 0);
   allow_lds<kernel>(bytes);
   const int64_t tiles = static_cast<int64_t>((a->num_rows + 32 * TT - 1) / (32 * TT)) * ((a->n + 32 * NN - 1) / (32 * NN));
   const int64_t most = 256 * (TT * NN > 8 ? 2 : TT * NN > 4 ? 3 : 4);
   kernel<<<static_cast<unsigned>(tiles < most ? tiles : most), 256, bytes, static_cast<hipStream_t>(a->stream)>>>(*a);
 }
-template <typename T, int TT, int NN> void launch_k(const MloraProjectArgs* a) {
-  if (a->num_slices) {
-    if (a->k % 128) launch<T, TT, NN, true, true>(a);
-    else launch<T, TT, NN, false, true>(a);
-  } else {
-    if (a->k % 128) launch<T, TT, NN, true, false>(a);
-    else launch<T, TT, NN, false, false>(a);
-  }
+template <typename T, int TT, int NN, int LORA> void launch_k(const MloraProjectArgs* a) {
+  if (a->k % 128) launch<T, TT, NN, true, LORA>(a);
+  else launch<T, TT, NN, false, LORA>(a);
+}
+template <typename T, int TT, int NN> void launch_lora(const MloraProjectArgs* a) {
+  if (!a->num_slices) launch_k<T, TT, NN, kNone>(a);
+  else if (a->r % 8 == 0) launch_k<T, TT, NN, kStaged>(a);
+  else launch_k<T, TT, NN, kLoose>(a);
 }
 template <typename T> void launch_size(const MloraProjectArgs* a, int kind) {
-  if (kind == kTiles128) launch_k<T, 4, 4>(a);
-  else if (kind == kTiles64x128) launch_k<T, 2, 4>(a);
-  else launch_k<T, 2, 2>(a);
+  if (kind == kTiles128) launch_lora<T, 4, 4>(a);
+  else if (kind == kTiles64x128) launch_lora<T, 2, 4>(a);
+  else launch_lora<T, 2, 2>(a);
 }
 
 }  // namespace
