@@ -35,10 +35,16 @@ __device__ __forceinline__ f32x4 mma8(const Eight& a, const Eight& b, f32x4 c) {
 
 // The intermediate h of the adapters, fp32 in value, lies in the workspace as two bf16 numbers hi + lo, [rows][slices][ranks rounded up to eight] each: the
 // second product multiplies 16-bit numbers, and with both pieces h is off by 2^-16 of itself there, not by 2^-8.
-// In front of it lie, for tiles, the rows by slot (their numbers, then their slots): h has their order then, else that of the rows.
+// In front of it lie, for tiles, the rows by slot (their numbers, then their slots; h has their order then, else that of the rows) and the groups of up to 64 rows of a slot.
 __host__ __device__ inline int padded_ranks(int r) { return (r + 7) & ~7; }
-__host__ __device__ inline int64_t order_bytes(int rows) { return (8ll * rows + 15) & ~15ll; }
-__device__ __forceinline__ uint16_t* intermediate(const MloraProjectArgs& a) { return reinterpret_cast<uint16_t*>(static_cast<char*>(a.workspace) + order_bytes(a.num_rows)); }
+constexpr int kGroup = 64;
+__host__ __device__ inline int group_capacity(int rows, int slots) { return rows / kGroup + (slots < rows ? slots : rows); }
+__host__ __device__ inline int64_t rows_bytes(int rows) { return (8ll * rows + 15) & ~15ll; }
+__host__ __device__ inline int64_t order_bytes(int rows, int slots) { return rows_bytes(rows) + 16ll * group_capacity(rows, slots); }
+__device__ __forceinline__ i32x4* group_list(const MloraProjectArgs& a) { return reinterpret_cast<i32x4*>(static_cast<char*>(a.workspace) + rows_bytes(a.num_rows)); }
+__device__ __forceinline__ uint16_t* intermediate(const MloraProjectArgs& a) {
+  return reinterpret_cast<uint16_t*>(static_cast<char*>(a.workspace) + order_bytes(a.num_rows, a.num_slots));
+}
 __device__ __forceinline__ void split(float h, __bf16* hi, __bf16* lo) {
   *hi = static_cast<__bf16>(h);
   const float rest = h - static_cast<float>(*hi);

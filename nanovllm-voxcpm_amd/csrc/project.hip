@@ -133,7 +133,7 @@ template <typename T> void launch(const MloraProjectArgs* a) {
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 size_t workspace_bytes(const MloraProjectArgs* a) {
-  return static_cast<size_t>(order_bytes(a->num_rows)) + static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * 4;
+  return static_cast<size_t>(order_bytes(a->num_rows, a->num_slots)) + static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * 4;
 }
 
 int check_project(const MloraProjectArgs* a) {

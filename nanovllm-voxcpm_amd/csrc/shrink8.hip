@@ -5,7 +5,9 @@
 // tiles' linear the rows are put in the order of their slots first, and a workgroup has 64 rows of that order, one slice, up to 64 ranks; few rows stay where they
 // are, and a workgroup has the rows of one slot, which it looks for itself, one slice and 16 ranks.
 #include "common.h"
+#include "dma.h"
 #include "launch.h"
+#include "lds.h"
 #include "project.h"
 
 namespace mlora {
@@ -100,7 +102,8 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void shrink8_
 constexpr int kOrderThreads = 1024;
 __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a) {
   __shared__ int next[MLORA_MAX_SLOTS];
-  __shared__ int sums[kOrderThreads / 64], without;
+  __shared__ int starts[MLORA_MAX_SLOTS], counts[MLORA_MAX_SLOTS], first_group[MLORA_MAX_SLOTS];
+  __shared__ int sums[kOrderThreads / 64], group_sums[kOrderThreads / 64], without;
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   static_assert(MLORA_MAX_SLOTS == kOrderThreads, "a slot a thread");
   int32_t* const order = static_cast<int32_t*>(a.workspace);
@@ -120,128 +123,199 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a
     }
     return t < a.num_rows ? atomicAdd(counter, 1) : 0;
   };
-  const int rounds = (a.num_rows + kOrderThreads - 1) / kOrderThreads;
-  for (int i = 0; i < rounds; ++i) {
-    const int t = i * kOrderThreads + tid;
-    take(slot_of(a, t), t);
+  // (sixteen rounds' slots are asked for at once: one trip to memory for up to 16384 rows)
+  constexpr int kAtOnce = 16;
+  int held[kAtOnce];
+  auto look_up = [&](int base) {
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int t = base + i * kOrderThreads + tid;
+      held[i] = base + i * kOrderThreads < a.num_rows ? a.token_to_slot[t < a.num_rows ? t : a.num_rows - 1] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i)
+      if (base + i * kOrderThreads + tid >= a.num_rows || held[i] < 0 || held[i] >= a.num_slots) held[i] = -1;
+  };
+  const bool few = a.num_rows <= kAtOnce * kOrderThreads;  // (then the first pass's places in the slots are the second's)
+  int place[kAtOnce];
+  for (int base = 0; base < a.num_rows; base += kAtOnce * kOrderThreads) {
+    look_up(base);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) place[i] = base + i * kOrderThreads < a.num_rows ? take(held[i], base + i * kOrderThreads + tid) : 0;
   }
   __syncthreads();
-  // exclusive sums over the slots
-  const int mine = next[tid];
-  int sum = mine;
+  // exclusive sums over the slots, of their rows and of the groups of up to 64 of them
+  const int mine = next[tid], groups = (mine + kGroup - 1) / kGroup;
+  int sum = mine, group_sum = groups;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
-    const int other = __shfl_up(sum, o, kWave);
-    if (lane >= o) sum += other;
+    const int other = __shfl_up(sum, o, kWave), group_other = __shfl_up(group_sum, o, kWave);
+    if (lane >= o) {
+      sum += other;
+      group_sum += group_other;
+    }
   }
-  if (lane == 63) sums[wave] = sum;
+  if (lane == 63) {
+    sums[wave] = sum;
+    group_sums[wave] = group_sum;
+  }
   __syncthreads();
-  int before = 0, all = 0;
+  int before = 0, all = 0, groups_before = 0, all_groups = 0;
 #pragma unroll
   for (int w = 0; w < kOrderThreads / 64; ++w) {
     before += w < wave ? sums[w] : 0;
+    groups_before += w < wave ? group_sums[w] : 0;
     all += sums[w];
+    all_groups += group_sums[w];
   }
-  next[tid] = before + sum - mine;
+  const int start = before + sum - mine;
+  starts[tid] = start;
+  counts[tid] = mine;
+  first_group[tid] = groups_before + group_sum - groups;
+  next[tid] = start;
   if (tid == 0) without = all;
   __syncthreads();
-  for (int i = 0; i < rounds; ++i) {
-    const int t = i * kOrderThreads + tid, s = slot_of(a, t);
-    const int at = take(s, t);
-    if (t < a.num_rows) {
-      order[at] = t;
-      slots[at] = s;
+  for (int base = 0; base < a.num_rows; base += kAtOnce * kOrderThreads) {
+    if (!few) look_up(base);
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int t = base + i * kOrderThreads + tid;
+      if (base + i * kOrderThreads >= a.num_rows) continue;
+      const int at = few ? place[i] + (held[i] >= 0 ? starts[held[i]] : all) : take(held[i], t);
+      if (t < a.num_rows) {
+        order[at] = t;
+        slots[at] = held[i];
+      }
     }
+  }
+  // the groups: a slot, its first row in the order, how many; the end is a group of none
+  i32x4* const list = group_list(a);
+  const int capacity = group_capacity(a.num_rows, a.num_slots);
+  for (int e = tid; e < capacity; e += kOrderThreads) {
+    int lo = 0, hi = MLORA_MAX_SLOTS;  // first_group[lo] <= e, the last such slot that has rows
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (first_group[mid] <= e) lo = mid;
+      else hi = mid;
+    }
+    const int in = (e - first_group[lo]) * kGroup;
+    list[e] = e < all_groups ? i32x4{lo, starts[lo] + in, counts[lo] - in < kGroup ? counts[lo] - in : kGroup, 0} : i32x4{0, 0, 0, 0};
   }
 }
 
-constexpr int kTileWaves = 4, kTileBlocks = 4;  // 64 rows
+// A group of up to 64 rows of a slot; 16 RB ranks of one slice.  Two teams of four wavefronts take every other 128 columns of K, a wavefront sixteen of the rows.  The columns of the rows and of
+// the slot's A come by direct loads into one of a team's two buffers, in whole lines, the 16-byte pieces of a row exchanged so that what the lanes read at once lies in all banks.
+// (One team, in which a wavefront waits for nobody but itself: 13.7 us where two take 8, K = 1024, 9392 rows, 2 slices of rank 64; 36 and 20 us of K = 4096, 8192 rows of 128 slots.)
+constexpr int kTeams = 2, kTileThreads = kTeams * 256;
 
-template <typename T, int RB> __global__ __launch_bounds__(kTileWaves * 64) void shrink8_tiles_kernel(MloraProjectArgs a) {
-  constexpr int kBlocks = kTileBlocks;
-  __shared__ f32x4 parts[kTileWaves][RB * kBlocks][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  const int groups = (a.r + 16 * RB - 1) / (16 * RB), slice = blockIdx.y / groups, first = (blockIdx.y - slice * groups) * 16 * RB;
+template <typename T, int RB> __global__ __launch_bounds__(kTileThreads) void shrink8_tiles_kernel(MloraProjectArgs a) {
+  constexpr int kStage = kGroup * 128 + 16 * RB * 256;
+  extern __shared__ char lds[];
+  const int everyone = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = everyone >> 2, wave = everyone & 3;
+  const int lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int ranges = (a.r + 16 * RB - 1) / (16 * RB), slice = blockIdx.y / ranges, first = (blockIdx.y - slice * ranges) * 16 * RB;
   const int32_t* const order = static_cast<const int32_t*>(a.workspace);
-  int mine[kBlocks];
-  unsigned left[kBlocks];
-  const uint8_t* x[kBlocks];
+  const i32x4 group = group_list(a)[blockIdx.x];
+  const int slot = __builtin_amdgcn_readfirstlane(group[0]), t0 = __builtin_amdgcn_readfirstlane(group[1]), rows = __builtin_amdgcn_readfirstlane(group[2]);
+  if (rows == 0) return;
+  uint32_t x_off[2], a_off[RB];
 #pragma unroll
-  for (int f = 0; f < kBlocks; ++f) {
-    const int at = blockIdx.x * (16 * kBlocks) + 16 * f + m, within = at < a.num_rows ? at : a.num_rows - 1;
-    mine[f] = at < a.num_rows ? order[a.num_rows + within] : -1;
-    left[f] = static_cast<unsigned>(__ballot(mine[f] >= 0)) & 0xffffu;
-    x[f] = static_cast<const uint8_t*>(a.x) + static_cast<int64_t>(order[within]) * a.x_row;
+  for (int i = 0; i < 2; ++i) {
+    const int row = (wave * 2 + i) * 8 + (lane >> 3);
+    x_off[i] = static_cast<uint32_t>(order[t0 + (row < rows ? row : rows - 1)]) * static_cast<uint32_t>(a.x_row) + 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * i));
   }
-  for (unsigned d = 0;; ++d) {
-    int slot = -1;
 #pragma unroll
-    for (int f = 0; f < kBlocks; ++f)
-      if (slot < 0 && left[f]) slot = __builtin_amdgcn_readlane(mine[f], __builtin_ctz(left[f]));
-    if (slot < 0) break;
-    unsigned has[kBlocks];
+  for (int i = 0; i < RB; ++i) {
+    const int at = (wave * RB + i) * 4 + (lane >> 4), j = first + at;
+    a_off[i] = static_cast<uint32_t>(j < a.r ? j : a.r - 1) * static_cast<uint32_t>(a.k) * 2 + 16 * ((lane & 15) ^ (at & 15));
+  }
+  char* const mine = lds + team * 2 * kStage;
+  const uint32_t home = lds_address(mine);
+  const int steps = (a.k + 127) / 128, turns = (steps + kTeams - 1) / kTeams;
+  const char* const x_base = static_cast<const char*>(a.x);
+  const char* const a_base = static_cast<const char*>(a.slices[slice].a) + static_cast<int64_t>(slot) * a.r * a.k * 2;
+  auto request = [&](int turn) {
+    const int k0 = (turn * kTeams + team) * 128;
+    if (k0 >= a.k) return;
+    const uint32_t to = home + (turn & 1) * kStage;
+    const bool whole = k0 + 128 <= a.k;
 #pragma unroll
-    for (int f = 0; f < kBlocks; ++f) {
-      has[f] = static_cast<unsigned>(__ballot(mine[f] == slot)) & 0xffffu;
-      left[f] &= ~has[f];
+    for (int i = 0; i < 2; ++i) {
+      uint32_t k = k0;  // (lanes behind the end of a row load its first bytes, which are multiplied by zero)
+      if (!whole && k0 + 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * i)) >= a.k) k = 0u - 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * i));
+      dma16_from(x_base, x_off[i] + k, to + (wave * 2 + i) * 1024);
     }
-    if (d % gridDim.z != blockIdx.z) continue;
-    const T* const A = static_cast<const T*>(a.slices[slice].a) + static_cast<int64_t>(slot) * a.r * a.k;
-    const T* ranks[RB];
-    f32x4 acc[RB][kBlocks];
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const int j = first + 16 * b + m;
-      ranks[b] = A + static_cast<int64_t>(j < a.r ? j : a.r - 1) * a.k;
-#pragma unroll
-      for (int f = 0; f < kBlocks; ++f) acc[b][f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < RB; ++i) {
+      const int piece = (lane & 15) ^ (((wave * RB + i) * 4 + (lane >> 4)) & 15);
+      uint32_t k = k0 * 2;
+      if (!whole && k0 + 8 * piece >= a.k) k = 0u - 16 * piece;
+      dma16_from(a_base, a_off[i] + k, to + kGroup * 128 + (wave * RB + i) * 1024);
     }
-    for (int k = wave * 64 + 16 * g; k < ((a.k + 63) & ~63); k += kTileWaves * 64) {
-      const bool there = k < a.k;  // (in the last columns lanes may have none)
-      const int at = there ? k : 0;
-      Pack8 as[RB][2];
+  };
+  f32x4 acc[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) acc[b] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  const bool some = wave * 16 < rows;
+  const char* const x_at = mine + (wave * 16 + m) * 128;
+  const char* const a_at = mine + kGroup * 128 + m * 256;
+  request(0);
+  for (int turn = 0; turn < turns; ++turn) {
+    wait_lds();
+    wait_loads<0>();
+    stage_barrier();
+    if (turn + 1 < turns) request(turn + 1);
+    const int k0 = (turn * kTeams + team) * 128, stage = (turn & 1) * kStage;
+    if (!some || k0 >= a.k) continue;
+    Pack8 as[RB][2][2];
+    i32x4 raw[2];
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      raw[p] = load128(x_at + stage + 16 * ((4 * p + g) ^ (m >> 1)));
 #pragma unroll
       for (int b = 0; b < RB; ++b)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          as[b][p].raw = load128(ranks[b] + at + 8 * p);
-          if (!there) as[b][p].raw = i32x4{0, 0, 0, 0};
+        for (int v = 0; v < 2; ++v) as[b][p][v].raw = load128(a_at + stage + b * 4096 + 16 * ((8 * p + 2 * g + v) ^ m));
+    }
+    if (k0 + 128 > a.k) {  // what lies behind the end of a row: zero on both sides
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (k0 + 64 * p + 16 * g >= a.k) {
+          raw[p] = i32x4{0, 0, 0, 0};
+#pragma unroll
+          for (int b = 0; b < RB; ++b) as[b][p][0].raw = as[b][p][1].raw = i32x4{0, 0, 0, 0};
         }
-#pragma unroll
-      for (int f = 0; f < kBlocks; ++f) {
-        if (!has[f]) continue;
-        i32x4 raw = load128(x[f] + at);
-        if (!there) raw = i32x4{0, 0, 0, 0};
-        Pack8 xs[2];
-        widen<T>(raw, xs);
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-          acc[b][f] = Mma<T>::run(as[b][0], xs[0], acc[b][f]);
-          acc[b][f] = Mma<T>::run(as[b][1], xs[1], acc[b][f]);
-        }
-      }
     }
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      mfma_settle(acc[b]);
+    for (int p = 0; p < 2; ++p) {
+      Pack8 xs[2];
+      widen<T>(raw[p], xs);
 #pragma unroll
-      for (int f = 0; f < kBlocks; ++f) parts[wave][b * kBlocks + f][lane] = acc[b][f];
+      for (int v = 0; v < 2; ++v)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) acc[b] = Mma<T>::run(as[b][p][v], xs[v], acc[b]);
     }
-    __syncthreads();
-    // a wavefront adds up every fourth block of rows
-#pragma unroll
-    for (int f = 0; f < kBlocks; ++f) {
-      if (f % kTileWaves != wave) continue;
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        f32x4 sum = parts[0][b * kBlocks + f][lane];
-#pragma unroll
-        for (int w = 1; w < kTileWaves; ++w) sum += parts[w][b * kBlocks + f][lane];
-        if (mine[f] == slot) store_h(a, blockIdx.x * (16 * kBlocks) + 16 * f + m, slice, first + 16 * b + 4 * g, sum);
-      }
-    }
-    __syncthreads();
+    mfma_settle(acc);
   }
+  // the teams' sums meet in the first one's buffers, which nobody reads any more
+  wait_lds();
+  stage_barrier();
+  f32x4* const parts = reinterpret_cast<f32x4*>(lds) + wave * (RB * 64) + lane;
+  if (team == 1) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) parts[b * 64] = acc[b];
+  }
+  __syncthreads();
+  if (team == 0 && wave * 16 + m < rows) {
+#pragma unroll
+    for (int b = 0; b < RB; ++b) store_h(a, t0 + wave * 16 + m, slice, first + 16 * b + 4 * g, acc[b] + parts[b * 64]);
+  }
+}
+
+template <typename T, int RB> void launch_tiles(const MloraProjectArgs* a, dim3 grid) {
+  constexpr int bytes = kTeams * 2 * (kGroup * 128 + 16 * RB * 256);
+  allow_lds<shrink8_tiles_kernel<T, RB>>(bytes);
+  shrink8_tiles_kernel<T, RB><<<grid, kTileThreads, bytes, static_cast<hipStream_t>(a->stream)>>>(*a);
 }
 
 template <typename T> void launch(const MloraProjectArgs* a, bool ordered) {
@@ -252,15 +326,11 @@ template <typename T> void launch(const MloraProjectArgs* a, bool ordered) {
     return;
   }
   order_kernel<<<1, kOrderThreads, 0, stream>>>(*a);
-  const unsigned tiles = static_cast<unsigned>((a->num_rows + 16 * kTileBlocks - 1) / (16 * kTileBlocks));
   const int blocks = a->r <= 16 ? 1 : a->r <= 32 ? 2 : 4;
-  const unsigned columns = static_cast<unsigned>(a->num_slices * ((a->r + 16 * blocks - 1) / (16 * blocks)));
-  unsigned together = 1024 / (tiles * columns);  // different slots of a tile side by side, as long as that is about what fills the chip
-  together = together < 1 ? 1 : together > 16 ? 16 : together;
-  const dim3 grid(tiles, columns, together);
-  if (blocks == 1) shrink8_tiles_kernel<T, 1><<<grid, kTileWaves * 64, 0, stream>>>(*a);
-  else if (blocks == 2) shrink8_tiles_kernel<T, 2><<<grid, kTileWaves * 64, 0, stream>>>(*a);
-  else shrink8_tiles_kernel<T, 4><<<grid, kTileWaves * 64, 0, stream>>>(*a);
+  const dim3 grid(static_cast<unsigned>(group_capacity(a->num_rows, a->num_slots)), static_cast<unsigned>(a->num_slices * ((a->r + 16 * blocks - 1) / (16 * blocks))));
+  if (blocks == 1) launch_tiles<T, 1>(a, grid);
+  else if (blocks == 2) launch_tiles<T, 2>(a, grid);
+  else launch_tiles<T, 4>(a, grid);
 }
 
 }  // namespace
