@@ -83,7 +83,7 @@ template <typename T, int TF, int WAVES> __global__ __launch_bounds__(WAVES * 64
         if (there && mine == slot) {
           const int64_t at = static_cast<int64_t>(t) * width + s * ranks + first;
           h[0].raw = load128(hi + at);
-          h[1].raw = load128(lo + at);
+          if constexpr (kParts<T> == 2) h[1].raw = load128(lo + at);
         }
         if (__ballot(any_beyond<T>(raw))) {  // (the four pieces of the list one behind the other)
           for (int v = 0; v < 4 && c0 + v < count * pieces; ++v) {
@@ -91,15 +91,17 @@ template <typename T, int TF, int WAVES> __global__ __launch_bounds__(WAVES * 64
             const int64_t at = static_cast<int64_t>(t) * width + s * ranks;
             if (mine == slot)
               add_slowly(static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(slot) * columns * a.r, columns, n0 + 4 * g - a.slices[s].y_col, a.r, 8 * (c0 + v - of * pieces), 8,
-                         hi + at, lo + at, acc[f]);
+                         hi + at, kParts<T> == 2 ? lo + at : nullptr, acc[f]);
           }
           continue;
         }
         BPiece<T> b;
         b.from(raw);
         acc[f] = Mma<__bf16>::run(b.hi, h[0], acc[f]);
-        acc[f] = Mma<__bf16>::run(b.hi, h[1], acc[f]);
-        if constexpr (BPiece<T>::kTwo) acc[f] = Mma<__bf16>::run(b.lo, h[0], acc[f]);
+        if constexpr (kParts<T> == 2) {
+          acc[f] = Mma<__bf16>::run(b.hi, h[1], acc[f]);
+          acc[f] = Mma<__bf16>::run(b.lo, h[0], acc[f]);
+        }
       }
     }
   }
@@ -133,7 +135,7 @@ template <typename T> void launch(const MloraProjectArgs* a) {
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 size_t workspace_bytes(const MloraProjectArgs* a) {
-  return static_cast<size_t>(order_bytes(a->num_rows, a->num_slots)) + static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * 4;
+  return static_cast<size_t>(order_bytes(a->num_rows, a->num_slots)) + static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * (a->dtype == MLORA_DTYPE_F16 ? 4 : 2);
 }
 
 int check_project(const MloraProjectArgs* a) {

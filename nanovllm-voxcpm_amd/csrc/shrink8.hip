@@ -31,16 +31,16 @@ template <> __device__ __forceinline__ void widen<_Float16>(const i32x4& in, Pac
   }
 }
 
-// h of four ranks from j on of one row, as hi and lo; ranks from r to `ranks` are zero.
-__device__ __forceinline__ void store_h(const MloraProjectArgs& a, int row, int slice, int j, const f32x4& sum) {
+// h of four ranks from j on of one row; ranks from r to `ranks` are zero.
+template <typename T> __device__ __forceinline__ void store_h(const MloraProjectArgs& a, int row, int slice, int j, const f32x4& sum) {
   const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
   if (j >= ranks) return;
   __bf16 h[4], l[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) split(j + i < a.r ? sum[i] : 0.0f, &h[i], &l[i]);
-  uint16_t* const hi = intermediate(a) + static_cast<int64_t>(row) * width + slice * ranks + j;
-  __builtin_memcpy(hi, h, 8);
-  __builtin_memcpy(hi + static_cast<int64_t>(a.num_rows) * width, l, 8);
+  uint16_t* const at = intermediate(a) + static_cast<int64_t>(row) * width + slice * ranks + j;
+  __builtin_memcpy(at, h, 8);
+  if constexpr (kParts<T> == 2) __builtin_memcpy(at + static_cast<int64_t>(a.num_rows) * width, l, 8);
 }
 
 constexpr int kRowWaves = 8, kRowBatch = kRowWaves * 64;
@@ -91,7 +91,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void shrink8_
         f32x4 sum = parts[0][lane];
 #pragma unroll
         for (int w = 1; w < kRowWaves; ++w) sum += parts[w][lane];
-        store_h(a, row, slice, first + 4 * g, sum);
+        store_h<T>(a, row, slice, first + 4 * g, sum);
       }
       __syncthreads();
     }
@@ -308,7 +308,7 @@ template <typename T, int RB> __global__ __launch_bounds__(kTileThreads) void sh
   __syncthreads();
   if (team == 0 && wave * 16 + m < rows) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b) store_h(a, t0 + wave * 16 + m, slice, first + 16 * b + 4 * g, acc[b] + parts[b * 64]);
+    for (int b = 0; b < RB; ++b) store_h<T>(a, t0 + wave * 16 + m, slice, first + 16 * b + 4 * g, acc[b] + parts[b * 64]);
   }
 }
 

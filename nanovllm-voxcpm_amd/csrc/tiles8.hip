@@ -79,10 +79,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     }
     if (lane == 0) table.count = count;
   };
-  // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 32 ranks at a time.
+  // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 64 ranks at a time, of h one part after the other.
   const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
   struct Extra {
-    int left, slice, c;  // slots that are not done yet
+    int left, slice, c, part;  // slots that are not done yet, ...
   };
   auto meeting = [&](int s, int n0) {  // the first slice from s on that the columns meet; num_slices for none
     while (s < a.num_slices && (n0 + BN <= a.slices[s].y_col || n0 >= a.slices[s].y_col + a.slices[s].n)) ++s;
@@ -90,10 +90,12 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   };
   auto first_extra = [&](const Table& table, int n0) {
     const int s = meeting(0, n0);
-    return Extra{s < a.num_slices ? __builtin_amdgcn_readfirstlane(table.count) : 0, s, 0};
+    return Extra{s < a.num_slices ? __builtin_amdgcn_readfirstlane(table.count) : 0, s, 0, 0};
   };
   auto advance = [&](Extra& e, int n0) {
-    e.c += 32;
+    if (++e.part < kParts<T>) return;
+    e.part = 0;
+    e.c += 64;
     if (e.c < ranks) return;
     e.c = 0;
     e.slice = meeting(e.slice + 1, n0);
@@ -101,7 +103,12 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     e.slice = meeting(0, n0);
     --e.left;
   };
-  Extra load_extra = {0, 0, 0};
+  Extra load_extra = {0, 0, 0, 0};
+  // The column that row `at` of the weights' part of a step is, from the tile's first on.
+  auto column_of = [&](int at) {
+    const int block = at >> 4, f = block % NN, r = at & 15;
+    return block / NN * (16 * NN) + 32 * (f >> 1) + 8 * (r >> 2) + 4 * (f & 1) + (r & 3);
+  };
   auto aim = [&]() {
     const Tile tile = tile_of(load_tile, rows, columns);
     load_t0 = tile.t * BT;
@@ -125,35 +132,46 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     }
 #pragma unroll
     for (int i = 0; i < NN; ++i) {
-      const int at = (wave * NN + i) * 8 + (lane >> 3), block = at >> 4, f = block % NN, r = at & 15, most = a.n - load_n0 - 1;
-      const int row = block / NN * (16 * NN) + 32 * (f >> 1) + 8 * (r >> 2) + 4 * (f & 1) + (r & 3);
+      const int row = column_of((wave * NN + i) * 8 + (lane >> 3)), most = a.n - load_n0 - 1;
       w_off[i] = static_cast<uint32_t>((row < most ? row : most) * a.w_row);
     }
   };
-  // Of an adapters' step: hi and lo of the rows' h, B of the columns, each in blocks of sixteen rows as the lanes want them.
-  auto request_extra = [&]() {
-    const uint32_t to = home + buffer * kStage;
-    const Table& table = tables[(turn - 1) & 3];
-    const int slot = __builtin_amdgcn_readfirstlane(table.list[__builtin_amdgcn_readfirstlane(table.count) - load_extra.left]);
-    const int rank = load_extra.c + 8 * g, at = rank < ranks ? rank : 0;  // (behind the last rank: what is multiplied by zero)
-    const char* const hi = reinterpret_cast<const char*>(intermediate(a) + static_cast<int64_t>(load_t0) * width + load_extra.slice * ranks);
-    const char* const lo = hi + static_cast<int64_t>(a.num_rows) * width * 2;
-    const int wide = a.slices[load_extra.slice].n, column = a.slices[load_extra.slice].y_col;
-    const char* const b = static_cast<const char*>(a.slices[load_extra.slice].b) + static_cast<int64_t>(slot) * wide * a.r * 2;
+  // One step's rows and columns, 128 bytes of each from byte `k` on, of which there are `bytes`.
+  auto load = [&](const char* x, const char* w, uint32_t k, uint32_t bytes, const uint32_t(&of_x)[TT], const uint32_t(&of_w)[NN]) {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(home + buffer * kStage);
+    x = uniform(x);
+    w = uniform(w);
+    // piece c of row r lies at c ^ (r / 2 % 8): sixteen rows' same piece, which a product reads at once, in all banks
 #pragma unroll
-    for (int i = 0; i < TT / 2; ++i) {
-      const int block = wave * (TT / 2) + i, row = block * 16 + m, most = a.num_rows - load_t0 - 1;
-      const uint32_t from = static_cast<uint32_t>(((row < most ? row : most) * width + at) * 2);
-      dma16_from(hi, from, to + block * 1024);
-      dma16_from(lo, from, to + (2 * TT + block) * 1024);
-    }
+    for (int odd = 0; odd < 2; ++odd) {  // (rows 8 .. 15 of a block of sixteen)
+      const uint32_t in = k + 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * odd));
+      const uint32_t at = (TAIL || LORA == kStaged) && in >= bytes ? 0 : in;  // (behind the end of a row: its first bytes, which are multiplied by zero)
 #pragma unroll
-    for (int i = 0; i < NN / 2; ++i) {
-      const int block = wave * (NN / 2) + i, f = block % NN;
-      const int in = load_n0 + block / NN * (16 * NN) + 32 * (f >> 1) + 8 * (m >> 2) + 4 * (f & 1) + (m & 3) - column;
-      dma16_from(b, (static_cast<uint32_t>(in < 0 ? 0 : in < wide ? in : wide - 1) * static_cast<uint32_t>(a.r) + at) * 2, to + (4 * TT + block) * 1024);
+      for (int i = odd; i < TT; i += 2) dma16_from(x, of_x[i] + at, to + (wave * TT + i) * 1024);
+#pragma unroll
+      for (int i = odd; i < NN; i += 2) dma16_from(w, of_w[i] + at, to + (4 * TT + wave * NN + i) * 1024);
     }
     buffer ^= 1;
+  };
+  // An adapters' step takes the rows' h for x and the columns' B for w.
+  auto request_extra = [&]() {
+    const Table& table = tables[(turn - 1) & 3];
+    const int slot = __builtin_amdgcn_readfirstlane(table.list[__builtin_amdgcn_readfirstlane(table.count) - load_extra.left]);
+    const int wide = a.slices[load_extra.slice].n, column = a.slices[load_extra.slice].y_col;
+    const char* const h = reinterpret_cast<const char*>(intermediate(a) + (static_cast<int64_t>(load_extra.part) * a.num_rows + load_t0) * width + load_extra.slice * ranks);
+    const char* const b = static_cast<const char*>(a.slices[load_extra.slice].b) + static_cast<int64_t>(slot) * wide * a.r * 2;
+    uint32_t h_off[TT], b_off[NN];
+#pragma unroll
+    for (int i = 0; i < TT; ++i) {
+      const int row = (wave * TT + i) * 8 + (lane >> 3), most = a.num_rows - load_t0 - 1;
+      h_off[i] = static_cast<uint32_t>((row < most ? row : most) * width * 2);
+    }
+#pragma unroll
+    for (int i = 0; i < NN; ++i) {
+      const int in = load_n0 + column_of((wave * NN + i) * 8 + (lane >> 3)) - column;
+      b_off[i] = static_cast<uint32_t>(in < 0 ? 0 : in < wide ? in : wide - 1) * static_cast<uint32_t>(a.r) * 2;
+    }
+    load(h, b, load_extra.c * 2, ranks * 2, h_off, b_off);
     advance(load_extra, load_n0);
     if (!load_extra.left) load_tile += gridDim.x;
   };
@@ -166,18 +184,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
       }
     }
     if (load_k == 0) aim();  // (everything that was asked for is there: the rows to load as well)
-    const uint32_t to = home + buffer * kStage;
-    // piece c of row r lies at c ^ (r / 2 % 8): sixteen rows' same piece, which a product reads at once, in all banks
-#pragma unroll
-    for (int odd = 0; odd < 2; ++odd) {  // (rows 8 .. 15 of a block of sixteen)
-      const int k = load_k + 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * odd));
-      const uint32_t at = !TAIL || k < a.k ? k : 0;  // (behind the end of a row: its first bytes, which are multiplied by zero)
-#pragma unroll
-      for (int i = odd; i < TT; i += 2) dma16_from(x_base, x_off[i] + at, to + (wave * TT + i) * 1024);
-#pragma unroll
-      for (int i = odd; i < NN; i += 2) dma16_from(w_base, w_off[i] + at, to + (4 * TT + wave * NN + i) * 1024);
-    }
-    buffer ^= 1;
+    load(x_base, w_base, load_k, a.k, x_off, w_off);
     load_k += 128;
     if (load_k >= a.k) {
       load_k = 0;
@@ -202,7 +209,27 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 
   f32x4 acc[TT][NN];
   int k = 0, now = 0;  // of the step that is multiplied
-  // One step: its blocks of w and the first two of x are in registers; leaves the next step's there.
+  // A step's first blocks into registers.
+  auto begin = [&](Eight(&w)[NN], Eight(&x01)[2], int stage) {
+#pragma unroll
+    for (int n = 0; n < NN; ++n) block_of(w_home + stage, n, w[n]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) block_of(x_home + stage, i, x01[i]);
+  };
+  // Everything of this step has been read: its buffer takes the step after the next, which is there.
+  auto turn_over = [&]() {
+    wait_lds();
+    wait_loads<0>();
+    stage_barrier();
+    request();
+  };
+  // (The last results may be read behind a branch that leaves a loop: the wait for a matrix instruction, which the next one would have to keep as well.)
+  auto settle = [&]() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // A step of the base product: its blocks of w and the first two of x are in registers; leaves the next step's there.
   auto step = [&](Eight(&w)[NN], Eight(&x01)[2], Eight(&next_w)[NN], Eight(&next_x)[2]) {
     const char* const xs = x_home + now * kStage;
     Eight x[TT];
@@ -212,16 +239,8 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     for (int t = 0; t < TT; ++t) {
       if (t + 2 < TT) block_of(xs, t + 2, x[t + 2]);
       if (t == TT - 2) {
-        // everything of this step has been read: its buffer takes the step after the next, which is there
-        wait_lds();
-        wait_loads<0>();
-        stage_barrier();
-        request();
-        const int other = (now ^ 1) * kStage;
-#pragma unroll
-        for (int n = 0; n < NN; ++n) block_of(w_home + other, n, next_w[n]);
-#pragma unroll
-        for (int i = 0; i < 2; ++i) block_of(x_home + other, i, next_x[i]);
+        turn_over();
+        begin(next_w, next_x, (now ^ 1) * kStage);
       }
       if constexpr (TAIL) {
 #pragma unroll
@@ -231,12 +250,59 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
       for (int n = 0; n < NN; ++n) acc[t][n] = mma8(w[n], x[t], acc[t][n]);
     }
-    // (the last results may be read behind a branch that leaves the loop: the wait for a matrix instruction, which the next one would have to keep as well)
-    __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
+    settle();
     k += 128;
     now ^= 1;
+  };
+  // A step of the adapters; leaves the next step's blocks where it found its own.
+  int mine[TT];
+  auto extra_step = [&](const Extra& e, int slot, int from, Eight(&w)[NN], Eight(&x01)[2]) {
+    const char* const xs = x_home + now * kStage;
+    const int wide = a.slices[e.slice].n;
+    Eight x[TT];
+    x[0] = x01[0];
+    x[1] = x01[1];
+#pragma unroll
+    for (int n = 0; n < NN; ++n) {  // (zero where there is no such rank or the column is none of the slice)
+      const int in = from + 32 * (n >> 1) + 4 * (n & 1);
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (!(e.c + 32 * p + 8 * g < ranks && in >= 0 && in < wide)) w[n].piece[p] = i32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int t = 2; t < TT; ++t) block_of(xs, t, x[t]);
+    turn_over();
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      // (a lane's results are of one row, and come from that row's h alone: rows of other slots keep what they have, whatever is in this one's B)
+      const bool own = mine[t] == slot;
+      if (!__ballot(own)) continue;
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (e.c + 32 * p + 8 * g >= ranks) x[t].piece[p] = i32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int n = 0; n < NN; ++n) {
+        f32x4 next = acc[t][n];
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          Pack8 h, raw;
+          h.raw = x[t].piece[p];
+          raw.raw = w[n].piece[p];
+          BPiece<T> b;
+          b.from(raw);
+          next = Mma<__bf16>::run(b.hi, h, next);
+          // (of the second part only the first piece counts)
+          if constexpr (kParts<T> == 2) {
+            if (e.part) b.lo.raw = i32x4{0, 0, 0, 0};
+            next = Mma<__bf16>::run(b.lo, h, next);
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][n][i] = own ? next[i] : acc[t][n][i];
+      }
+    }
+    now ^= 1;
+    begin(w, x01, now * kStage);
   };
 
   if constexpr (LORA) {
@@ -246,28 +312,22 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     wait_lds();
     stage_barrier();
   }
-  request();
-  wait_lds();
-  wait_loads<0>();
-  stage_barrier();
-  request();
+#pragma unroll 1
+  for (int i = 0; i < 2; ++i) {
+    request();
+    if (i) break;
+    wait_lds();
+    wait_loads<0>();
+    stage_barrier();
+  }
   Eight w[2][NN], x01[2][2];
-  auto begin = [&]() {
-#pragma unroll
-    for (int n = 0; n < NN; ++n) block_of(w_home + now * kStage, n, w[0][n]);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) block_of(x_home + now * kStage, i, x01[0][i]);
-  };
-  begin();
+  begin(w[0], x01[0], 0);
   int done = 0;
   for (int id = blockIdx.x; id < total; id += gridDim.x, ++done) {
-    if (LORA && id != blockIdx.x) begin();  // (again: the adapters want the registers)
 #pragma unroll
     for (int t = 0; t < TT; ++t)
 #pragma unroll
       for (int n = 0; n < NN; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    const Tile tile = tile_of(id, rows, columns);
-    const int t0 = tile.t * BT + wt * (16 * TT), n0 = tile.n * BN + wn * (16 * NN) + 8 * g;  // the lane's columns: n0 + 32 c + 0 .. 7
     for (k = 0; k < a.k;) {
       step(w[0], x01[0], w[1], x01[1]);
       if (k < a.k) {
@@ -279,72 +339,33 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
         for (int i = 0; i < 2; ++i) x01[0][i] = x01[1][i];
       }
     }
-    const bool whole = (tile.n + 1) * BN <= a.n && ((reinterpret_cast<uintptr_t>(a.y) | static_cast<uintptr_t>(a.y_row * 2)) & 15) == 0;
-    float scales[NN / 2][8];
-#pragma unroll
-    for (int c = 0; c < NN / 2; ++c)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) scales[c][i] = a.w_scales[n0 + 32 * c + i < a.n ? n0 + 32 * c + i : a.n - 1];
-#pragma unroll
-    for (int t = 0; t < TT; ++t)
-#pragma unroll
-      for (int n = 0; n < NN; ++n)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][n][i] *= scales[n / 2][n % 2 * 4 + i];
-
-    int mine[TT];
+    const Tile tile = tile_of(id, rows, columns);
+    const int t0 = tile.t * BT + wt * (16 * TT), n0 = tile.n * BN + wn * (16 * NN) + 8 * g;  // the lane's columns: n0 + 32 c + 0 .. 7
     const Table& table = tables[done & 3];
+    {
+      float scales[NN / 2][8];
+#pragma unroll
+      for (int c = 0; c < NN / 2; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) scales[c][i] = a.w_scales[n0 + 32 * c + i < a.n ? n0 + 32 * c + i : a.n - 1];
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[t][n][i] *= scales[n / 2][n % 2 * 4 + i];
+    }
     if constexpr (LORA) {
 #pragma unroll
       for (int t = 0; t < TT; ++t) mine[t] = table.slots[wt * (16 * TT) + 16 * t + m];
     }
     if constexpr (LORA == kStaged) {
-      const int begin = tile.n * BN, count = __builtin_amdgcn_readfirstlane(table.count);
-      for (Extra e = first_extra(table, begin); e.left; advance(e, begin)) {
-        const int slot = __builtin_amdgcn_readfirstlane(table.list[count - e.left]);
-        const char* const stage = lds + now * kStage + lane * 16;
-        Pack8 h[TT][2], raw[NN];
-#pragma unroll
-        for (int n = 0; n < NN; ++n) raw[n].raw = load128(stage + (4 * TT + wn * NN + n) * 1024);
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          h[t][0].raw = load128(stage + (wt * TT + t) * 1024);
-          h[t][1].raw = load128(stage + (2 * TT + wt * TT + t) * 1024);
-        }
-        wait_lds();
-        wait_loads<0>();
-        stage_barrier();
-        request();
-        now ^= 1;
-        const bool some = e.c + 8 * g < ranks;
-        const int wide = a.slices[e.slice].n, from = begin + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - a.slices[e.slice].y_col;
-        BPiece<T> b[NN];
-#pragma unroll
-        for (int n = 0; n < NN; ++n) {
-          const int in = from + 32 * (n >> 1) + 4 * (n & 1);
-          if (!(some && in >= 0 && in < wide)) raw[n].raw = i32x4{0, 0, 0, 0};
-          b[n].from(raw[n]);
-        }
-#pragma unroll
-        for (int t = 0; t < TT; ++t) {
-          // (a lane's results are of one row, and come from that row's h alone: rows of other slots keep what they have, whatever is in this one's B)
-          const bool own = mine[t] == slot;
-          if (!__ballot(own)) continue;
-#pragma unroll
-          for (int v = 0; v < 2; ++v)
-            if (!some) h[t][v].raw = i32x4{0, 0, 0, 0};
-#pragma unroll
-          for (int n = 0; n < NN; ++n) {
-            f32x4 next = Mma<__bf16>::run(b[n].hi, h[t][0], acc[t][n]);
-            next = Mma<__bf16>::run(b[n].hi, h[t][1], next);
-            if constexpr (BPiece<T>::kTwo) next = Mma<__bf16>::run(b[n].lo, h[t][0], next);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[t][n][i] = own ? next[i] : acc[t][n][i];
-          }
-        }
-      }
+      const int count = __builtin_amdgcn_readfirstlane(table.count);
+      for (Extra e = first_extra(table, tile.n * BN); e.left; advance(e, tile.n * BN))
+        extra_step(e, __builtin_amdgcn_readfirstlane(table.list[count - e.left]), tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - a.slices[e.slice].y_col, w[0], x01[0]);
+      settle();
     }
-
+    const bool whole = (tile.n + 1) * BN <= a.n && ((reinterpret_cast<uintptr_t>(a.y) | static_cast<uintptr_t>(a.y_row * 2)) & 15) == 0;
     if constexpr (LORA == kLoose) {  // every different slot among the wavefront's rows
       const uint16_t* const hi = intermediate(a);
       const uint16_t* const lo = hi + static_cast<int64_t>(a.num_rows) * width;
@@ -378,7 +399,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
               const int at = t0 + 16 * t + m < a.num_rows ? t0 + 16 * t + m : a.num_rows - 1;
               const int64_t from = static_cast<int64_t>(at) * width + s * ranks + (some ? rank : 0);
               h[t][0].raw = load128(hi + from);
-              h[t][1].raw = load128(lo + from);
+              h[t][1].raw = kParts<T> == 2 ? load128(lo + from) : i32x4{0, 0, 0, 0};
               if (!some) h[t][0].raw = h[t][1].raw = i32x4{0, 0, 0, 0};
             }
 #pragma unroll
@@ -405,8 +426,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
               for (int n = 0; n < NN; ++n) {
                 f32x4 next = Mma<__bf16>::run(b[n].hi, h[t][0], acc[t][n]);
-                next = Mma<__bf16>::run(b[n].hi, h[t][1], next);
-                if constexpr (BPiece<T>::kTwo) next = Mma<__bf16>::run(b[n].lo, h[t][0], next);
+                if constexpr (kParts<T> == 2) {
+                  next = Mma<__bf16>::run(b[n].hi, h[t][1], next);
+                  next = Mma<__bf16>::run(b[n].lo, h[t][0], next);
+                }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[t][n][i] = own ? next[i] : acc[t][n][i];
               }
@@ -460,12 +483,12 @@ template <typename T, int TT, int NN, int LORA> void launch_k(const MloraProject
   else launch<T, TT, NN, false, LORA>(a);
 }
 template <typename T, int TT, int NN> void launch_lora(const MloraProjectArgs* a) {
-  if (!a->num_slices) launch_k<T, TT, NN, kNone>(a);
-  else if (a->r % 8 == 0) launch_k<T, TT, NN, kStaged>(a);
-  else launch_k<T, TT, NN, kLoose>(a);
+  if (a->num_slices) launch_k<T, TT, NN, kStaged>(a);
+  else launch_k<T, TT, NN, kNone>(a);
 }
 template <typename T> void launch_size(const MloraProjectArgs* a, int kind) {
-  if (kind == kTiles128) launch_lora<T, 4, 4>(a);
+  if (a->num_slices && a->r % 8) launch_k<T, 2, 2, kLoose>(a);
+  else if (kind == kTiles128) launch_lora<T, 4, 4>(a);
   else if (kind == kTiles64x128) launch_lora<T, 2, 4>(a);
   else launch_lora<T, 2, 2>(a);
 }
