@@ -38,11 +38,11 @@ __device__ __forceinline__ f32x4 mma8(const Eight& a, const Eight& b, f32x4 c) {
 // fp16 ones, whose B has three bits more, a second array holds what the first leaves over, and B goes in two pieces as well: 2^-16.
 template <typename T> constexpr int kParts = 1;
 template <> constexpr int kParts<_Float16> = 2;
-// In front of it lie, for tiles, the rows by slot (their numbers, then their slots; h has their order then, else that of the rows) and the groups of up to 64 rows of a slot.
+// In front of it lie, for tiles, the rows by slot (their numbers, their slots, where the slots end; h has their order then, else that of the rows) and the groups of up to 64 rows of a slot.
 __host__ __device__ inline int padded_ranks(int r) { return (r + 7) & ~7; }
 constexpr int kGroup = 64;
 __host__ __device__ inline int group_capacity(int rows, int slots) { return rows / kGroup + (slots < rows ? slots : rows); }
-__host__ __device__ inline int64_t rows_bytes(int rows) { return (8ll * rows + 15) & ~15ll; }
+__host__ __device__ inline int64_t rows_bytes(int rows) { return (12ll * rows + 15) & ~15ll; }
 __host__ __device__ inline int64_t order_bytes(int rows, int slots) { return rows_bytes(rows) + 16ll * group_capacity(rows, slots); }
 __device__ __forceinline__ i32x4* group_list(const MloraProjectArgs& a) { return reinterpret_cast<i32x4*>(static_cast<char*>(a.workspace) + rows_bytes(a.num_rows)); }
 __device__ __forceinline__ uint16_t* intermediate(const MloraProjectArgs& a) {

@@ -107,7 +107,7 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   static_assert(MLORA_MAX_SLOTS == kOrderThreads, "a slot a thread");
   int32_t* const order = static_cast<int32_t*>(a.workspace);
-  int32_t* const slots = order + a.num_rows;
+  int32_t *const slots = order + a.num_rows, *const ends = slots + a.num_rows;
   next[tid] = 0;
   if (tid == 0) without = 0;
   __syncthreads();
@@ -185,6 +185,7 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a
       if (t < a.num_rows) {
         order[at] = t;
         slots[at] = held[i];
+        ends[at] = held[i] >= 0 ? starts[held[i]] + counts[held[i]] : a.num_rows;
       }
     }
   }

@@ -15,34 +15,46 @@ namespace {
 
 constexpr int kXcds = 8;
 
+// How the tiles of a call follow one another.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles, in strips of eight row tiles (the last one of
+// what is left), columns by columns, so that what works on an XCD at one time shares rows and columns in its L2.  The host divides: a tile's place takes no division.
+struct Grid {
+  int total, rows, columns;
+  uint32_t strip_inverse, last_inverse;  // 2^32 over the tiles of a strip, and over the height of the last one, rounded down
+};
+constexpr int kStrip = 8;
 struct Tile {
   int t, n;
 };
-// Which tile comes `id`-th.  Workgroups go to the eight XCDs in turn; each XCD gets a run of tiles, in strips of eight row tiles, columns by columns, so that what
-// works on an XCD at one time shares rows and columns in its L2.
-__device__ __forceinline__ Tile tile_of(int id, int rows, int columns) {
-  const int total = rows * columns, share = total / kXcds, more = total % kXcds, xcd = id % kXcds;
-  const int at = xcd * share + (xcd < more ? xcd : more) + id / kXcds;
-  constexpr int kStrip = 8;
-  const int strip = at / (kStrip * columns), in = at - strip * (kStrip * columns);
-  const int high = rows - strip * kStrip < kStrip ? rows - strip * kStrip : kStrip;
-  return Tile{strip * kStrip + in % high, in / high};
+__host__ __device__ __forceinline__ uint32_t inverse_of(uint32_t d) { return d > 1 ? static_cast<uint32_t>((1ull << 32) / d) : 0xffffffffu; }
+__device__ __forceinline__ uint32_t divide(uint32_t v, uint32_t d, uint32_t inverse) {  // (the product is short of v / d by less than one)
+  const uint32_t q = __umulhi(v, inverse);
+  return v - q * d >= d ? q + 1 : q;
+}
+__device__ __forceinline__ Tile tile_of(const Grid& grid, int id) {
+  const int share = grid.total / kXcds, more = grid.total % kXcds, xcd = id % kXcds;
+  const uint32_t at = xcd * share + (xcd < more ? xcd : more) + id / kXcds;
+  const uint32_t of_strip = kStrip * grid.columns, strip = divide(at, of_strip, grid.strip_inverse), in = at - strip * of_strip;
+  const uint32_t high = grid.rows - strip * kStrip < kStrip ? grid.rows - strip * kStrip : kStrip;
+  const uint32_t n = high == kStrip ? in / kStrip : divide(in, high, grid.last_inverse);
+  return Tile{static_cast<int>(strip * kStrip + in - n * high), static_cast<int>(n)};
 }
 
 // Adapters: none, through LDS like the rest, or by loads of the lanes (ranks that are no multiple of eight, whose rows of B lie anywhere).
 enum { kNone, kStaged, kLoose };
 
-template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_bounds__(256, LORA || TT * NN > 8 ? 2 : 3) void tiles8_kernel(MloraProjectArgs a) {
+template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_bounds__(256, LORA || TT * NN > 8 ? 2 : 3) void tiles8_kernel(MloraProjectArgs a, Grid grid) {
   constexpr int BT = 32 * TT, BN = 32 * NN, kStage = (BT + BN) * 128;
   extern __shared__ char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int wt = wave >> 1, wn = wave & 1;
-  const int rows = (a.num_rows + BT - 1) / BT, columns = (a.n + BN - 1) / BN, total = rows * columns;
+  const int total = grid.total;
   const uint32_t home = lds_address(lds);
 
   // the loads run two steps ahead of the products, over the tiles of this workgroup one behind the other
   int load_tile = blockIdx.x, load_k = 0, buffer = 0;
-  const char *x_base = nullptr, *w_base = nullptr;
+  bool loading = true;
+  const char *x_from = nullptr, *w_from = nullptr;  // of the load that comes next
+  uint32_t in_row[2];                               // where in its row a lane's piece lies, of rows 0 .. 7 and 8 .. 15 of sixteen
   uint32_t x_off[TT], w_off[NN];  // eight rows a load, whole lines of 128 bytes; a row's 16-byte pieces lie exchanged in LDS
   int load_t0 = 0, load_n0 = 0;
 
@@ -50,76 +62,91 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   // behind them, which is written a tile ahead of its use by what was asked for a tile before that.
   const int32_t* const order = static_cast<const int32_t*>(a.workspace);
   struct Table {
-    int32_t rows[BT], slots[BT], list[BT];  // the last: the different slots among the tile's rows, `count` of them
-    int32_t count, unused[3];
+    int32_t rows[BT], slots[BT], ends[BT];  // the last: where, from the tile's first row on, the row's slot ends
   };
   Table* const tables = reinterpret_cast<Table*>(lds + 2 * kStage);
-  int coming_row = 0, coming_slot = -1, turn = 0;
+  int coming_row = 0, coming_slot = -1, coming_end = 0, turn = 0;
   auto look_up = [&](int id) {
     if (id >= total || threadIdx.x >= BT) return;
-    const int at = tile_of(id, rows, columns).t * BT + static_cast<int>(threadIdx.x), within = at < a.num_rows ? at : a.num_rows - 1;
+    const int t0 = tile_of(grid, id).t * BT, at = t0 + static_cast<int>(threadIdx.x), within = at < a.num_rows ? at : a.num_rows - 1;
     coming_row = order[within];
     coming_slot = order[a.num_rows + within];
+    coming_end = order[2 * a.num_rows + within] - t0;
     if (at >= a.num_rows) coming_slot = -1;
   };
   auto write_table = [&](int which) {
     if (threadIdx.x >= BT) return;
     tables[which & 3].rows[threadIdx.x] = coming_row;
     tables[which & 3].slots[threadIdx.x] = coming_slot;
+    tables[which & 3].ends[threadIdx.x] = coming_end;
   };
-  auto write_list = [&](Table& table) {  // (by one wavefront; equal slots lie side by side, -1 last)
-    int count = 0;
-#pragma unroll
-    for (int i = 0; i < BT; i += 64) {
-      const int mine = table.slots[i + lane], before = i + lane ? table.slots[i + lane - 1] : -1;
-      const bool first = mine >= 0 && mine != before;
-      const unsigned long long all = __ballot(first);
-      if (first) table.list[count + __builtin_popcountll(all & ((1ull << lane) - 1))] = mine;
-      count += __builtin_popcountll(all);
-    }
-    if (lane == 0) table.count = count;
-  };
-  // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 64 ranks at a time, of h one part after the other.
+  // The slices, one a lane.
   const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
+  int slice_column = 0, slice_wide = 0, slice_b[2] = {0, 0};
+  if constexpr (LORA == kStaged) {
+    const int s = lane < a.num_slices ? lane : 0;
+    slice_column = a.slices[s].y_col;
+    slice_wide = lane < a.num_slices ? a.slices[s].n : 0;
+    const uint64_t at = reinterpret_cast<uint64_t>(a.slices[s].b);
+    slice_b[0] = static_cast<int>(at);
+    slice_b[1] = static_cast<int>(at >> 32);
+  }
+  // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 64 ranks at a time, of h one part after the other.
   struct Extra {
-    int left, slice, c, part;  // slots that are not done yet, ...
+    int row, slot, first, end, slice, c, part;  // the slot's first row in the tile (BT: no more), the slices
   };
-  auto meeting = [&](int s, int n0) {  // the first slice from s on that the columns meet; num_slices for none
-    while (s < a.num_slices && (n0 + BN <= a.slices[s].y_col || n0 >= a.slices[s].y_col + a.slices[s].n)) ++s;
-    return s;
+  auto at_row = [&](const Table& table, Extra& e, int row) {
+    e.row = row;
+    if (row >= BT) return;
+    e.slot = __builtin_amdgcn_readfirstlane(table.slots[row]);
+    if (e.slot < 0) e.row = BT;  // (rows without a slot come last)
   };
   auto first_extra = [&](const Table& table, int n0) {
-    const int s = meeting(0, n0);
-    return Extra{s < a.num_slices ? __builtin_amdgcn_readfirstlane(table.count) : 0, s, 0, 0};
+    Extra e = {BT, -1, 0, 0, 0, 0, 0};
+    const unsigned long long meeting = __ballot(slice_wide && n0 + BN > slice_column && n0 < slice_column + slice_wide);
+    if (!meeting) return e;
+    e.first = e.slice = __builtin_ctzll(meeting);
+    e.end = 64 - __builtin_clzll(meeting);
+    at_row(table, e, 0);
+    return e;
   };
-  auto advance = [&](Extra& e, int n0) {
+  auto advance = [&](const Table& table, Extra& e) {
     if (++e.part < kParts<T>) return;
     e.part = 0;
     e.c += 64;
     if (e.c < ranks) return;
     e.c = 0;
-    e.slice = meeting(e.slice + 1, n0);
-    if (e.slice < a.num_slices) return;
-    e.slice = meeting(0, n0);
-    --e.left;
+    if (++e.slice < e.end) return;
+    e.slice = e.first;
+    at_row(table, e, __builtin_amdgcn_readfirstlane(table.ends[e.row]));
   };
-  Extra load_extra = {0, 0, 0, 0};
+  Extra load_extra = {BT, -1, 0, 0, 0, 0, 0};
   // The column that row `at` of the weights' part of a step is, from the tile's first on.
   auto column_of = [&](int at) {
     const int block = at >> 4, f = block % NN, r = at & 15;
     return block / NN * (16 * NN) + 32 * (f >> 1) + 8 * (r >> 2) + 4 * (f & 1) + (r & 3);
   };
+  // Piece c of a row's 128 bytes lies in LDS at c ^ (r / 2 % 8): sixteen rows' same piece, which a product reads at once, in all banks.  `bytes`: of a row; lanes behind its
+  // end load its first ones, which are multiplied by zero.
+  auto place = [&](uint32_t k, uint32_t bytes, bool ends) {
+#pragma unroll
+    for (int odd = 0; odd < 2; ++odd) {
+      const uint32_t in = k + 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * odd));
+      in_row[odd] = ends && in >= bytes ? 0 : in;
+    }
+  };
   auto aim = [&]() {
-    const Tile tile = tile_of(load_tile, rows, columns);
+    const Tile tile = tile_of(grid, load_tile);
     load_t0 = tile.t * BT;
     load_n0 = tile.n * BN;
-    x_base = static_cast<const char*>(a.x) + (LORA ? 0 : static_cast<int64_t>(load_t0) * a.x_row);
-    w_base = static_cast<const char*>(a.w) + static_cast<int64_t>(load_n0) * a.w_row;
+    load_k = 0;
+    place(0, a.k, TAIL);
+    x_from = static_cast<const char*>(a.x) + (LORA ? 0 : static_cast<int64_t>(load_t0) * a.x_row);
+    w_from = static_cast<const char*>(a.w) + static_cast<int64_t>(load_n0) * a.w_row;
     if constexpr (LORA) {
-      Table& table = tables[turn & 3];
+      const Table& table = tables[turn & 3];
 #pragma unroll
       for (int i = 0; i < TT; ++i) x_off[i] = static_cast<uint32_t>(table.rows[(wave * TT + i) * 8 + (lane >> 3)]) * static_cast<uint32_t>(a.x_row);
-      if (wave == 0) write_list(table);
       ++turn;
       write_table(turn);
       look_up(load_tile + 2 * gridDim.x);
@@ -136,68 +163,59 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
       w_off[i] = static_cast<uint32_t>((row < most ? row : most) * a.w_row);
     }
   };
-  // One step's rows and columns, 128 bytes of each from byte `k` on, of which there are `bytes`.
-  auto load = [&](const char* x, const char* w, uint32_t k, uint32_t bytes, const uint32_t(&of_x)[TT], const uint32_t(&of_w)[NN]) {
-    const uint32_t to = __builtin_amdgcn_readfirstlane(home + buffer * kStage);
-    x = uniform(x);
-    w = uniform(w);
-    // piece c of row r lies at c ^ (r / 2 % 8): sixteen rows' same piece, which a product reads at once, in all banks
-#pragma unroll
-    for (int odd = 0; odd < 2; ++odd) {  // (rows 8 .. 15 of a block of sixteen)
-      const uint32_t in = k + 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * odd));
-      const uint32_t at = (TAIL || LORA == kStaged) && in >= bytes ? 0 : in;  // (behind the end of a row: its first bytes, which are multiplied by zero)
-#pragma unroll
-      for (int i = odd; i < TT; i += 2) dma16_from(x, of_x[i] + at, to + (wave * TT + i) * 1024);
-#pragma unroll
-      for (int i = odd; i < NN; i += 2) dma16_from(w, of_w[i] + at, to + (4 * TT + wave * NN + i) * 1024);
-    }
-    buffer ^= 1;
-  };
   // An adapters' step takes the rows' h for x and the columns' B for w.
-  auto request_extra = [&]() {
-    const Table& table = tables[(turn - 1) & 3];
-    const int slot = __builtin_amdgcn_readfirstlane(table.list[__builtin_amdgcn_readfirstlane(table.count) - load_extra.left]);
-    const int wide = a.slices[load_extra.slice].n, column = a.slices[load_extra.slice].y_col;
-    const char* const h = reinterpret_cast<const char*>(intermediate(a) + (static_cast<int64_t>(load_extra.part) * a.num_rows + load_t0) * width + load_extra.slice * ranks);
-    const char* const b = static_cast<const char*>(a.slices[load_extra.slice].b) + static_cast<int64_t>(slot) * wide * a.r * 2;
-    uint32_t h_off[TT], b_off[NN];
+  auto aim_extra = [&]() {
+    const int wide = __builtin_amdgcn_readlane(slice_wide, load_extra.slice), column = __builtin_amdgcn_readlane(slice_column, load_extra.slice);
+    const uint64_t b_of = static_cast<uint32_t>(__builtin_amdgcn_readlane(slice_b[0], load_extra.slice)) |
+                          static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(slice_b[1], load_extra.slice))) << 32;
+    x_from = reinterpret_cast<const char*>(intermediate(a) + (static_cast<int64_t>(load_extra.part) * a.num_rows + load_t0) * width + load_extra.slice * ranks);
+    w_from = reinterpret_cast<const char*>(b_of) + static_cast<int64_t>(load_extra.slot) * wide * a.r * 2;
+    place(load_extra.c * 2, ranks * 2, true);
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
       const int row = (wave * TT + i) * 8 + (lane >> 3), most = a.num_rows - load_t0 - 1;
-      h_off[i] = static_cast<uint32_t>((row < most ? row : most) * width * 2);
+      x_off[i] = static_cast<uint32_t>((row < most ? row : most) * width * 2);
     }
 #pragma unroll
     for (int i = 0; i < NN; ++i) {
       const int in = load_n0 + column_of((wave * NN + i) * 8 + (lane >> 3)) - column;
-      b_off[i] = static_cast<uint32_t>(in < 0 ? 0 : in < wide ? in : wide - 1) * static_cast<uint32_t>(a.r) * 2;
+      w_off[i] = static_cast<uint32_t>(in < 0 ? 0 : in < wide ? in : wide - 1) * static_cast<uint32_t>(a.r) * 2;
     }
-    load(h, b, load_extra.c * 2, ranks * 2, h_off, b_off);
-    advance(load_extra, load_n0);
-    if (!load_extra.left) load_tile += gridDim.x;
   };
-  auto request = [&]() {
-    if (load_tile >= total) return;
+  // What the next load takes, behind the one before it; between steps, since its branches would cut a step's code in pieces.
+  auto prepare = [&]() {
+    if (load_extra.row >= BT && load_k + 128 < a.k) {
+      load_k += 128;
+      if constexpr (TAIL) {
+        place(load_k, a.k, true);
+      } else {
+        in_row[0] += 128;
+        in_row[1] += 128;
+      }
+      return;
+    }
     if constexpr (LORA == kStaged) {
-      if (load_extra.left) {
-        request_extra();
+      const Table& table = tables[(turn - 1) & 3];
+      if (load_extra.row >= BT) load_extra = first_extra(table, load_n0);
+      else advance(table, load_extra);
+      if (load_extra.row < BT) {
+        aim_extra();
         return;
       }
     }
-    if (load_k == 0) aim();  // (everything that was asked for is there: the rows to load as well)
-    load(x_base, w_base, load_k, a.k, x_off, w_off);
-    load_k += 128;
-    if (load_k >= a.k) {
-      load_k = 0;
-      // (the list of a tile of one step is another wavefront's work of this very request)
-      if constexpr (LORA == kStaged) {
-        if (a.k <= 128) {
-          wait_lds();
-          stage_barrier();
-        }
-        load_extra = first_extra(tables[(turn - 1) & 3], load_n0);
-      }
-      if (LORA != kStaged || !load_extra.left) load_tile += gridDim.x;
-    }
+    load_tile += gridDim.x;
+    loading = load_tile < total;
+    if (loading) aim();
+  };
+  auto request = [&]() {
+    if (!loading) return;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(home + buffer * kStage);
+    const char *const x = uniform(x_from), *const w = uniform(w_from);
+#pragma unroll
+    for (int i = 0; i < TT; ++i) dma16_from(x, x_off[i] + in_row[i & 1], to + (wave * TT + i) * 1024);
+#pragma unroll
+    for (int i = 0; i < NN; ++i) dma16_from(w, w_off[i] + in_row[i & 1], to + (4 * TT + wave * NN + i) * 1024);
+    buffer ^= 1;
   };
   const char* const x_home = lds + wt * (TT * 2048) + m * 128;
   const char* const w_home = lds + (2 * TT + wn * NN) * 2048 + m * 128;
@@ -256,9 +274,9 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   };
   // A step of the adapters; leaves the next step's blocks where it found its own.
   int mine[TT];
-  auto extra_step = [&](const Extra& e, int slot, int from, Eight(&w)[NN], Eight(&x01)[2]) {
+  auto extra_step = [&](const Extra& e, int from, Eight(&w)[NN], Eight(&x01)[2]) {
     const char* const xs = x_home + now * kStage;
-    const int wide = a.slices[e.slice].n;
+    const int wide = __builtin_amdgcn_readlane(slice_wide, e.slice);
     Eight x[TT];
     x[0] = x01[0];
     x[1] = x01[1];
@@ -275,7 +293,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
       // (a lane's results are of one row, and come from that row's h alone: rows of other slots keep what they have, whatever is in this one's B)
-      const bool own = mine[t] == slot;
+      const bool own = mine[t] == e.slot;
       if (!__ballot(own)) continue;
 #pragma unroll
       for (int p = 0; p < 2; ++p)
@@ -312,14 +330,13 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     wait_lds();
     stage_barrier();
   }
-#pragma unroll 1
-  for (int i = 0; i < 2; ++i) {
-    request();
-    if (i) break;
-    wait_lds();
-    wait_loads<0>();
-    stage_barrier();
-  }
+  aim();
+  request();
+  wait_lds();
+  wait_loads<0>();
+  stage_barrier();
+  prepare();
+  request();
   Eight w[2][NN], x01[2][2];
   begin(w[0], x01[0], 0);
   int done = 0;
@@ -329,8 +346,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
       for (int n = 0; n < NN; ++n) acc[t][n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     for (k = 0; k < a.k;) {
+      prepare();
       step(w[0], x01[0], w[1], x01[1]);
       if (k < a.k) {
+        prepare();
         step(w[1], x01[1], w[0], x01[0]);
       } else {
 #pragma unroll
@@ -339,7 +358,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
         for (int i = 0; i < 2; ++i) x01[0][i] = x01[1][i];
       }
     }
-    const Tile tile = tile_of(id, rows, columns);
+    const Tile tile = tile_of(grid, id);
     const int t0 = tile.t * BT + wt * (16 * TT), n0 = tile.n * BN + wn * (16 * NN) + 8 * g;  // the lane's columns: n0 + 32 c + 0 .. 7
     const Table& table = tables[done & 3];
     {
@@ -360,9 +379,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
       for (int t = 0; t < TT; ++t) mine[t] = table.slots[wt * (16 * TT) + 16 * t + m];
     }
     if constexpr (LORA == kStaged) {
-      const int count = __builtin_amdgcn_readfirstlane(table.count);
-      for (Extra e = first_extra(table, tile.n * BN); e.left; advance(e, tile.n * BN))
-        extra_step(e, __builtin_amdgcn_readfirstlane(table.list[count - e.left]), tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - a.slices[e.slice].y_col, w[0], x01[0]);
+      for (Extra e = first_extra(table, tile.n * BN); e.row < BT; advance(table, e)) {
+        prepare();
+        extra_step(e, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, e.slice), w[0], x01[0]);
+      }
       settle();
     }
     const bool whole = (tile.n + 1) * BN <= a.n && ((reinterpret_cast<uintptr_t>(a.y) | static_cast<uintptr_t>(a.y_row * 2)) & 15) == 0;
@@ -472,11 +492,16 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 
 template <typename T, int TT, int NN, bool TAIL, int LORA> void launch(const MloraProjectArgs* a) {
   constexpr auto kernel = tiles8_kernel<T, TT, NN, TAIL, LORA>;
-  constexpr int bytes = 2 * (32 * TT + 32 * NN) * 128 + (LORA ? 4 * (3 * 32 * TT + 4) * 4 : 0);
+  constexpr int bytes = 2 * (32 * TT + 32 * NN) * 128 + (LORA ? 4 * 3 * 32 * TT * 4 : 0);
   allow_lds<kernel>(bytes);
-  const int64_t tiles = static_cast<int64_t>((a->num_rows + 32 * TT - 1) / (32 * TT)) * ((a->n + 32 * NN - 1) / (32 * NN));
-  const int64_t most = 256 * (TT * NN > 8 ? 2 : TT * NN > 4 ? 3 : 4);
-  kernel<<<static_cast<unsigned>(tiles < most ? tiles : most), 256, bytes, static_cast<hipStream_t>(a->stream)>>>(*a);
+  Grid grid = {};
+  grid.rows = (a->num_rows + 32 * TT - 1) / (32 * TT);
+  grid.columns = (a->n + 32 * NN - 1) / (32 * NN);
+  grid.total = grid.rows * grid.columns;
+  grid.strip_inverse = inverse_of(kStrip * grid.columns);
+  grid.last_inverse = inverse_of(grid.rows % kStrip);
+  const int most = 256 * (TT * NN > 8 ? 2 : TT * NN > 4 ? 3 : 4);
+  kernel<<<grid.total < most ? grid.total : most, 256, bytes, static_cast<hipStream_t>(a->stream)>>>(*a, grid);
 }
 template <typename T, int TT, int NN, int LORA> void launch_k(const MloraProjectArgs* a) {
   if (a->k % 128) launch<T, TT, NN, true, LORA>(a);
