@@ -61,32 +61,6 @@ __device__ __forceinline__ int slot_of(const MloraProjectArgs& a, int row) {
   return s >= 0 && s < a.num_slots ? s : -1;
 }
 
-// The different slots of the sixteen rows whose slots lanes 0..15 (and again 16..31, ...) hold: lane i keeps the i-th; returns how many.
-__device__ __forceinline__ int different(int mine, int lane, int* list) {
-  unsigned long long left = __ballot(mine >= 0) & 0xffffull;
-  int count = 0;
-  *list = -1;
-  while (left) {
-    const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
-    left &= ~__ballot(mine == s);
-    if (lane == count) *list = s;
-    ++count;
-  }
-  return count;
-}
-
-// Whether one of eight 16-bit numbers is an infinity or a NaN.
-template <typename T> __device__ __forceinline__ bool any_beyond(const Pack8& p) {
-  constexpr uint32_t kExponent = sizeof(T) == 2 && __is_same(T, __bf16) ? 0x7f807f80u : 0x7c007c00u;
-  bool any = false;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const uint32_t e = p.u[i] & kExponent;
-    any |= (e & 0xffffu) == (kExponent & 0xffffu) || (e >> 16) == (kExponent >> 16);
-  }
-  return any;
-}
-
 // Eight elements of B as bf16 numbers hi + lo (of bf16 adapters lo is nothing).
 template <typename T> struct BPiece;
 template <> struct BPiece<__bf16> {

@@ -6,130 +6,355 @@
 // product continues in the same accumulators: its contraction is a list of pieces of eight ranks, those of the different slots among sixteen rows one behind the other, in which a
 // row's h is zero outside its own slot's.
 #include "common.h"
+#include "dma.h"
 #include "launch.h"
+#include "lds.h"
 #include "project.h"
 
 namespace mlora {
 
 namespace {
 
-// Sixteen columns of y, up to 16 TF rows; K by the wavefronts, every WAVES-th 128 columns each.
-template <typename T, int TF, int WAVES> __global__ __launch_bounds__(WAVES * 64) void project_rows_kernel(MloraProjectArgs a) {
-  __shared__ f32x4 parts[WAVES][TF][64];
-  const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, t0 = blockIdx.y * (16 * TF);
-  const uint8_t* w = static_cast<const uint8_t*>(a.w) + static_cast<int64_t>(n0 + m < a.n ? n0 + m : a.n - 1) * a.w_row;
-  const uint8_t* x[TF];
-  f32x4 acc[TF];
+// 16 NF columns of y, 16 TF rows.
+//
+// A stage is 128 columns of K for each of kSplit = 8 / TF wavefronts a block of sixteen rows has; stages come by direct loads, whole 128-byte lines, into a ring in LDS as deep as it holds,
+// so that for K up to some thousand everything is asked for at once.  A wavefront multiplies one block of rows with all columns of its share of a stage; the shares meet in LDS at the end.
+// The adapters follow as more stages: pieces of eight ranks of one of the different slots among a block's sixteen rows go to the block's wavefronts in turn, four of them a product, and a stage
+// holds each wavefront's own B and h.  (Ranks that are no multiple of eight, whose rows of B lie anywhere, are loaded by the lanes behind the last stage.)
+constexpr int kRowWaves = 8;
+
+template <int TF, int NF> struct RowsShape {
+  static constexpr int kSplit = kRowWaves / TF, kRows = 16 * (TF + NF);
+  static constexpr int kPer = (kRows * 128 * kSplit + 1024 * kRowWaves - 1) / (1024 * kRowWaves), kStage = kPer * 1024 * kRowWaves;  // (as many loads for every wavefront: some of nothing)
+  static constexpr int kRing = kStage > 40 * 1024 ? 3 : kStage > 24 * 1024 ? 4 : 6, kLds = kRing * kStage + 64;
+  static_assert(kLds <= kMostLds && kRowWaves * NF * 1024 <= kLds && NF < kPer, "stages");
+};
+
+// The column of y that row `at` of a workgroup's weights is: a lane ends up with 4 NF of them side by side.
+template <int NF> __device__ __forceinline__ int column_of(int at) { return 4 * NF * ((at & 15) >> 2) + 4 * (at >> 4) + (at & 3); }
+
+template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(kRowWaves * 64) void project_rows_kernel(MloraProjectArgs a) {
+  using S = RowsShape<TF, NF>;
+  extern __shared__ char lds[];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int f = wave % TF, part = wave / TF;
+  const int n0 = blockIdx.x * (16 * NF), t0 = blockIdx.y * (16 * TF);
+  const int row = t0 + 16 * f + m;
+  const int mine = a.num_slices ? slot_of(a, row) : -1;  // first of all: the adapters' loads wait for it
+
+  // what this wavefront loads of a stage: blocks of eight rows, of x or of w
+  const char* from[S::kPer];
+  int column[S::kPer];  // the first of K, without the stage's
 #pragma unroll
-  for (int f = 0; f < TF; ++f) {
-    const int t = t0 + 16 * f + m;
-    x[f] = static_cast<const uint8_t*>(a.x) + static_cast<int64_t>(t < a.num_rows ? t : a.num_rows - 1) * a.x_row;
-    acc[f] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int i = 0; i < S::kPer; ++i) {
+    const int block = wave * S::kPer + i, share = block / (S::kRows / 8), at = (block - share * (S::kRows / 8)) * 8 + (lane >> 3);
+    column[i] = share * 128 + 16 * ((lane & 7) ^ ((at >> 1) & 7));
+    if (at < 16 * TF) {
+      const int t = t0 + at < a.num_rows ? t0 + at : a.num_rows - 1;
+      from[i] = static_cast<const char*>(a.x) + static_cast<int64_t>(t) * a.x_row;
+    } else {
+      const int n = n0 + column_of<NF>(at - 16 * TF);
+      from[i] = static_cast<const char*>(a.w) + static_cast<int64_t>(n < a.n ? n : a.n - 1) * a.w_row;
+    }
   }
-  for (int base = wave * 128; base < a.k; base += WAVES * 128) {
-    Eight ws, xs[TF];
+  const uint32_t home = lds_address(lds) + wave * (S::kPer * 1024);
+  const int stages = (a.k + 128 * S::kSplit - 1) / (128 * S::kSplit);
+  int put = 0, asked = 0;
+  auto request = [&]() {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(home + put * S::kStage);
+#pragma unroll
+    for (int i = 0; i < S::kPer; ++i) {
+      const int k = asked * (128 * S::kSplit) + column[i];
+      dma16v(from[i] + (k < a.k ? k : 0), to + i * 1024);  // (behind the end of a row: its first bytes, which nobody or a zero multiplies)
+    }
+    put = put == S::kRing - 1 ? 0 : put + 1;
+    ++asked;
+  };
+#pragma unroll
+  for (int i = 0; i < S::kRing - 1; ++i)
+    if (i < stages) request();
+
+  // the different slots among the block's rows: lane d (and d + 16, ...) holds the d-th, `ordinal` is which one the row's is
+  const int ranks = padded_ranks(a.r), pieces = ranks / 8, width = a.num_slices * ranks;
+  int list = -1, ordinal = -1, count = 0;
+  if (a.num_slices) {
+    unsigned long long left = __ballot(mine >= 0) & 0xffffull;
+    while (left) {
+      const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+      const unsigned long long has = __ballot(mine == s);
+      left &= ~has;
+      if (mine == s) ordinal = count;
+      if (m == count) list = s;
+      ++count;
+    }
+  }
+  const float inverse = 1.0f / static_cast<float>(pieces);
+  auto slot_place = [&](int c) {  // which slot the c-th piece is of
+    const int d = static_cast<int>((static_cast<float>(c) + 0.5f) * inverse);
+    return d < count ? d : count - 1;
+  };
+  const int total = count * pieces, groups = (total + 3) / 4;
+  auto meeting = [&](int s) {  // the first slice from s on that the columns meet
+    while (s < a.num_slices && (n0 + 16 * NF <= a.slices[s].y_col || n0 >= a.slices[s].y_col + a.slices[s].n)) ++s;
+    return s;
+  };
+  // What a lane takes of a group: piece `first` of slot d, none where `there` is not set.
+  struct Place {
+    int d, first;
+    bool there;
+  };
+  auto place_of = [&](int group) {
+    const int c = 4 * group + g, d = slot_place(c);
+    return Place{d, c < total ? 8 * (c - d * pieces) : 0, c < total};
+  };
+  const uint16_t* const h_row = intermediate(a) + static_cast<int64_t>(row < a.num_rows ? row : a.num_rows - 1) * width;
+  // Of a slice: where its B is, how far apart two slots are in it, and the lane's rows (any for a column that is none of the slice's).
+  struct Slice {
+    const T* b;
+    uint32_t slot_stride, in[NF];
+    bool whole;
+  };
+  auto slice_of = [&](int s) {
+    const int columns = a.slices[s].n, first = n0 - a.slices[s].y_col;
+    Slice of;
+    of.b = static_cast<const T*>(a.slices[s].b);
+    of.slot_stride = static_cast<uint32_t>(columns) * static_cast<uint32_t>(a.r);
+    of.whole = first >= 0 && first + 16 * NF <= columns;
+#pragma unroll
+    for (int n = 0; n < NF; ++n) {
+      const int in = first + column_of<NF>(16 * n + m);
+      of.in[n] = static_cast<uint32_t>(in < 0 ? 0 : in < columns ? in : columns - 1) * static_cast<uint32_t>(a.r);
+    }
+    return of;
+  };
+  // The adapters' stages, the same number for every wavefront: of each slice, as many as the block with most groups has for a wavefront, each once for either part of h.
+  int rounds = 0;
+  struct Extra {
+    int slice, round, part;
+  };
+  Extra load_extra = {a.num_slices, 0, 0};
+  Slice load_slice = {};
+  int extras = 0;
+  if (!LOOSE && a.num_slices) {
+    int32_t* const most = reinterpret_cast<int32_t*>(lds + S::kRing * S::kStage);
+    if (part == 0 && lane == 0) most[f] = groups;
+    wait_lds();
+    stage_barrier();
+    for (int i = 0; i < TF; ++i) rounds = most[i] > rounds ? most[i] : rounds;
+    rounds = __builtin_amdgcn_readfirstlane((rounds + S::kSplit - 1) / S::kSplit);
+    load_extra.slice = meeting(0);
+    if (rounds)
+      for (int s = load_extra.slice; s < a.num_slices; s = meeting(s + 1)) extras += rounds * kParts<T>;
+    if (extras) load_slice = slice_of(load_extra.slice);
+  }
+  auto advance = [&](Extra& e, Slice& slice) {
+    if (++e.part < kParts<T>) return;
+    e.part = 0;
+    if (++e.round < rounds) return;
+    e.round = 0;
+    e.slice = meeting(e.slice + 1);
+    if (e.slice < a.num_slices) slice = slice_of(e.slice);
+  };
+  auto request_extra = [&]() {
+    const uint32_t to = __builtin_amdgcn_readfirstlane(home + put * S::kStage);
+    const int group = load_extra.round * S::kSplit + part;
+    const Place p = place_of(group < groups ? group : 0);
+    const uint16_t* const h = h_row + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width : 0) + load_extra.slice * ranks + p.first;
+    const T* const b = load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * load_slice.slot_stride + p.first;
+#pragma unroll
+    for (int i = 0; i < S::kPer; ++i) {  // (as many as of any stage; without a group, and behind the last piece, of something that is there)
+      if (i < NF && count) dma16v(reinterpret_cast<const char*>(b + load_slice.in[i]), to + i * 1024);
+      else dma16v(reinterpret_cast<const char*>(h), to + i * 1024);
+    }
+    put = put == S::kRing - 1 ? 0 : put + 1;
+    ++asked;
+    advance(load_extra, load_slice);
+  };
+  auto request_next = [&]() {
+    if (asked < stages) request();
+    else if (asked < stages + extras) request_extra();
+  };
+  while (asked < S::kRing - 1 && asked < stages + extras) request_next();
+
+  f32x4 acc[NF];
+#pragma unroll
+  for (int n = 0; n < NF; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  // Four pieces of B with the block's h.  What is not the row's, or no piece, is zero in h; columns outside the slice are in B.
+  auto add_group = [&](int slice, const Place& p, bool whole, int h_part, Pack8(&raw)[NF], Pack8(&h)[kParts<T>]) {
+    if (!whole) {
+#pragma unroll
+      for (int n = 0; n < NF; ++n) {
+        const int in = n0 + column_of<NF>(16 * n + m) - a.slices[slice].y_col;
+        if (in < 0 || in >= a.slices[slice].n) raw[n].raw = i32x4{0, 0, 0, 0};
+      }
+    }
+    const bool own = p.there && ordinal == p.d;
+#pragma unroll
+    for (int v = 0; v < kParts<T>; ++v)
+      if (!own) h[v].raw = i32x4{0, 0, 0, 0};
+#pragma unroll
+    for (int n = 0; n < NF; ++n) {
+      BPiece<T> b;
+      b.from(raw[n]);
+      acc[n] = Mma<__bf16>::run(b.hi, h[0], acc[n]);
+      if constexpr (kParts<T> == 2) {  // (a stage has one part of h: the other one here is zero)
+        if (h_part) b.lo.raw = i32x4{0, 0, 0, 0};
+        acc[n] = Mma<__bf16>::run(b.lo, h[0], acc[n]);
+        if constexpr (LOOSE) acc[n] = Mma<__bf16>::run(b.hi, h[1], acc[n]);
+      }
+    }
+    mfma_settle(acc);
+  };
+
+  const char* const share = lds + part * (S::kRows * 128) + m * 128;
+  const int piece[2] = {16 * (g ^ (m >> 1)), 16 * ((4 + g) ^ (m >> 1))};
+  int now = 0;
+  auto next_stage = [&](int stage) {  // (is there; what came before it has been read)
+    wait_lds();
+    wait_stages<S::kPer, S::kRing - 2>(stages + extras - 1 - stage);
+    stage_barrier();
+    request_next();
+  };
+  for (int stage = 0; stage < stages; ++stage) {
+    next_stage(stage);
+    const int base = (stage * S::kSplit + part) * 128;
+    const char* const at = share + now * S::kStage;
+    now = now == S::kRing - 1 ? 0 : now + 1;
+    if (base >= a.k) continue;
+    Eight x, w[NF];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
-      const int k = base + 64 * p + 16 * g;
-      const bool there = k < a.k;  // (else zeros of x, and some of w's row, which is NaN only where y is)
-      ws.piece[p] = load128(w + (there ? k : 0));
+      x.piece[p] = load128(at + f * 2048 + piece[p]);
 #pragma unroll
-      for (int f = 0; f < TF; ++f) {
-        xs[f].piece[p] = load128(x[f] + (there ? k : 0));
-        if (!there) xs[f].piece[p] = i32x4{0, 0, 0, 0};
-      }
+      for (int n = 0; n < NF; ++n) w[n].piece[p] = load128(at + (TF + n) * 2048 + piece[p]);
+    }
+    if (base + 128 > a.k) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (base + 64 * p + 16 * g >= a.k) x.piece[p] = i32x4{0, 0, 0, 0};
     }
 #pragma unroll
-    for (int f = 0; f < TF; ++f) acc[f] = mma8(ws, xs[f], acc[f]);
+    for (int n = 0; n < NF; ++n) acc[n] = mma8(w[n], x, acc[n]);
+    mfma_settle(acc);
   }
-  mfma_settle(acc);
-  float scales[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) scales[i] = n0 + 4 * g + i < a.n ? a.w_scales[n0 + 4 * g + i] : 0.0f;
-  const int ranks = padded_ranks(a.r), pieces = ranks / 8, width = a.num_slices * ranks;
-  const uint16_t* hi = intermediate(a);
-  const uint16_t* lo = hi + static_cast<int64_t>(a.num_rows) * width;
-  const bool words = a.r % 8 == 0;
+  for (int n = 0; n < NF; ++n) {
+    const int c = n0 + 4 * NF * g + 4 * n;
 #pragma unroll
-  for (int f = 0; f < TF; ++f) {
-    const int t = t0 + 16 * f + m;
+    for (int i = 0; i < 4; ++i) acc[n][i] *= a.w_scales[c + i < a.n ? c + i : a.n - 1];
+  }
+  f32x4 product[NF];  // the base product by itself
 #pragma unroll
-    for (int i = 0; i < 4; ++i) acc[f][i] *= scales[i];
-    if (!a.num_slices) continue;
-    const int mine = slot_of(a, t);
-    int list;
-    const int count = different(mine, lane, &list);
-    for (int s = 0; s < a.num_slices; ++s) {
-      const int columns = a.slices[s].n, n = n0 + m - a.slices[s].y_col;
-      if (n0 + 16 <= a.slices[s].y_col || n0 >= a.slices[s].y_col + columns) continue;
-      for (int c0 = 4 * wave; c0 < count * pieces; c0 += 4 * WAVES) {
-        const int c = c0 + g, d = c / pieces < count ? c / pieces : count - 1, first = 8 * (c - c / pieces * pieces);
-        const int slot = __shfl(list, d, kWave);
-        const bool there = c < count * pieces;
-        Pack8 raw, h[2];
-        raw.raw = h[0].raw = h[1].raw = i32x4{0, 0, 0, 0};
-        if (there && n >= 0 && n < columns) {
-          const T* b = static_cast<const T*>(a.slices[s].b) + (static_cast<int64_t>(slot) * columns + n) * a.r + first;
-          if (words) {
-            raw.raw = load128(b);
-          } else {
-            T* e = reinterpret_cast<T*>(&raw);
+  for (int n = 0; n < NF; ++n) product[n] = acc[n];
+  if (!LOOSE && extras) {
+    Extra e = {meeting(0), 0, 0};
+    Slice slice = slice_of(e.slice);
+    for (int stage = stages; stage < stages + extras; ++stage) {
+      next_stage(stage);
+      const int group = e.round * S::kSplit + part;
+      const char* const at = lds + now * S::kStage + wave * (S::kPer * 1024) + lane * 16;
+      now = now == S::kRing - 1 ? 0 : now + 1;
+      if (group < groups) {
+        Pack8 raw[NF], h[kParts<T>];
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (first + i < a.r) e[i] = b[i];
+        for (int n = 0; n < NF; ++n) raw[n].raw = load128(at + n * 1024);
+        h[0].raw = load128(at + NF * 1024);
+        if constexpr (kParts<T> == 2) h[1].raw = i32x4{0, 0, 0, 0};
+        add_group(e.slice, place_of(group), slice.whole, e.part, raw, h);
+      }
+      advance(e, slice);
+    }
+  }
+  if constexpr (LOOSE) {
+    for (int s = meeting(0); s < a.num_slices; s = meeting(s + 1)) {
+      const Slice slice = slice_of(s);
+      for (int group = part; group < groups; group += S::kSplit) {
+        const Place p = place_of(group);
+        const T* const b_slot = slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * slice.slot_stride;
+        Pack8 raw[NF], h[kParts<T>];
+#pragma unroll
+        for (int n = 0; n < NF; ++n) {
+          T* const to = reinterpret_cast<T*>(&raw[n]);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            to[i] = b_slot[slice.in[n] + (p.first + i < a.r ? p.first + i : 0)];
+            if (p.first + i >= a.r) to[i] = static_cast<T>(0.0f);
           }
         }
-        if (there && mine == slot) {
-          const int64_t at = static_cast<int64_t>(t) * width + s * ranks + first;
-          h[0].raw = load128(hi + at);
-          if constexpr (kParts<T> == 2) h[1].raw = load128(lo + at);
-        }
-        if (__ballot(any_beyond<T>(raw))) {  // (the four pieces of the list one behind the other)
-          for (int v = 0; v < 4 && c0 + v < count * pieces; ++v) {
-            const int of = (c0 + v) / pieces, slot = __builtin_amdgcn_readlane(list, of);
-            const int64_t at = static_cast<int64_t>(t) * width + s * ranks;
-            if (mine == slot)
-              add_slowly(static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(slot) * columns * a.r, columns, n0 + 4 * g - a.slices[s].y_col, a.r, 8 * (c0 + v - of * pieces), 8,
-                         hi + at, kParts<T> == 2 ? lo + at : nullptr, acc[f]);
-          }
-          continue;
-        }
-        BPiece<T> b;
-        b.from(raw);
-        acc[f] = Mma<__bf16>::run(b.hi, h[0], acc[f]);
-        if constexpr (kParts<T> == 2) {
-          acc[f] = Mma<__bf16>::run(b.hi, h[1], acc[f]);
-          acc[f] = Mma<__bf16>::run(b.lo, h[0], acc[f]);
-        }
+#pragma unroll
+        for (int v = 0; v < kParts<T>; ++v) h[v].raw = load128(h_row + v * static_cast<int64_t>(a.num_rows) * width + s * ranks + p.first);
+        add_group(s, p, slice.whole, 0, raw, h);
       }
     }
   }
-  mfma_settle(acc);
+  // An infinity or a NaN in B goes through a matrix product to the rows of other slots (0 times it is NaN): where one came out the rows' own adapters are added again, one number at a time.
+  bool beyond = false;
 #pragma unroll
-  for (int f = 0; f < TF; ++f) parts[wave][f][lane] = acc[f];
+  for (int n = 0; n < NF; ++n)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) beyond |= (__float_as_uint(acc[n][i]) & 0x7f800000u) == 0x7f800000u;
+  if (groups > part && __ballot(beyond)) {
+#pragma unroll
+    for (int n = 0; n < NF; ++n) acc[n] = product[n];
+    for (int s = meeting(0); s < a.num_slices; s = meeting(s + 1))
+      for (int c = 0; c < total; ++c) {
+        const int of = __builtin_amdgcn_readfirstlane(slot_place(c));
+        if (c / 4 % S::kSplit != part || ordinal != of) continue;
+        const T* const b = static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(__builtin_amdgcn_readlane(list, of)) * a.slices[s].n * a.r;
+        const uint16_t* const hi = h_row + s * ranks;
+#pragma unroll
+        for (int n = 0; n < NF; ++n)
+          add_slowly(b, a.slices[s].n, n0 + 4 * NF * g + 4 * n - a.slices[s].y_col, a.r, 8 * (c - of * pieces), 8, hi, kParts<T> == 2 ? hi + static_cast<int64_t>(a.num_rows) * width : nullptr, acc[n]);
+      }
+  }
+  // the shares meet
+  wait_lds();
+  wait_loads<0>();
   __syncthreads();
-  for (int f = wave; f < TF; f += WAVES) {
-    const int t = t0 + 16 * f + m, n = n0 + 4 * g;
-    if (t >= a.num_rows) continue;
-    f32x4 sum = parts[0][f][lane];
+  f32x4* const parts = reinterpret_cast<f32x4*>(lds);
 #pragma unroll
-    for (int v = 1; v < WAVES; ++v) sum += parts[v][f][lane];
+  for (int n = 0; n < NF; ++n) parts[(wave * NF + n) * 64 + lane] = acc[n];
+  __syncthreads();
+  for (int block = wave; block < TF * NF; block += kRowWaves) {
+    const int of = block / NF, t = t0 + 16 * of + m, c = n0 + 4 * NF * g + 4 * (block % NF);
+    if (t >= a.num_rows || c >= a.n) continue;
+    f32x4 sum = parts[(of * NF + block % NF) * 64 + lane];
+#pragma unroll
+    for (int v = 1; v < S::kSplit; ++v) sum += parts[((v * TF + of) * NF + block % NF) * 64 + lane];
     const float scale = a.x_scales[t];
-    T* y = static_cast<T*>(a.y) + static_cast<int64_t>(t) * a.y_row + n;
+    T out[4];
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (n + i < a.n) y[i] = from_f32<T>(__builtin_fmaf(sum[i], scale, a.bias ? to_f32(static_cast<const T*>(a.bias)[n + i]) : 0.0f));
+    for (int i = 0; i < 4; ++i) out[i] = from_f32<T>(__builtin_fmaf(sum[i], scale, a.bias ? to_f32(static_cast<const T*>(a.bias)[c + i < a.n ? c + i : a.n - 1]) : 0.0f));
+    T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(t) * a.y_row + c;
+    if (c + 4 <= a.n && ((reinterpret_cast<uintptr_t>(a.y) | static_cast<uintptr_t>(a.y_row * 2)) & 7) == 0) {
+      __builtin_memcpy(__builtin_assume_aligned(y, 8), out, 8);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (c + i < a.n) y[i] = out[i];
+    }
   }
 }
 
-template <typename T> void launch(const MloraProjectArgs* a) {
-  const hipStream_t stream = static_cast<hipStream_t>(a->stream);
-  const unsigned columns = static_cast<unsigned>((a->n + 15) / 16);
-  auto rows = [&](int tile) { return dim3(columns, static_cast<unsigned>((a->num_rows + tile - 1) / tile)); };
-  if (a->num_rows <= 16) project_rows_kernel<T, 1, 8><<<rows(16), 512, 0, stream>>>(*a);
-  else if (a->num_rows <= 32) project_rows_kernel<T, 2, 8><<<rows(32), 512, 0, stream>>>(*a);
-  else project_rows_kernel<T, 4, 8><<<rows(64), 512, 0, stream>>>(*a);
+template <typename T, int TF, int NF, bool LOOSE> void launch_ranks(const MloraProjectArgs* a) {
+  allow_lds<project_rows_kernel<T, TF, NF, LOOSE>>(RowsShape<TF, NF>::kLds);
+  const dim3 grid(static_cast<unsigned>((a->n + 16 * NF - 1) / (16 * NF)), static_cast<unsigned>((a->num_rows + 16 * TF - 1) / (16 * TF)));
+  project_rows_kernel<T, TF, NF, LOOSE><<<grid, kRowWaves * 64, RowsShape<TF, NF>::kLds, static_cast<hipStream_t>(a->stream)>>>(*a);
+}
+template <typename T, int TF, int NF> void launch(const MloraProjectArgs* a) {
+  if (a->num_slices && a->r % 8) launch_ranks<T, TF, NF, true>(a);
+  else launch_ranks<T, TF, NF, false>(a);
+}
+template <typename T, int TF> void launch_columns(const MloraProjectArgs* a) {
+  // 32 columns a workgroup where that still gives every compute unit one
+  const int64_t wide = static_cast<int64_t>((a->n + 31) / 32) * ((a->num_rows + 16 * TF - 1) / (16 * TF));
+  if (wide >= 256) launch<T, TF, 2>(a);
+  else launch<T, TF, 1>(a);
+}
+template <typename T> void launch_rows(const MloraProjectArgs* a) {
+  if (a->num_rows <= 16) launch_columns<T, 1>(a);
+  else if (a->num_rows <= 32) launch_columns<T, 2>(a);
+  else launch_columns<T, 4>(a);
 }
 
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -183,8 +408,8 @@ int project_kind(const MloraProjectArgs* a) {
 }
 
 int launch_project_rows(const MloraProjectArgs* a) {
-  if (a->dtype == MLORA_DTYPE_BF16) launch<__bf16>(a);
-  else launch<_Float16>(a);
+  if (a->dtype == MLORA_DTYPE_BF16) launch_rows<__bf16>(a);
+  else launch_rows<_Float16>(a);
   return check_launch("project");
 }
 
