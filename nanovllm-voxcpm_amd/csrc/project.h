@@ -72,10 +72,9 @@ template <> struct BPiece<_Float16> {
   __device__ __forceinline__ void from(const Pack8& raw) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      __bf16 h, l;
-      split(static_cast<float>(raw.hf[i]), &h, &l);  // (an fp16 number has eleven bits: hi + lo is all of it)
-      hi.bf[i] = h;
-      lo.bf[i] = l;
+      const float v = static_cast<float>(raw.hf[i]);  // (an fp16 number has eleven bits: hi + lo is all of it; of an infinity lo is NaN, and so is what it meets)
+      hi.bf[i] = static_cast<__bf16>(v);
+      lo.bf[i] = static_cast<__bf16>(v - static_cast<float>(hi.bf[i]));
     }
   }
 };

@@ -108,6 +108,9 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     return Place{d, c < total ? 8 * (c - d * pieces) : 0, c < total};
   };
   const uint16_t* const h_row = intermediate(a) + static_cast<int64_t>(row < a.num_rows ? row : a.num_rows - 1) * width;
+  const int block_row = t0 + 16 * f < a.num_rows ? t0 + 16 * f : a.num_rows - 1;  // (a block behind the last row: its loads are of that)
+  const char* const h_block = reinterpret_cast<const char*>(intermediate(a) + static_cast<int64_t>(block_row) * width);
+  const uint32_t h_lane = static_cast<uint32_t>((row < a.num_rows ? row - block_row : a.num_rows - 1 - block_row) * width * 2 + 16 * g);
   // Of a slice: where its B is, how far apart two slots are in it, and the lane's rows (any for a column that is none of the slice's).
   struct Slice {
     const T* b;
@@ -131,8 +134,18 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   int rounds = 0;
   struct Extra {
     int slice, round, part;
+    int d, quarter;  // where a slot is whole groups of four pieces: the group's slot and which of its groups it is
   };
-  Extra load_extra = {a.num_slices, 0, 0};
+  const int quarters = pieces / 4;
+  const bool even = pieces % 4 == 0;
+  auto settle_quarter = [&](Extra& e) {
+    if (!even) return;
+    while (e.quarter >= quarters) {
+      e.quarter -= quarters;
+      ++e.d;
+    }
+  };
+  Extra load_extra = {a.num_slices, 0, 0, 0, part};
   Slice load_slice = {};
   int extras = 0;
   if (!LOOSE && a.num_slices) {
@@ -146,25 +159,43 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     if (rounds)
       for (int s = load_extra.slice; s < a.num_slices; s = meeting(s + 1)) extras += rounds * kParts<T>;
     if (extras) load_slice = slice_of(load_extra.slice);
+    settle_quarter(load_extra);
   }
   auto advance = [&](Extra& e, Slice& slice) {
     if (++e.part < kParts<T>) return;
     e.part = 0;
+    e.quarter += S::kSplit;
+    settle_quarter(e);
     if (++e.round < rounds) return;
     e.round = 0;
+    e.d = 0;
+    e.quarter = part;
+    settle_quarter(e);
     e.slice = meeting(e.slice + 1);
     if (e.slice < a.num_slices) slice = slice_of(e.slice);
   };
   auto request_extra = [&]() {
     const uint32_t to = __builtin_amdgcn_readfirstlane(home + put * S::kStage);
     const int group = load_extra.round * S::kSplit + part;
-    const Place p = place_of(group < groups ? group : 0);
-    const uint16_t* const h = h_row + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width : 0) + load_extra.slice * ranks + p.first;
-    const T* const b = load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * load_slice.slot_stride + p.first;
+    if (even && group < groups) {
+      // a slot's 32 ranks: everything but the lane's row and its eight ranks is the same for all
+      const char* const b = reinterpret_cast<const char*>(load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(list, load_extra.d))) * load_slice.slot_stride) +
+                            64 * load_extra.quarter;
+      const char* const h = h_block + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width * 2 : 0) + load_extra.slice * ranks * 2 + 64 * load_extra.quarter;
 #pragma unroll
-    for (int i = 0; i < S::kPer; ++i) {  // (as many as of any stage; without a group, and behind the last piece, of something that is there)
-      if (i < NF && count) dma16v(reinterpret_cast<const char*>(b + load_slice.in[i]), to + i * 1024);
-      else dma16v(reinterpret_cast<const char*>(h), to + i * 1024);
+      for (int i = 0; i < S::kPer; ++i) {
+        if (i < NF) dma16_from(uniform(b), load_slice.in[i] * 2 + 16 * g, to + i * 1024);
+        else dma16_from(uniform(h), h_lane, to + i * 1024);
+      }
+    } else {
+      const Place p = place_of(group < groups ? group : 0);
+      const uint16_t* const h = h_row + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width : 0) + load_extra.slice * ranks + p.first;
+      const T* const b = load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * load_slice.slot_stride + p.first;
+#pragma unroll
+      for (int i = 0; i < S::kPer; ++i) {  // (as many as of any stage; without a group, and behind the last piece, of something that is there)
+        if (i < NF && count) dma16v(reinterpret_cast<const char*>(b + load_slice.in[i]), to + i * 1024);
+        else dma16v(reinterpret_cast<const char*>(h), to + i * 1024);
+      }
     }
     put = put == S::kRing - 1 ? 0 : put + 1;
     ++asked;
@@ -247,10 +278,15 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
 #pragma unroll
   for (int n = 0; n < NF; ++n) product[n] = acc[n];
   if (!LOOSE && extras) {
-    Extra e = {meeting(0), 0, 0};
+    Extra e = {meeting(0), 0, 0, 0, part};
+    settle_quarter(e);
     Slice slice = slice_of(e.slice);
     for (int stage = stages; stage < stages + extras; ++stage) {
-      next_stage(stage);
+      // (a wavefront reads what it has loaded itself: only the last stage of the base product has to be everybody's)
+      wait_lds();
+      wait_stages<S::kPer, S::kRing - 2>(stages + extras - 1 - stage);
+      if (stage == stages) stage_barrier();
+      request_next();
       const int group = e.round * S::kSplit + part;
       const char* const at = lds + now * S::kStage + wave * (S::kPer * 1024) + lane * 16;
       now = now == S::kRing - 1 ? 0 : now + 1;
@@ -260,7 +296,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
         for (int n = 0; n < NF; ++n) raw[n].raw = load128(at + n * 1024);
         h[0].raw = load128(at + NF * 1024);
         if constexpr (kParts<T> == 2) h[1].raw = i32x4{0, 0, 0, 0};
-        add_group(e.slice, place_of(group), slice.whole, e.part, raw, h);
+        add_group(e.slice, even ? Place{e.d, 0, true} : place_of(group), slice.whole, e.part, raw, h);
       }
       advance(e, slice);
     }
