@@ -5,7 +5,7 @@
 
 namespace mlora {
 
-// Which kernel serves a call.  Rows by themselves where they are few, else tiles; with or without adapters the same, so that a row's base product is the same.
+// Which kernel serves a call: rows by themselves where they are few, else tiles.  Which of the two does not depend on the adapters, so that a row's base product does not.
 enum { kRows, kTiles64, kTiles64x128, kTiles128 };
 int project_kind(const MloraProjectArgs* a);
 

@@ -436,11 +436,17 @@ int check_project(const MloraProjectArgs* a) {
 
 }  // namespace
 
+// Rows by themselves up to 64, and up to 256 while their workgroups are no more than the compute units: what they share out along K a tile has to go through alone, and tiles want the rows in
+// the order of their slots first; beyond, a second round of them costs as much as the first.  (us, graph replay, bf16, 8 slots of rank 32, random; in brackets without adapters:
+// 128 rows, k 4096, n 4096, 256 workgroups: 29.5 [12.6], by tiles 39.1 [13.0]; 192 rows: 43.7 [22.4], 38.4 [13.2]; 96 rows, k 1024, n 8192, 512 workgroups: 22.3 [10.8], 23.9 [6.6].)
+// Of the tiles the smallest that are all at work at once, 64 x 64 three a compute unit, 64 x 128 three or, with adapters, two, else 128 x 128, which loads least.  (k 4096, n 4096: 768 rows
+// 21.6 / 24.0 / 26.0 without adapters, 49.4 / 50.7 / 51.6 with; 1024 rows 26.6 / 26.5 / 27.2, 70.2 / 51.8 / 51.8; 2048 rows 48.4 / 48.7 / 35.9, 113 / 80 / 63.)
+// Which of the tiles changes nothing in the result: all go through K in the same steps.
 int project_kind(const MloraProjectArgs* a) {
-  const int forced = env_int("MLORA_TILE8", 0);
-  if (forced) return forced - 1;
-  if (a->num_rows <= 256 || !tiles8_supported(a)) return kRows;
-  return a->num_rows > 2048 ? kTiles128 : kTiles64;
+  auto tiles = [&](int rows, int columns) { return static_cast<int64_t>((a->num_rows + rows - 1) / rows) * ((a->n + columns - 1) / columns); };
+  if (a->num_rows <= 64 || (a->num_rows <= 256 && tiles(64, 32) <= 256) || !tiles8_supported(a)) return kRows;
+  if (tiles(64, 64) <= 3 * 256) return kTiles64;
+  return tiles(64, 128) <= (a->num_slices ? 2 : 3) * 256 ? kTiles64x128 : kTiles128;
 }
 
 int launch_project_rows(const MloraProjectArgs* a) {

@@ -45,7 +45,7 @@ template <typename T> __device__ __forceinline__ void store_h(const MloraProject
 
 constexpr int kRowWaves = 8, kRowBatch = kRowWaves * 64;
 
-// The rows of slot blockIdx.x, sixteen of its ranks in one slice.
+// The rows of slot blockIdx.x, sixteen of its ranks in one slice; where that leaves compute units without work, sixteen rows in turn a workgroup (blockIdx.z).
 template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void shrink8_rows_kernel(MloraProjectArgs a) {
   __shared__ int32_t found[kRowBatch];
   __shared__ int counts[kRowWaves];
@@ -66,7 +66,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void shrink8_
     }
     if (here >> lane & 1) found[before + __builtin_popcountll(here & ((1ull << lane) - 1))] = t;
     __syncthreads();
-    for (int i0 = 0; i0 < count; i0 += 16) {
+    for (int i0 = 16 * blockIdx.z; i0 < count; i0 += 16 * gridDim.z) {
       const int row = found[i0 + m < count ? i0 + m : count - 1];
       const uint8_t* const x = static_cast<const uint8_t*>(a.x) + static_cast<int64_t>(row) * a.x_row;
       f32x4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -322,7 +322,8 @@ template <typename T, int RB> void launch_tiles(const MloraProjectArgs* a, dim3 
 template <typename T> void launch(const MloraProjectArgs* a, bool ordered) {
   const hipStream_t stream = static_cast<hipStream_t>(a->stream);
   if (!ordered) {
-    const dim3 grid(static_cast<unsigned>(a->num_slots), static_cast<unsigned>(a->num_slices * ((a->r + 15) / 16)));
+    const int groups = a->num_slices * ((a->r + 15) / 16), spare = 256 / (a->num_slots * groups), blocks = (a->num_rows + 15) / 16;
+    const dim3 grid(static_cast<unsigned>(a->num_slots), static_cast<unsigned>(groups), static_cast<unsigned>(spare < 1 ? 1 : spare < blocks ? spare : blocks));
     shrink8_rows_kernel<T><<<grid, kRowWaves * 64, 0, stream>>>(*a);
     return;
   }

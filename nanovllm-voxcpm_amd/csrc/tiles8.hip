@@ -520,9 +520,10 @@ template <typename T> void launch_size(const MloraProjectArgs* a, int kind) {
 
 }  // namespace
 
-// A tile's weights lie within 32 bits of its first, and so do its rows, which with adapters may be any.
+// A tile's weights lie within 32 bits of its first, so do its rows, which with adapters may be any, and a slot's A, of up to 256 ranks.
 bool tiles8_supported(const MloraProjectArgs* a) {
-  return a->x_row >= 0 && a->w_row >= 0 && a->x_row <= 1 << 22 && a->w_row <= 1 << 22 && static_cast<int64_t>(a->num_rows) * a->x_row + a->k < 1ll << 32;
+  static_assert(MLORA_MAX_RANK <= 1024, "a slot's A");
+  return a->k <= 1 << 20 && a->x_row >= 0 && a->w_row >= 0 && a->x_row <= 1 << 22 && a->w_row <= 1 << 22 && static_cast<int64_t>(a->num_rows) * a->x_row + a->k < 1ll << 32;
 }
 
 int launch_tiles8(const MloraProjectArgs* a, int kind) {
