@@ -3,7 +3,8 @@
 Not a served model: random-init weights, plain torch for everything that is not LoRA (RMSNorm,
 rotary embedding, attention over a dense padded KV cache, SwiGLU), and this package's LoRA
 linears for the four stacked projections of every layer.  ``forward_paged`` runs the same layers over a
-paged cache with this package's attention (``layers.attention``): prompts, chunks of them, and decode steps.  The shape follows the end-to-end
+paged cache with this package's attention (``layers.attention``): prompts, chunks of them, and decode steps.  After ``quantize_base_`` the base weights
+have 8 bits and ``forward_paged`` runs on this package's kernels throughout (``quant_ops``).  The shape follows the end-to-end
 benchmark configuration: 24 layers, hidden 1024, 16 query heads / 2 KV heads of 64, SwiGLU
 intermediate 4096, RMSNorm; decode streams with one new token each.
 """
@@ -16,6 +17,7 @@ import torch.nn.functional as F
 
 from .layers.attention import AttentionBatch, PagedAttention, unserved_sizes
 from .layers.lora import LoRAMergedColumnParallelLinear, LoRAQKVParallelLinear, LoRARowParallelLinear
+from .quant_ops import add_rms_norm, quantize_rows, silu_mul
 
 
 class RMSNorm(nn.Module):
@@ -83,6 +85,13 @@ class DecoderLayer(nn.Module):
         gate, up = self.gate_up(self.post_norm(x)).chunk(2, dim=-1)
         return x + self.down(F.silu(gate) * up)
 
+    def forward_paged_in_8_bits(self, x, update, k_cache, v_cache, batch: AttentionBatch):
+        """The rows x + update (None: x) through the layer -> rows and the update to them that the next norm adds."""
+        rows, x = add_rms_norm(x if update is None else update, self.input_norm.weight, residual=None if update is None else x, eps=self.input_norm.eps, quantize=True)
+        attended = self.o(quantize_rows(self.attention(self.qkv(rows), k_cache, v_cache, batch)))
+        rows, x = add_rms_norm(attended, self.post_norm.weight, residual=x, eps=self.post_norm.eps, quantize=True)
+        return x, self.down(silu_mul(self.gate_up(rows), quantize=True))
+
 
 class MiniDecoder(nn.Module):
     """``attention``: options of ``PagedAttention`` (norms of the heads, window, first tokens) that ``forward_paged`` has and
@@ -119,6 +128,12 @@ class MiniDecoder(nn.Module):
                 a, b2 = ab(inter, hid)
                 layer.down.set_slot_lora(slot, a.to(w.device), b2.to(w.device), rank, alpha / rank)
 
+    def quantize_base_(self) -> None:
+        """Put the base weights of all linears in 8 bits (fp16 and bf16 models on the GPU)."""
+        for layer in self.layers:
+            for linear in (layer.qkv, layer.o, layer.gate_up, layer.down):
+                linear.quantize_base_()
+
     def make_cache(self, streams: int, max_len: int, dtype, device, seed: int):
         """Seeded KV caches [layers][2] of shape [streams, kv_heads, max_len, head_dim] (filled on
         the device: they are filler for the attention, not part of any parity claim)."""
@@ -145,6 +160,11 @@ class MiniDecoder(nn.Module):
         return [(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)) for _ in self.layers]
 
     def forward_paged(self, x, caches, batch: AttentionBatch):
+        if self.layers and self.layers[0].qkv.base_in_8_bits:
+            update = None
+            for layer, (k_cache, v_cache) in zip(self.layers, caches):
+                x, update = layer.forward_paged_in_8_bits(x, update, k_cache, v_cache, batch)
+            return add_rms_norm(update, self.norm.weight, residual=x, eps=self.norm.eps)[0]
         for layer, (k_cache, v_cache) in zip(self.layers, caches):
             x = layer.forward_paged(x, k_cache, v_cache, batch)
         return self.norm(x)

@@ -11,6 +11,8 @@ Weight buffers: ``A = [slots, r, in]`` and ``B = [slots, out, r]`` with the adap
 ``alpha / r`` folded into B when a slot is installed; rows / columns at or above an adapter's
 own rank stay zero, which is what makes rank padding numerically inert
 (reference :395-417).
+
+``quantize_base_`` puts a layer's base weight in 8 bits: from then on base product and adapters are one call of ``quant_ops``.
 """
 
 from __future__ import annotations
@@ -25,6 +27,8 @@ import torch.nn.functional as F
 
 from nanovllm_voxcpm_amd import _hip
 from nanovllm_voxcpm_amd.lora import LoRAMetadata, get_backend
+from nanovllm_voxcpm_amd.lora_ops.segment_meta import as_slot_vector
+from nanovllm_voxcpm_amd.quant_ops import QuantizedRows, quantize_rows, quantized_linear
 from nanovllm_voxcpm_amd.utils.context import LM_LORA_DOMAIN, get_lora_context, installed_lora_context
 
 ShardId = str | int
@@ -82,6 +86,9 @@ class _LoRALayerBase(nn.Module):
         self._rank_summary_of: list | None = None  # the mirror the summary below was made from
         self._rank_summary = (False, False)
         self._targets_in_order = True  # every output block has a target, in order
+        self.base_in_8_bits = False
+        self._base_dtype: torch.dtype | None = None
+        self._base_rows: tuple | None = None  # the buffers of the 8-bit weight, and that weight
 
     # ---- subclass contract ------------------------------------------------------------------
     def _target_keys(self) -> list:
@@ -229,6 +236,60 @@ class _LoRALayerBase(nn.Module):
         if x.ndim == 2:
             return out_flat
         return out_flat.reshape(*x.shape[:-1], out_flat.size(-1))
+
+    # ---- base weights in 8 bits ---------------------------------------------------------------
+    @torch.no_grad()
+    def quantize_base_(self) -> None:
+        """Put the base weight in 8 bits, e4m3 numbers with a scale an output column, and let the 16-bit one go.
+
+        The forward then takes rows in 8 bits (``QuantizedRows``) or in the layer's type, which it puts in 8 bits itself, and adds the same adapters as before; it has no derivatives.
+        For fp16 and bf16 layers on the GPU whose input features are a multiple of 16; call it after the base weight is loaded.  The state dict has ``weight_values`` and
+        ``weight_scales`` (both as integers, which a change of the module's type leaves as they are) in place of ``weight``.
+        """
+        if self.base_in_8_bits:
+            raise RuntimeError("the base weight is in 8 bits already")
+        weight = self.weight
+        if weight.dtype not in (torch.float16, torch.bfloat16):
+            raise ValueError(f"a base weight in 8 bits is for fp16 and bf16 layers, this one is {weight.dtype}")
+        if weight.size(1) % 16:
+            raise ValueError(f"a base weight in 8 bits takes a multiple of 16 input features, this layer has {weight.size(1)}")
+        values, scales = quantize_rows(weight.detach())
+        self._base_dtype = weight.dtype
+        self.weight = None
+        self.register_buffer("weight_values", values.view(torch.uint8))
+        self.register_buffer("weight_scales", scales.view(torch.int32))
+        self.base_in_8_bits = True
+
+    def base_weight_rows(self) -> QuantizedRows:
+        """The base weight in 8 bits."""
+        values, scales = self._buffers["weight_values"], self._buffers["weight_scales"]
+        held = self._base_rows
+        if held is None or held[0] is not values or held[1] is not scales:  # (moved or loaded since)
+            held = self._base_rows = (values, scales, QuantizedRows(values.view(torch.float8_e4m3fn), scales.view(torch.float32)))
+        return held[2]
+
+    def _forward_in_8_bits(self, x: torch.Tensor | QuantizedRows, bias: torch.Tensor | None, block_sizes: list[int], block_of_target: list[int]) -> torch.Tensor:
+        eight = isinstance(x, QuantizedRows)
+        dtype = self.lora_A.dtype if self.supports_lora else self.bias.dtype if self.bias is not None else self._base_dtype if eight else x.dtype
+        if eight:
+            rows, shape = x, None
+        else:
+            if x.dtype != dtype:
+                raise ValueError(f"the input is {x.dtype}, the layer {dtype}")
+            shape = None if x.ndim == 2 else x.shape[:-1]
+            rows = quantize_rows(x if shape is None else x.reshape(-1, x.size(-1)))
+        slots = self._resolve_token_slots(rows.values)
+        if slots is None:
+            y = quantized_linear(rows, self.base_weight_rows(), bias=bias, dtype=dtype)
+        else:
+            by_column = sorted(range(len(block_of_target)), key=block_of_target.__getitem__)
+            columns = None
+            if not self._targets_in_order:
+                starts = [sum(block_sizes[:b]) for b in range(len(block_sizes))]
+                columns = [starts[block_of_target[p]] for p in by_column]
+            y = quantized_linear(rows, self.base_weight_rows(), bias=bias, dtype=dtype, lora_a=[self._a_of(p) for p in by_column], lora_b=[self._b_of(p) for p in by_column],
+                                 token_to_slot=as_slot_vector(slots), lora_columns=columns)
+        return y if shape is None else y.view(*shape, y.size(-1))
 
     def _wants_rank_masking(self) -> bool:
         """Whether the backend should be told the per-slot ranks: only buffers of more than one
@@ -497,6 +558,8 @@ class LoRAQKVParallelLinear(_MultiTargetMixin, _LoRALayerBase):
         rows.copy_(loaded_weight.chunk(self.tp_size, 0)[self.tp_rank])
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.base_in_8_bits:
+            return self._forward_in_8_bits(x, self.bias, [self.q_size, self.kv_size, self.kv_size], [self._BLOCK[t] for t in self.lora_targets])
         qkv = F.linear(x, self.weight, self.bias)
         if self._add_lora_quickly(x, qkv):
             return qkv
@@ -551,6 +614,8 @@ class LoRAMergedColumnParallelLinear(_MultiTargetMixin, _LoRALayerBase):
         rows.copy_(loaded_weight.chunk(self.tp_size, 0)[self.tp_rank])
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.base_in_8_bits:
+            return self._forward_in_8_bits(x, self.bias, list(self.shard_output_sizes), list(self.lora_targets))
         out = F.linear(x, self.weight, self.bias)
         if self._add_lora_quickly(x, out):
             return out
@@ -617,9 +682,13 @@ class LoRARowParallelLinear(_SingleTargetMixin, _LoRALayerBase):
         param.data[0, : loaded_weight.size(0)].copy_(shard)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        y = F.linear(x, self.weight, self.bias if self.tp_rank == 0 else None)
-        if not self._add_lora_quickly(x, y):
-            y = self._add_lora(x, y, [self.output_size], [0])
+        bias = self.bias if self.tp_rank == 0 else None
+        if self.base_in_8_bits:
+            y = self._forward_in_8_bits(x, bias, [self.output_size], [0])
+        else:
+            y = F.linear(x, self.weight, bias)
+            if not self._add_lora_quickly(x, y):
+                y = self._add_lora(x, y, [self.output_size], [0])
         if self.tp_size > 1 and dist.is_available() and dist.is_initialized():
             dist.all_reduce(y)
         return y
@@ -654,6 +723,8 @@ class LoRALinear(_SingleTargetMixin, _LoRALayerBase):
             self.lora_B = nn.Parameter(torch.zeros(max_loras, out_features, rank))
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if self.base_in_8_bits:
+            return self._forward_in_8_bits(x, self.bias, [self.out_features], [0])
         y = F.linear(x, self.weight, self.bias)
         if self._add_lora_quickly(x, y):
             return y

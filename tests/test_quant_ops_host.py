@@ -177,3 +177,38 @@ def test_the_oracle_is_torch_in_64_bits():
     for t, s in ((0, 0), (2, 2), (4, 1)):
         want[t, 2:8] += b[0][s].double() @ (a[0][s].double() @ x[t])
     assert torch.allclose(y, want, rtol=1e-12) and (bound > 0).all()
+
+
+def test_base_weights_that_stay_as_they_are():
+    from nanovllm_voxcpm_amd.layers.lora import LoRALinear
+
+    for layer, error, match in ((LoRALinear(32, 8), ValueError, "fp16 and bf16"), (LoRALinear(40, 8).half(), ValueError, "multiple of 16"), (LoRALinear(32, 8).half(), RuntimeError, "GPU")):
+        with pytest.raises(error, match=match):
+            layer.quantize_base_()
+        assert not layer.base_in_8_bits and layer.weight is not None and "weight_values" not in layer.state_dict()
+
+
+@torch.no_grad()
+def test_a_sharded_row_parallel_linear_adds_its_bias_once(monkeypatch):
+    """The ops stand in by their definitions: on the first rank with the bias, on the others without."""
+    from nanovllm_voxcpm_amd.layers import lora as layers
+
+    def quantize(x):
+        scales, _, values, _ = oracle.eight_bits(x.double(), 0.0)
+        return QuantizedRows(values.to(torch.float8_e4m3fn), scales.float())
+
+    def linear(rows, weight, *, bias=None, dtype=None, **adapters):
+        assert not adapters
+        return oracle.linear(rows.values.float(), rows.scales, weight.values.float(), weight.scales, bias, dtype=dtype)[0].to(dtype)
+
+    monkeypatch.setattr(layers, "quantize_rows", quantize)
+    monkeypatch.setattr(layers, "quantized_linear", linear)
+    x, sums = torch.randn(3, 32).half(), []
+    for rank in (0, 1):
+        layer = layers.LoRARowParallelLinear(32, 8, bias=True).half()
+        layer.weight.copy_(torch.ones(8, 32))
+        layer.bias.copy_(torch.full((8,), 64.0))
+        layer.tp_size, layer.tp_rank = 2, rank
+        layer.quantize_base_()
+        sums.append(layer(x))
+    assert ((sums[0] - sums[1]).float() - 64).abs().max() <= 0.07  # (fp16 up to 128 and below 64: two halves of steps of 2^-4)
