@@ -21,17 +21,50 @@ namespace {
 // so that for K up to some thousand everything is asked for at once.  A wavefront multiplies one block of rows with all columns of its share of a stage; the shares meet in LDS at the end.
 // The adapters follow as more stages: pieces of eight ranks of one of the different slots among a block's sixteen rows go to the block's wavefronts in turn, four of them a product, and a stage
 // holds each wavefront's own B and h.  (Ranks that are no multiple of eight, whose rows of B lie anywhere, are loaded by the lanes behind the last stage.)
-constexpr int kRowWaves = 8;
+//
+// Rows in four blocks (more than 32, up to kSorted) are taken in the order of their slots where there are eight slots or more; every workgroup works the order out for itself.  The sixteen rows of a block then
+// have few different slots.  (us in their own order / sorted, bf16: 256 rows, k 1024, n 1536, 48 slots of rank 64 36.8 / 26.5, 8 of rank 32 20.6 / 20.7, one slot 16.9 / 20.7; 64 rows, k 2048, n 2048,
+// 16 slots of rank 64 21.4 / 18.1; 32 rows, k 1024, n 8192, 8 slots of rank 32 11.8 / 12.3.  201 rows of 48 fp16 slots of rank 64, k 8192, n 2048: 55.8 / 43.3.)
+constexpr int kRowWaves = 8, kSorted = 256;
 
 template <int TF, int NF> struct RowsShape {
   static constexpr int kSplit = kRowWaves / TF, kRows = 16 * (TF + NF);
   static constexpr int kPer = (kRows * 128 * kSplit + 1024 * kRowWaves - 1) / (1024 * kRowWaves), kStage = kPer * 1024 * kRowWaves;  // (as many loads for every wavefront: some of nothing)
-  static constexpr int kRing = kStage > 40 * 1024 ? 3 : kStage > 24 * 1024 ? 4 : 6, kLds = kRing * kStage + 64;
+  static constexpr int kRing = kStage > 40 * 1024 ? 3 : kStage > 24 * 1024 ? 4 : 6;
+  static constexpr int kMost = kRing * kStage, kOrder = kMost + 64, kLds = kOrder + (TF == 4 ? kSorted * 4 : 0);  // (behind the ring: the blocks' numbers of groups, the rows' order)
   static_assert(kLds <= kMostLds && kRowWaves * NF * 1024 <= kLds && NF < kPer, "stages");
 };
 
 // The column of y that row `at` of a workgroup's weights is: a lane ends up with 4 NF of them side by side.
 template <int NF> __device__ __forceinline__ int column_of(int at) { return 4 * NF * ((at & 15) >> 2) + 4 * (at >> 4) + (at & 3); }
+
+// The numbers of up to kSorted rows, those of a slot side by side, rows without one last: a row's place is how many come before it, which two threads count.
+__device__ __forceinline__ void sort_rows(const MloraProjectArgs& a, int32_t* keys, int32_t* order) {
+  static_assert(kRowWaves * 64 == 2 * kSorted, "two threads a row");
+  const int t = threadIdx.x % kSorted, half = threadIdx.x / kSorted;
+  uint32_t key = 0xffffffffu;  // (the slot, then the row: no two alike)
+  if (t < a.num_rows) {
+    const int s = slot_of(a, t);
+    key = static_cast<uint32_t>(s < 0 ? MLORA_MAX_SLOTS : s) * kSorted + t;
+  }
+  if (half == 0) keys[t] = static_cast<int32_t>(key);
+  __syncthreads();
+  int before = 0;
+  if (t < a.num_rows) {
+    for (int i = 16 * half; i < a.num_rows; i += 32) {
+#pragma unroll
+      for (int v = 0; v < 16; v += 4) {
+        const i32x4 others = *reinterpret_cast<const i32x4*>(keys + i + v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) before += static_cast<uint32_t>(others[e]) < key;
+      }
+    }
+  }
+  if (half == 0) keys[kSorted + t] = before;
+  __syncthreads();
+  if (half == 1 && t < a.num_rows) order[keys[kSorted + t] + before] = t;
+  __syncthreads();
+}
 
 template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(kRowWaves * 64) void project_rows_kernel(MloraProjectArgs a) {
   using S = RowsShape<TF, NF>;
@@ -39,7 +72,11 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int f = wave % TF, part = wave / TF;
   const int n0 = blockIdx.x * (16 * NF), t0 = blockIdx.y * (16 * TF);
-  const int row = t0 + 16 * f + m;
+  const bool sorted = TF == 4 && a.num_slices && a.num_slots >= 8 && a.num_rows <= kSorted;
+  const int32_t* const order = reinterpret_cast<const int32_t*>(lds + S::kOrder);
+  if (sorted) sort_rows(a, reinterpret_cast<int32_t*>(lds), reinterpret_cast<int32_t*>(lds + S::kOrder));
+  auto row_at = [&](int t) { return sorted && t < a.num_rows ? order[t] : t; };
+  const int row = row_at(t0 + 16 * f + m);
   const int mine = a.num_slices ? slot_of(a, row) : -1;  // first of all: the adapters' loads wait for it
 
   // what this wavefront loads of a stage: blocks of eight rows, of x or of w
@@ -50,7 +87,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     const int block = wave * S::kPer + i, share = block / (S::kRows / 8), at = (block - share * (S::kRows / 8)) * 8 + (lane >> 3);
     column[i] = share * 128 + 16 * ((lane & 7) ^ ((at >> 1) & 7));
     if (at < 16 * TF) {
-      const int t = t0 + at < a.num_rows ? t0 + at : a.num_rows - 1;
+      const int t = row_at(t0 + at < a.num_rows ? t0 + at : a.num_rows - 1);
       from[i] = static_cast<const char*>(a.x) + static_cast<int64_t>(t) * a.x_row;
     } else {
       const int n = n0 + column_of<NF>(at - 16 * TF);
@@ -108,7 +145,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     return Place{d, c < total ? 8 * (c - d * pieces) : 0, c < total};
   };
   const uint16_t* const h_row = intermediate(a) + static_cast<int64_t>(row < a.num_rows ? row : a.num_rows - 1) * width;
-  const int block_row = t0 + 16 * f < a.num_rows ? t0 + 16 * f : a.num_rows - 1;  // (a block behind the last row: its loads are of that)
+  const int block_row = sorted ? 0 : t0 + 16 * f < a.num_rows ? t0 + 16 * f : a.num_rows - 1;  // (a block behind the last row: its loads are of that)
   const char* const h_block = reinterpret_cast<const char*>(intermediate(a) + static_cast<int64_t>(block_row) * width);
   const uint32_t h_lane = static_cast<uint32_t>((row < a.num_rows ? row - block_row : a.num_rows - 1 - block_row) * width * 2 + 16 * g);
   // Of a slice: where its B is, how far apart two slots are in it, and the lane's rows (any for a column that is none of the slice's).
@@ -149,7 +186,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   Slice load_slice = {};
   int extras = 0;
   if (!LOOSE && a.num_slices) {
-    int32_t* const most = reinterpret_cast<int32_t*>(lds + S::kRing * S::kStage);
+    int32_t* const most = reinterpret_cast<int32_t*>(lds + S::kMost);
     if (part == 0 && lane == 0) most[f] = groups;
     wait_lds();
     stage_barrier();
@@ -246,19 +283,21 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     stage_barrier();
     request_next();
   };
-  for (int stage = 0; stage < stages; ++stage) {
+  // A stage's operands come to registers while those of the one before it are multiplied.
+  auto read_stage = [&](int stage, Eight& x, Eight(&w)[NF]) {
     next_stage(stage);
     const int base = (stage * S::kSplit + part) * 128;
     const char* const at = share + now * S::kStage;
     now = now == S::kRing - 1 ? 0 : now + 1;
-    if (base >= a.k) continue;
-    Eight x, w[NF];
 #pragma unroll
     for (int p = 0; p < 2; ++p) {
       x.piece[p] = load128(at + f * 2048 + piece[p]);
 #pragma unroll
       for (int n = 0; n < NF; ++n) w[n].piece[p] = load128(at + (TF + n) * 2048 + piece[p]);
     }
+    return base;
+  };
+  auto multiply = [&](int base, Eight& x, const Eight(&w)[NF]) {
     if (base + 128 > a.k) {
 #pragma unroll
       for (int p = 0; p < 2; ++p)
@@ -266,6 +305,24 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     }
 #pragma unroll
     for (int n = 0; n < NF; ++n) acc[n] = mma8(w[n], x, acc[n]);
+  };
+  {
+    Eight x[2], w[2][NF];
+    int base = read_stage(0, x[0], w[0]), next = 0;
+    for (int stage = 1; stage < stages; stage += 2) {
+      next = read_stage(stage, x[1], w[1]);
+      multiply(base, x[0], w[0]);
+      if (stage + 1 >= stages) {
+        x[0] = x[1];
+#pragma unroll
+        for (int n = 0; n < NF; ++n) w[0][n] = w[1][n];
+        base = next;
+        break;
+      }
+      base = read_stage(stage + 1, x[0], w[0]);
+      multiply(next, x[1], w[1]);
+    }
+    multiply(base, x[0], w[0]);
     mfma_settle(acc);
   }
 #pragma unroll
@@ -352,8 +409,9 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   for (int n = 0; n < NF; ++n) parts[(wave * NF + n) * 64 + lane] = acc[n];
   __syncthreads();
   for (int block = wave; block < TF * NF; block += kRowWaves) {
-    const int of = block / NF, t = t0 + 16 * of + m, c = n0 + 4 * NF * g + 4 * (block % NF);
-    if (t >= a.num_rows || c >= a.n) continue;
+    const int of = block / NF, c = n0 + 4 * NF * g + 4 * (block % NF);
+    if (t0 + 16 * of + m >= a.num_rows || c >= a.n) continue;
+    const int t = row_at(t0 + 16 * of + m);
     f32x4 sum = parts[(of * NF + block % NF) * 64 + lane];
 #pragma unroll
     for (int v = 1; v < S::kSplit; ++v) sum += parts[((v * TF + of) * NF + block % NF) * 64 + lane];
