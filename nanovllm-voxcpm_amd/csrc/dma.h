@@ -48,6 +48,11 @@ __device__ __forceinline__ void dma16v(const char* p, uint32_t lds) {
   asm volatile("s_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"{m0}"(lds), "v"(p) : "memory");
 }
 
+// The same of four bytes a lane: lane i's go to LDS byte lds + 4 i.
+__device__ __forceinline__ void dma4v(const void* p, uint32_t lds) {
+  asm volatile("s_nop 0\n\tglobal_load_lds_dword %1, off" ::"{m0}"(lds), "v"(p) : "memory");
+}
+
 // Waits until no more than `younger` (at most MOST) stages of PER loads each are on their way.
 template <int PER, int MOST> __device__ __forceinline__ void wait_stages(int younger) {
   if (younger >= MOST) wait_loads<MOST * PER>();

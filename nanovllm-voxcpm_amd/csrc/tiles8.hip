@@ -59,26 +59,26 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   int load_t0 = 0, load_n0 = 0;
 
   // With adapters: rows in the order of their slots.  What a tile's rows are lies in LDS for four tiles, the one that is multiplied, those that are loaded and the one
-  // behind them, which is written a tile ahead of its use by what was asked for a tile before that.
+  // behind them, which is asked for a tile ahead.
   const int32_t* const order = static_cast<const int32_t*>(a.workspace);
   struct Table {
-    int32_t rows[BT], slots[BT], ends[BT];  // the last: where, from the tile's first row on, the row's slot ends
+    int32_t rows[BT], slots[BT], ends[BT];  // the last: where the row's slot ends
   };
-  Table* const tables = reinterpret_cast<Table*>(lds + 2 * kStage);
-  int coming_row = 0, coming_slot = -1, coming_end = 0, turn = 0;
-  auto look_up = [&](int id) {
-    if (id >= total || threadIdx.x >= BT) return;
-    const int t0 = tile_of(grid, id).t * BT, at = t0 + static_cast<int>(threadIdx.x), within = at < a.num_rows ? at : a.num_rows - 1;
-    coming_row = order[within];
-    coming_slot = order[a.num_rows + within];
-    coming_end = order[2 * a.num_rows + within] - t0;
-    if (at >= a.num_rows) coming_slot = -1;
-  };
-  auto write_table = [&](int which) {
-    if (threadIdx.x >= BT) return;
-    tables[which & 3].rows[threadIdx.x] = coming_row;
-    tables[which & 3].slots[threadIdx.x] = coming_slot;
-    tables[which & 3].ends[threadIdx.x] = coming_end;
+  // The scales of the tiles' rows and columns likewise, by direct loads that come with a tile's first step.
+  float* const scales = reinterpret_cast<float*>(lds + 2 * kStage);  // [4][BT + BN]
+  Table* const tables = reinterpret_cast<Table*>(lds + 2 * kStage + 4 * (BT + BN) * 4);
+  int turn = 0;
+  auto load_table = [&](int id, int which) {  // (64 rows a wavefront; the last row stands for those behind it)
+    const int at = (wave & 1) * 64 + lane;
+    if ((wave & 1) * 64 >= BT) return;
+    const int t = tile_of(grid, id < total ? id : total - 1).t * BT + at, within = t < a.num_rows ? t : a.num_rows - 1;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(tables + (which & 3)) + (wave & 1) * 256);
+    if (wave >> 1) {
+      dma4v(order + 2 * a.num_rows + within, to + BT * 8);
+    } else {
+      dma4v(order + within, to);
+      dma4v(order + a.num_rows + within, to + BT * 4);
+    }
   };
   // The slices, one a lane.
   const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
@@ -110,7 +110,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     at_row(table, e, 0);
     return e;
   };
-  auto advance = [&](const Table& table, Extra& e) {
+  auto advance = [&](const Table& table, Extra& e, int t0) {
     if (++e.part < kParts<T>) return;
     e.part = 0;
     e.c += 64;
@@ -118,7 +118,8 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     e.c = 0;
     if (++e.slice < e.end) return;
     e.slice = e.first;
-    at_row(table, e, __builtin_amdgcn_readfirstlane(table.ends[e.row]));
+    const int end = __builtin_amdgcn_readfirstlane(table.ends[e.row]);
+    at_row(table, e, end < a.num_rows ? end - t0 : BT);
   };
   Extra load_extra = {BT, -1, 0, 0, 0, 0, 0};
   // The column that row `at` of the weights' part of a step is, from the tile's first on.
@@ -135,6 +136,20 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
       in_row[odd] = ends && in >= bytes ? 0 : in;
     }
   };
+  int aimed = 0;  // tiles so far
+  auto load_scales = [&]() {  // (the first half of the wavefronts has the rows, the other one the columns, 64 each; of smaller tiles not all have some)
+    const int at = (wave & 1) * 64 + lane;
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(scales + (aimed & 3) * (BT + BN)) + (wave >> 1 ? BT * 4 : 0) + (wave & 1) * 256);
+    if (wave >> 1) {
+      if ((wave & 1) * 64 < BN) dma4v(a.w_scales + (load_n0 + at < a.n ? load_n0 + at : a.n - 1), to);
+    } else if ((wave & 1) * 64 < BT) {
+      int row;
+      if constexpr (LORA != kNone) row = tables[(turn - 1) & 3].rows[at];
+      else row = load_t0 + at < a.num_rows ? load_t0 + at : a.num_rows - 1;
+      dma4v(a.x_scales + row, to);
+    }
+    ++aimed;
+  };
   auto aim = [&]() {
     const Tile tile = tile_of(grid, load_tile);
     load_t0 = tile.t * BT;
@@ -148,8 +163,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
       for (int i = 0; i < TT; ++i) x_off[i] = static_cast<uint32_t>(table.rows[(wave * TT + i) * 8 + (lane >> 3)]) * static_cast<uint32_t>(a.x_row);
       ++turn;
-      write_table(turn);
-      look_up(load_tile + 2 * gridDim.x);
+      load_table(load_tile + gridDim.x, turn);
     } else {
 #pragma unroll
       for (int i = 0; i < TT; ++i) {
@@ -162,6 +176,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
       const int row = column_of((wave * NN + i) * 8 + (lane >> 3)), most = a.n - load_n0 - 1;
       w_off[i] = static_cast<uint32_t>((row < most ? row : most) * a.w_row);
     }
+    load_scales();
   };
   // An adapters' step takes the rows' h for x and the columns' B for w.
   auto aim_extra = [&]() {
@@ -197,7 +212,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     if constexpr (LORA == kStaged) {
       const Table& table = tables[(turn - 1) & 3];
       if (load_extra.row >= BT) load_extra = first_extra(table, load_n0);
-      else advance(table, load_extra);
+      else advance(table, load_extra, load_t0);
       if (load_extra.row < BT) {
         aim_extra();
         return;
@@ -235,9 +250,12 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     for (int i = 0; i < 2; ++i) block_of(x_home + stage, i, x01[i]);
   };
   // Everything of this step has been read: its buffer takes the step after the next, which is there.
+  bool stored = false;  // a whole tile's stores are younger than the loads of the step that has to be there: they need not have ended
   auto turn_over = [&]() {
     wait_lds();
-    wait_loads<0>();
+    if (stored) wait_loads<TT * NN / 2>();
+    else wait_loads<0>();
+    stored = false;
     stage_barrier();
     request();
   };
@@ -324,10 +342,8 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   };
 
   if constexpr (LORA) {
-    look_up(load_tile);
-    write_table(0);
-    look_up(load_tile + gridDim.x);
-    wait_lds();
+    load_table(load_tile, 0);
+    wait_loads<0>();
     stage_barrier();
   }
   aim();
@@ -361,25 +377,22 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     const Tile tile = tile_of(grid, id);
     const int t0 = tile.t * BT + wt * (16 * TT), n0 = tile.n * BN + wn * (16 * NN) + 8 * g;  // the lane's columns: n0 + 32 c + 0 .. 7
     const Table& table = tables[done & 3];
+    const float* const scale = scales + (done & 3) * (BT + BN);
     {
-      float scales[NN / 2][8];
+      f32x4 columns[NN];
 #pragma unroll
-      for (int c = 0; c < NN / 2; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) scales[c][i] = a.w_scales[n0 + 32 * c + i < a.n ? n0 + 32 * c + i : a.n - 1];
+      for (int n = 0; n < NN; ++n) columns[n] = *reinterpret_cast<const f32x4*>(scale + BT + wn * (16 * NN) + 8 * g + 32 * (n >> 1) + 4 * (n & 1));
 #pragma unroll
       for (int t = 0; t < TT; ++t)
 #pragma unroll
-        for (int n = 0; n < NN; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) acc[t][n][i] *= scales[n / 2][n % 2 * 4 + i];
+        for (int n = 0; n < NN; ++n) acc[t][n] *= columns[n];
     }
     if constexpr (LORA) {
 #pragma unroll
       for (int t = 0; t < TT; ++t) mine[t] = table.slots[wt * (16 * TT) + 16 * t + m];
     }
     if constexpr (LORA == kStaged) {
-      for (Extra e = first_extra(table, tile.n * BN); e.row < BT; advance(table, e)) {
+      for (Extra e = first_extra(table, tile.n * BN); e.row < BT; advance(table, e, tile.t * BT)) {
         prepare();
         extra_step(e, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, e.slice), w[0], x01[0]);
       }
@@ -469,13 +482,13 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
       const int at = t0 + 16 * t + m;
       if (at >= a.num_rows) continue;
       const int row = LORA ? table.rows[wt * (16 * TT) + 16 * t + m] : at;
-      const float scale = a.x_scales[row];
+      const float of_row = scale[wt * (16 * TT) + 16 * t + m];
       T* const y = static_cast<T*>(a.y) + static_cast<int64_t>(row) * a.y_row + n0;
 #pragma unroll
       for (int c = 0; c < NN / 2; ++c) {
         T out[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(__builtin_fmaf(acc[t][2 * c + i / 4][i % 4], scale, bias[c][i]));
+        for (int i = 0; i < 8; ++i) out[i] = from_f32<T>(__builtin_fmaf(acc[t][2 * c + i / 4][i % 4], of_row, bias[c][i]));
         if (whole) {
           i32x4 word;
           __builtin_memcpy(&word, out, 16);
@@ -487,12 +500,13 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
         }
       }
     }
+    stored = whole && (tile.t + 1) * BT <= a.num_rows && (LORA == kNone || a.k > 128);  // (of tiles of one step the next table comes behind the stores and has to be there)
   }
 }
 
 template <typename T, int TT, int NN, bool TAIL, int LORA> void launch(const MloraProjectArgs* a) {
   constexpr auto kernel = tiles8_kernel<T, TT, NN, TAIL, LORA>;
-  constexpr int bytes = 2 * (32 * TT + 32 * NN) * 128 + (LORA ? 4 * 3 * 32 * TT * 4 : 0);
+  constexpr int bytes = 2 * (32 * TT + 32 * NN) * 128 + 4 * (32 * TT + 32 * NN) * 4 + (LORA ? 4 * 3 * 32 * TT * 4 : 0);
   allow_lds<kernel>(bytes);
   Grid grid = {};
   grid.rows = (a->num_rows + 32 * TT - 1) / (32 * TT);
