@@ -54,6 +54,23 @@ __device__ __forceinline__ void split(float h, __bf16* hi, __bf16* lo) {
   *lo = static_cast<__bf16>((__float_as_uint(rest) & 0x7f800000u) == 0x7f800000u ? 0.0f : rest);  // (of an infinity or a NaN hi is all there is)
 }
 
+// Sixteen e4m3 numbers as two operands of eight.
+template <typename T> __device__ __forceinline__ void widen(const i32x4& in, Pack8 (&out)[2]);
+template <> [[maybe_unused]] __device__ __forceinline__ void widen<__bf16>(const i32x4& in, Pack8 (&out)[2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    out[i / 2].u[2 * (i % 2)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], 1.0f, false));
+    out[i / 2].u[2 * (i % 2) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], 1.0f, true));
+  }
+}
+template <> [[maybe_unused]] __device__ __forceinline__ void widen<_Float16>(const i32x4& in, Pack8 (&out)[2]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    out[i / 2].u[2 * (i % 2)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[i], 1.0f, false));
+    out[i / 2].u[2 * (i % 2) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[i], 1.0f, true));
+  }
+}
+
 // A row's slot, -1 where it has no adapter.
 __device__ __forceinline__ int slot_of(const MloraProjectArgs& a, int row) {
   if (row >= a.num_rows) return -1;

@@ -430,6 +430,172 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   }
 }
 
+// Very few rows with their adapters in one launch: sixteen columns a workgroup, which works out the rows' whole h for itself.
+//
+// A second launch and the trip of h through memory cost more than every workgroup's reading of the rows' A, from L2, as long as that is little (few_rows below).  The wavefronts share K, 128 columns each in turn, of the base product and of
+// h; h is added up in LDS, rounded as in the other kernels, and the wavefronts share its ranks in the second product.
+constexpr int kFewGroups = 2;  // of sixteen ranks of a slot, all rows together
+
+template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_few_kernel(MloraProjectArgs a) {
+  __shared__ f32x4 parts[kFewGroups][kRowWaves][64];
+  __shared__ __align__(16) uint16_t h_of[kParts<T>][16][16 * kFewGroups];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * 16, mine = slot_of(a, m);
+  // the different slots among the rows: lane d holds the d-th, `ordinal` is which one the row's is
+  int list = 0, ordinal = -1, count = 0;
+  unsigned long long left = __ballot(mine >= 0) & 0xffffull;
+  while (left) {
+    const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
+    const unsigned long long has = __ballot(mine == s);
+    left &= ~has;
+    if (mine == s) ordinal = count;
+    if (m == count) list = s;
+    ++count;
+  }
+  const int ranks = padded_ranks(a.r), pieces = ranks / 8, of_slot = (ranks + 15) / 16, groups = count * of_slot, total = count * pieces;
+  const char* const x = static_cast<const char*>(a.x) + static_cast<int64_t>(m < a.num_rows ? m : a.num_rows - 1) * a.x_row;
+  const char* const w = static_cast<const char*>(a.w) + static_cast<int64_t>(n0 + m < a.n ? n0 + m : a.n - 1) * a.w_row;
+  f32x4 acc[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
+  auto meets = [&](int s) { return n0 < a.slices[s].y_col + a.slices[s].n && n0 + 16 > a.slices[s].y_col; };
+  // eight ranks of B of the lane's column, those of the c-th piece; zero where there are none
+  auto load_b = [&](int s, int c) {
+    Pack8 b;
+    b.raw = i32x4{0, 0, 0, 0};
+    const int d = c / pieces, in = n0 + m - a.slices[s].y_col;
+    const int slot = __shfl(list, c < total ? d : 0, kWave);
+    if (c < total && in >= 0 && in < a.slices[s].n)
+      b.raw = load128(static_cast<const T*>(a.slices[s].b) + (static_cast<int64_t>(slot) * a.slices[s].n + in) * a.r + 8 * (c - d * pieces));
+    return b;
+  };
+  // of a lane's piece behind the last column the row's first one is read, and nothing kept
+  auto load_x = [&](int k, Eight& to) {
+#pragma unroll
+    for (int p = 0; p < 2; ++p) {
+      const int at = k + 64 * p + 16 * g;
+      to.piece[p] = load128(x + (at < a.k ? at : 0));
+      if (at >= a.k) to.piece[p] = i32x4{0, 0, 0, 0};
+    }
+  };
+  for (int k = wave * 128; k < a.k; k += kRowWaves * 128) {
+    Eight xs, ws;
+    load_x(k, xs);
+#pragma unroll
+    for (int p = 0; p < 2; ++p) ws.piece[p] = load128(w + (k + 64 * p + 16 * g < a.k ? k + 64 * p + 16 * g : 0));
+    acc[0] = mma8(ws, xs, acc[0]);
+  }
+  mfma_settle(acc);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[0][i] *= a.w_scales[n0 + 4 * g + i < a.n ? n0 + 4 * g + i : a.n - 1];
+  for (int s = 0; s < a.num_slices; ++s) {
+    if (!meets(s)) continue;
+    Pack8 b = load_b(s, 4 * wave + g);  // (on its way while h comes about)
+    const T* rows[kFewGroups];
+#pragma unroll
+    for (int v = 0; v < kFewGroups; ++v) {
+      const int of = v < groups ? v : 0, d = of / of_slot, j = (of - d * of_slot) * 16 + m;
+      rows[v] = static_cast<const T*>(a.slices[s].a) + (static_cast<int64_t>(__builtin_amdgcn_readlane(list, d)) * a.r + (j < a.r ? j : a.r - 1)) * a.k;
+    }
+    f32x4 h[kFewGroups];
+#pragma unroll
+    for (int v = 0; v < kFewGroups; ++v) h[v] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int k = wave * 128; k < a.k && groups; k += kRowWaves * 128) {
+      Eight xs;
+      load_x(k, xs);
+      Pack8 as[kFewGroups][2][2];
+#pragma unroll
+      for (int v = 0; v < kFewGroups; ++v)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          const int at = k + 64 * p + 16 * g < a.k ? k + 64 * p + 16 * g : 0;
+          as[v][p][0].raw = load128(rows[v] + at);
+          as[v][p][1].raw = load128(rows[v] + at + 8);
+        }
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        Pack8 wide[2];
+        widen<T>(xs.piece[p], wide);
+        const bool there = k + 64 * p + 16 * g < a.k;
+#pragma unroll
+        for (int v = 0; v < kFewGroups; ++v)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            if (!there) as[v][p][e].raw = i32x4{0, 0, 0, 0};
+            h[v] = Mma<T>::run(as[v][p][e], wide[e], h[v]);
+          }
+      }
+    }
+    mfma_settle(h);
+#pragma unroll
+    for (int v = 0; v < kFewGroups; ++v) parts[v][wave][lane] = h[v];
+    __syncthreads();
+    if (wave < groups) {  // a wavefront adds up one group's
+      f32x4 sum = parts[wave][0][lane];
+#pragma unroll
+      for (int v = 1; v < kRowWaves; ++v) sum += parts[wave][v][lane];
+      const int d = wave / of_slot, j = (wave - d * of_slot) * 16 + 4 * g;
+      if (ordinal == d) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          __bf16 hi, lo;
+          split(j + i < a.r ? sum[i] : 0.0f, &hi, &lo);
+          h_of[0][m][j + i] = __builtin_bit_cast(uint16_t, hi);
+          if constexpr (kParts<T> == 2) h_of[1][m][j + i] = __builtin_bit_cast(uint16_t, lo);
+        }
+      }
+    }
+    __syncthreads();
+    const f32x4 before = acc[0];
+    for (int first = 4 * wave; first < total; first += 4 * kRowWaves) {
+      const int c = first + g, d = c / pieces;
+      if (first != 4 * wave) b = load_b(s, c);
+      const bool own = c < total && ordinal == d;
+      BPiece<T> of;
+      of.from(b);
+      Pack8 h;
+#pragma unroll
+      for (int v = 0; v < kParts<T>; ++v) {
+        h.raw = own ? load128(&h_of[v][m][8 * (c - d * pieces)]) : i32x4{0, 0, 0, 0};
+        acc[0] = Mma<__bf16>::run(of.hi, h, acc[0]);
+        if constexpr (kParts<T> == 2)
+          if (v == 0) acc[0] = Mma<__bf16>::run(of.lo, h, acc[0]);
+      }
+    }
+    mfma_settle(acc);
+    // (infinities and NaN in B: see the kernel above)
+    bool beyond = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) beyond |= (__float_as_uint(acc[0][i]) & 0x7f800000u) == 0x7f800000u;
+    if (4 * wave < total && __ballot(beyond)) {
+      acc[0] = before;
+      for (int c = 0; c < total; ++c) {
+        const int d = c / pieces, j = 8 * (c - d * pieces);
+        if (c / 4 % kRowWaves != wave || ordinal != d) continue;
+        const T* const of = static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(__builtin_amdgcn_readlane(list, d)) * a.slices[s].n * a.r;
+        add_slowly(of, a.slices[s].n, n0 + 4 * g - a.slices[s].y_col, a.r, j, 8, h_of[0][m], kParts<T> == 2 ? h_of[kParts<T> - 1][m] : nullptr, acc[0]);
+      }
+    }
+    __syncthreads();  // (the next slice has another h)
+  }
+  parts[0][wave][lane] = acc[0];
+  __syncthreads();
+  if (wave || m >= a.num_rows) return;
+  f32x4 sum = parts[0][0][lane];
+#pragma unroll
+  for (int v = 1; v < kRowWaves; ++v) sum += parts[0][v][lane];
+  const float scale = a.x_scales[m];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = n0 + 4 * g + i;
+    if (c < a.n) static_cast<T*>(a.y)[static_cast<int64_t>(m) * a.y_row + c] = from_f32<T>(__builtin_fmaf(sum[i], scale, a.bias ? to_f32(static_cast<const T*>(a.bias)[c]) : 0.0f));
+  }
+}
+
+// The rows' A of at most two times sixteen ranks, a K of two turns, and few enough workgroups that they do not wait for each other in L2: as in one launch / in two, us, graph replay, 1 row, rank 32: k 1024,
+// n 1536 6.8 / 9.3, n 8192 9.2 / 10.1; k 2048, n 2048 9.2 / 10.6, n 8192 14.0 / 12.9; k 4096, n 1024 13.9 / 13.1; of rank 64 (four times sixteen) k 1024, n 1536 8.8 / 8.9, n 8192 13.0 / 9.8.
+bool few_rows(const MloraProjectArgs* a) {
+  return a->num_slices && a->r % 8 == 0 && a->num_rows <= kFewGroups && a->num_rows * ((a->r + 15) / 16) <= kFewGroups && a->k <= 2048 && static_cast<int64_t>(a->n) * a->k <= 1 << 23;
+}
+
 template <typename T, int TF, int NF, bool LOOSE> void launch_ranks(const MloraProjectArgs* a) {
   allow_lds<project_rows_kernel<T, TF, NF, LOOSE>>(RowsShape<TF, NF>::kLds);
   const dim3 grid(static_cast<unsigned>((a->n + 16 * NF - 1) / (16 * NF)), static_cast<unsigned>((a->num_rows + 16 * TF - 1) / (16 * TF)));
@@ -444,6 +610,9 @@ template <typename T, int TF> void launch_columns(const MloraProjectArgs* a) {
   const int64_t wide = static_cast<int64_t>((a->n + 31) / 32) * ((a->num_rows + 16 * TF - 1) / (16 * TF));
   if (wide >= 256) launch<T, TF, 2>(a);
   else launch<T, TF, 1>(a);
+}
+template <typename T> void launch_few(const MloraProjectArgs* a) {
+  project_few_kernel<T><<<static_cast<unsigned>((a->n + 15) / 16), kRowWaves * 64, 0, static_cast<hipStream_t>(a->stream)>>>(*a);
 }
 template <typename T> void launch_rows(const MloraProjectArgs* a) {
   if (a->num_rows <= 16) launch_columns<T, 1>(a);
@@ -520,6 +689,11 @@ using namespace mlora;
 extern "C" int mlora_project(const MloraProjectArgs* a) {
   const int rc = check_project(a);
   if (rc) return rc == kNothingToDo ? 0 : rc;
+  if (few_rows(a)) {
+    if (a->dtype == MLORA_DTYPE_BF16) launch_few<__bf16>(a);
+    else launch_few<_Float16>(a);
+    return check_launch("project");
+  }
   const int kind = project_kind(a);
   if (a->num_slices)
     if (const int failed = launch_shrink8(a, kind != kRows)) return failed;

@@ -14,23 +14,6 @@ namespace mlora {
 
 namespace {
 
-// Sixteen e4m3 numbers as two operands of eight.
-template <typename T> __device__ __forceinline__ void widen(const i32x4& in, Pack8 (&out)[2]);
-template <> __device__ __forceinline__ void widen<__bf16>(const i32x4& in, Pack8 (&out)[2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    out[i / 2].u[2 * (i % 2)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], 1.0f, false));
-    out[i / 2].u[2 * (i % 2) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(in[i], 1.0f, true));
-  }
-}
-template <> __device__ __forceinline__ void widen<_Float16>(const i32x4& in, Pack8 (&out)[2]) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    out[i / 2].u[2 * (i % 2)] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[i], 1.0f, false));
-    out[i / 2].u[2 * (i % 2) + 1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(in[i], 1.0f, true));
-  }
-}
-
 // h of four ranks from j on of one row; ranks from r to `ranks` are zero.
 template <typename T> __device__ __forceinline__ void store_h(const MloraProjectArgs& a, int row, int slice, int j, const f32x4& sum) {
   const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
