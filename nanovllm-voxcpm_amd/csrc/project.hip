@@ -5,6 +5,9 @@
 // The base product runs on the 16x16x128 e4m3 matrix instruction, weights as its rows, so that a lane holds consecutive columns of one row of y.  The adapters' second
 // product continues in the same accumulators: its contraction is a list of pieces of eight ranks, those of the different slots among sixteen rows one behind the other, in which a
 // row's h is zero outside its own slot's.
+//
+// Few rows are bound by the weights' way to the compute units: 64 rows, k 1024, n 8192 6.4 us (8.4 MB; with 32 slots of rank 32, 21 MB more, 16.2), 201 rows, k 8192, n 2048 17 us (all workgroups together take 200 MB from L2 in that time, 46 bytes a ns
+// each; with 48 fp16 slots of rank 64, 63 MB more, 41 us, of which the first product 12.5), one row 3.8 us, with its adapter 7.0.
 #include "common.h"
 #include "dma.h"
 #include "launch.h"
@@ -664,10 +667,10 @@ int check_project(const MloraProjectArgs* a) {
 }  // namespace
 
 // Rows by themselves up to 64, and up to 256 while their workgroups are no more than the compute units: what they share out along K a tile has to go through alone, and tiles want the rows in
-// the order of their slots first; beyond, a second round of them costs as much as the first.  (us, graph replay, bf16, 8 slots of rank 32, random; in brackets without adapters:
-// 128 rows, k 4096, n 4096, 256 workgroups: 29.5 [12.6], by tiles 39.1 [13.0]; 192 rows: 43.7 [22.4], 38.4 [13.2]; 96 rows, k 1024, n 8192, 512 workgroups: 22.3 [10.8], 23.9 [6.6].)
+// the order of their slots first; beyond, a second round of them costs a base product as much as the first.  (us, graph replay, bf16, 8 slots of rank 32, random; in brackets without adapters:
+// 128 rows, k 4096, n 4096, 256 workgroups: 23.5 [11.5], by tiles 37.8 [13.1]; 192 rows: 35.2 [20.6], 37.3 [13.7]; 96 rows, k 1024, n 8192, 512 workgroups: 20.4 [10.9], 23.1 [6.4].)
 // Of the tiles the smallest that are all at work at once, 64 x 64 three a compute unit, 64 x 128 three or, with adapters, two, else 128 x 128, which loads least.  (k 4096, n 4096: 768 rows
-// 21.6 / 24.0 / 26.0 without adapters, 49.4 / 50.7 / 51.6 with; 1024 rows 26.6 / 26.5 / 27.2, 70.2 / 51.8 / 51.8; 2048 rows 48.4 / 48.7 / 35.9, 113 / 80 / 63.)
+// 21.7 / 24.0 / 26.0 without adapters, 48.0 / 48.2 / 50.9 with; 1024 rows 26.0 / 24.3 / 26.1, 52.7 / 48.4 / 49.9; 2048 rows 47.0 / 45.2 / 34.2, 78.7 / 72.0 / 60.1.)
 // Which of the tiles changes nothing in the result: all go through K in the same steps.
 int project_kind(const MloraProjectArgs* a) {
   auto tiles = [&](int rows, int columns) { return static_cast<int64_t>((a->num_rows + rows - 1) / rows) * ((a->n + columns - 1) / columns); };

@@ -82,6 +82,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void shrink8_
 }
 
 // The rows by slot, those without one last: a counting sort by one workgroup.  Where in its slot a row comes is left to chance; no result depends on it.
+// Bound by latency: 9392 rows 9 us, 8192 rows of 128 slots 10.8.  (Sixteen workgroups that count all rows and place a share each, or places written side by side from LDS: the same.)
 constexpr int kOrderThreads = 1024;
 __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a) {
   __shared__ int next[MLORA_MAX_SLOTS];
@@ -189,7 +190,7 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a
 
 // A group of up to 64 rows of a slot; 16 RB ranks of one slice.  Two teams of four wavefronts take every other 128 columns of K, a wavefront sixteen of the rows.  The columns of the rows and of
 // the slot's A come by direct loads into one of a team's two buffers, in whole lines, the 16-byte pieces of a row exchanged so that what the lanes read at once lies in all banks.
-// (One team, in which a wavefront waits for nobody but itself: 13.7 us where two take 8, K = 1024, 9392 rows, 2 slices of rank 64; 36 and 20 us of K = 4096, 8192 rows of 128 slots.)
+// (One team, in which a wavefront waits for nobody but itself: 13.7 us where two take 8.6, K = 1024, 9392 rows, 2 slices of rank 64; 36 and 21 us of K = 4096, 8192 rows of 128 slots, 100 MB: 4.8 TB/s.)
 constexpr int kTeams = 2, kTileThreads = kTeams * 256;
 
 template <typename T, int RB> __global__ __launch_bounds__(kTileThreads) void shrink8_tiles_kernel(MloraProjectArgs a) {
