@@ -103,6 +103,7 @@ class MiniDecoder(nn.Module):
         self.hidden, self.kv_heads, self.head_dim = hidden, kv_heads, head_dim
         self.layers = nn.ModuleList(DecoderLayer(hidden, heads, kv_heads, head_dim, inter, max_loras, rank, **attention) for _ in range(layers))
         self.norm = RMSNorm(hidden)
+        self.base_in_8_bits = False  # all linears'
 
     @torch.no_grad()
     def init_random(self, seed: int, adapters: int, rank: int, alpha: float = 32.0) -> None:
@@ -130,9 +131,12 @@ class MiniDecoder(nn.Module):
 
     def quantize_base_(self) -> None:
         """Put the base weights of all linears in 8 bits (fp16 and bf16 models on the GPU)."""
-        for layer in self.layers:
-            for linear in (layer.qkv, layer.o, layer.gate_up, layer.down):
-                linear.quantize_base_()
+        linears = [linear for layer in self.layers for linear in (layer.qkv, layer.o, layer.gate_up, layer.down)]
+        for linear in linears:  # (all or none)
+            linear.check_base_for_8_bits()
+        for linear in linears:
+            linear.quantize_base_()
+        self.base_in_8_bits = True
 
     def make_cache(self, streams: int, max_len: int, dtype, device, seed: int):
         """Seeded KV caches [layers][2] of shape [streams, kv_heads, max_len, head_dim] (filled on
@@ -160,11 +164,11 @@ class MiniDecoder(nn.Module):
         return [(torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)) for _ in self.layers]
 
     def forward_paged(self, x, caches, batch: AttentionBatch):
-        if self.layers and self.layers[0].qkv.base_in_8_bits:
+        if self.base_in_8_bits:
             update = None
             for layer, (k_cache, v_cache) in zip(self.layers, caches):
                 x, update = layer.forward_paged_in_8_bits(x, update, k_cache, v_cache, batch)
-            return add_rms_norm(update, self.norm.weight, residual=x, eps=self.norm.eps)[0]
+            return add_rms_norm(x if update is None else update, self.norm.weight, residual=None if update is None else x, eps=self.norm.eps)[0]
         for layer, (k_cache, v_cache) in zip(self.layers, caches):
             x = layer.forward_paged(x, k_cache, v_cache, batch)
         return self.norm(x)

@@ -246,6 +246,17 @@ class _LoRALayerBase(nn.Module):
         For fp16 and bf16 layers on the GPU whose input features are a multiple of 16; call it after the base weight is loaded.  The state dict has ``weight_values`` and
         ``weight_scales`` (both as integers, which a change of the module's type leaves as they are) in place of ``weight``.
         """
+        self.check_base_for_8_bits()
+        weight = self.weight
+        values, scales = quantize_rows(weight.detach())
+        self._base_dtype = weight.dtype
+        self.weight = None
+        self.register_buffer("weight_values", values.view(torch.uint8))
+        self.register_buffer("weight_scales", scales.view(torch.int32))
+        self.base_in_8_bits = True
+
+    def check_base_for_8_bits(self) -> None:
+        """Raise what ``quantize_base_`` would, and change nothing."""
         if self.base_in_8_bits:
             raise RuntimeError("the base weight is in 8 bits already")
         weight = self.weight
@@ -253,12 +264,8 @@ class _LoRALayerBase(nn.Module):
             raise ValueError(f"a base weight in 8 bits is for fp16 and bf16 layers, this one is {weight.dtype}")
         if weight.size(1) % 16:
             raise ValueError(f"a base weight in 8 bits takes a multiple of 16 input features, this layer has {weight.size(1)}")
-        values, scales = quantize_rows(weight.detach())
-        self._base_dtype = weight.dtype
-        self.weight = None
-        self.register_buffer("weight_values", values.view(torch.uint8))
-        self.register_buffer("weight_scales", scales.view(torch.int32))
-        self.base_in_8_bits = True
+        if not weight.is_cuda:
+            raise RuntimeError(f"a base weight is put in 8 bits on the GPU, this one lives on {weight.device}")
 
     def base_weight_rows(self) -> QuantizedRows:
         """The base weight in 8 bits."""

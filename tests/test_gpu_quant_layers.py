@@ -260,3 +260,26 @@ def test_a_decode_step_in_a_graph_with_padding_and_adapters_that_come_later():
         assert torch.equal(got, model.forward_paged(x, caches, batch)), step
         assert last is None or not torch.equal(got, last)
         last = got
+
+
+@torch.no_grad()
+def test_models_with_some_linears_in_8_bits_and_models_that_stay_as_they_are():
+    from nanovllm_voxcpm_amd.backbone import MiniDecoder
+    from nanovllm_voxcpm_amd.layers.attention import build_attention_batch
+
+    dtype, g = torch.bfloat16, torch.Generator().manual_seed(6)
+    wide, some = _model(dtype), _model(dtype)
+    some.layers[0].qkv.quantize_base_()
+    some.layers[1].down.quantize_base_()
+    batch = build_attention_batch([5, 9], [0, 0], [[0], [1]], 16, device="cuda")
+    x = torch.randn(14, 256, generator=g).to(dtype).cuda()
+    _with_slots([1] * 5 + [-1] * 9)
+    want, got = (m.forward_paged(x, m.make_paged_cache(2, 16, dtype, "cuda"), batch).float() for m in (wide, some))
+    assert not torch.equal(got, want) and (got - want).norm() < 0.35 * want.norm()
+    with pytest.raises(RuntimeError, match="already"):
+        some.quantize_base_()
+    assert not some.layers[0].o.base_in_8_bits  # all or none
+    odd = MiniDecoder(layers=1, hidden=32, heads=3, kv_heads=1, head_dim=8, inter=64, max_loras=1, rank=8).to(device="cuda", dtype=dtype)  # (o has 24 input features)
+    with pytest.raises(ValueError, match="multiple of 16"):
+        odd.quantize_base_()
+    assert not odd.layers[0].qkv.base_in_8_bits and not odd.base_in_8_bits

@@ -203,6 +203,7 @@ def test_a_sharded_row_parallel_linear_adds_its_bias_once(monkeypatch):
 
     monkeypatch.setattr(layers, "quantize_rows", quantize)
     monkeypatch.setattr(layers, "quantized_linear", linear)
+    monkeypatch.setattr(layers.LoRARowParallelLinear, "check_base_for_8_bits", lambda self: None)
     x, sums = torch.randn(3, 32).half(), []
     for rank in (0, 1):
         layer = layers.LoRARowParallelLinear(32, 8, bias=True).half()
