@@ -97,16 +97,18 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   }
   // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 64 ranks at a time, of h one part after the other.
   struct Extra {
-    int row, slot, first, end, slice, c, part;  // the slot's first row in the tile (BT: no more), the slices
+    int row, slot, stop, first, end, slice, c, part;  // the slot's first row in the tile (BT: no more) and where it stops, the slices
   };
   auto at_row = [&](const Table& table, Extra& e, int row) {
     e.row = row;
     if (row >= BT) return;
-    e.slot = __builtin_amdgcn_readfirstlane(table.slots[row]);
+    const int slot = table.slots[row], stop = table.ends[row];
+    e.slot = __builtin_amdgcn_readfirstlane(slot);
+    e.stop = __builtin_amdgcn_readfirstlane(stop);
     if (e.slot < 0) e.row = BT;  // (rows without a slot come last)
   };
   auto first_extra = [&](const Table& table, int n0) {
-    Extra e = {BT, -1, 0, 0, 0, 0, 0};
+    Extra e = {BT, -1, 0, 0, 0, 0, 0, 0};
     const unsigned long long meeting = __ballot(slice_wide && n0 + BN > slice_column && n0 < slice_column + slice_wide);
     if (!meeting) return e;
     e.first = e.slice = __builtin_ctzll(meeting);
@@ -122,10 +124,9 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     e.c = 0;
     if (++e.slice < e.end) return;
     e.slice = e.first;
-    const int end = __builtin_amdgcn_readfirstlane(table.ends[e.row]);
-    at_row(table, e, end < a.num_rows ? end - t0 : BT);
+    at_row(table, e, e.stop < a.num_rows ? e.stop - t0 : BT);
   };
-  Extra load_extra = {BT, -1, 0, 0, 0, 0, 0};
+  Extra load_extra = {BT, -1, 0, 0, 0, 0, 0, 0}, coming = load_extra, current = load_extra;  // of the step that is loaded next, of the two that are multiplied in front of it
   // The column that row `at` of the weights' part of a step is, from the tile's first on.
   auto column_of = [&](int at) {
     const int block = at >> 4, f = block % NN, r = at & 15;
@@ -203,6 +204,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   };
   // What the next load takes, behind the one before it; between steps, since its branches would cut a step's code in pieces.
   auto prepare = [&]() {
+    if constexpr (LORA == kStaged) {
+      current = coming;
+      coming = load_extra;
+    }
     if (load_extra.row >= BT && load_k + 128 < a.k) {
       load_k += 128;
       if constexpr (TAIL) {
@@ -357,6 +362,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   stage_barrier();
   prepare();
   request();
+  if (LORA != kNone && a.k <= 128) {  // (where that was the second tile's only step, the third one's table has to be there)
+    wait_loads<0>();
+    stage_barrier();
+  }
   Eight w[2][NN], x01[2][2];
   begin(w[0], x01[0], 0);
   int done = 0;
@@ -396,9 +405,9 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
       for (int t = 0; t < TT; ++t) mine[t] = table.slots[wt * (16 * TT) + 16 * t + m];
     }
     if constexpr (LORA == kStaged) {
-      for (Extra e = first_extra(table, tile.n * BN); e.row < BT; advance(table, e, tile.t * BT)) {
+      while (coming.row < BT) {
         prepare();
-        extra_step(e, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, e.slice), w[0], x01[0]);
+        extra_step(current, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, current.slice), w[0], x01[0]);
       }
       settle();
     }
@@ -503,6 +512,11 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
             if (n0 + 32 * c + i < a.n) y[32 * c + i] = out[i];
         }
       }
+    }
+    // Tiles of one step run three ahead of a wavefront that is still here: the table that is asked for next is the one that it reads.  (Of two steps and more the loads are two tiles ahead at most.)
+    if (LORA != kNone && a.k <= 128) {
+      wait_lds();
+      stage_barrier();
     }
     stored = whole && (tile.t + 1) * BT <= a.num_rows && (LORA == kNone || a.k > 128);  // (of tiles of one step the next table comes behind the stores and has to be there)
   }

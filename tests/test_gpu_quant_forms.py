@@ -208,3 +208,22 @@ def test_two_graphs_in_turn():
             graphs[i].replay()
             got = out.clone()
             assert torch.equal(got, call()), (step, i)
+
+
+@pytest.mark.parametrize("rank", [8, 20])
+@pytest.mark.parametrize("k", [16, 128, 144])
+def test_many_tiles_of_one_step_and_two(rank, k):
+    """Workgroups with many tiles of a step or two, whose wavefronts take different times at a tile's end (ranks that are no multiple of eight most of all): the same every time, and the definition's."""
+    g = torch.Generator().manual_seed(rank + k)
+    t, n, slots, dtype = 9000, 2048, 11, torch.float16
+    x, w = _rows8(g, t, k), _rows8(g, n, k, k**-0.5)
+    a, b = _adapters(g, slots, rank, k, [n // 3, n // 2], dtype)
+    x, w, a, b = ([v.cuda() for v in group] for group in (x, w, a, b))
+    of = torch.randint(-1, slots, (t,), generator=g, dtype=torch.int32)
+    first = _call(x, w, dtype=dtype, lora_a=a, lora_b=b, token_to_slot=of)
+    rows = torch.randperm(t, generator=g)[:300]
+    held = [v.cpu() for v in (x[0].float().cpu()[rows], x[1].cpu()[rows], w[0].float(), w[1])]
+    want, bound = oracle.linear(*held, a=[v.cpu() for v in a], b=[v.cpu() for v in b], slots=of[rows], dtype=dtype)
+    assert ((first.cpu()[rows].double() - want).abs() <= bound).all()
+    for _ in range(30):
+        assert torch.equal(_call(x, w, dtype=dtype, lora_a=a, lora_b=b, token_to_slot=of), first)
