@@ -5,8 +5,8 @@
 // whole 128-byte lines of eight rows: with halves of lines of sixteen rows, which want no exchange in LDS, every line was fetched twice (8192 x 8192 x 8192: 655 us; this way 463).
 // Nothing in a tile's end waits for memory of its own: scales and tables come by direct loads a tile ahead, the stores end under the next tile's first step (9392 rows, k 1024, n 8192, 8 slots of rank 64: 166 us
 // without that, 150 with).  Measured in graph replay: 8192 x 8192 x 8192 493-505 us (2.2 PFLOP/s; the library's product with a scale a row and a column 480), 9392 rows, k 1024, n 8192 87-101 us as y's
-// 154 MB fit the cache behind L2 or do not (library 106), with the adapters 147-150, of which this kernel 130-135, the matrix pipes busy for a third of the time.  Tiles of 256 x 128 with three
-// buffers and eight wavefronts: 102 and 181 us.
+// 154 MB fit the cache behind L2 or do not (library 106), with the adapters 146-150, of which this kernel 132-136, the matrix pipes busy for a third of the time.  Tiles of 256 x 128 with three
+// buffers and eight wavefronts: 102 and 181 us.  A word of every line of B asked for a tile ahead of the adapters' steps cost 1 us a tile more than it saved.
 #include "common.h"
 #include "dma.h"
 #include "launch.h"
