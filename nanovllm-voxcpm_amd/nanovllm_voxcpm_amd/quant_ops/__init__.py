@@ -41,9 +41,14 @@ def _no_grad(*tensors: torch.Tensor | None) -> None:
         raise RuntimeError("the 8-bit ops have no backward, nor a forward derivative: a tensor carries a tangent")
 
 
+_MOST = 2**31 - 1  # (sizes are 32-bit numbers in the library, which refuses what it does not serve below that)
+
+
 def _rows(t: torch.Tensor, name: str, like: torch.Tensor | None = None) -> None:
     if t.dim() != 2:
         raise ValueError(f"{name} must be [rows, width], got shape {tuple(t.shape)}")
+    if max(t.shape) > _MOST:
+        raise ValueError(f"{name} {tuple(t.shape)} is larger than a call takes")
     if t.size(1) < 1:
         raise ValueError(f"{name} has rows without elements")
     if t.numel() and t.stride(1) != 1 and t.size(1) != 1:
@@ -153,6 +158,8 @@ def _quantized(rows: QuantizedRows, name: str, device: torch.device | None = Non
     values, scales = rows
     if values.dtype != torch.float8_e4m3fn or values.dim() != 2:
         raise ValueError(f"values of {name} must be float8_e4m3fn [rows, width], got {values.dtype} {tuple(values.shape)}")
+    if max(values.shape) > _MOST:
+        raise ValueError(f"{name} {tuple(values.shape)} is larger than a call takes")
     if values.size(1) < 1 or values.size(1) % 16:
         raise ValueError(f"rows of {name} have {values.size(1)} elements, which is no multiple of 16")
     if values.numel() and (values.stride(1) != 1 or values.data_ptr() % 16 or (values.size(0) > 1 and values.stride(0) % 16)):
@@ -205,7 +212,7 @@ def quantized_linear(
     ``dtype``: fp16 or bf16, of the result, the bias ``[out]`` and the adapters.  ``lora_a``, ``lora_b``: buffers ``[slots, rank, in]`` and ``[slots,
     columns, rank]`` of every target (q, k and v of a stacked projection), whose columns lie one behind the other, or from ``lora_columns`` on;
     ``token_to_slot``: int32 ``[T]``, ids outside the slots stand for rows without an adapter.  Sums are fp32, the result is rounded
-    once.  ``in`` is a multiple of 16 and rows start on 16 bytes.
+    once.  ``in`` is a multiple of 16 and rows start on 16 bytes; up to 2^20 rows a call, ``in`` and ``out`` up to 2^22.
     """
     fast = _hip.load_fastcall()
     if fast is not None and out is None and lora_columns is None:

@@ -213,3 +213,15 @@ def test_a_sharded_row_parallel_linear_adds_its_bias_once(monkeypatch):
         layer.quantize_base_()
         sums.append(layer(x))
     assert ((sums[0] - sums[1]).float() - 64).abs().max() <= 0.07  # (fp16 up to 128 and below 64: two halves of steps of 2^-4)
+
+
+def test_sizes_beyond_32_bits_are_refused():
+    wide, many = torch.empty(1, 2**31 + 512, dtype=torch.bfloat16, device="meta"), torch.empty(2**31 + 512, 16, dtype=torch.bfloat16, device="meta")
+    for x in (wide, many):
+        for call in (lambda: quantize_rows(x), lambda: silu_mul(x), lambda: add_rms_norm(x, torch.ones(1))):
+            with pytest.raises(ValueError, match="larger than"):
+                call()
+        eight = QuantizedRows(torch.empty(x.shape, dtype=torch.float8_e4m3fn, device="meta"), torch.empty(x.size(0), device="meta"))
+        for rows, weight in ((eight, _eight(5, 16)), (_eight(5, 16), eight)):
+            with pytest.raises(ValueError, match="larger than"):
+                quantized_linear(rows, weight)
