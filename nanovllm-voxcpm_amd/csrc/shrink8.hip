@@ -188,12 +188,12 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a
   }
 }
 
-// A group of up to 64 rows of a slot; 16 RB ranks of one slice.  Two teams of four wavefronts take every other 128 columns of K, a wavefront sixteen of the rows.  The columns of the rows and of
+// A group of up to 64 rows of a slot; 16 RB ranks of one slice.  TEAMS of four wavefronts take 128 columns of K each in turn, a wavefront sixteen of the rows.  The columns of the rows and of
 // the slot's A come by direct loads into one of a team's two buffers, in whole lines, the 16-byte pieces of a row exchanged so that what the lanes read at once lies in all banks.
 // (One team, in which a wavefront waits for nobody but itself: 13.7 us where two take 8.6, K = 1024, 9392 rows, 2 slices of rank 64; 36 and 21 us of K = 4096, 8192 rows of 128 slots, 100 MB: 4.8 TB/s.)
-constexpr int kTeams = 2, kTileThreads = kTeams * 256;
-
-template <typename T, int RB> __global__ __launch_bounds__(kTileThreads) void shrink8_tiles_kernel(MloraProjectArgs a) {
+// Four teams, of 32 ranks at most, where that gives a compute unit one workgroup at most: the whole call with two teams and with four, 600 rows of 32 slots of rank 64: k 8192, n 1024 69.6 and 59.5 us, k 1024, n 1536
+// 23.8 and 22.6; 2000 rows of 8 slots of rank 32, k 4096, n 4096 59.9 and 57.9.
+template <typename T, int RB, int TEAMS> __global__ __launch_bounds__(TEAMS * 256) void shrink8_tiles_kernel(MloraProjectArgs a) {
   constexpr int kStage = kGroup * 128 + 16 * RB * 256;
   extern __shared__ char lds[];
   const int everyone = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), team = everyone >> 2, wave = everyone & 3;
@@ -216,11 +216,11 @@ template <typename T, int RB> __global__ __launch_bounds__(kTileThreads) void sh
   }
   char* const mine = lds + team * 2 * kStage;
   const uint32_t home = lds_address(mine);
-  const int steps = (a.k + 127) / 128, turns = (steps + kTeams - 1) / kTeams;
+  const int steps = (a.k + 127) / 128, turns = (steps + TEAMS - 1) / TEAMS;
   const char* const x_base = static_cast<const char*>(a.x);
   const char* const a_base = static_cast<const char*>(a.slices[slice].a) + static_cast<int64_t>(slot) * a.r * a.k * 2;
   auto request = [&](int turn) {
-    const int k0 = (turn * kTeams + team) * 128;
+    const int k0 = (turn * TEAMS + team) * 128;
     if (k0 >= a.k) return;
     const uint32_t to = home + (turn & 1) * kStage;
     const bool whole = k0 + 128 <= a.k;
@@ -250,7 +250,7 @@ template <typename T, int RB> __global__ __launch_bounds__(kTileThreads) void sh
     wait_loads<0>();
     stage_barrier();
     if (turn + 1 < turns) request(turn + 1);
-    const int k0 = (turn * kTeams + team) * 128, stage = (turn & 1) * kStage;
+    const int k0 = (turn * TEAMS + team) * 128, stage = (turn & 1) * kStage;
     if (!some || k0 >= a.k) continue;
     Pack8 as[RB][2][2];
     i32x4 raw[2];
@@ -282,25 +282,32 @@ template <typename T, int RB> __global__ __launch_bounds__(kTileThreads) void sh
     }
     mfma_settle(acc);
   }
-  // the teams' sums meet in the first one's buffers, which nobody reads any more
+  // the teams' sums meet in the buffers, which nobody reads any more
   wait_lds();
   stage_barrier();
   f32x4* const parts = reinterpret_cast<f32x4*>(lds) + wave * (RB * 64) + lane;
-  if (team == 1) {
+  constexpr int kTeam = 4 * RB * 64;
+  if (team) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b) parts[b * 64] = acc[b];
+    for (int b = 0; b < RB; ++b) parts[(team - 1) * kTeam + b * 64] = acc[b];
   }
   __syncthreads();
   if (team == 0 && wave * 16 + m < rows) {
 #pragma unroll
-    for (int b = 0; b < RB; ++b) store_h<T>(a, t0 + wave * 16 + m, slice, first + 16 * b + 4 * g, acc[b] + parts[b * 64]);
+    for (int b = 0; b < RB; ++b) {
+#pragma unroll
+      for (int v = 0; v < TEAMS - 1; ++v) acc[b] += parts[v * kTeam + b * 64];
+      store_h<T>(a, t0 + wave * 16 + m, slice, first + 16 * b + 4 * g, acc[b]);
+    }
   }
 }
 
-template <typename T, int RB> void launch_tiles(const MloraProjectArgs* a, dim3 grid) {
-  constexpr int bytes = kTeams * 2 * (kGroup * 128 + 16 * RB * 256);
-  allow_lds<shrink8_tiles_kernel<T, RB>>(bytes);
-  shrink8_tiles_kernel<T, RB><<<grid, kTileThreads, bytes, static_cast<hipStream_t>(a->stream)>>>(*a);
+template <typename T, int RB, int TEAMS> void launch_tiles(const MloraProjectArgs* a) {
+  constexpr int bytes = TEAMS * 2 * (kGroup * 128 + 16 * RB * 256);
+  static_assert(bytes <= kMostLds && (TEAMS - 1) * 4 * RB * 1024 <= bytes, "buffers");
+  allow_lds<shrink8_tiles_kernel<T, RB, TEAMS>>(bytes);
+  const dim3 grid(static_cast<unsigned>(group_capacity(a->num_rows, a->num_slots)), static_cast<unsigned>(a->num_slices * ((a->r + 16 * RB - 1) / (16 * RB))));
+  shrink8_tiles_kernel<T, RB, TEAMS><<<grid, TEAMS * 256, bytes, static_cast<hipStream_t>(a->stream)>>>(*a);
 }
 
 template <typename T> void launch(const MloraProjectArgs* a, bool ordered) {
@@ -312,11 +319,12 @@ template <typename T> void launch(const MloraProjectArgs* a, bool ordered) {
     return;
   }
   order_kernel<<<1, kOrderThreads, 0, stream>>>(*a);
-  const int blocks = a->r <= 16 ? 1 : a->r <= 32 ? 2 : 4;
-  const dim3 grid(static_cast<unsigned>(group_capacity(a->num_rows, a->num_slots)), static_cast<unsigned>(a->num_slices * ((a->r + 16 * blocks - 1) / (16 * blocks))));
-  if (blocks == 1) launch_tiles<T, 1>(a, grid);
-  else if (blocks == 2) launch_tiles<T, 2>(a, grid);
-  else launch_tiles<T, 4>(a, grid);
+  const int64_t groups = static_cast<int64_t>(group_capacity(a->num_rows, a->num_slots)) * a->num_slices;
+  const bool few = groups * ((a->r + 31) / 32) <= 256;
+  if (a->r <= 16) few ? launch_tiles<T, 1, 4>(a) : launch_tiles<T, 1, 2>(a);
+  else if (few) launch_tiles<T, 2, 4>(a);
+  else if (a->r <= 32) launch_tiles<T, 2, 2>(a);
+  else launch_tiles<T, 4, 2>(a);
 }
 
 }  // namespace
