@@ -668,9 +668,9 @@ int check_project(const MloraProjectArgs* a) {
 
 // Rows by themselves up to 64, and up to 256 while their workgroups are no more than the compute units: what they share out along K a tile has to go through alone, and tiles want the rows in
 // the order of their slots first; beyond, a second round of them costs a base product as much as the first.  (us, graph replay, bf16, 8 slots of rank 32, random; in brackets without adapters:
-// 128 rows, k 4096, n 4096, 256 workgroups: 23.5 [11.5], by tiles 37.8 [13.1]; 192 rows: 35.2 [20.6], 37.3 [13.7]; 96 rows, k 1024, n 8192, 512 workgroups: 20.4 [10.9], 23.1 [6.4].)
+// 128 rows, k 4096, n 4096, 256 workgroups: 23.4 [11.6], by tiles 36.0 [12.7]; 192 rows: 35.1 [20.1], 35.7 [12.9]; 96 rows, k 1024, n 8192, 512 workgroups: 20.3 [10.6], 22.2 [6.2].)
 // Of the tiles the smallest that are all at work at once, 64 x 64 three a compute unit, 64 x 128 three or, with adapters, two, else 128 x 128, which loads least.  (k 4096, n 4096: 768 rows
-// 21.7 / 24.0 / 26.0 without adapters, 48.0 / 48.2 / 50.9 with; 1024 rows 26.0 / 24.3 / 26.1, 52.7 / 48.4 / 49.9; 2048 rows 47.0 / 45.2 / 34.2, 78.7 / 72.0 / 60.1.)
+// 21.5 / 24.6 / 26.7 without adapters, 44.3 / 44.9 / 47.5 with; 1024 rows 26.4 / 23.8 / 26.7, 49.8 / 45.4 / 47.2; 2048 rows 47.3 / 45.4 / 35.0, 76.2 / 70.7 / 57.7.)
 // Which of the tiles changes nothing in the result: all go through K in the same steps.
 int project_kind(const MloraProjectArgs* a) {
   auto tiles = [&](int rows, int columns) { return static_cast<int64_t>((a->num_rows + rows - 1) / rows) * ((a->n + columns - 1) / columns); };
