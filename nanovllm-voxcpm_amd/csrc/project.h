@@ -40,13 +40,15 @@ __device__ __forceinline__ f32x4 mma8(const Eight& a, const Eight& b, f32x4 c) {
 // fp16 ones, whose B has three bits more, a second array holds what the first leaves over, and B goes in two pieces as well: 2^-16.
 template <typename T> constexpr int kParts = 1;
 template <> constexpr int kParts<_Float16> = 2;
-// In front of it lie, for tiles, the rows by slot (their numbers, their slots, where the slots end; h has their order then, else that of the rows) and the groups of up to 64 rows of a slot.
+// In front of it lie, for tiles, the rows by slot (their numbers, their slots, where the slots end; h has their order then, else that of the rows), the groups of up to 64 rows of a slot, and whether
+// any h is an infinity or a NaN.
 __host__ __device__ inline int padded_ranks(int r) { return (r + 7) & ~7; }
 constexpr int kGroup = 64;
 __host__ __device__ inline int group_capacity(int rows, int slots) { return rows / kGroup + (slots < rows ? slots : rows); }
 __host__ __device__ inline int64_t rows_bytes(int rows) { return (12ll * rows + 15) & ~15ll; }
-__host__ __device__ inline int64_t order_bytes(int rows, int slots) { return rows_bytes(rows) + 16ll * group_capacity(rows, slots); }
+__host__ __device__ inline int64_t order_bytes(int rows, int slots) { return rows_bytes(rows) + 16ll * group_capacity(rows, slots) + 16; }
 __device__ __forceinline__ i32x4* group_list(const MloraProjectArgs& a) { return reinterpret_cast<i32x4*>(static_cast<char*>(a.workspace) + rows_bytes(a.num_rows)); }
+__device__ __forceinline__ int32_t* any_h_beyond(const MloraProjectArgs& a) { return reinterpret_cast<int32_t*>(group_list(a) + group_capacity(a.num_rows, a.num_slots)); }
 __device__ __forceinline__ uint16_t* intermediate(const MloraProjectArgs& a) {
   return reinterpret_cast<uint16_t*>(static_cast<char*>(a.workspace) + order_bytes(a.num_rows, a.num_slots));
 }
@@ -55,6 +57,10 @@ __device__ __forceinline__ void split(float h, __bf16* hi, __bf16* lo) {
   const float rest = h - static_cast<float>(*hi);
   *lo = static_cast<__bf16>((__float_as_uint(rest) & 0x7f800000u) == 0x7f800000u ? 0.0f : rest);  // (of an infinity or a NaN hi is all there is)
 }
+
+// An infinity or a NaN among two bf16 numbers side by side.
+__device__ __forceinline__ bool pair_beyond(uint32_t two) { return (((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u) != 0; }
+__device__ __forceinline__ uint32_t pair_mask(uint32_t two) { return ((((two & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 15) * 0xffffu; }  // which of them
 
 // Sixteen e4m3 numbers as two operands of eight.
 template <typename T> __device__ __forceinline__ void widen(const i32x4& in, Pack8 (&out)[2]);

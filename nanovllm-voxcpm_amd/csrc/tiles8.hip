@@ -86,6 +86,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   };
   // The slices, one a lane.
   const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
+  const bool beyond = LORA && *any_h_beyond(a);  // some row's h is an infinity or a NaN
   int slice_column = 0, slice_wide = 0, slice_b[2] = {0, 0};
   if constexpr (LORA == kStaged) {
     const int s = lane < a.num_slices ? lane : 0;
@@ -301,7 +302,20 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   };
   // A step of the adapters; leaves the next step's blocks where it found its own.
   int mine[TT];
-  auto extra_step = [&](const Extra& e, int from, Eight(&w)[NN], Eight(&x01)[2]) {
+  // What the lane's row of block t gains from `some` ranks of a slot in one slice, one number at a time; where everything is NaN already, nothing.
+  auto add_row = [&](int t, int slot, int s, int first, int some, int t0, int n0) {
+    const int at = t0 + 16 * t + m < a.num_rows ? t0 + 16 * t + m : a.num_rows - 1;
+    const uint16_t* const hi = intermediate(a) + static_cast<int64_t>(at) * width + s * ranks;
+    const T* const b = static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(slot) * a.slices[s].n * a.r;
+#pragma unroll
+    for (int n = 0; n < NN; ++n) {
+      f32x4 sum = acc[t][n];
+      if (sum[0] != sum[0] && sum[1] != sum[1] && sum[2] != sum[2] && sum[3] != sum[3]) continue;
+      add_slowly(b, a.slices[s].n, n0 + 32 * (n >> 1) + 4 * (n & 1) - a.slices[s].y_col, a.r, first, some, hi, kParts<T> == 2 ? hi + static_cast<int64_t>(a.num_rows) * width : nullptr, sum);
+      acc[t][n] = sum;
+    }
+  };
+  auto extra_step = [&](const Extra& e, int from, int t0, int n0, Eight(&w)[NN], Eight(&x01)[2]) {
     const char* const xs = x_home + now * kStage;
     const int wide = __builtin_amdgcn_readlane(slice_wide, e.slice);
     Eight x[TT];
@@ -317,8 +331,31 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
     for (int t = 2; t < TT; ++t) block_of(xs, t, x[t]);
     turn_over();
+    // Of an infinity in B only the product with all of h is what the definition says, not the two that its parts and those of h would make: then one number at a time.
+    bool wild = false;
+    if constexpr (kParts<T> == 2) {
+      Pack8 zero;
+      zero.raw = i32x4{0, 0, 0, 0};
+      f32x4 none = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // (of numbers nothing but zero comes out, of others NaN)
+#pragma unroll
+      for (int n = 0; n < NN; ++n)
+#pragma unroll
+        for (int p = 0; p < 2; ++p) {
+          Pack8 raw;
+          raw.raw = w[n].piece[p];
+          none = Mma<T>::run(raw, zero, none);
+        }
+      settle();
+      wild = __ballot(!(none[0] + none[1] + none[2] + none[3] == 0.0f)) != 0;
+    }
+    if (wild && e.part == 0) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+        if (mine[t] == e.slot) add_row(t, e.slot, e.slice, e.c, 64, t0, n0);
+    }
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
+      if (wild) break;
       // (a lane's results are of one row, and come from that row's h alone: rows of other slots keep what they have, whatever is in this one's B)
       const bool own = mine[t] == e.slot;
       if (!__ballot(own)) continue;
@@ -400,14 +437,25 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
         for (int n = 0; n < NN; ++n) acc[t][n] *= columns[n];
     }
+    // Rows whose h is not all numbers (bits of `odd`) are left out by the products, in which an infinity or a NaN would reach other targets' columns (B is zero there), and come last.
+    unsigned odd = 0;
     if constexpr (LORA) {
 #pragma unroll
-      for (int t = 0; t < TT; ++t) mine[t] = table.slots[wt * (16 * TT) + 16 * t + m];
+      for (int t = 0; t < TT; ++t) {
+        mine[t] = table.slots[wt * (16 * TT) + 16 * t + m];
+        if (!beyond || mine[t] < 0) continue;
+        const int at = t0 + 16 * t + m < a.num_rows ? t0 + 16 * t + m : a.num_rows - 1;
+        for (int j = 0; j < width; j += 8) {
+          const i32x4 h = load128(intermediate(a) + static_cast<int64_t>(at) * width + j);
+          if (pair_beyond(h[0]) || pair_beyond(h[1]) || pair_beyond(h[2]) || pair_beyond(h[3])) odd |= 1u << t;
+        }
+        if (odd >> t & 1) mine[t] = -1;
+      }
     }
     if constexpr (LORA == kStaged) {
       while (coming.row < BT) {
         prepare();
-        extra_step(current, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, current.slice), w[0], x01[0]);
+        extra_step(current, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, current.slice), t0, n0, w[0], x01[0]);
       }
       settle();
     }
@@ -462,8 +510,20 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
               if (!there) raw[n].raw = i32x4{0, 0, 0, 0};
             }
             BPiece<T> b[NN];
+            Pack8 finite[NN];  // (an infinity in B meets the first part of h alone)
 #pragma unroll
-            for (int n = 0; n < NN; ++n) b[n].from(raw[n]);
+            for (int n = 0; n < NN; ++n) {
+              b[n].from(raw[n]);
+              finite[n] = b[n].hi;
+              if constexpr (kParts<T> == 2) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const uint32_t keep = ~pair_mask(finite[n].u[i]);
+                  finite[n].u[i] &= keep;
+                  b[n].lo.u[i] &= keep;
+                }
+              }
+            }
 #pragma unroll
             for (int t = 0; t < TT; ++t) {
               if (!has[t]) continue;
@@ -473,7 +533,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
               for (int n = 0; n < NN; ++n) {
                 f32x4 next = Mma<__bf16>::run(b[n].hi, h[t][0], acc[t][n]);
                 if constexpr (kParts<T> == 2) {
-                  next = Mma<__bf16>::run(b[n].hi, h[t][1], next);
+                  next = Mma<__bf16>::run(finite[n], h[t][1], next);
                   next = Mma<__bf16>::run(b[n].lo, h[t][0], next);
                 }
 #pragma unroll
@@ -483,6 +543,13 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
           }
         }
       }
+    }
+
+    if (LORA && __ballot(odd != 0)) {
+#pragma unroll
+      for (int t = 0; t < TT; ++t)
+        if (odd >> t & 1)
+          for (int s = 0; s < a.num_slices; ++s) add_row(t, table.slots[wt * (16 * TT) + 16 * t + m], s, 0, a.r, t0, n0);
     }
 
     float bias[NN / 2][8];
