@@ -436,7 +436,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
 // Very few rows with their adapters in one launch: sixteen columns a workgroup, which works out the rows' whole h for itself.
 //
 // A second launch and the trip of h through memory cost more than every workgroup's reading of the rows' A, from L2, as long as that is little (few_rows below).  The wavefronts share K, 128 columns each in turn, of the base product and of
-// h; h is added up in LDS, rounded as in the other kernels, and the wavefronts share its ranks in the second product.
+// h; h is added up in LDS and rounded as in the other kernels, and the first wavefront multiplies it with B, in one product: there are four pieces of eight ranks at most.
 constexpr int kFewGroups = 2;  // of sixteen ranks of a slot, all rows together
 
 template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_few_kernel(MloraProjectArgs a) {
@@ -460,16 +460,8 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
   const char* const w = static_cast<const char*>(a.w) + static_cast<int64_t>(n0 + m < a.n ? n0 + m : a.n - 1) * a.w_row;
   f32x4 acc[1] = {f32x4{0.0f, 0.0f, 0.0f, 0.0f}};
   auto meets = [&](int s) { return n0 < a.slices[s].y_col + a.slices[s].n && n0 + 16 > a.slices[s].y_col; };
-  // eight ranks of B of the lane's column, those of the c-th piece; zero where there are none
-  auto load_b = [&](int s, int c) {
-    Pack8 b;
-    b.raw = i32x4{0, 0, 0, 0};
-    const int d = c / pieces, in = n0 + m - a.slices[s].y_col;
-    const int slot = __shfl(list, c < total ? d : 0, kWave);
-    if (c < total && in >= 0 && in < a.slices[s].n)
-      b.raw = load128(static_cast<const T*>(a.slices[s].b) + (static_cast<int64_t>(slot) * a.slices[s].n + in) * a.r + 8 * (c - d * pieces));
-    return b;
-  };
+  // The lane's piece of the contraction: eight ranks of the d-th slot, from `first` on.
+  const int d = g / pieces, first = 8 * (g - d * pieces), slot = __shfl(list, g < total ? d : 0, kWave);
   // of a lane's piece behind the last column the row's first one is read, and nothing kept
   auto load_x = [&](int k, Eight& to) {
 #pragma unroll
@@ -491,12 +483,15 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
   for (int i = 0; i < 4; ++i) acc[0][i] *= a.w_scales[n0 + 4 * g + i < a.n ? n0 + 4 * g + i : a.n - 1];
   for (int s = 0; s < a.num_slices; ++s) {
     if (!meets(s)) continue;
-    Pack8 b = load_b(s, 4 * wave + g);  // (on its way while h comes about)
+    Pack8 b;  // (on its way while h comes about; zero where there is no piece, or the column is none of the slice's)
+    b.raw = i32x4{0, 0, 0, 0};
+    const int in = n0 + m - a.slices[s].y_col;
+    if (wave == 0 && g < total && in >= 0 && in < a.slices[s].n) b.raw = load128(static_cast<const T*>(a.slices[s].b) + (static_cast<int64_t>(slot) * a.slices[s].n + in) * a.r + first);
     const T* rows[kFewGroups];
 #pragma unroll
     for (int v = 0; v < kFewGroups; ++v) {
-      const int of = v < groups ? v : 0, d = of / of_slot, j = (of - d * of_slot) * 16 + m;
-      rows[v] = static_cast<const T*>(a.slices[s].a) + (static_cast<int64_t>(__builtin_amdgcn_readlane(list, d)) * a.r + (j < a.r ? j : a.r - 1)) * a.k;
+      const int of = v < groups ? v : 0, its = of / of_slot, j = (of - its * of_slot) * 16 + m;
+      rows[v] = static_cast<const T*>(a.slices[s].a) + (static_cast<int64_t>(__builtin_amdgcn_readlane(list, its)) * a.r + (j < a.r ? j : a.r - 1)) * a.k;
     }
     f32x4 h[kFewGroups];
 #pragma unroll
@@ -535,8 +530,8 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
       f32x4 sum = parts[wave][0][lane];
 #pragma unroll
       for (int v = 1; v < kRowWaves; ++v) sum += parts[wave][v][lane];
-      const int d = wave / of_slot, j = (wave - d * of_slot) * 16 + 4 * g;
-      if (ordinal == d) {
+      const int its = wave / of_slot, j = (wave - its * of_slot) * 16 + 4 * g;
+      if (ordinal == its) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           __bf16 hi, lo;
@@ -547,34 +542,29 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
       }
     }
     __syncthreads();
-    const f32x4 before = acc[0];
-    for (int first = 4 * wave; first < total; first += 4 * kRowWaves) {
-      const int c = first + g, d = c / pieces;
-      if (first != 4 * wave) b = load_b(s, c);
-      const bool own = c < total && ordinal == d;
+    if (wave == 0 && total) {
+      const f32x4 before = acc[0];
+      const bool own = g < total && ordinal == d;
       BPiece<T> of;
       of.from(b);
       Pack8 h;
 #pragma unroll
       for (int v = 0; v < kParts<T>; ++v) {
-        h.raw = own ? load128(&h_of[v][m][8 * (c - d * pieces)]) : i32x4{0, 0, 0, 0};
+        h.raw = own ? load128(&h_of[v][m][first]) : i32x4{0, 0, 0, 0};
         acc[0] = Mma<__bf16>::run(of.hi, h, acc[0]);
         if constexpr (kParts<T> == 2)
           if (v == 0) acc[0] = Mma<__bf16>::run(of.lo, h, acc[0]);
       }
-    }
-    mfma_settle(acc);
-    // (infinities and NaN in B: see the kernel above)
-    bool beyond = false;
+      mfma_settle(acc);
+      // (infinities and NaN in B: see the kernel above)
+      bool beyond = false;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) beyond |= (__float_as_uint(acc[0][i]) & 0x7f800000u) == 0x7f800000u;
-    if (4 * wave < total && __ballot(beyond)) {
-      acc[0] = before;
-      for (int c = 0; c < total; ++c) {
-        const int d = c / pieces, j = 8 * (c - d * pieces);
-        if (c / 4 % kRowWaves != wave || ordinal != d) continue;
-        const T* const of = static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(__builtin_amdgcn_readlane(list, d)) * a.slices[s].n * a.r;
-        add_slowly(of, a.slices[s].n, n0 + 4 * g - a.slices[s].y_col, a.r, j, 8, h_of[0][m], kParts<T> == 2 ? h_of[kParts<T> - 1][m] : nullptr, acc[0]);
+      for (int i = 0; i < 4; ++i) beyond |= (__float_as_uint(acc[0][i]) & 0x7f800000u) == 0x7f800000u;
+      if (__ballot(beyond)) {
+        acc[0] = before;
+        if (ordinal >= 0)
+          add_slowly(static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(mine) * a.slices[s].n * a.r, a.slices[s].n, n0 + 4 * g - a.slices[s].y_col, a.r, 0, a.r, h_of[0][m],
+                     kParts<T> == 2 ? h_of[kParts<T> - 1][m] : nullptr, acc[0]);
       }
     }
     __syncthreads();  // (the next slice has another h)
