@@ -2,9 +2,10 @@
 //
 //   y[t, n] = xs[t] ws[n] sum_k x8[t, k] w8[n, k] + bias[n] + sum_j h[t, j] B[slot of t, n, j]
 //
-// The base product runs on the 16x16x128 e4m3 matrix instruction, weights as its rows, so that a lane holds consecutive columns of one row of y.  The adapters' second
-// product continues in the same accumulators: its contraction is a list of pieces of eight ranks, those of the different slots among sixteen rows one behind the other, in which a
-// row's h is zero outside its own slot's.
+// The base product runs on the 16x16x128 e4m3 matrix instruction, weights as its rows, so that a lane holds consecutive columns of one row of y.  The contraction of the adapters' second
+// product is a list of pieces of eight ranks, those of the different slots among sixteen rows one behind the other, in which a row's h is zero outside its own slot's; it has accumulators of its own, and
+// a row's pieces are added in the order of its ranks wherever its slot stands in the list: a row's result does not depend on which adapters the rows beside it have (but for one of infinities or NaN, beside which
+// the row's sum is taken in another order).
 //
 // Few rows are bound by the weights' way to the compute units: 64 rows, k 1024, n 8192 6.4 us (8.4 MB; with 32 slots of rank 32, 21 MB more, 16.2), 201 rows, k 8192, n 2048 17 us (all workgroups together take 200 MB from L2 in that time, 46 bytes a ns
 // each; with 48 fp16 slots of rank 64, 63 MB more, 41 us, of which the first product 12.5), one row 3.8 us, with its adapter 7.0.
@@ -22,8 +23,8 @@ namespace {
 //
 // A stage is 128 columns of K for each of kSplit = 8 / TF wavefronts a block of sixteen rows has; stages come by direct loads, whole 128-byte lines, into a ring in LDS as deep as it holds,
 // so that for K up to some thousand everything is asked for at once.  A wavefront multiplies one block of rows with all columns of its share of a stage; the shares meet in LDS at the end.
-// The adapters follow as more stages: pieces of eight ranks of one of the different slots among a block's sixteen rows go to the block's wavefronts in turn, four of them a product, and a stage
-// holds each wavefront's own B and h.  (Ranks that are no multiple of eight, whose rows of B lie anywhere, are loaded by the lanes behind the last stage.)
+// The adapters follow as more stages: pieces of eight ranks of one of the different slots among a block's sixteen rows go to the block's wavefronts in turn, four of them a product (of one slot, or of four or two whole slots
+// of one piece or two), and a stage holds each wavefront's own B and h.  (Ranks that are no multiple of eight, whose rows of B lie anywhere, are loaded by the lanes behind the last stage.)
 //
 // Rows in four blocks (more than 32, up to kSorted) are taken in the order of their slots where there are eight slots or more; every workgroup works the order out for itself.  The sixteen rows of a block then
 // have few different slots.  (us in their own order / sorted, bf16: 256 rows, k 1024, n 1536, 48 slots of rank 64 36.8 / 26.5, 8 of rank 32 20.6 / 20.7, one slot 16.9 / 20.7; 64 rows, k 2048, n 2048,
@@ -35,7 +36,7 @@ template <int TF, int NF> struct RowsShape {
   static constexpr int kPer = (kRows * 128 * kSplit + 1024 * kRowWaves - 1) / (1024 * kRowWaves), kStage = kPer * 1024 * kRowWaves;  // (as many loads for every wavefront: some of nothing)
   static constexpr int kRing = kStage > 40 * 1024 ? 3 : kStage > 24 * 1024 ? 4 : 6;
   static constexpr int kMost = kRing * kStage, kOrder = kMost + 64, kLds = kOrder + (TF == 4 ? kSorted * 4 : 0);  // (behind the ring: the blocks' numbers of groups, the rows' order)
-  static_assert(kLds <= kMostLds && kRowWaves * NF * 1024 <= kLds && NF < kPer, "stages");
+  static_assert(kLds <= kMostLds && 2 * kRowWaves * NF * 1024 + 64 * TF <= kMost && NF < kPer, "stages");
 };
 
 // The column of y that row `at` of a workgroup's weights is: a lane ends up with 4 NF of them side by side.
@@ -115,7 +116,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     if (i < stages) request();
 
   // the different slots among the block's rows: lane d (and d + 16, ...) holds the d-th, `ordinal` is which one the row's is
-  const int ranks = padded_ranks(a.r), pieces = ranks / 8, width = a.num_slices * ranks;
+  const int ranks = padded_ranks(a.r), pieces = ranks ? ranks / 8 : 1, width = a.num_slices * ranks;
   int list = -1, ordinal = -1, count = 0;
   if (a.num_slices) {
     unsigned long long left = __ballot(mine >= 0) & 0xffffull;
@@ -128,12 +129,12 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
       ++count;
     }
   }
-  const float inverse = 1.0f / static_cast<float>(pieces);
-  auto slot_place = [&](int c) {  // which slot the c-th piece is of
-    const int d = static_cast<int>((static_cast<float>(c) + 0.5f) * inverse);
-    return d < count ? d : count - 1;
-  };
-  const int total = count * pieces, groups = (total + 3) / 4;
+  // Groups of four pieces, a product's: slots of one piece or two share one, others have as many of their own as they need.
+  const bool packed = pieces <= 2;
+  const int quarters = (pieces + 3) >> 2, shift = packed ? 3 - pieces : 0;  // a slot's groups; a group has 2^shift slots
+  const int groups = packed ? (count + (1 << shift) - 1) >> shift : count * quarters;
+  // The wavefront that has the first of the row's groups: the others follow it in turn.
+  const int leader = (packed ? ordinal >> shift : ordinal * quarters) & (S::kSplit - 1);
   auto meeting = [&](int s) {  // the first slice from s on that the columns meet
     while (s < a.num_slices && (n0 + 16 * NF <= a.slices[s].y_col || n0 >= a.slices[s].y_col + a.slices[s].n)) ++s;
     return s;
@@ -143,14 +144,18 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     int d, first;
     bool there;
   };
-  auto place_of = [&](int group) {
-    const int c = 4 * group + g, d = slot_place(c);
-    return Place{d, c < total ? 8 * (c - d * pieces) : 0, c < total};
+  auto packed_place = [&](int group) {
+    const int c = 4 * group + g, d = c >> (pieces - 1);
+    return Place{d, d < count ? 8 * (c - d * pieces) : 0, d < count};
+  };
+  auto place_in = [&](int d, int quarter) {
+    const int first = 32 * quarter + 8 * g;
+    return Place{d, first < ranks ? first : 0, first < ranks};
   };
   const uint16_t* const h_row = intermediate(a) + static_cast<int64_t>(row < a.num_rows ? row : a.num_rows - 1) * width;
   const int block_row = sorted ? 0 : t0 + 16 * f < a.num_rows ? t0 + 16 * f : a.num_rows - 1;  // (a block behind the last row: its loads are of that)
   const char* const h_block = reinterpret_cast<const char*>(intermediate(a) + static_cast<int64_t>(block_row) * width);
-  const uint32_t h_lane = static_cast<uint32_t>((row < a.num_rows ? row - block_row : a.num_rows - 1 - block_row) * width * 2 + 16 * g);
+  const uint32_t h_lane = static_cast<uint32_t>((row < a.num_rows ? row - block_row : a.num_rows - 1 - block_row) * width * 2);
   // Of a slice: where its B is, how far apart two slots are in it, and the lane's rows (any for a column that is none of the slice's).
   struct Slice {
     const T* b;
@@ -174,12 +179,10 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   int rounds = 0;
   struct Extra {
     int slice, round, part;
-    int d, quarter;  // where a slot is whole groups of four pieces: the group's slot and which of its groups it is
+    int d, quarter;  // where a slot has groups of its own: the group's slot and which of its groups it is
   };
-  const int quarters = pieces / 4;
-  const bool even = pieces % 4 == 0;
   auto settle_quarter = [&](Extra& e) {
-    if (!even) return;
+    if (packed) return;
     while (e.quarter >= quarters) {
       e.quarter -= quarters;
       ++e.d;
@@ -217,18 +220,18 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   auto request_extra = [&]() {
     const uint32_t to = __builtin_amdgcn_readfirstlane(home + put * S::kStage);
     const int group = load_extra.round * S::kSplit + part;
-    if (even && group < groups) {
-      // a slot's 32 ranks: everything but the lane's row and its eight ranks is the same for all
-      const char* const b = reinterpret_cast<const char*>(load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(list, load_extra.d))) * load_slice.slot_stride) +
-                            64 * load_extra.quarter;
-      const char* const h = h_block + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width * 2 : 0) + load_extra.slice * ranks * 2 + 64 * load_extra.quarter;
+    if (!packed && group < groups) {
+      // a slot's 32 ranks: everything but the lane's row and its eight ranks (of which the last group may have fewer) is the same for all
+      const uint32_t in = 64 * load_extra.quarter + 16 * g, at = in < static_cast<uint32_t>(2 * ranks) ? in : 0;
+      const char* const b = reinterpret_cast<const char*>(load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(list, load_extra.d))) * load_slice.slot_stride);
+      const char* const h = h_block + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width * 2 : 0) + load_extra.slice * ranks * 2;
 #pragma unroll
       for (int i = 0; i < S::kPer; ++i) {
-        if (i < NF) dma16_from(uniform(b), load_slice.in[i] * 2 + 16 * g, to + i * 1024);
-        else dma16_from(uniform(h), h_lane, to + i * 1024);
+        if (i < NF) dma16_from(uniform(b), load_slice.in[i] * 2 + at, to + i * 1024);
+        else dma16_from(uniform(h), h_lane + at, to + i * 1024);
       }
     } else {
-      const Place p = place_of(group < groups ? group : 0);
+      const Place p = packed ? packed_place(group < groups ? group : 0) : Place{0, 0, false};
       const uint16_t* const h = h_row + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width : 0) + load_extra.slice * ranks + p.first;
       const T* const b = load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * load_slice.slot_stride + p.first;
 #pragma unroll
@@ -247,9 +250,9 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   };
   while (asked < S::kRing - 1 && asked < stages + extras) request_next();
 
-  f32x4 acc[NF];
+  f32x4 acc[NF], update[NF];  // the base product, the adapters'
 #pragma unroll
-  for (int n = 0; n < NF; ++n) acc[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+  for (int n = 0; n < NF; ++n) acc[n] = update[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // Four pieces of B with the block's h.  What is not the row's, or no piece, is zero in h; columns outside the slice are in B.
   auto add_group = [&](int slice, const Place& p, bool whole, int h_part, Pack8(&raw)[NF], Pack8(&h)[kParts<T>]) {
     if (!whole) {
@@ -267,14 +270,14 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     for (int n = 0; n < NF; ++n) {
       BPiece<T> b;
       b.from(raw[n]);
-      acc[n] = Mma<__bf16>::run(b.hi, h[0], acc[n]);
+      update[n] = Mma<__bf16>::run(b.hi, h[0], update[n]);
       if constexpr (kParts<T> == 2) {  // (a stage has one part of h: the other one here is zero)
         if (h_part) b.lo.raw = i32x4{0, 0, 0, 0};
-        acc[n] = Mma<__bf16>::run(b.lo, h[0], acc[n]);
-        if constexpr (LOOSE) acc[n] = Mma<__bf16>::run(b.hi, h[1], acc[n]);
+        update[n] = Mma<__bf16>::run(b.lo, h[0], update[n]);
+        if constexpr (LOOSE) update[n] = Mma<__bf16>::run(b.hi, h[1], update[n]);
       }
     }
-    mfma_settle(acc);
+    mfma_settle(update);
   };
 
   const char* const share = lds + part * (S::kRows * 128) + m * 128;
@@ -334,9 +337,6 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n][i] *= a.w_scales[c + i < a.n ? c + i : a.n - 1];
   }
-  f32x4 product[NF];  // the base product by itself
-#pragma unroll
-  for (int n = 0; n < NF; ++n) product[n] = acc[n];
   if (!LOOSE && extras) {
     Extra e = {meeting(0), 0, 0, 0, part};
     settle_quarter(e);
@@ -356,7 +356,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
         for (int n = 0; n < NF; ++n) raw[n].raw = load128(at + n * 1024);
         h[0].raw = load128(at + NF * 1024);
         if constexpr (kParts<T> == 2) h[1].raw = i32x4{0, 0, 0, 0};
-        add_group(e.slice, even ? Place{e.d, 0, true} : place_of(group), slice.whole, e.part, raw, h);
+        add_group(e.slice, packed ? packed_place(group) : place_in(e.d, e.quarter), slice.whole, e.part, raw, h);
       }
       advance(e, slice);
     }
@@ -364,8 +364,12 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   if constexpr (LOOSE) {
     for (int s = meeting(0); s < a.num_slices; s = meeting(s + 1)) {
       const Slice slice = slice_of(s);
+      Extra e = {s, 0, 0, 0, part};
+      settle_quarter(e);
       for (int group = part; group < groups; group += S::kSplit) {
-        const Place p = place_of(group);
+        const Place p = packed ? packed_place(group) : place_in(e.d, e.quarter);
+        e.quarter += S::kSplit;
+        settle_quarter(e);
         const T* const b_slot = slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * slice.slot_stride;
         Pack8 raw[NF], h[kParts<T>];
 #pragma unroll
@@ -383,33 +387,42 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
       }
     }
   }
-  // An infinity or a NaN in B goes through a matrix product to the rows of other slots (0 times it is NaN): where one came out the rows' own adapters are added again, one number at a time.
-  bool beyond = false;
+  // An infinity or a NaN in B goes through a matrix product to the rows of other slots (0 times it is NaN): where one came out the row's own adapter is added again, one number at a time.
+  unsigned beyond = 0;
 #pragma unroll
   for (int n = 0; n < NF; ++n)
 #pragma unroll
-    for (int i = 0; i < 4; ++i) beyond |= (__float_as_uint(acc[n][i]) & 0x7f800000u) == 0x7f800000u;
-  if (groups > part && __ballot(beyond)) {
+    for (int i = 0; i < 4; ++i) beyond |= (__float_as_uint(update[n][i]) & 0x7f800000u) == 0x7f800000u ? 1u << n : 0;
+  if (beyond) {
 #pragma unroll
-    for (int n = 0; n < NF; ++n) acc[n] = product[n];
-    for (int s = meeting(0); s < a.num_slices; s = meeting(s + 1))
-      for (int c = 0; c < total; ++c) {
-        const int of = __builtin_amdgcn_readfirstlane(slot_place(c));
-        if (c / 4 % S::kSplit != part || ordinal != of) continue;
-        const T* const b = static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(__builtin_amdgcn_readlane(list, of)) * a.slices[s].n * a.r;
-        const uint16_t* const hi = h_row + s * ranks;
+    for (int n = 0; n < NF; ++n)
+      if (beyond >> n & 1) update[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int ahead = (part - leader) & (S::kSplit - 1);  // which of the row's groups the wavefront has first
+    if (ordinal >= 0)
+      for (int s = meeting(0); s < a.num_slices; s = meeting(s + 1))
+        for (int quarter = ahead; quarter < quarters; quarter += S::kSplit) {
+          const T* const b = static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(mine) * a.slices[s].n * a.r;
+          const uint16_t* const hi = h_row + s * ranks;
 #pragma unroll
-        for (int n = 0; n < NF; ++n)
-          add_slowly(b, a.slices[s].n, n0 + 4 * NF * g + 4 * n - a.slices[s].y_col, a.r, 8 * (c - of * pieces), 8, hi, kParts<T> == 2 ? hi + static_cast<int64_t>(a.num_rows) * width : nullptr, acc[n]);
-      }
+          for (int n = 0; n < NF; ++n)
+            if (beyond >> n & 1)
+              add_slowly(b, a.slices[s].n, n0 + 4 * NF * g + 4 * n - a.slices[s].y_col, a.r, 32 * quarter, 32, hi, kParts<T> == 2 ? hi + static_cast<int64_t>(a.num_rows) * width : nullptr, update[n]);
+        }
   }
   // the shares meet
   wait_lds();
   wait_loads<0>();
   __syncthreads();
+  constexpr int kUpdates = kRowWaves * NF * 64;
   f32x4* const parts = reinterpret_cast<f32x4*>(lds);
+  int32_t* const leaders = reinterpret_cast<int32_t*>(lds + 2 * kUpdates * 16);
 #pragma unroll
   for (int n = 0; n < NF; ++n) parts[(wave * NF + n) * 64 + lane] = acc[n];
+  if (a.num_slices) {
+#pragma unroll
+    for (int n = 0; n < NF; ++n) parts[kUpdates + (wave * NF + n) * 64 + lane] = update[n];
+    if (part == 0 && g == 0) leaders[16 * f + m] = leader;
+  }
   __syncthreads();
   for (int block = wave; block < TF * NF; block += kRowWaves) {
     const int of = block / NF, c = n0 + 4 * NF * g + 4 * (block % NF);
@@ -418,6 +431,12 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     f32x4 sum = parts[(of * NF + block % NF) * 64 + lane];
 #pragma unroll
     for (int v = 1; v < S::kSplit; ++v) sum += parts[((v * TF + of) * NF + block % NF) * 64 + lane];
+    if (a.num_slices) {
+      const int first = leaders[16 * of + m];
+      f32x4 added = parts[kUpdates + ((first * TF + of) * NF + block % NF) * 64 + lane];
+      for (int v = 1; v < S::kSplit && v < quarters; ++v) added += parts[kUpdates + ((((first + v) & (S::kSplit - 1)) * TF + of) * NF + block % NF) * 64 + lane];
+      sum += added;
+    }
     const float scale = a.x_scales[t];
     T out[4];
 #pragma unroll
@@ -560,7 +579,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
       bool beyond = false;
 #pragma unroll
       for (int i = 0; i < 4; ++i) beyond |= (__float_as_uint(acc[0][i]) & 0x7f800000u) == 0x7f800000u;
-      if (__ballot(beyond)) {
+      if (beyond) {
         acc[0] = before;
         if (ordinal >= 0)
           add_slowly(static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(mine) * a.slices[s].n * a.r, a.slices[s].n, n0 + 4 * g - a.slices[s].y_col, a.r, 0, a.r, h_of[0][m],
