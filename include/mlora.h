@@ -447,8 +447,8 @@ int mlora_quantize_rows(const MloraRowsArgs* args);
  *   y[t, n] = x_scales[t] w_scales[n] sum_k x[t, k] w[n, k] + bias[n]
  *             + sum_j h[t, j] b[slot, n - y_col, j],  h[t, j] = x_scales[t] sum_k x[t, k] a[slot, j, k]
  * for the slice that column n lies in (if any) and slot = token_to_slot[t] (an id outside [0, num_slots): no adapter).  Sums are
- * fp32 and y is rounded once; h, without the row's scale, is kept in bf16: beside bf16 adapters
- * one number (2^-8 of it), beside fp16 ones two (2^-16).  Infinities and NaN in an adapter give what the formula does, in the rows of its slot and the
+ * fp32 and y is rounded once; h, without the row's scale, is kept in bf16: two numbers a
+ * value (2^-16 of it).  Infinities and NaN in an adapter give what the formula does, in the rows of its slot and the
  * columns of its slice alone.  y lies on none of the inputs.
  * (reference: nanovllm_voxcpm/layers/lora.py, the linears' forward, with weights in 16 bits there) */
 typedef struct MloraProjectArgs {

@@ -63,6 +63,16 @@ template <int PER, int MOST> __device__ __forceinline__ void wait_stages(int you
   else wait_loads<0>();
 }
 
+// Waits until no more than `most` loads (of which as many as N are counted) are on their way.
+template <int N> __device__ __forceinline__ void wait_at_most(int most) {
+  if constexpr (N == 0) {
+    wait_loads<0>();
+  } else {
+    if (most >= N) wait_loads<N>();
+    else wait_at_most<N - 1>(most);
+  }
+}
+
 // A barrier that waits for no load.
 __device__ __forceinline__ void stage_barrier() { asm volatile("s_barrier" ::: "memory"); }
 

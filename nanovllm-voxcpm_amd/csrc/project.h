@@ -7,6 +7,8 @@ namespace mlora {
 
 // Which kernel serves a call: rows by themselves where they are few, else tiles.  Which of the two does not depend on the adapters, so that a row's base product does not.
 enum { kRows, kTiles64, kTiles64x128, kTiles128 };
+// Adapters: none, through LDS like the rest, or by loads of the lanes (ranks that are no multiple of eight, whose rows of B lie anywhere).
+enum { kNone, kStaged, kLoose };
 int project_kind(const MloraProjectArgs* a);
 
 // shrink8.hip: the adapters' first product, and in front of tiles the rows' order by slot
@@ -35,11 +37,9 @@ __device__ __forceinline__ f32x4 mma8(const Eight& a, const Eight& b, f32x4 c) {
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a.all, b.all, c, 0, 0, 0, 0, 0, 0);
 }
 
-// The intermediate h of the adapters, fp32 in value, lies in the workspace as bf16 numbers, [rows][slices][ranks rounded up to eight]: the second product multiplies 16-bit numbers, and unlike
-// fp16's the range of bf16 holds any h.  Beside bf16 adapters it is rounded once (2^-8 of h at most, as the base product's 16-bit input and the other forms' intermediate are); beside
-// fp16 ones, whose B has three bits more, a second array holds what the first leaves over, and B goes in two pieces as well: 2^-16.
-template <typename T> constexpr int kParts = 1;
-template <> constexpr int kParts<_Float16> = 2;
+// The intermediate h of the adapters, fp32 in value, lies in the workspace as two bf16 numbers, its leading part and what that leaves over, [rows][slices][ranks rounded up to eight] each: the second
+// product multiplies 16-bit numbers, and unlike fp16's the range of bf16 holds any h.  h is off by 2^-16 of itself at most (one part alone by 2^-8, which shows wherever ranks cancel).  B of bf16 adapters is
+// multiplied with both parts; fp16's, which has three bits more, goes in two pieces as well, of which the second meets the leading part of h alone: 2^-16 once more.
 // In front of it lie, for tiles, the rows by slot (their numbers, their slots, where the slots end; h has their order then, else that of the rows), the groups of up to 64 rows of a slot, and whether
 // any h is an infinity or a NaN.
 __host__ __device__ inline int padded_ranks(int r) { return (r + 7) & ~7; }
@@ -86,14 +86,16 @@ __device__ __forceinline__ int slot_of(const MloraProjectArgs& a, int row) {
   return s >= 0 && s < a.num_slots ? s : -1;
 }
 
-// Eight elements of B as bf16 numbers hi + lo (of bf16 adapters lo is nothing).
+// Eight elements of B as bf16 numbers hi + lo, or hi alone.
 template <typename T> struct BPiece;
 template <> struct BPiece<__bf16> {
-    Pack8 hi;
+  static constexpr bool kTwo = false;
+  Pack8 hi;
   __device__ __forceinline__ void from(const Pack8& raw) { hi = raw; }
 };
 template <> struct BPiece<_Float16> {
-    Pack8 hi, lo;
+  static constexpr bool kTwo = true;
+  Pack8 hi, lo;
   __device__ __forceinline__ void from(const Pack8& raw) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -109,7 +111,7 @@ template <> struct BPiece<_Float16> {
 template <typename T>
 __device__ inline void add_slowly(const T* b, int columns, int n, int r, int first, int some, const uint16_t* hi, const uint16_t* lo, f32x4& acc) {
   for (int j = first; j < first + some && j < r; ++j) {
-    const float h = static_cast<float>(__builtin_bit_cast(__bf16, hi[j])) + (lo ? static_cast<float>(__builtin_bit_cast(__bf16, lo[j])) : 0.0f);
+    const float h = static_cast<float>(__builtin_bit_cast(__bf16, hi[j])) + static_cast<float>(__builtin_bit_cast(__bf16, lo[j]));
 #pragma unroll
     for (int i = 0; i < 4; ++i)
       if (n + i >= 0 && n + i < columns) acc[i] += h * to_f32(b[static_cast<int64_t>(n + i) * r + j]);

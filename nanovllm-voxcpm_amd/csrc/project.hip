@@ -31,9 +31,11 @@ namespace {
 // 16 slots of rank 64 21.4 / 18.1; 32 rows, k 1024, n 8192, 8 slots of rank 32 11.8 / 12.3.  201 rows of 48 fp16 slots of rank 64, k 8192, n 2048: 55.8 / 43.3.)
 constexpr int kRowWaves = 8, kSorted = 256;
 
-template <int TF, int NF> struct RowsShape {
+template <int TF, int NF, int LORA> struct RowsShape {
   static constexpr int kSplit = kRowWaves / TF, kRows = 16 * (TF + NF);
-  static constexpr int kPer = (kRows * 128 * kSplit + 1024 * kRowWaves - 1) / (1024 * kRowWaves), kStage = kPer * 1024 * kRowWaves;  // (as many loads for every wavefront: some of nothing)
+  static constexpr int kPer = (kRows * 128 * kSplit + 1024 * kRowWaves - 1) / (1024 * kRowWaves);  // loads of a wavefront in a stage of the base product (as many for every one: some of nothing)
+  static constexpr int kExtra = NF + 2, kMore = LORA == kStaged && kExtra > kPer ? kExtra - kPer : 0;  // in one of the adapters: B, and both parts of h
+  static constexpr int kStage = (kPer + kMore) * 1024 * kRowWaves;
   static constexpr int kRing = kStage > 40 * 1024 ? 3 : kStage > 24 * 1024 ? 4 : 6;
   static constexpr int kMost = kRing * kStage, kOrder = kMost + 64, kLds = kOrder + (TF == 4 ? kSorted * 4 : 0);  // (behind the ring: the blocks' numbers of groups, the rows' order)
   static_assert(kLds <= kMostLds && 2 * kRowWaves * NF * 1024 + 64 * TF <= kMost && NF < kPer, "stages");
@@ -70,18 +72,18 @@ __device__ __forceinline__ void sort_rows(const MloraProjectArgs& a, int32_t* ke
   __syncthreads();
 }
 
-template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(kRowWaves * 64) void project_rows_kernel(MloraProjectArgs a) {
-  using S = RowsShape<TF, NF>;
+template <typename T, int TF, int NF, int LORA> __global__ __launch_bounds__(kRowWaves * 64) void project_rows_kernel(MloraProjectArgs a) {
+  using S = RowsShape<TF, NF, LORA>;
   extern __shared__ char lds[];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int f = wave % TF, part = wave / TF;
   const int n0 = blockIdx.x * (16 * NF), t0 = blockIdx.y * (16 * TF);
-  const bool sorted = TF == 4 && a.num_slices && a.num_slots >= 8 && a.num_rows <= kSorted;
+  const bool sorted = TF == 4 && LORA && a.num_slots >= 8 && a.num_rows <= kSorted;
   const int32_t* const order = reinterpret_cast<const int32_t*>(lds + S::kOrder);
   if (sorted) sort_rows(a, reinterpret_cast<int32_t*>(lds), reinterpret_cast<int32_t*>(lds + S::kOrder));
   auto row_at = [&](int t) { return sorted && t < a.num_rows ? order[t] : t; };
   const int row = row_at(t0 + 16 * f + m);
-  const int mine = a.num_slices ? slot_of(a, row) : -1;  // first of all: the adapters' loads wait for it
+  const int mine = LORA ? slot_of(a, row) : -1;  // first of all: the adapters' loads wait for it
 
   // what this wavefront loads of a stage: blocks of eight rows, of x or of w
   const char* from[S::kPer];
@@ -116,9 +118,9 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     if (i < stages) request();
 
   // the different slots among the block's rows: lane d (and d + 16, ...) holds the d-th, `ordinal` is which one the row's is
-  const int ranks = padded_ranks(a.r), pieces = ranks ? ranks / 8 : 1, width = a.num_slices * ranks;
+  const int ranks = padded_ranks(a.r), pieces = ranks / 8, width = a.num_slices * ranks;
   int list = -1, ordinal = -1, count = 0;
-  if (a.num_slices) {
+  if constexpr (LORA) {
     unsigned long long left = __ballot(mine >= 0) & 0xffffull;
     while (left) {
       const int s = __builtin_amdgcn_readlane(mine, __builtin_ctzll(left));
@@ -175,10 +177,10 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     }
     return of;
   };
-  // The adapters' stages, the same number for every wavefront: of each slice, as many as the block with most groups has for a wavefront, each once for either part of h.
+  // The adapters' stages, the same number for every wavefront: of each slice, as many as the block with most groups has for a wavefront.
   int rounds = 0;
   struct Extra {
-    int slice, round, part;
+    int slice, round;
     int d, quarter;  // where a slot has groups of its own: the group's slot and which of its groups it is
   };
   auto settle_quarter = [&](Extra& e) {
@@ -188,10 +190,10 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
       ++e.d;
     }
   };
-  Extra load_extra = {a.num_slices, 0, 0, 0, part};
+  Extra load_extra = {a.num_slices, 0, 0, part};
   Slice load_slice = {};
   int extras = 0;
-  if (!LOOSE && a.num_slices) {
+  if constexpr (LORA == kStaged) {
     int32_t* const most = reinterpret_cast<int32_t*>(lds + S::kMost);
     if (part == 0 && lane == 0) most[f] = groups;
     wait_lds();
@@ -200,13 +202,11 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     rounds = __builtin_amdgcn_readfirstlane((rounds + S::kSplit - 1) / S::kSplit);
     load_extra.slice = meeting(0);
     if (rounds)
-      for (int s = load_extra.slice; s < a.num_slices; s = meeting(s + 1)) extras += rounds * kParts<T>;
+      for (int s = load_extra.slice; s < a.num_slices; s = meeting(s + 1)) extras += rounds;
     if (extras) load_slice = slice_of(load_extra.slice);
     settle_quarter(load_extra);
   }
   auto advance = [&](Extra& e, Slice& slice) {
-    if (++e.part < kParts<T>) return;
-    e.part = 0;
     e.quarter += S::kSplit;
     settle_quarter(e);
     if (++e.round < rounds) return;
@@ -217,27 +217,30 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     e.slice = meeting(e.slice + 1);
     if (e.slice < a.num_slices) slice = slice_of(e.slice);
   };
+  // Where the i-th of a wavefront's loads of an adapters' stage goes: those that the base product's stages do not have lie behind theirs.
+  auto place_of = [&](int i) { return i < S::kPer ? wave * (S::kPer * 1024) + i * 1024 : S::kPer * 1024 * kRowWaves + (wave * S::kMore + i - S::kPer) * 1024; };
+  const int64_t h_rest = static_cast<int64_t>(a.num_rows) * width;  // from one part of h to the other
   auto request_extra = [&]() {
-    const uint32_t to = __builtin_amdgcn_readfirstlane(home + put * S::kStage);
+    const uint32_t to = __builtin_amdgcn_readfirstlane(lds_address(lds) + put * S::kStage);
     const int group = load_extra.round * S::kSplit + part;
     if (!packed && group < groups) {
       // a slot's 32 ranks: everything but the lane's row and its eight ranks (of which the last group may have fewer) is the same for all
       const uint32_t in = 64 * load_extra.quarter + 16 * g, at = in < static_cast<uint32_t>(2 * ranks) ? in : 0;
       const char* const b = reinterpret_cast<const char*>(load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(list, load_extra.d))) * load_slice.slot_stride);
-      const char* const h = h_block + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width * 2 : 0) + load_extra.slice * ranks * 2;
+      const char* const h = h_block + load_extra.slice * ranks * 2;
 #pragma unroll
-      for (int i = 0; i < S::kPer; ++i) {
-        if (i < NF) dma16_from(uniform(b), load_slice.in[i] * 2 + at, to + i * 1024);
-        else dma16_from(uniform(h), h_lane + at, to + i * 1024);
+      for (int i = 0; i < S::kExtra; ++i) {
+        if (i < NF) dma16_from(uniform(b), load_slice.in[i] * 2 + at, to + place_of(i));
+        else dma16_from(uniform(i == NF ? h : h + 2 * h_rest), h_lane + at, to + place_of(i));
       }
     } else {
       const Place p = packed ? packed_place(group < groups ? group : 0) : Place{0, 0, false};
-      const uint16_t* const h = h_row + (load_extra.part ? static_cast<int64_t>(a.num_rows) * width : 0) + load_extra.slice * ranks + p.first;
+      const uint16_t* const h = h_row + load_extra.slice * ranks + p.first;
       const T* const b = load_slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * load_slice.slot_stride + p.first;
 #pragma unroll
-      for (int i = 0; i < S::kPer; ++i) {  // (as many as of any stage; without a group, and behind the last piece, of something that is there)
-        if (i < NF && count) dma16v(reinterpret_cast<const char*>(b + load_slice.in[i]), to + i * 1024);
-        else dma16v(reinterpret_cast<const char*>(h), to + i * 1024);
+      for (int i = 0; i < S::kExtra; ++i) {  // (as many as of any stage; without a group, and behind the last piece, of something that is there)
+        if (i < NF && count) dma16v(reinterpret_cast<const char*>(b + load_slice.in[i]), to + place_of(i));
+        else dma16v(reinterpret_cast<const char*>(i <= NF ? h : h + h_rest), to + place_of(i));
       }
     }
     put = put == S::kRing - 1 ? 0 : put + 1;
@@ -254,7 +257,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
 #pragma unroll
   for (int n = 0; n < NF; ++n) acc[n] = update[n] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
   // Four pieces of B with the block's h.  What is not the row's, or no piece, is zero in h; columns outside the slice are in B.
-  auto add_group = [&](int slice, const Place& p, bool whole, int h_part, Pack8(&raw)[NF], Pack8(&h)[kParts<T>]) {
+  auto add_group = [&](int slice, const Place& p, bool whole, Pack8(&raw)[NF], Pack8(&h)[2]) {
     if (!whole) {
 #pragma unroll
       for (int n = 0; n < NF; ++n) {
@@ -264,18 +267,15 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     }
     const bool own = p.there && ordinal == p.d;
 #pragma unroll
-    for (int v = 0; v < kParts<T>; ++v)
+    for (int v = 0; v < 2; ++v)
       if (!own) h[v].raw = i32x4{0, 0, 0, 0};
 #pragma unroll
     for (int n = 0; n < NF; ++n) {
       BPiece<T> b;
       b.from(raw[n]);
       update[n] = Mma<__bf16>::run(b.hi, h[0], update[n]);
-      if constexpr (kParts<T> == 2) {  // (a stage has one part of h: the other one here is zero)
-        if (h_part) b.lo.raw = i32x4{0, 0, 0, 0};
-        update[n] = Mma<__bf16>::run(b.lo, h[0], update[n]);
-        if constexpr (LOOSE) update[n] = Mma<__bf16>::run(b.hi, h[1], update[n]);
-      }
+      update[n] = Mma<__bf16>::run(b.hi, h[1], update[n]);
+      if constexpr (BPiece<T>::kTwo) update[n] = Mma<__bf16>::run(b.lo, h[0], update[n]);
     }
     mfma_settle(update);
   };
@@ -283,9 +283,14 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   const char* const share = lds + part * (S::kRows * 128) + m * 128;
   const int piece[2] = {16 * (g ^ (m >> 1)), 16 * ((4 + g) ^ (m >> 1))};
   int now = 0;
+  // Waits for a stage: no more loads may be on their way than those of the stages that were asked for behind it.
+  auto wait_stage = [&](int stage) {
+    const int younger = asked - 1 - stage, of_extras = asked - stages < 0 ? 0 : asked - stages < younger ? asked - stages : younger;
+    wait_at_most<(S::kRing - 2) * (LORA == kStaged && S::kExtra > S::kPer ? S::kExtra : S::kPer)>(S::kPer * (younger - of_extras) + S::kExtra * of_extras);
+  };
   auto next_stage = [&](int stage) {  // (is there; what came before it has been read)
     wait_lds();
-    wait_stages<S::kPer, S::kRing - 2>(stages + extras - 1 - stage);
+    wait_stage(stage);
     stage_barrier();
     request_next();
   };
@@ -337,41 +342,41 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[n][i] *= a.w_scales[c + i < a.n ? c + i : a.n - 1];
   }
-  if (!LOOSE && extras) {
-    Extra e = {meeting(0), 0, 0, 0, part};
+  if (LORA == kStaged && extras) {
+    Extra e = {meeting(0), 0, 0, part};
     settle_quarter(e);
     Slice slice = slice_of(e.slice);
     for (int stage = stages; stage < stages + extras; ++stage) {
       // (a wavefront reads what it has loaded itself: only the last stage of the base product has to be everybody's)
       wait_lds();
-      wait_stages<S::kPer, S::kRing - 2>(stages + extras - 1 - stage);
+      wait_stage(stage);
       if (stage == stages) stage_barrier();
       request_next();
       const int group = e.round * S::kSplit + part;
-      const char* const at = lds + now * S::kStage + wave * (S::kPer * 1024) + lane * 16;
+      const char* const at = lds + now * S::kStage + lane * 16;
       now = now == S::kRing - 1 ? 0 : now + 1;
       if (group < groups) {
-        Pack8 raw[NF], h[kParts<T>];
+        Pack8 raw[NF], h[2];
 #pragma unroll
-        for (int n = 0; n < NF; ++n) raw[n].raw = load128(at + n * 1024);
-        h[0].raw = load128(at + NF * 1024);
-        if constexpr (kParts<T> == 2) h[1].raw = i32x4{0, 0, 0, 0};
-        add_group(e.slice, packed ? packed_place(group) : place_in(e.d, e.quarter), slice.whole, e.part, raw, h);
+        for (int n = 0; n < NF; ++n) raw[n].raw = load128(at + place_of(n));
+#pragma unroll
+        for (int v = 0; v < 2; ++v) h[v].raw = load128(at + place_of(NF + v));
+        add_group(e.slice, packed ? packed_place(group) : place_in(e.d, e.quarter), slice.whole, raw, h);
       }
       advance(e, slice);
     }
   }
-  if constexpr (LOOSE) {
+  if constexpr (LORA == kLoose) {
     for (int s = meeting(0); s < a.num_slices; s = meeting(s + 1)) {
       const Slice slice = slice_of(s);
-      Extra e = {s, 0, 0, 0, part};
+      Extra e = {s, 0, 0, part};
       settle_quarter(e);
       for (int group = part; group < groups; group += S::kSplit) {
         const Place p = packed ? packed_place(group) : place_in(e.d, e.quarter);
         e.quarter += S::kSplit;
         settle_quarter(e);
         const T* const b_slot = slice.b + static_cast<uint64_t>(static_cast<uint32_t>(__shfl(list, p.there ? p.d : 0, kWave))) * slice.slot_stride;
-        Pack8 raw[NF], h[kParts<T>];
+        Pack8 raw[NF], h[2];
 #pragma unroll
         for (int n = 0; n < NF; ++n) {
           T* const to = reinterpret_cast<T*>(&raw[n]);
@@ -382,8 +387,8 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
           }
         }
 #pragma unroll
-        for (int v = 0; v < kParts<T>; ++v) h[v].raw = load128(h_row + v * static_cast<int64_t>(a.num_rows) * width + s * ranks + p.first);
-        add_group(s, p, slice.whole, 0, raw, h);
+        for (int v = 0; v < 2; ++v) h[v].raw = load128(h_row + v * h_rest + s * ranks + p.first);
+        add_group(s, p, slice.whole, raw, h);
       }
     }
   }
@@ -406,7 +411,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
 #pragma unroll
           for (int n = 0; n < NF; ++n)
             if (beyond >> n & 1)
-              add_slowly(b, a.slices[s].n, n0 + 4 * NF * g + 4 * n - a.slices[s].y_col, a.r, 32 * quarter, 32, hi, kParts<T> == 2 ? hi + static_cast<int64_t>(a.num_rows) * width : nullptr, update[n]);
+              add_slowly(b, a.slices[s].n, n0 + 4 * NF * g + 4 * n - a.slices[s].y_col, a.r, 32 * quarter, 32, hi, hi + h_rest, update[n]);
         }
   }
   // the shares meet
@@ -418,7 +423,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
   int32_t* const leaders = reinterpret_cast<int32_t*>(lds + 2 * kUpdates * 16);
 #pragma unroll
   for (int n = 0; n < NF; ++n) parts[(wave * NF + n) * 64 + lane] = acc[n];
-  if (a.num_slices) {
+  if constexpr (LORA) {
 #pragma unroll
     for (int n = 0; n < NF; ++n) parts[kUpdates + (wave * NF + n) * 64 + lane] = update[n];
     if (part == 0 && g == 0) leaders[16 * f + m] = leader;
@@ -431,7 +436,7 @@ template <typename T, int TF, int NF, bool LOOSE> __global__ __launch_bounds__(k
     f32x4 sum = parts[(of * NF + block % NF) * 64 + lane];
 #pragma unroll
     for (int v = 1; v < S::kSplit; ++v) sum += parts[((v * TF + of) * NF + block % NF) * 64 + lane];
-    if (a.num_slices) {
+    if constexpr (LORA) {
       const int first = leaders[16 * of + m];
       f32x4 added = parts[kUpdates + ((first * TF + of) * NF + block % NF) * 64 + lane];
       for (int v = 1; v < S::kSplit && v < quarters; ++v) added += parts[kUpdates + ((((first + v) & (S::kSplit - 1)) * TF + of) * NF + block % NF) * 64 + lane];
@@ -460,7 +465,7 @@ constexpr int kFewGroups = 2;  // of sixteen ranks of a slot, all rows together
 
 template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_few_kernel(MloraProjectArgs a) {
   __shared__ f32x4 parts[kFewGroups][kRowWaves][64];
-  __shared__ __align__(16) uint16_t h_of[kParts<T>][16][16 * kFewGroups];
+  __shared__ __align__(16) uint16_t h_of[2][16][16 * kFewGroups];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, m = lane & 15, g = lane >> 4;
   const int n0 = blockIdx.x * 16, mine = slot_of(a, m);
   // the different slots among the rows: lane d holds the d-th, `ordinal` is which one the row's is
@@ -556,7 +561,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
           __bf16 hi, lo;
           split(j + i < a.r ? sum[i] : 0.0f, &hi, &lo);
           h_of[0][m][j + i] = __builtin_bit_cast(uint16_t, hi);
-          if constexpr (kParts<T> == 2) h_of[1][m][j + i] = __builtin_bit_cast(uint16_t, lo);
+          h_of[1][m][j + i] = __builtin_bit_cast(uint16_t, lo);
         }
       }
     }
@@ -568,10 +573,10 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
       of.from(b);
       Pack8 h;
 #pragma unroll
-      for (int v = 0; v < kParts<T>; ++v) {
+      for (int v = 0; v < 2; ++v) {
         h.raw = own ? load128(&h_of[v][m][first]) : i32x4{0, 0, 0, 0};
         acc[0] = Mma<__bf16>::run(of.hi, h, acc[0]);
-        if constexpr (kParts<T> == 2)
+        if constexpr (BPiece<T>::kTwo)
           if (v == 0) acc[0] = Mma<__bf16>::run(of.lo, h, acc[0]);
       }
       mfma_settle(acc);
@@ -583,7 +588,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
         acc[0] = before;
         if (ordinal >= 0)
           add_slowly(static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(mine) * a.slices[s].n * a.r, a.slices[s].n, n0 + 4 * g - a.slices[s].y_col, a.r, 0, a.r, h_of[0][m],
-                     kParts<T> == 2 ? h_of[kParts<T> - 1][m] : nullptr, acc[0]);
+                     h_of[1][m], acc[0]);
       }
     }
     __syncthreads();  // (the next slice has another h)
@@ -608,14 +613,16 @@ bool few_rows(const MloraProjectArgs* a) {
   return a->num_slices && a->r % 8 == 0 && a->num_rows <= kFewGroups && a->num_rows * ((a->r + 15) / 16) <= kFewGroups && a->k <= 2048 && static_cast<int64_t>(a->n) * a->k <= 1 << 23;
 }
 
-template <typename T, int TF, int NF, bool LOOSE> void launch_ranks(const MloraProjectArgs* a) {
-  allow_lds<project_rows_kernel<T, TF, NF, LOOSE>>(RowsShape<TF, NF>::kLds);
+template <typename T, int TF, int NF, int LORA> void launch_ranks(const MloraProjectArgs* a) {
+  constexpr int bytes = RowsShape<TF, NF, LORA>::kLds;
+  allow_lds<project_rows_kernel<T, TF, NF, LORA>>(bytes);
   const dim3 grid(static_cast<unsigned>((a->n + 16 * NF - 1) / (16 * NF)), static_cast<unsigned>((a->num_rows + 16 * TF - 1) / (16 * TF)));
-  project_rows_kernel<T, TF, NF, LOOSE><<<grid, kRowWaves * 64, RowsShape<TF, NF>::kLds, static_cast<hipStream_t>(a->stream)>>>(*a);
+  project_rows_kernel<T, TF, NF, LORA><<<grid, kRowWaves * 64, bytes, static_cast<hipStream_t>(a->stream)>>>(*a);
 }
 template <typename T, int TF, int NF> void launch(const MloraProjectArgs* a) {
-  if (a->num_slices && a->r % 8) launch_ranks<T, TF, NF, true>(a);
-  else launch_ranks<T, TF, NF, false>(a);
+  if (!a->num_slices) launch_ranks<T, TF, NF, kNone>(a);
+  else if (a->r % 8) launch_ranks<T, TF, NF, kLoose>(a);
+  else launch_ranks<T, TF, NF, kStaged>(a);
 }
 template <typename T, int TF> void launch_columns(const MloraProjectArgs* a) {
   // 32 columns a workgroup where that still gives every compute unit one
@@ -635,7 +642,7 @@ template <typename T> void launch_rows(const MloraProjectArgs* a) {
 bool on16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 size_t workspace_bytes(const MloraProjectArgs* a) {
-  return static_cast<size_t>(order_bytes(a->num_rows, a->num_slots)) + static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * (a->dtype == MLORA_DTYPE_F16 ? 4 : 2);
+  return static_cast<size_t>(order_bytes(a->num_rows, a->num_slots)) + static_cast<size_t>(a->num_rows) * a->num_slices * padded_ranks(a->r) * 4;
 }
 
 int check_project(const MloraProjectArgs* a) {

@@ -15,7 +15,7 @@ namespace mlora {
 namespace {
 
 // h of four ranks from j on of one row; ranks from r to `ranks` are zero.  Whether an infinity or a NaN is among them.
-template <typename T> __device__ __forceinline__ bool store_h(const MloraProjectArgs& a, int row, int slice, int j, const f32x4& sum) {
+__device__ __forceinline__ bool store_h(const MloraProjectArgs& a, int row, int slice, int j, const f32x4& sum) {
   const int ranks = padded_ranks(a.r), width = a.num_slices * ranks;
   if (j >= ranks) return false;
   __bf16 h[4], l[4];
@@ -23,7 +23,7 @@ template <typename T> __device__ __forceinline__ bool store_h(const MloraProject
   for (int i = 0; i < 4; ++i) split(j + i < a.r ? sum[i] : 0.0f, &h[i], &l[i]);
   uint16_t* const at = intermediate(a) + static_cast<int64_t>(row) * width + slice * ranks + j;
   __builtin_memcpy(at, h, 8);
-  if constexpr (kParts<T> == 2) __builtin_memcpy(at + static_cast<int64_t>(a.num_rows) * width, l, 8);
+  __builtin_memcpy(at + static_cast<int64_t>(a.num_rows) * width, l, 8);
   uint32_t words[2];
   __builtin_memcpy(words, h, 8);
   return pair_beyond(words[0]) || pair_beyond(words[1]);
@@ -77,7 +77,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void shrink8_
         f32x4 sum = parts[0][lane];
 #pragma unroll
         for (int w = 1; w < kRowWaves; ++w) sum += parts[w][lane];
-        store_h<T>(a, row, slice, first + 4 * g, sum);
+        store_h(a, row, slice, first + 4 * g, sum);
       }
       __syncthreads();
     }
@@ -303,7 +303,7 @@ template <typename T, int RB, int TEAMS> __global__ __launch_bounds__(TEAMS * 25
     for (int b = 0; b < RB; ++b) {
 #pragma unroll
       for (int v = 0; v < TEAMS - 1; ++v) acc[b] += parts[v * kTeam + b * 64];
-      if (store_h<T>(a, t0 + wave * 16 + m, slice, first + 16 * b + 4 * g, acc[b])) *any_h_beyond(a) = 1;  // (whoever finds one writes the same)
+      if (store_h(a, t0 + wave * 16 + m, slice, first + 16 * b + 4 * g, acc[b])) *any_h_beyond(a) = 1;  // (whoever finds one writes the same)
     }
   }
 }

@@ -13,6 +13,8 @@
 #include "lds.h"
 #include "project.h"
 
+#include <type_traits>
+
 namespace mlora {
 
 namespace {
@@ -42,9 +44,6 @@ __device__ __forceinline__ Tile tile_of(const Grid& grid, int id) {
   const uint32_t n = high == kStrip ? in / kStrip : divide(in, high, grid.last_inverse);
   return Tile{static_cast<int>(strip * kStrip + in - n * high), static_cast<int>(n)};
 }
-
-// Adapters: none, through LDS like the rest, or by loads of the lanes (ranks that are no multiple of eight, whose rows of B lie anywhere).
-enum { kNone, kStaged, kLoose };
 
 template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_bounds__(256, LORA || TT * NN > 8 ? 2 : 3) void tiles8_kernel(MloraProjectArgs a, Grid grid) {
   constexpr int BT = 32 * TT, BN = 32 * NN, kStage = (BT + BN) * 128;
@@ -96,7 +95,8 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     slice_b[0] = static_cast<int>(at);
     slice_b[1] = static_cast<int>(at >> 32);
   }
-  // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 64 ranks at a time, of h one part after the other.
+  // The adapters' steps of a tile: its slots, for each the slices that its columns meet, of each 64 ranks at a time, of h one part after the other; of up to 32 ranks both parts at once, side by side.
+  const bool narrow = ranks <= 32;
   struct Extra {
     int row, slot, stop, first, end, slice, c, part;  // the slot's first row in the tile (BT: no more) and where it stops, the slices
   };
@@ -118,7 +118,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     return e;
   };
   auto advance = [&](const Table& table, Extra& e, int t0) {
-    if (++e.part < kParts<T>) return;
+    if (!narrow && ++e.part < 2) return;
     e.part = 0;
     e.c += 64;
     if (e.c < ranks) return;
@@ -184,23 +184,38 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     }
     load_scales();
   };
-  // An adapters' step takes the rows' h for x and the columns' B for w.
+  // An adapters' step takes the rows' h for x, first one part of it and then the other, and the columns' B for w, which stays in registers for the second.
   auto aim_extra = [&]() {
+    if (load_extra.part) {
+      x_from += static_cast<int64_t>(a.num_rows) * width * 2;
+      return;
+    }
     const int wide = __builtin_amdgcn_readlane(slice_wide, load_extra.slice), column = __builtin_amdgcn_readlane(slice_column, load_extra.slice);
     const uint64_t b_of = static_cast<uint32_t>(__builtin_amdgcn_readlane(slice_b[0], load_extra.slice)) |
                           static_cast<uint64_t>(static_cast<uint32_t>(__builtin_amdgcn_readlane(slice_b[1], load_extra.slice))) << 32;
-    x_from = reinterpret_cast<const char*>(intermediate(a) + (static_cast<int64_t>(load_extra.part) * a.num_rows + load_t0) * width + load_extra.slice * ranks);
+    x_from = reinterpret_cast<const char*>(intermediate(a) + static_cast<int64_t>(load_t0) * width + load_extra.slice * ranks);
     w_from = reinterpret_cast<const char*>(b_of) + static_cast<int64_t>(load_extra.slot) * wide * a.r * 2;
-    place(load_extra.c * 2, ranks * 2, true);
+    // (narrow: the second four pieces of a row are the first four's ranks, of h's other part and of B once more)
+    const uint32_t h_rest = static_cast<uint32_t>(a.num_rows) * static_cast<uint32_t>(width * 2);
+    auto again = [&](int i) { return narrow && (((lane >> 2) ^ i) & 1); };
+    if (narrow) {
+#pragma unroll
+      for (int odd = 0; odd < 2; ++odd) {
+        const uint32_t in = 16 * ((lane & 7) ^ (((lane >> 4) & 3) + 4 * odd));
+        in_row[odd] = (in & 63) < static_cast<uint32_t>(ranks * 2) ? in : in & 64;
+      }
+    } else {
+      place(load_extra.c * 2, ranks * 2, true);
+    }
 #pragma unroll
     for (int i = 0; i < TT; ++i) {
       const int row = (wave * TT + i) * 8 + (lane >> 3), most = a.num_rows - load_t0 - 1;
-      x_off[i] = static_cast<uint32_t>((row < most ? row : most) * width * 2);
+      x_off[i] = static_cast<uint32_t>((row < most ? row : most) * width * 2) + (again(i) ? h_rest - 64 : 0);
     }
 #pragma unroll
     for (int i = 0; i < NN; ++i) {
       const int in = load_n0 + column_of((wave * NN + i) * 8 + (lane >> 3)) - column;
-      w_off[i] = static_cast<uint32_t>(in < 0 ? 0 : in < wide ? in : wide - 1) * static_cast<uint32_t>(a.r) * 2;
+      w_off[i] = static_cast<uint32_t>(in < 0 ? 0 : in < wide ? in : wide - 1) * static_cast<uint32_t>(a.r) * 2 - (again(i) ? 64 : 0);
     }
   };
   // What the next load takes, behind the one before it; between steps, since its branches would cut a step's code in pieces.
@@ -238,8 +253,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     const char *const x = uniform(x_from), *const w = uniform(w_from);
 #pragma unroll
     for (int i = 0; i < TT; ++i) dma16_from(x, x_off[i] + in_row[i & 1], to + (wave * TT + i) * 1024);
+    if (load_extra.row >= BT || !load_extra.part) {
 #pragma unroll
-    for (int i = 0; i < NN; ++i) dma16_from(w, w_off[i] + in_row[i & 1], to + (4 * TT + wave * NN + i) * 1024);
+      for (int i = 0; i < NN; ++i) dma16_from(w, w_off[i] + in_row[i & 1], to + (4 * TT + wave * NN + i) * 1024);
+    }
     buffer ^= 1;
   };
   const char* const x_home = lds + wt * (TT * 2048) + m * 128;
@@ -302,8 +319,8 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
   };
   // A step of the adapters; leaves the next step's blocks where it found its own.
   int mine[TT];
-  // What the lane's row of block t gains from `some` ranks of a slot in one slice, one number at a time; where everything is NaN already, nothing.
-  auto add_row = [&](int t, int slot, int s, int first, int some, int t0, int n0) {
+  // What the lane's row of block t gains from a slot in one slice, one number at a time; where everything is NaN already, nothing.
+  auto add_row = [&](int t, int slot, int s, int t0, int n0) {
     const int at = t0 + 16 * t + m < a.num_rows ? t0 + 16 * t + m : a.num_rows - 1;
     const uint16_t* const hi = intermediate(a) + static_cast<int64_t>(at) * width + s * ranks;
     const T* const b = static_cast<const T*>(a.slices[s].b) + static_cast<int64_t>(slot) * a.slices[s].n * a.r;
@@ -311,80 +328,120 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     for (int n = 0; n < NN; ++n) {
       f32x4 sum = acc[t][n];
       if (sum[0] != sum[0] && sum[1] != sum[1] && sum[2] != sum[2] && sum[3] != sum[3]) continue;
-      add_slowly(b, a.slices[s].n, n0 + 32 * (n >> 1) + 4 * (n & 1) - a.slices[s].y_col, a.r, first, some, hi, kParts<T> == 2 ? hi + static_cast<int64_t>(a.num_rows) * width : nullptr, sum);
+      add_slowly(b, a.slices[s].n, n0 + 32 * (n >> 1) + 4 * (n & 1) - a.slices[s].y_col, a.r, 0, a.r, hi, hi + static_cast<int64_t>(a.num_rows) * width, sum);
       acc[t][n] = sum;
     }
   };
-  auto extra_step = [&](const Extra& e, int from, int t0, int n0, Eight(&w)[NN], Eight(&x01)[2]) {
+  auto extra_step = [&](auto second, const Extra& e, int from, Eight(&w)[NN], Eight(&x01)[2]) {
+    constexpr bool SECOND = decltype(second)::value;  // the second part of h: w is what the first one's step has made of it
     const char* const xs = x_home + now * kStage;
-    const int wide = __builtin_amdgcn_readlane(slice_wide, e.slice);
     Eight x[TT];
     x[0] = x01[0];
     x[1] = x01[1];
+    auto rank_of = [&](const Extra& e, int p) { return e.c + (narrow ? 0 : 32 * p) + 8 * g; };
+    if constexpr (!SECOND) {
+      const int wide = __builtin_amdgcn_readlane(slice_wide, e.slice);
 #pragma unroll
-    for (int n = 0; n < NN; ++n) {  // (zero where there is no such rank or the column is none of the slice)
-      const int in = from + 32 * (n >> 1) + 4 * (n & 1);
+      for (int n = 0; n < NN; ++n) {  // (zero where there is no such rank or the column is none of the slice)
+        const int in = from + 32 * (n >> 1) + 4 * (n & 1);
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
-        if (!(e.c + 32 * p + 8 * g < ranks && in >= 0 && in < wide)) w[n].piece[p] = i32x4{0, 0, 0, 0};
+        for (int p = 0; p < 2; ++p)
+          if (!(rank_of(e, p) < ranks && in >= 0 && in < wide)) w[n].piece[p] = i32x4{0, 0, 0, 0};
+      }
     }
 #pragma unroll
     for (int t = 2; t < TT; ++t) block_of(xs, t, x[t]);
-    turn_over();
-    // Of an infinity in B only the product with all of h is what the definition says, not the two that its parts and those of h would make: then one number at a time.
-    bool wild = false;
-    if constexpr (kParts<T> == 2) {
+    // An infinity in B meets the leading part of h alone: with the other one, or its own second piece, it would make NaN.  Whether there is one a product with zeros shows: of numbers it is zero.
+    f32x4 none[NN];
+    if constexpr (!SECOND) {
       Pack8 zero;
       zero.raw = i32x4{0, 0, 0, 0};
-      f32x4 none = f32x4{0.0f, 0.0f, 0.0f, 0.0f};  // (of numbers nothing but zero comes out, of others NaN)
 #pragma unroll
-      for (int n = 0; n < NN; ++n)
+      for (int p = 0; p < 2; ++p)
 #pragma unroll
-        for (int p = 0; p < 2; ++p) {
+        for (int n = 0; n < NN; ++n) {
           Pack8 raw;
           raw.raw = w[n].piece[p];
-          none = Mma<T>::run(raw, zero, none);
+          none[n] = Mma<T>::run(raw, zero, p ? none[n] : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         }
+    }
+    turn_over();
+    bool wild = false;
+    if constexpr (!SECOND) {
       settle();
-      wild = __ballot(!(none[0] + none[1] + none[2] + none[3] == 0.0f)) != 0;
-    }
-    if (wild && e.part == 0) {
+      f32x4 sum = none[0];
 #pragma unroll
-      for (int t = 0; t < TT; ++t)
-        if (mine[t] == e.slot) add_row(t, e.slot, e.slice, e.c, 64, t0, n0);
+      for (int n = 1; n < NN; ++n) sum += none[n];
+      wild = __ballot(!(sum[0] + sum[1] + sum[2] + sum[3] == 0.0f)) != 0;
     }
+#pragma unroll
+    for (int t = 0; t < TT; ++t)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (rank_of(e, p) >= ranks) x[t].piece[p] = i32x4{0, 0, 0, 0};
+    auto finite = [&](const Pack8& hi, Pack8& of) {  // `of` where hi is a number, else zero
+#pragma unroll
+      for (int i = 0; i < 4; ++i) of.u[i] &= ~pair_mask(hi.u[i]);
+    };
+    auto keep_finite = [&](int p) {
+#pragma unroll
+      for (int n = 0; n < NN; ++n) {
+        Pack8 b;
+        b.raw = w[n].piece[p];
+        finite(b, b);
+        w[n].piece[p] = b.raw;
+      }
+    };
+    [[maybe_unused]] Pack8 rest[NN][2];  // the second pieces of fp16's B
+    if constexpr (BPiece<T>::kTwo) {
+      if constexpr (!SECOND) {
+#pragma unroll
+        for (int n = 0; n < NN; ++n)
+#pragma unroll
+          for (int p = 0; p < 2; ++p) {
+            Pack8 raw;
+            raw.raw = w[n].piece[p];
+            BPiece<T> b;
+            b.from(raw);
+            if (wild) finite(b.hi, b.lo);
+            w[n].piece[p] = b.hi.raw;
+            rest[n][p] = b.lo;
+            if (narrow && p) rest[n][p].raw = i32x4{0, 0, 0, 0};
+          }
+      }
+    }
+    auto product = [&](int t, int n, f32x4 sum) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p) {
+        Pack8 h, b;
+        h.raw = x[t].piece[p];
+        b.raw = w[n].piece[p];
+        sum = Mma<__bf16>::run(b, h, sum);
+        if constexpr (BPiece<T>::kTwo && !SECOND) sum = Mma<__bf16>::run(rest[n][p], h, sum);
+      }
+      return sum;
+    };
+    // (a lane's results are of one row, and come from that row's h alone: rows of other slots keep what they have, whatever is in this one's B)
+    if (wild && narrow) keep_finite(1);
 #pragma unroll
     for (int t = 0; t < TT; ++t) {
-      if (wild) break;
-      // (a lane's results are of one row, and come from that row's h alone: rows of other slots keep what they have, whatever is in this one's B)
       const bool own = mine[t] == e.slot;
       if (!__ballot(own)) continue;
 #pragma unroll
-      for (int p = 0; p < 2; ++p)
-        if (e.c + 32 * p + 8 * g >= ranks) x[t].piece[p] = i32x4{0, 0, 0, 0};
+        for (int n = 0; n < NN; ++n) {
+          const f32x4 next = product(t, n, acc[t][n]);
 #pragma unroll
-      for (int n = 0; n < NN; ++n) {
-        f32x4 next = acc[t][n];
-#pragma unroll
-        for (int p = 0; p < 2; ++p) {
-          Pack8 h, raw;
-          h.raw = x[t].piece[p];
-          raw.raw = w[n].piece[p];
-          BPiece<T> b;
-          b.from(raw);
-          next = Mma<__bf16>::run(b.hi, h, next);
-          // (of the second part only the first piece counts)
-          if constexpr (kParts<T> == 2) {
-            if (e.part) b.lo.raw = i32x4{0, 0, 0, 0};
-            next = Mma<__bf16>::run(b.lo, h, next);
-          }
+          for (int i = 0; i < 4; ++i) acc[t][n][i] = own ? next[i] : acc[t][n][i];
         }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[t][n][i] = own ? next[i] : acc[t][n][i];
-      }
     }
+    if (wild && !narrow) keep_finite(0), keep_finite(1);
     now ^= 1;
-    begin(w, x01, now * kStage);
+    if (SECOND || narrow) {
+      begin(w, x01, now * kStage);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) block_of(x_home + now * kStage, i, x01[i]);
+    }
   };
 
   if constexpr (LORA) {
@@ -455,7 +512,10 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
     if constexpr (LORA == kStaged) {
       while (coming.row < BT) {
         prepare();
-        extra_step(current, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, current.slice), t0, n0, w[0], x01[0]);
+        extra_step(std::false_type(), current, tile.n * BN + wn * (16 * NN) + 8 * (m >> 2) + (m & 3) - __builtin_amdgcn_readlane(slice_column, current.slice), w[0], x01[0]);
+        if (narrow) continue;
+        prepare();
+        extra_step(std::true_type(), current, 0, w[0], x01[0]);
       }
       settle();
     }
@@ -493,7 +553,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
               const int at = t0 + 16 * t + m < a.num_rows ? t0 + 16 * t + m : a.num_rows - 1;
               const int64_t from = static_cast<int64_t>(at) * width + s * ranks + (some ? rank : 0);
               h[t][0].raw = load128(hi + from);
-              h[t][1].raw = kParts<T> == 2 ? load128(lo + from) : i32x4{0, 0, 0, 0};
+              h[t][1].raw = load128(lo + from);
               if (!some) h[t][0].raw = h[t][1].raw = i32x4{0, 0, 0, 0};
             }
 #pragma unroll
@@ -515,13 +575,11 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
             for (int n = 0; n < NN; ++n) {
               b[n].from(raw[n]);
               finite[n] = b[n].hi;
-              if constexpr (kParts<T> == 2) {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                  const uint32_t keep = ~pair_mask(finite[n].u[i]);
-                  finite[n].u[i] &= keep;
-                  b[n].lo.u[i] &= keep;
-                }
+              for (int i = 0; i < 4; ++i) {
+                const uint32_t keep = ~pair_mask(finite[n].u[i]);
+                finite[n].u[i] &= keep;
+                if constexpr (BPiece<T>::kTwo) b[n].lo.u[i] &= keep;
               }
             }
 #pragma unroll
@@ -532,10 +590,8 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
               for (int n = 0; n < NN; ++n) {
                 f32x4 next = Mma<__bf16>::run(b[n].hi, h[t][0], acc[t][n]);
-                if constexpr (kParts<T> == 2) {
-                  next = Mma<__bf16>::run(finite[n], h[t][1], next);
-                  next = Mma<__bf16>::run(b[n].lo, h[t][0], next);
-                }
+                next = Mma<__bf16>::run(finite[n], h[t][1], next);
+                if constexpr (BPiece<T>::kTwo) next = Mma<__bf16>::run(b[n].lo, h[t][0], next);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) acc[t][n][i] = own ? next[i] : acc[t][n][i];
               }
@@ -549,7 +605,7 @@ template <typename T, int TT, int NN, bool TAIL, int LORA> __global__ __launch_b
 #pragma unroll
       for (int t = 0; t < TT; ++t)
         if (odd >> t & 1)
-          for (int s = 0; s < a.num_slices; ++s) add_row(t, table.slots[wt * (16 * TT) + 16 * t + m], s, 0, a.r, t0, n0);
+          for (int s = 0; s < a.num_slices; ++s) add_row(t, table.slots[wt * (16 * TT) + 16 * t + m], s, t0, n0);
     }
 
     float bias[NN / 2][8];

@@ -66,9 +66,8 @@ def linear(x, x_scales, w, w_scales, bias=None, a=(), b=(), columns=None, slots=
             aa, bb = a_of[s].double(), b_of[s].double()
             h, h_size = aa @ x[t], aa.abs() @ x[t].abs()
             y[t, first : first + n] += bb @ h
-            # h: K additions; beside bf16 adapters it is rounded to bf16, 2^-8 of it; beside fp16 ones it is two bf16 numbers, as is B, and three of the
-            # four products are taken: 2^-16 each; then rank additions
-            rounded = HALF_STEP[torch.bfloat16] if dtype == torch.bfloat16 else 2 * 2.0**-16
+            # h: K additions; it is two bf16 numbers, 2^-16 of it, and fp16's B two as well, of whose four products with h three are taken, 2^-16 once more; then rank additions
+            rounded = 2.0**-16 if dtype == torch.bfloat16 else 2 * 2.0**-16
             bound[t, first : first + n] += bb.abs() @ ((h_size * (k + 8) * UNIT) * (1 + rounded) + h.abs() * (rounded + (rank + 8) * 2 * UNIT))
             size[t, first : first + n] += bb.abs() @ h.abs()
         first += n
