@@ -15,8 +15,8 @@ def eight_bits(y, wrong):
     """y [rows, width] in 64 bits, known to `wrong` (relative) -> (scales, bound, values before their rounding, bound)."""
     scales = (y.abs().amax(-1) / TOP).clamp(min=LEAST)
     values = y / scales[:, None]
-    # max / 448 rounds once; 448 / max and its product with z twice; e4m3 keeps four bits (2^-4 of the value) down to steps of 2^-9
-    off = values.abs() * (2 * wrong + 4 * UNIT) if torch.is_tensor(wrong) else values.abs() * (2 * wrong + 4 * UNIT)
+    # max / 448 rounds once, and so does the quotient by it; e4m3 keeps four bits (2^-4 of the value) down to steps of 2^-9
+    off = values.abs() * (2 * wrong + 4 * UNIT)
     most = wrong.amax(-1) if torch.is_tensor(wrong) else wrong
     return scales, scales * (most + 2 * UNIT), values, off + (values.abs() + off) * 2.0**-4 + 2.0**-10
 
