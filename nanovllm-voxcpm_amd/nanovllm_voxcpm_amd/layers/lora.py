@@ -28,7 +28,7 @@ import torch.nn.functional as F
 from nanovllm_voxcpm_amd import _hip
 from nanovllm_voxcpm_amd.lora import LoRAMetadata, get_backend
 from nanovllm_voxcpm_amd.lora_ops.segment_meta import as_slot_vector
-from nanovllm_voxcpm_amd.quant_ops import QuantizedRows, quantize_rows, quantized_linear
+from nanovllm_voxcpm_amd.quant_ops import MOST_FEATURES, QuantizedRows, quantize_rows, quantized_linear
 from nanovllm_voxcpm_amd.utils.context import LM_LORA_DOMAIN, get_lora_context, installed_lora_context
 
 ShardId = str | int
@@ -248,7 +248,7 @@ class _LoRALayerBase(nn.Module):
         """
         self.check_base_for_8_bits()
         weight = self.weight
-        values, scales = quantize_rows(weight.detach())
+        values, scales = quantize_rows(weight.detach().contiguous())
         self._base_dtype = weight.dtype
         self.weight = None
         self.register_buffer("weight_values", values.view(torch.uint8))
@@ -264,6 +264,14 @@ class _LoRALayerBase(nn.Module):
             raise ValueError(f"a base weight in 8 bits is for fp16 and bf16 layers, this one is {weight.dtype}")
         if weight.size(1) % 16:
             raise ValueError(f"a base weight in 8 bits takes a multiple of 16 input features, this layer has {weight.size(1)}")
+        if max(weight.shape) > MOST_FEATURES:
+            raise ValueError(f"a base weight in 8 bits takes up to {MOST_FEATURES} features, this layer has {tuple(weight.shape)}")
+        if self.supports_lora:
+            if self._num_targets() > _hip.MAX_SLICES or self.max_lora_rank > _hip.MAX_RANK or self.max_loras > _hip.MAX_SLOTS:
+                raise ValueError(f"a base weight in 8 bits takes up to {_hip.MAX_SLICES} adapter targets, rank {_hip.MAX_RANK} and {_hip.MAX_SLOTS} slots beside it, "
+                                 f"this layer has {self._num_targets()}, {self.max_lora_rank} and {self.max_loras}")
+            if any(t.dtype != weight.dtype for t in (self.lora_A, *(self._b_of(p) for p in range(self._num_targets())))):
+                raise ValueError(f"a base weight in 8 bits takes adapters of its own type, these are {self.lora_A.dtype} beside {weight.dtype}")
         if not weight.is_cuda:
             raise RuntimeError(f"a base weight is put in 8 bits on the GPU, this one lives on {weight.device}")
 

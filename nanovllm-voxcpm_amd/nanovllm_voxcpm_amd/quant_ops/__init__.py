@@ -41,6 +41,7 @@ def _no_grad(*tensors: torch.Tensor | None) -> None:
         raise RuntimeError("the 8-bit ops have no backward, nor a forward derivative: a tensor carries a tangent")
 
 
+MOST_FEATURES = 2**22  # of a linear, in or out
 _MOST = 2**31 - 1  # (sizes are 32-bit numbers in the library, which refuses what it does not serve below that)
 
 
