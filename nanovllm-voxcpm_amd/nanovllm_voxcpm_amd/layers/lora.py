@@ -87,7 +87,6 @@ class _LoRALayerBase(nn.Module):
         self._rank_summary = (False, False)
         self._targets_in_order = True  # every output block has a target, in order
         self.base_in_8_bits = False
-        self._base_dtype: torch.dtype | None = None
         self._base_rows: tuple | None = None  # the buffers of the 8-bit weight, and that weight
 
     # ---- subclass contract ------------------------------------------------------------------
@@ -249,7 +248,7 @@ class _LoRALayerBase(nn.Module):
         self.check_base_for_8_bits()
         weight = self.weight
         values, scales = quantize_rows(weight.detach().contiguous())
-        self._base_dtype = weight.dtype
+        self.register_buffer("base_type", weight.new_empty(0), persistent=False)  # (of no elements: its type is the layer's, and changes with it)
         self.weight = None
         self.register_buffer("weight_values", values.view(torch.uint8))
         self.register_buffer("weight_scales", scales.view(torch.int32))
@@ -285,7 +284,7 @@ class _LoRALayerBase(nn.Module):
 
     def _forward_in_8_bits(self, x: torch.Tensor | QuantizedRows, bias: torch.Tensor | None, block_sizes: list[int], block_of_target: list[int]) -> torch.Tensor:
         eight = isinstance(x, QuantizedRows)
-        dtype = self.lora_A.dtype if self.supports_lora else self.bias.dtype if self.bias is not None else self._base_dtype if eight else x.dtype
+        dtype = self.lora_A.dtype if self.supports_lora else self._buffers["base_type"].dtype
         if eight:
             rows, shape = x, None
         else:

@@ -1,9 +1,12 @@
-"""What a layer refuses before its base weight is put in 8 bits, so that no layer is left that its forward cannot serve; no GPU."""
+"""LoRA linears with base weights in 8 bits: what a layer refuses beforehand, so that none is left that its forward cannot serve, and what it does on the host around its two calls; no GPU."""
 
 import pytest
 import torch
 
+from nanovllm_voxcpm_amd.layers import lora as layers
 from nanovllm_voxcpm_amd.layers.lora import LoRALinear, LoRAMergedColumnParallelLinear
+from nanovllm_voxcpm_amd.quant_ops import QuantizedRows
+from oracle import quant as oracle
 
 
 def _kept(layer):
@@ -38,3 +41,41 @@ def test_eight_targets_pass():
     layer = LoRAMergedColumnParallelLinear(32, [16] * 8, max_loras=2, max_lora_rank=8).to(torch.bfloat16)
     with pytest.raises(RuntimeError, match="GPU"):  # (the last that is looked at)
         layer.quantize_base_()
+
+
+@pytest.fixture
+def on_the_host(monkeypatch):
+    """The ops by their definitions."""
+
+    def quantize(x):
+        assert x.dim() == 2 and (x.stride(1) == 1 or x.size(1) == 1)  # (as the op does)
+        scales, _, values, _ = oracle.eight_bits(x.double(), 0.0)
+        return QuantizedRows(values.to(torch.float8_e4m3fn), scales.float())
+
+    def linear(rows, weight, *, bias=None, dtype=None, **adapters):
+        assert not adapters and (bias is None or bias.dtype == dtype)
+        return oracle.linear(rows.values.float(), rows.scales, weight.values.float(), weight.scales, bias, dtype=dtype)[0].to(dtype)
+
+    monkeypatch.setattr(layers, "quantize_rows", quantize)
+    monkeypatch.setattr(layers, "quantized_linear", linear)
+    monkeypatch.setattr(layers._LoRALayerBase, "check_base_for_8_bits", lambda self: None)
+    return quantize
+
+
+@torch.no_grad()
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("loras", [0, 2])
+def test_the_output_has_the_layers_type_after_a_change_of_it(on_the_host, bias, loras):
+    layer = LoRALinear(32, 8, bias=bias, max_loras=loras, max_lora_rank=4 if loras else 0).to(torch.bfloat16)
+    layer.weight.copy_(torch.randn(8, 32, generator=torch.Generator().manual_seed(1)))
+    layer.quantize_base_()
+    names = set(layer.state_dict())
+    x = torch.randn(3, 32)
+    for dtype in (torch.bfloat16, torch.float16, torch.bfloat16):
+        layer.to(dtype)
+        want = layer(x.to(dtype))
+        got = layer(on_the_host(x.to(dtype)))
+        assert want.dtype == got.dtype == dtype and torch.equal(got, want)
+        with pytest.raises(ValueError, match="the layer"):
+            layer(x.to(torch.bfloat16 if dtype == torch.float16 else torch.float16))
+    assert set(layer.state_dict()) == names == {"weight_values", "weight_scales"} | ({"bias"} if bias else set()) | ({"lora_A", "lora_B"} if loras else set())
