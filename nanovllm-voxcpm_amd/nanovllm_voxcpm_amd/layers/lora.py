@@ -87,7 +87,6 @@ class _LoRALayerBase(nn.Module):
         self._rank_summary = (False, False)
         self._targets_in_order = True  # every output block has a target, in order
         self.base_in_8_bits = False
-        self._base_rows: tuple | None = None  # the buffers of the 8-bit weight, and that weight
 
     # ---- subclass contract ------------------------------------------------------------------
     def _target_keys(self) -> list:
@@ -276,11 +275,7 @@ class _LoRALayerBase(nn.Module):
 
     def base_weight_rows(self) -> QuantizedRows:
         """The base weight in 8 bits."""
-        values, scales = self._buffers["weight_values"], self._buffers["weight_scales"]
-        held = self._base_rows
-        if held is None or held[0] is not values or held[1] is not scales:  # (moved or loaded since)
-            held = self._base_rows = (values, scales, QuantizedRows(values.view(torch.float8_e4m3fn), scales.view(torch.float32)))
-        return held[2]
+        return QuantizedRows(self._buffers["weight_values"].view(torch.float8_e4m3fn), self._buffers["weight_scales"].view(torch.float32))
 
     def _forward_in_8_bits(self, x: torch.Tensor | QuantizedRows, bias: torch.Tensor | None, block_sizes: list[int], block_of_target: list[int]) -> torch.Tensor:
         eight = isinstance(x, QuantizedRows)

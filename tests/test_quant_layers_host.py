@@ -1,5 +1,9 @@
 """LoRA linears with base weights in 8 bits: what a layer refuses beforehand, so that none is left that its forward cannot serve, and what it does on the host around its two calls; no GPU."""
 
+import copy
+import gc
+import weakref
+
 import pytest
 import torch
 
@@ -79,3 +83,31 @@ def test_the_output_has_the_layers_type_after_a_change_of_it(on_the_host, bias, 
         with pytest.raises(ValueError, match="the layer"):
             layer(x.to(torch.bfloat16 if dtype == torch.float16 else torch.float16))
     assert set(layer.state_dict()) == names == {"weight_values", "weight_scales"} | ({"bias"} if bias else set()) | ({"lora_A", "lora_B"} if loras else set())
+
+
+@torch.no_grad()
+def test_the_8_bit_weight_is_what_its_buffers_hold(on_the_host):
+    """Whichever way other numbers come into them; and a layer whose weight lies elsewhere now keeps nothing of where it was."""
+    g = torch.Generator().manual_seed(2)
+    one, other = (LoRALinear(32, 8, bias=False).half() for _ in range(2))
+    for layer in (one, other):
+        layer.weight.copy_(torch.randn(8, 32, generator=g))
+        layer.quantize_base_()
+    x = torch.randn(3, 32, generator=g).half()
+    first, want = one(x), other(x)
+    assert not torch.equal(first, want)
+    held = {name: t.clone() for name, t in one.state_dict().items()}
+    for take in (lambda: one.load_state_dict(other.state_dict()), lambda: one.load_state_dict(copy.deepcopy(other.state_dict()), assign=True),
+                 lambda: [setattr(one._buffers[n], "data", t.clone()) for n, t in other.state_dict().items()], lambda: [one._buffers[n].set_(t.clone()) for n, t in other.state_dict().items()],
+                 lambda: [one.register_buffer(n, t.clone()) for n, t in other.state_dict().items()]):
+        one.load_state_dict(held)
+        assert torch.equal(one(x), first)
+        take()
+        assert torch.equal(one(x), want)
+    twin = copy.deepcopy(one)
+    one.load_state_dict(held)
+    assert torch.equal(twin(x), want) and torch.equal(one(x), first)
+    gone = weakref.ref(one._buffers["weight_values"])
+    one.register_buffer("weight_values", held["weight_values"].clone())
+    gc.collect()
+    assert gone() is None
