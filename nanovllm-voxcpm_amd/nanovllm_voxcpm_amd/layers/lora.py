@@ -286,7 +286,8 @@ class _LoRALayerBase(nn.Module):
             if x.dtype != dtype:
                 raise ValueError(f"the input is {x.dtype}, the layer {dtype}")
             shape = None if x.ndim == 2 else x.shape[:-1]
-            rows = quantize_rows(x if shape is None else x.reshape(-1, x.size(-1)))
+            flat = x if shape is None else x.reshape(-1, x.size(-1))
+            rows = quantize_rows(flat if flat.stride(1) == 1 else flat.contiguous())  # (a row's elements may lie anywhere, as a linear's in 16 bits may)
         slots = self._resolve_token_slots(rows.values)
         if slots is None:
             y = quantized_linear(rows, self.base_weight_rows(), bias=bias, dtype=dtype)

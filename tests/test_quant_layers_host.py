@@ -111,3 +111,20 @@ def test_the_8_bit_weight_is_what_its_buffers_hold(on_the_host):
     one.register_buffer("weight_values", held["weight_values"].clone())
     gc.collect()
     assert gone() is None
+
+
+@torch.no_grad()
+def test_inputs_lie_as_a_linear_takes_them(on_the_host):
+    g = torch.Generator().manual_seed(3)
+    layer = LoRALinear(32, 8, bias=False).half()
+    layer.weight.copy_(torch.randn(8, 32, generator=g))
+    layer.quantize_base_()
+    x = torch.randn(6, 32, generator=g).half()
+    want = layer(x)
+    apart = torch.zeros(6, 64).half()
+    apart[:, ::2] = x
+    for same in (x.t().contiguous().t(), apart[:, ::2], x.view(2, 3, 32), x.view(2, 3, 32).permute(2, 0, 1).contiguous().permute(1, 2, 0), x.view(3, 2, 32).transpose(0, 1).contiguous().transpose(0, 1)):
+        assert torch.equal(layer(same).reshape(6, 8), want) and layer(same).shape == (*same.shape[:-1], 8)
+    assert torch.equal(layer(x[2]), want[2])
+    assert torch.equal(layer(x[:1, 0:1].expand(4, 32)), layer(x[:1, 0:1].expand(4, 32).contiguous()))
+    assert layer(x[:0]).shape == (0, 8) and layer(x[:0].view(0, 3, 32)).shape == (0, 3, 8)
