@@ -836,7 +836,7 @@ bool plain_vector(const at::Tensor& t, int64_t n, c10::ScalarType type, const at
 PyObject* op_rows(PyObject* const* args) {
   bool ok = true;
   const at::Tensor *x = optional_tensor(args[1], &ok), *weight = optional_tensor(args[4], &ok), *residual = optional_tensor(args[5], &ok), *sum_out = optional_tensor(args[7], &ok);
-  if (!ok || !x || !plain_rows(*x) || code_of(x->scalar_type()) < 0 || learns(x) || learns(weight) || learns(residual)) return nullptr;
+  if (!ok || !x || !plain_rows(*x) || code_of(x->scalar_type()) < 0 || learns(x) || learns(weight) || learns(residual) || learns(sum_out)) return nullptr;
   const long per = PyLong_AsLong(args[2]);
   const bool quantize = PyObject_IsTrue(args[3]) == 1;
   if (per < 1 || x->size(1) % per) return nullptr;

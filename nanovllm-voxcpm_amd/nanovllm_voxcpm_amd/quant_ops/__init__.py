@@ -111,7 +111,7 @@ def add_rms_norm(
         if result is not None:
             return QuantizedRows(result[0], result[1]) if quantize else result[0], x if residual is None else result[2]
     _rows(x, "x")
-    _no_grad(x, weight, residual)
+    _no_grad(x, weight, residual, sum_out)
     if weight.device != x.device:
         raise ValueError(f"weight lives on {weight.device}, x on {x.device}")
     if weight.dtype not in (x.dtype, torch.float32) or weight.shape != (x.size(1),) or not weight.is_contiguous():
@@ -236,7 +236,7 @@ def quantized_linear(
         raise ValueError("lora_a, lora_b and token_to_slot are given together or not at all")
     first: list[int] = []
     a, b = list(lora_a or ()), list(lora_b or ())
-    _no_grad(*rows, *weight, bias, *a, *b)
+    _no_grad(*rows, *weight, bias, *a, *b, out)
     if all(given):
         first = _adapters(a, b, lora_columns, width, columns, dtype, device)
         if token_to_slot.dtype != torch.int32 or token_to_slot.shape != (x.size(0),) or not token_to_slot.is_contiguous() or token_to_slot.device != device:
