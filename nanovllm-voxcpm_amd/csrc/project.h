@@ -106,8 +106,8 @@ template <> struct BPiece<_Float16> {
   }
 };
 
-// What four columns from n on (of the slice; -3 .. columns - 1) of one row gain from `some` ranks, one number at a time: for pieces of B that hold infinities or NaN, which
-// a matrix product would carry to the rows of other slots (0 times them is NaN).
+// What four columns from n on (of the slice; -3 .. columns - 1) of one row gain from `some` ranks, one number at a time: for infinities and NaN in h or B, which a matrix
+// product would carry to the rows of other slots or to other columns (0 times them is NaN).
 template <typename T>
 __device__ inline void add_slowly(const T* b, int columns, int n, int r, int first, int some, const uint16_t* hi, const uint16_t* lo, f32x4& acc) {
   for (int j = first; j < first + some && j < r; ++j) {

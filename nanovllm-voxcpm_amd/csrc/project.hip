@@ -7,8 +7,8 @@
 // a row's pieces are added in the order of its ranks wherever its slot stands in the list: a row's result does not depend on which adapters the rows beside it have (but for one of infinities or NaN, beside which
 // the row's sum is taken in another order).
 //
-// Few rows are bound by the weights' way to the compute units: 64 rows, k 1024, n 8192 6.4 us (8.4 MB; with 32 slots of rank 32, 21 MB more, 16.2), 201 rows, k 8192, n 2048 17 us (all workgroups together take 200 MB from L2 in that time, 46 bytes a ns
-// each; with 48 fp16 slots of rank 64, 63 MB more, 41 us, of which the first product 12.5), one row 3.8 us, with its adapter 7.0.
+// Few rows are bound by the weights' way to the compute units: 64 rows, k 1024, n 8192 6.0 us (8.4 MB; with 32 slots of rank 32, 21 MB more, 17), 201 rows, k 8192, n 2048 17 us (all workgroups together take 200 MB from L2 in that time, 46 bytes a ns
+// each; with 48 fp16 slots of rank 64, 63 MB more, 41 us, of which the first product 12.5), one row 3.6 us, with its adapter 7.0.
 #include "common.h"
 #include "dma.h"
 #include "launch.h"
@@ -27,8 +27,9 @@ namespace {
 // of one piece or two), and a stage holds each wavefront's own B and h.  (Ranks that are no multiple of eight, whose rows of B lie anywhere, are loaded by the lanes behind the last stage.)
 //
 // Rows in four blocks (more than 32, up to kSorted) are taken in the order of their slots where there are eight slots or more; every workgroup works the order out for itself.  The sixteen rows of a block then
-// have few different slots.  (us in their own order / sorted, bf16: 256 rows, k 1024, n 1536, 48 slots of rank 64 36.8 / 26.5, 8 of rank 32 20.6 / 20.7, one slot 16.9 / 20.7; 64 rows, k 2048, n 2048,
-// 16 slots of rank 64 21.4 / 18.1; 32 rows, k 1024, n 8192, 8 slots of rank 32 11.8 / 12.3.  201 rows of 48 fp16 slots of rank 64, k 8192, n 2048: 55.8 / 43.3.)
+// have few different slots.  (us in their own order / sorted, bf16: 256 rows, k 1024, n 1536, 48 slots of rank 64 36.9 / 27.6, 8 of rank 32 21.8 / 21.4, one slot of eight 17.3 / 21.0; 64 rows, k 2048, n 2048,
+// 16 slots of rank 64 21.0 / 18.0, k 1024, n 8192, 32 of rank 32 17.1 / 16.0; 201 rows of 48 fp16 slots of rank 64, k 8192, n 2048 49.0 / 41.7.  Two blocks, 32 rows, k 1024, n 8192, 8 slots of rank 32, lost when they
+// were tried: 11.8 / 12.3.)
 constexpr int kRowWaves = 8, kSorted = 256;
 
 template <int TF, int NF, int LORA> struct RowsShape {
@@ -608,7 +609,7 @@ template <typename T> __global__ __launch_bounds__(kRowWaves * 64) void project_
 }
 
 // The rows' A of at most two times sixteen ranks, a K of two turns, and few enough workgroups that they do not wait for each other in L2: as in one launch / in two, us, graph replay, 1 row, rank 32: k 1024,
-// n 1536 6.8 / 9.3, n 8192 9.2 / 10.1; k 2048, n 2048 9.2 / 10.6, n 8192 14.0 / 12.9; k 4096, n 1024 13.9 / 13.1; of rank 64 (four times sixteen) k 1024, n 1536 8.8 / 8.9, n 8192 13.0 / 9.8.
+// n 1536 7.0 / 9.4, n 8192 9.4 / 10.4; k 2048, n 2048 9.4 / 11.0, n 8192 14.2 / 12.6; k 4096, n 1024 13.9 / 13.5; of rank 64 (four times sixteen), when it was tried, k 1024, n 1536 8.8 / 8.9, n 8192 13.0 / 9.8.
 bool few_rows(const MloraProjectArgs* a) {
   return a->num_slices && a->r % 8 == 0 && a->num_rows <= kFewGroups && a->num_rows * ((a->r + 15) / 16) <= kFewGroups && a->k <= 2048 && static_cast<int64_t>(a->n) * a->k <= 1 << 23;
 }
@@ -684,9 +685,10 @@ int check_project(const MloraProjectArgs* a) {
 
 // Rows by themselves up to 64, and up to 256 while their workgroups are no more than the compute units: what they share out along K a tile has to go through alone, and tiles want the rows in
 // the order of their slots first; beyond, a second round of them costs a base product as much as the first.  (us, graph replay, bf16, 8 slots of rank 32, random; in brackets without adapters:
-// 128 rows, k 4096, n 4096, 256 workgroups: 23.4 [11.6], by tiles 36.0 [12.7]; 192 rows: 35.1 [20.1], 35.7 [12.9]; 96 rows, k 1024, n 8192, 512 workgroups: 20.3 [10.6], 22.2 [6.2].)
+// 128 rows, k 4096, n 4096, 256 workgroups: 24.3 [10.6], by tiles 38.1 [12.5]; 192 rows: 36.9 [18.9], 37.4 [13.1]; 96 rows, k 1024, n 8192, 512 workgroups: 21.7 [9.6], 24.5 [6.1].  Of short K the rule gives up
+// without adapters about what it gains with them: 256 rows, k 1024, n 1536 21.2 [8.3], 23.2 [5.8]; 192 rows, k 2048, n 2048 23.9 [10.6], 27.7 [7.9].)
 // Of the tiles the smallest that are all at work at once, 64 x 64 three a compute unit, 64 x 128 three or, with adapters, two, else 128 x 128, which loads least.  (k 4096, n 4096: 768 rows
-// 21.5 / 24.6 / 26.7 without adapters, 44.3 / 44.9 / 47.5 with; 1024 rows 26.4 / 23.8 / 26.7, 49.8 / 45.4 / 47.2; 2048 rows 47.3 / 45.4 / 35.0, 76.2 / 70.7 / 57.7.)
+// 20.5 / 22.9 / 25.7 without adapters, 45.8 / 46.5 / 52.0 with; 1024 rows 25.3 / 23.0 / 25.6, 60.8 / 46.6 / 50.7; 2048 rows 48.7 / 45.1 / 34.8, 99.1 / 72.4 / 61.4.)
 // Which of the tiles changes nothing in the result: all go through K in the same steps.
 int project_kind(const MloraProjectArgs* a) {
   auto tiles = [&](int rows, int columns) { return static_cast<int64_t>((a->num_rows + rows - 1) / rows) * ((a->n + columns - 1) / columns); };

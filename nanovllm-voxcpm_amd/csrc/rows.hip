@@ -8,8 +8,8 @@
 // on 16 bytes in one or two loads, of others one by one, to the same sums in the same order: where a row lies does not change what comes out.
 // (16 bytes a load is what counts: as unaligned copies, which the compiler splits, the norm of 9392 rows of 1024 bf16 took 20 us and the gate of 9392 rows of 2 x 4096 took 44.)
 // Few rows cost a launch and one trip to memory: the lanes meet between registers, and up to 1024 elements are one wavefront's.
-// Measured (graph replay): norm with residual of 9392 rows of 1024 bf16 14.2 us (67 MB, 4.7 TB/s; an elementwise sum of two such tensors 10.4 for 58 MB), of 3001 rows of 2048 fp16 10.5 us (49 MB); gate of 9392 rows of 2 x 4096 bf16 29.9 us (6.4 TB/s);
-// one row 3.7 us.  Workgroups that stay and fetch their next row ahead gained nothing at any width.
+// Measured (graph replay): norm with residual of 9392 rows of 1024 bf16 14.0 us (67 MB, 4.8 TB/s; an elementwise sum of two such tensors 10.4 for 58 MB), of 3001 rows of 2048 fp16 10.0 us (49 MB); gate of 9392 rows of 2 x 4096 bf16 31.3 us (6.1 TB/s);
+// one row 3.0 us.  Workgroups that stay and fetch their next row ahead gained nothing at any width.
 #include "common.h"
 #include "launch.h"
 

@@ -196,9 +196,9 @@ __global__ __launch_bounds__(kOrderThreads) void order_kernel(MloraProjectArgs a
 
 // A group of up to 64 rows of a slot; 16 RB ranks of one slice.  TEAMS of four wavefronts take 128 columns of K each in turn, a wavefront sixteen of the rows.  The columns of the rows and of
 // the slot's A come by direct loads into one of a team's two buffers, in whole lines, the 16-byte pieces of a row exchanged so that what the lanes read at once lies in all banks.
-// (One team, in which a wavefront waits for nobody but itself: 13.7 us where two take 8.6, K = 1024, 9392 rows, 2 slices of rank 64; 36 and 21 us of K = 4096, 8192 rows of 128 slots, 100 MB: 4.8 TB/s.)
-// Four teams, of 32 ranks at most, where that gives a compute unit one workgroup at most: the whole call with two teams and with four, 600 rows of 32 slots of rank 64: k 8192, n 1024 69.6 and 59.5 us, k 1024, n 1536
-// 23.8 and 22.6; 2000 rows of 8 slots of rank 32, k 4096, n 4096 59.9 and 57.9.
+// (9392 rows, K = 1024, 2 slices of rank 64 10 us; 8192 rows of 128 slots, K = 4096, 23 us: 100 MB of A, 4.3 TB/s.  The whole call with one team in place of two: 181 and 181 us, 90.7 and 89.0.)
+// Four teams, of 32 ranks at most, where that gives a compute unit one workgroup at most: the whole call with two teams and with four, 600 rows of 32 slots of rank 64: k 8192, n 1024 73.9 and 63.9 us, k 1024, n 1536
+// 28.3 and 26.8; 2000 rows of 8 slots of rank 32, k 4096, n 4096 66.4 and 64.0.
 template <typename T, int RB, int TEAMS> __global__ __launch_bounds__(TEAMS * 256) void shrink8_tiles_kernel(MloraProjectArgs a) {
   constexpr int kStage = kGroup * 128 + 16 * RB * 256;
   extern __shared__ char lds[];

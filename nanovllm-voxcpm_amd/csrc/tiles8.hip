@@ -3,10 +3,11 @@
 // Four wavefronts have a tile of y, each a quarter.  128 columns of K of the tile's rows and weights come by direct loads into one of two buffers in LDS, two steps
 // ahead of the products and on into the workgroup's next tile, so that the loads of a tile's beginning run under the end of the one before it.  A load takes
 // whole 128-byte lines of eight rows: with halves of lines of sixteen rows, which want no exchange in LDS, every line was fetched twice (8192 x 8192 x 8192: 655 us; this way 463).
-// Nothing in a tile's end waits for memory of its own: scales and tables come by direct loads a tile ahead, the stores end under the next tile's first step (9392 rows, k 1024, n 8192, 8 slots of rank 64: 166 us
-// without that, 150 with).  Measured in graph replay: 8192 x 8192 x 8192 493-505 us (2.2 PFLOP/s; the library's product with a scale a row and a column 480), 9392 rows, k 1024, n 8192 87-101 us as y's
-// 154 MB fit the cache behind L2 or do not (library 106), with the adapters 146-150, of which this kernel 132-136, the matrix pipes busy for a third of the time.  Tiles of 256 x 128 with three
-// buffers and eight wavefronts: 102 and 181 us.  A word of every line of B asked for a tile ahead of the adapters' steps cost 1 us a tile more than it saved.
+// Nothing in a tile's end waits for memory of its own: scales and tables come by direct loads a tile ahead, the stores end under the next tile's first step (which took 16 us off 9392 rows, k 1024, n 8192, 8 slots of
+// rank 64).  Measured in graph replay: 8192 x 8192 x 8192 493-510 us (2.2 PFLOP/s; the library's product with a scale a row and a column 480), 9392 rows, k 1024, n 8192 94-111 us as y's
+// 154 MB fit the cache behind L2 or do not (library 106), with the adapters of 16 prompts 160-164, the matrix pipes busy for a third of this kernel's time.  What an adapters' step costs is less its products than what it
+// finds out first and waits for.  Tiles of 256 x 128 with three buffers and eight wavefronts took 102 us for the base product where these took 95.  A word of every line of B asked for a tile ahead of the adapters' steps
+// cost 1 us a tile more than it saved.
 #include "common.h"
 #include "dma.h"
 #include "launch.h"

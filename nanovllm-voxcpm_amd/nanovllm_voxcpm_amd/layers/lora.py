@@ -240,8 +240,8 @@ class _LoRALayerBase(nn.Module):
     def quantize_base_(self) -> None:
         """Put the base weight in 8 bits, e4m3 numbers with a scale an output column, and let the 16-bit one go.
 
-        The forward then takes rows in 8 bits (``QuantizedRows``) or in the layer's type, which it puts in 8 bits itself, and adds the same adapters as before; it has no derivatives.
-        For fp16 and bf16 layers on the GPU whose input features are a multiple of 16; call it after the base weight is loaded.  The state dict has ``weight_values`` and
+        The forward then takes rows in 8 bits (``QuantizedRows``) or in the layer's type, which it puts in 8 bits itself, and adds the same adapters as before, whose input are those 8-bit rows too; it has no
+        derivatives.  For fp16 and bf16 layers on the GPU whose input features are a multiple of 16, with up to 8 adapter targets; call it after the base weight is loaded.  The state dict has ``weight_values`` and
         ``weight_scales`` (both as integers, which a change of the module's type leaves as they are) in place of ``weight``.
         """
         self.check_base_for_8_bits()
